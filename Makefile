@@ -1,7 +1,7 @@
 # Builds everything in-tree (the .so files travel to the GPU box with the snapshot).
 #   make            HIP library + pybind11 modules + CPU oracle
 #   make lib        envpool_amd/libenvpool_amd.so   (hipcc, gfx950)
-#   make pymod      envpool_amd/dummy/dummy_envpool*.so, envpool_amd/ygopro/ygopro_envpool*.so
+#   make pymod      envpool_amd/dummy/dummy_envpool*.so, envpool_amd/ygopro/ygopro_envpool*.so, envpool_amd/policy_native*.so
 #   make oracle     oracle/liboracle.so             (gcc; test infrastructure)
 HIPCC ?= /opt/rocm/bin/hipcc
 CXX ?= g++
@@ -15,14 +15,14 @@ CSRC := envpool_amd/csrc
 LIB := envpool_amd/libenvpool_amd.so
 HIP_SRCS := $(wildcard $(CSRC)/*.hip)
 HIP_DEPS := $(wildcard $(CSRC)/*.hpp) $(wildcard $(CSRC)/*.inl) $(wildcard include/*.h)
-PYMODS := envpool_amd/dummy/dummy_envpool$(EXT) $(if $(wildcard $(CSRC)/py_ygopro.cpp),envpool_amd/ygopro/ygopro_envpool$(EXT))
+PYMODS := envpool_amd/dummy/dummy_envpool$(EXT) envpool_amd/policy_native$(EXT) $(if $(wildcard $(CSRC)/py_ygopro.cpp),envpool_amd/ygopro/ygopro_envpool$(EXT))
 
 all: lib pymod oracle synth examples
 
 lib: $(LIB)
 
 $(LIB): $(HIP_SRCS) $(HIP_DEPS)
-	$(HIPCC) --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -shared -Iinclude -o $@ $(HIP_SRCS)
+	$(HIPCC) --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -shared -Xclang -target-feature -Xclang -packed-fp32-ops -Iinclude -o $@ $(HIP_SRCS)
 
 pymod: $(PYMODS)
 
@@ -33,6 +33,10 @@ envpool_amd/dummy/dummy_envpool$(EXT): $(CSRC)/py_dummy.cpp $(CSRC)/py_common.h 
 envpool_amd/ygopro/ygopro_envpool$(EXT): $(CSRC)/py_ygopro.cpp $(CSRC)/py_common.h include/envpool_amd.h include/envpool_amd_ygo.h $(LIB)
 	$(CXX) -O2 -std=c++17 -fPIC -shared -fvisibility=hidden $(PYINC) -Iinclude -o $@ $< \
 	  -Lenvpool_amd -lenvpool_amd -Wl,-rpath,'$$ORIGIN/..'
+
+envpool_amd/policy_native$(EXT): $(CSRC)/py_policy.cpp $(CSRC)/py_common.h include/envpool_amd.h include/envpool_amd_policy.h $(LIB)
+	$(CXX) -O2 -std=c++17 -fPIC -shared -fvisibility=hidden $(PYINC) -Iinclude -o $@ $< \
+	  -Lenvpool_amd -lenvpool_amd -Wl,-rpath,'$$ORIGIN'
 
 oracle:
 	$(MAKE) -C oracle

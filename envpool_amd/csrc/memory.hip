@@ -1,0 +1,158 @@
+// memory.hip - ep_memory_step / ep_memory_scan: checks and launches.
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/envpool_amd_policy.h"
+#include "common.hpp"
+#include "memory_kernels.hpp"
+
+namespace {
+
+using epc::fail;
+
+bool float_type(int32_t dtype) { return dtype == EP_F32 || dtype == EP_F16 || dtype == EP_BF16; }
+size_t size_of(int32_t dtype) { return dtype == EP_F32 ? 4 : 2; }
+
+template <class F> void with_type(int32_t dtype, F f) {
+  if (dtype == EP_F32) f(float{});
+  else if (dtype == EP_F16) f(epm::f16{});
+  else f(epm::bf16{});
+}
+
+int check_workspace(const void* ws, int64_t have, int64_t need) {
+  if (need > 0 && (!ws || have < need))
+    return fail(EP_ERR_INVALID, "workspace of %lld bytes is smaller than the %lld this call needs", (long long)(ws ? have : 0), (long long)need);
+  if ((uintptr_t)ws % 16) return fail(EP_ERR_INVALID, "workspace: not aligned to 16 bytes");
+  return EP_OK;
+}
+
+// Up to this many rows every workgroup looks the whole batch's ids through for a second row of its env
+// (a few KB out of L2); above it two small launches count the rows of each env first.
+constexpr int64_t kLookThrough = 1024;
+
+int64_t step_workspace(const ep_memory_step_args* a) {
+  return a->env_id && a->rows > kLookThrough ? a->num_envs * 4 : 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t ep_memory_step_workspace(const ep_memory_step_args* a) { return a ? step_workspace(a) : 0; }
+
+int ep_memory_step(const ep_memory_step_args* a) {
+  if (!a) return fail(EP_ERR_INVALID, "null argument");
+  if (!float_type(a->dtype)) return fail(EP_ERR_INVALID, "dtype = %d is none of EP_F32, EP_F16, EP_BF16", a->dtype);
+  if (a->num_envs < 1 || a->num_envs > INT32_MAX) return fail(EP_ERR_INVALID, "num_envs = %lld", (long long)a->num_envs);
+  if (a->rows < 0 || a->rows > INT32_MAX) return fail(EP_ERR_INVALID, "rows = %lld", (long long)a->rows);
+  if (a->heads < 1 || a->heads > 65535) return fail(EP_ERR_INVALID, "heads = %d is outside [1, 65535]", a->heads);
+  if (a->kv_heads < 1 || a->heads % a->kv_heads) return fail(EP_ERR_INVALID, "kv_heads = %d does not divide heads = %d", a->kv_heads, a->heads);
+  if (a->key_dim < 1 || a->key_dim > 256 || a->value_dim < 1 || a->value_dim > 256)
+    return fail(EP_ERR_INVALID, "key_dim = %d, value_dim = %d: not both in [1, 256]", a->key_dim, a->value_dim);
+  if (!a->env_id && a->rows > a->num_envs) return fail(EP_ERR_INVALID, "rows = %lld of %lld envs without env_id", (long long)a->rows, (long long)a->num_envs);
+  if (a->rows > 0 && (!a->q || !a->k || !a->v || !a->out || !a->log_decay || !a->state)) return fail(EP_ERR_INVALID, "q, k, v, out, log_decay, state: null pointer");
+  if (a->fresh && a->fresh_dtype != EP_BOOL && a->fresh_dtype != EP_U8 && a->fresh_dtype != EP_I32)
+    return fail(EP_ERR_INVALID, "fresh_dtype = %d is none of EP_BOOL, EP_U8, EP_I32", a->fresh_dtype);
+  if (!std::isfinite(a->scale)) return fail(EP_ERR_INVALID, "scale = %g", (double)a->scale);
+  const void* typed[] = {a->q, a->k, a->v, a->out};
+  for (const void* ptr : typed)
+    if ((uintptr_t)ptr % size_of(a->dtype)) return fail(EP_ERR_INVALID, "q, k, v, out: not aligned to their type");
+  const void* words[] = {a->log_decay, a->state, a->env_id, a->fresh_dtype == EP_I32 ? a->fresh : nullptr, a->error};
+  for (const void* ptr : words)
+    if ((uintptr_t)ptr % 4) return fail(EP_ERR_INVALID, "an array of 4-byte values is not aligned to 4 bytes");
+  if (int rc = check_workspace(a->workspace, a->workspace_bytes, step_workspace(a))) return rc;
+  if (a->rows == 0) return EP_OK;
+  EP_ENTER_DEVICE(a->device_id);
+  const hipStream_t stream = (hipStream_t)a->stream;
+  epm::Step k{};
+  k.num_envs = a->num_envs, k.rows = a->rows;
+  k.heads = a->heads, k.kv_group = a->heads / a->kv_heads, k.dk = a->key_dim, k.dv = a->value_dim;
+  k.q = a->q, k.k = a->k, k.v = a->v, k.out = a->out;
+  for (int i = 0; i < 2; ++i)
+    k.q_stride[i] = a->q_stride[i], k.k_stride[i] = a->k_stride[i], k.v_stride[i] = a->v_stride[i], k.out_stride[i] = a->out_stride[i];
+  k.log_decay = a->log_decay, k.state = a->state, k.env_id = a->env_id, k.env_id_offset = a->env_id_offset;
+  k.fresh = a->fresh, k.fresh_i32 = a->fresh_dtype == EP_I32;
+  k.scale = a->scale, k.error = a->error;
+  k.claims = step_workspace(a) ? (int32_t*)a->workspace : nullptr;
+  if (k.claims) {
+    const dim3 grid((unsigned)((a->rows + 255) / 256));
+    hipLaunchKernelGGL(epm::clear_claims, grid, dim3(256), 0, stream, k);
+    hipLaunchKernelGGL(epm::count_claims, grid, dim3(256), 0, stream, k);
+    HIP_TRY(hipGetLastError());
+  }
+  with_type(a->dtype, [&](auto t) {
+    hipLaunchKernelGGL(epm::step_row<decltype(t)>, dim3((unsigned)std::min<int64_t>(a->rows, 1 << 20), (unsigned)a->heads), dim3(256), 0, stream, k);
+  });
+  HIP_TRY(hipGetLastError());
+  return EP_OK;
+}
+
+int64_t ep_memory_scan_workspace(const ep_memory_scan_args*) { return 0; }
+
+int ep_memory_scan(const ep_memory_scan_args* a) {
+  if (!a) return fail(EP_ERR_INVALID, "null argument");
+  if (!float_type(a->dtype)) return fail(EP_ERR_INVALID, "dtype = %d is none of EP_F32, EP_F16, EP_BF16", a->dtype);
+  if (a->out_dtype != a->dtype && a->out_dtype != EP_F32) return fail(EP_ERR_INVALID, "out_dtype = %d is neither dtype nor EP_F32", a->out_dtype);
+  if (a->steps < 0 || a->steps > INT32_MAX) return fail(EP_ERR_INVALID, "steps = %lld", (long long)a->steps);
+  if (a->rows < 0 || a->rows > INT32_MAX) return fail(EP_ERR_INVALID, "rows = %lld", (long long)a->rows);
+  if (a->heads < 1 || a->heads > 65535) return fail(EP_ERR_INVALID, "heads = %d is outside [1, 65535]", a->heads);
+  const int32_t groups[] = {a->q_group, a->k_group, a->v_group};
+  for (int32_t g : groups)
+    if (g < 1 || a->heads % g) return fail(EP_ERR_INVALID, "a head group of %d does not divide heads = %d", g, a->heads);
+  if (a->key_dim < 1 || a->key_dim > 128 || a->value_dim < 1 || a->value_dim > 128)
+    return fail(EP_ERR_INVALID, "key_dim = %d, value_dim = %d: not both in [1, 128]", a->key_dim, a->value_dim);
+  if (a->rows > 0 && !a->log_decay) return fail(EP_ERR_INVALID, "log_decay: null pointer");
+  if (a->rows > 0 && a->steps > 0 && (!a->q || !a->k || !a->v)) return fail(EP_ERR_INVALID, "q, k, v: null pointer");
+  if (a->rows > 0 && a->steps > 0 && !a->out && !a->state_out) return fail(EP_ERR_INVALID, "neither out nor state_out is wanted");
+  if (!std::isfinite(a->inc_scale) || !std::isfinite(a->out_scale)) return fail(EP_ERR_INVALID, "inc_scale = %g, out_scale = %g", (double)a->inc_scale, (double)a->out_scale);
+  const void* typed[] = {a->q, a->k, a->v};
+  for (const void* ptr : typed)
+    if ((uintptr_t)ptr % size_of(a->dtype)) return fail(EP_ERR_INVALID, "q, k, v: not aligned to their type");
+  if ((uintptr_t)a->out % size_of(a->out_dtype)) return fail(EP_ERR_INVALID, "out: not aligned to its type");
+  const void* words[] = {a->log_decay, a->state_in, a->state_out};
+  for (const void* ptr : words)
+    if ((uintptr_t)ptr % 4) return fail(EP_ERR_INVALID, "an array of 4-byte values is not aligned to 4 bytes");
+  if (int rc = check_workspace(a->workspace, a->workspace_bytes, ep_memory_scan_workspace(a))) return rc;
+  if (a->rows == 0 || (a->steps == 0 && !a->state_out)) return EP_OK;
+  EP_ENTER_DEVICE(a->device_id);
+  const hipStream_t stream = (hipStream_t)a->stream;
+  epm::Scan k{};
+  k.steps = a->steps, k.rows = a->rows, k.heads = a->heads;
+  k.q_group = a->q_group, k.k_group = a->k_group, k.v_group = a->v_group, k.dk = a->key_dim, k.dv = a->value_dim;
+  k.q = a->q, k.k = a->k, k.v = a->v, k.out = a->out, k.out_f32 = a->out_dtype == EP_F32;
+  for (int i = 0; i < 3; ++i)
+    k.q_stride[i] = a->q_stride[i], k.k_stride[i] = a->k_stride[i], k.v_stride[i] = a->v_stride[i], k.out_stride[i] = a->out_stride[i];
+  k.log_decay = a->log_decay, k.fresh = a->fresh;
+  for (int i = 0; i < 2; ++i) k.fresh_stride[i] = a->fresh_stride[i];
+  k.state_in = a->state_in, k.state_out = a->state_out;
+  for (int i = 0; i < 4; ++i) k.in_stride[i] = a->state_in_stride[i], k.outs_stride[i] = a->state_out_stride[i];
+  k.inc_scale = a->inc_scale, k.out_scale = a->out_scale, k.reverse = a->reverse;
+  with_type(a->dtype, [&](auto t) {
+    const size_t lds = (size_t)(a->key_dim * 130) * 4;
+    const auto fn = epm::scan_steps<decltype(t)>;
+    (void)hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    hipLaunchKernelGGL(fn, dim3((unsigned)std::min<int64_t>(a->rows, 1 << 20), (unsigned)a->heads), dim3(128), lds, stream, k);
+  });
+  HIP_TRY(hipGetLastError());
+  return EP_OK;
+}
+
+int ep_memory_sum_heads(int32_t device_id, const float* src, int64_t n, int32_t heads_out, int32_t group, int32_t dim, void* out, int32_t dtype,
+                        void* stream) {
+  if (!float_type(dtype)) return fail(EP_ERR_INVALID, "dtype = %d is none of EP_F32, EP_F16, EP_BF16", dtype);
+  if (n < 0 || heads_out < 1 || group < 1 || dim < 1) return fail(EP_ERR_INVALID, "n, heads_out, group, dim: out of range");
+  const int64_t total = n * heads_out * dim;
+  if (total == 0) return EP_OK;
+  if (!src || !out) return fail(EP_ERR_INVALID, "src, out: null pointer");
+  if ((uintptr_t)src % 4 || (uintptr_t)out % size_of(dtype)) return fail(EP_ERR_INVALID, "src, out: not aligned to their type");
+  if ((total + 255) / 256 > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld elements", (long long)total);
+  EP_ENTER_DEVICE(device_id);
+  with_type(dtype, [&](auto t) {
+    hipLaunchKernelGGL(epm::sum_heads<decltype(t)>, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, (hipStream_t)stream, src, total, group, dim,
+                       (decltype(t)*)out);
+  });
+  HIP_TRY(hipGetLastError());
+  return EP_OK;
+}
+
+}  // extern "C"
