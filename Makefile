@@ -21,8 +21,12 @@ all: lib pymod oracle synth examples
 
 lib: $(LIB)
 
-$(LIB): $(HIP_SRCS) $(HIP_DEPS)
-	$(HIPCC) --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -shared -Xclang -target-feature -Xclang -packed-fp32-ops -Iinclude -o $@ $(HIP_SRCS)
+HIP_OBJS := $(patsubst $(CSRC)/%.hip,build/%.o,$(HIP_SRCS))
+build/%.o: $(CSRC)/%.hip $(HIP_DEPS)
+	@mkdir -p build
+	$(HIPCC) --offload-arch=$(ARCH) -O3 -std=c++17 -fPIC -Xclang -target-feature -Xclang -packed-fp32-ops -Iinclude -c -o $@ $<
+$(LIB): $(HIP_OBJS)
+	$(HIPCC) --offload-arch=$(ARCH) -fPIC -shared -o $@ $(HIP_OBJS)
 
 pymod: $(PYMODS)
 

@@ -5,6 +5,7 @@
 #include "../../include/envpool_amd_policy.h"
 #include "common.hpp"
 #include "memory_kernels.hpp"
+#include "memory_scan.hpp"
 
 namespace {
 
@@ -32,6 +33,66 @@ constexpr int64_t kLookThrough = 1024;
 
 int64_t step_workspace(const ep_memory_step_args* a) {
   return a->env_id && a->rows > kLookThrough ? a->num_envs * 4 : 0;
+}
+
+template <class T, int DK, int DV> int scan_tile(const epm::Scan& k, epm::Parts parts, unsigned states, hipStream_t stream) {
+  constexpr size_t lds = epm::ScanTile<T, DK, DV>::kLds;
+  const auto fn = epm::scan_chunks<T, DK, DV>;
+  if (lds > 65536) HIP_TRY(hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+  if (parts.n_seg > 1) {
+    parts.state_only = 1;
+    hipLaunchKernelGGL(fn, dim3(states, (unsigned)parts.n_seg - 1), dim3(256), lds, stream, k, parts);
+    hipLaunchKernelGGL((epm::join_parts<DK, DV>), dim3(states, DK * DV / 1024), dim3(256), 0, stream, k, parts);
+    parts.state_only = 0;
+  }
+  hipLaunchKernelGGL(fn, dim3(states, (unsigned)parts.n_seg), dim3(256), lds, stream, k, parts);
+  return EP_OK;
+}
+
+int padded(int dim) { return dim <= 64 ? 64 : 128; }
+
+// Split of the time axis. One part per state keeps everything single-pass. With fewer states than fill the
+// chip, parts of at least two chunks are walked side by side: keys and values are then read twice (first for
+// the states between the parts).
+constexpr int64_t kFill = 1024;  // workgroups
+int64_t scan_parts(const ep_memory_scan_args* a) {
+  const int64_t states = a->rows * a->heads, chunks = (a->steps + epm::kChunk - 1) / epm::kChunk;
+  if (states <= 0 || states * 2 > kFill || chunks < 4) return 1;
+  return std::min<int64_t>(std::min<int64_t>(chunks / 2, (kFill + states - 1) / states), 65535);
+}
+int64_t scan_workspace(const ep_memory_scan_args* a, int64_t n_seg) {
+  if (n_seg <= 1) return 0;
+  return a->rows * a->heads * n_seg * ((int64_t)padded(a->key_dim) * padded(a->value_dim) * 4 + 4);
+}
+
+int scan_launch(const ep_memory_scan_args* a, const epm::Scan& k, hipStream_t stream) {
+  epm::Parts parts{};
+  const int64_t chunks = std::max<int64_t>(1, (a->steps + epm::kChunk - 1) / epm::kChunk);
+  const int64_t want = scan_parts(a), per = (chunks + want - 1) / want;
+  parts.seg_len = per * epm::kChunk;
+  parts.n_seg = (int32_t)((chunks + per - 1) / per);
+  if (parts.n_seg > 1) {
+    parts.ws_state = (epm::f32x4*)a->workspace;
+    parts.ws_carry = (float*)((char*)a->workspace + a->rows * a->heads * parts.n_seg * ((int64_t)padded(a->key_dim) * padded(a->value_dim) * 4));
+  }
+  const int64_t size = size_of(a->dtype), vec = 16 / size;
+  const auto aligned = [&](const void* ptr, const int64_t* stride, int64_t unit, int64_t bytes) {
+    return (uintptr_t)ptr % unit == 0 && stride[0] * bytes % unit == 0 && stride[1] * bytes % unit == 0 && stride[2] * bytes % unit == 0;
+  };
+  parts.vec = aligned(a->q, a->q_stride, 16, size) && aligned(a->k, a->k_stride, 16, size) && aligned(a->v, a->v_stride, 16, size) &&
+              a->key_dim % vec == 0 && a->value_dim % vec == 0;
+  const int64_t out_size = size_of(a->out_dtype);
+  parts.vec_out = aligned(a->out, a->out_stride, 4 * out_size, out_size);
+  const int64_t states = a->rows * a->heads;
+  if (states > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld states", (long long)states);
+  int rc = EP_OK;
+  with_type(a->dtype, [&](auto t) {
+    using T = decltype(t);
+    const unsigned n = (unsigned)states;
+    if (a->key_dim <= 64) rc = a->value_dim <= 64 ? scan_tile<T, 64, 64>(k, parts, n, stream) : scan_tile<T, 64, 128>(k, parts, n, stream);
+    else rc = a->value_dim <= 64 ? scan_tile<T, 128, 64>(k, parts, n, stream) : scan_tile<T, 128, 128>(k, parts, n, stream);
+  });
+  return rc;
 }
 
 }  // namespace
@@ -87,7 +148,7 @@ int ep_memory_step(const ep_memory_step_args* a) {
   return EP_OK;
 }
 
-int64_t ep_memory_scan_workspace(const ep_memory_scan_args*) { return 0; }
+int64_t ep_memory_scan_workspace(const ep_memory_scan_args* a) { return a ? scan_workspace(a, scan_parts(a)) : 0; }
 
 int ep_memory_scan(const ep_memory_scan_args* a) {
   if (!a) return fail(EP_ERR_INVALID, "null argument");
@@ -127,12 +188,7 @@ int ep_memory_scan(const ep_memory_scan_args* a) {
   k.state_in = a->state_in, k.state_out = a->state_out;
   for (int i = 0; i < 4; ++i) k.in_stride[i] = a->state_in_stride[i], k.outs_stride[i] = a->state_out_stride[i];
   k.inc_scale = a->inc_scale, k.out_scale = a->out_scale, k.reverse = a->reverse;
-  with_type(a->dtype, [&](auto t) {
-    const size_t lds = (size_t)(a->key_dim * 130) * 4;
-    const auto fn = epm::scan_steps<decltype(t)>;
-    (void)hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    hipLaunchKernelGGL(fn, dim3((unsigned)std::min<int64_t>(a->rows, 1 << 20), (unsigned)a->heads), dim3(128), lds, stream, k);
-  });
+  if (int rc = scan_launch(a, k, stream)) return rc;
   HIP_TRY(hipGetLastError());
   return EP_OK;
 }

@@ -127,55 +127,6 @@ struct Scan {
   int32_t reverse;
 };
 
-// The recurrence step by step: one workgroup per (row, head), one thread per value column, the state in
-// LDS (column by column: a thread touches its own only).
-template <class T> __global__ __launch_bounds__(128) void scan_steps(Scan p) {
-  extern __shared__ float lds[];
-  float* s = lds;                  // [dk][128]
-  float* qs = lds + p.dk * 128;    // [dk]
-  float* ks = qs + p.dk;
-  const int h = blockIdx.y;
-  const int j = threadIdx.x;
-  const float decay = expf(p.log_decay[h]);
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    for (int i = 0; i < p.dk; ++i)
-      s[i * 128 + j] = p.state_in && j < p.dv ? p.state_in[row * p.in_stride[0] + h * p.in_stride[1] + i * p.in_stride[2] + j * p.in_stride[3]] : 0.f;
-    for (int64_t n = 0; n < p.steps; ++n) {
-      const int64_t t = p.reverse ? p.steps - 1 - n : n;
-      // forward: d_t before step t; backward: d_{t+1}, and none before the first
-      float keep = 1.f;
-      const int64_t gate = p.reverse ? t + 1 : t;
-      if (gate < p.steps) keep = p.fresh && p.fresh[gate * p.fresh_stride[0] + row * p.fresh_stride[1]] ? 0.f : decay;
-      const T* q = (const T*)p.q + t * p.q_stride[0] + row * p.q_stride[1] + (h / p.q_group) * p.q_stride[2];
-      const T* k = (const T*)p.k + t * p.k_stride[0] + row * p.k_stride[1] + (h / p.k_group) * p.k_stride[2];
-      const T* v = (const T*)p.v + t * p.v_stride[0] + row * p.v_stride[1] + (h / p.v_group) * p.v_stride[2];
-      __syncthreads();
-      if (j < p.dk) qs[j] = (float)q[j], ks[j] = (float)k[j] * p.inc_scale;
-      __syncthreads();
-      const float vj = j < p.dv ? (float)v[j] : 0.f;
-      float acc = 0.f;
-      for (int i = 0; i < p.dk; ++i) {
-        const float now = (keep == 0.f ? 0.f : keep * s[i * 128 + j]) + ks[i] * vj;
-        s[i * 128 + j] = now;
-        acc += qs[i] * now;
-      }
-      if (p.out && j < p.dv) {
-        const int64_t at = t * p.out_stride[0] + row * p.out_stride[1] + h * p.out_stride[2] + j;
-        if (p.out_f32) ((float*)p.out)[at] = acc * p.out_scale;
-        else ((T*)p.out)[at] = (T)(acc * p.out_scale);
-      }
-    }
-    if (p.state_out && j < p.dv) {
-      float last = 1.f;
-      if (p.reverse && p.steps > 0) last = p.fresh && p.fresh[row * p.fresh_stride[1]] ? 0.f : decay;
-      for (int i = 0; i < p.dk; ++i)
-        p.state_out[row * p.outs_stride[0] + h * p.outs_stride[1] + i * p.outs_stride[2] + j * p.outs_stride[3]] =
-            last == 0.f ? 0.f : last * s[i * 128 + j];
-    }
-    __syncthreads();
-  }
-}
-
 template <class T> __global__ __launch_bounds__(256) void sum_heads(const float* src, int64_t total, int32_t group, int32_t dim, T* out) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;  // over [n][heads_out][dim]
   if (i >= total) return;

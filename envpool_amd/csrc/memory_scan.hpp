@@ -1,0 +1,425 @@
+// memory_scan.hpp - the chunked form of the memory on matrix cores.
+//
+// A workgroup of four waves owns one state (row, head) and walks along time in chunks of 64 steps. Inside a
+// chunk, with D[t, s] = decay^|t-s| where s reaches t (no episode starts between them), else 0:
+//   P = (Q K^T) * D                       scores, 64 x 64
+//   O = w_in[t] * (Q S) + P V             S: the state the chunk starts from
+//   S = carry * S + (K * w_up[s])^T V
+// Everything is computed transposed (scores as [s, t], outputs as [v, t]): the accumulators of one product are
+// then laid out as an operand of the next up to a permutation of the summed index, which is applied to the
+// other operand as well. So the state never leaves its registers (32 bits; a copy rounded to the operands' type
+// feeds Q S), scores cross LDS once because each wave computes 16 of the 64 query columns and needs all of
+// them for its quarter of the value columns, and an output row is written 4 values a lane.
+// Time backwards (for gradients) is the same chunk with the triangle and the weights mirrored.
+#pragma once
+#include "memory_kernels.hpp"
+
+namespace epm {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+constexpr int kChunk = 64;
+
+template <class T> struct Mma;
+
+template <class T, class V8, class V4> struct Mma16 {
+  using frag = V8;
+  static constexpr int K = 32;  // summed index per fragment: lane group g = lane / 16 holds 8g .. 8g+7
+  static __device__ frag row(const T* tile, int stride, int r0, int k0) {
+    return *(const V8*)(tile + (r0 + (threadIdx.x & 15)) * stride + k0 + 8 * ((threadIdx.x >> 4) & 3));
+  }
+  // the order that a pair of accumulators has: 4g .. 4g+3, then 16 + 4g .. 16 + 4g+3
+  static __device__ frag row_as_acc(const T* tile, int stride, int r0, int k0) {
+    const T* p = tile + (r0 + (threadIdx.x & 15)) * stride + k0 + 4 * ((threadIdx.x >> 4) & 3);
+    const V4 a = *(const V4*)p, b = *(const V4*)(p + 16);
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  // column c0 + lane % 16 of rows k0 + 8g .. k0 + 8g + 7: the transposing LDS read takes 4 rows x 16 columns
+  // per 16 lanes, lane i addressing 4 values of row i / 4
+  static __device__ frag col(const T* tile, int stride, int k0, int c0) {
+    const int i = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+    const T* p = tile + (k0 + 8 * g + (i >> 2)) * stride + c0 + 4 * (i & 3);
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4* lp;
+    union { s4 s[2]; V8 v; } u;
+    u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p));
+    u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 4 * stride));
+    return u.v;
+  }
+  static __device__ frag from_acc(f32x4 a, f32x4 b) {
+    frag f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f[r] = (T)a[r], f[r + 4] = (T)b[r];
+    return f;
+  }
+  static __device__ frag weighted(frag f, const float* w) {  // element e times w[e], e = 0 .. 7
+    frag o;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) o[r] = (T)(w[r] != 0.f ? (float)f[r] * w[r] : 0.f);
+    return o;
+  }
+  static __device__ void put4(T* p, f32x4 a) {
+    V4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = (T)a[r];
+    *(V4*)p = v;
+  }
+};
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+template <> struct Mma<bf16> : Mma16<bf16, bf16x8, bf16x4> {
+  static constexpr uint32_t kExp = 0x7f807f80u;
+  static __device__ f32x4 mul(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mma<f16> : Mma16<f16, f16x8, f16x4> {
+  static constexpr uint32_t kExp = 0x7c007c00u;
+  static __device__ f32x4 mul(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mma<float> {
+  using frag = f32x4;
+  static constexpr int K = 16;  // four products of 4: lane group g holds 4g + r in step r
+  static constexpr uint32_t kExp = 0x7f800000u;
+  static __device__ frag row(const float* tile, int stride, int r0, int k0) {
+    return *(const f32x4*)(tile + (r0 + (threadIdx.x & 15)) * stride + k0 + 4 * ((threadIdx.x >> 4) & 3));
+  }
+  static __device__ frag row_as_acc(const float* tile, int stride, int r0, int k0) { return row(tile, stride, r0, k0); }
+  static __device__ frag col(const float* tile, int stride, int k0, int c0) {
+    const float* p = tile + (k0 + 4 * ((threadIdx.x >> 4) & 3)) * stride + c0 + (threadIdx.x & 15);
+    return frag{p[0], p[stride], p[2 * stride], p[3 * stride]};
+  }
+  static __device__ frag weighted(frag f, const float* w) {
+    frag o;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = w[r] != 0.f ? f[r] * w[r] : 0.f;
+    return o;
+  }
+  static __device__ void put4(float* p, f32x4 a) { *(f32x4*)p = a; }
+  static __device__ f32x4 mul(frag a, frag b, f32x4 c) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b[r], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// how a launch's states come and go
+struct Parts {
+  int64_t seg_len;     // steps per part of the time axis (a multiple of 64), blockIdx.y counts parts in time
+  int32_t n_seg;
+  f32x4* ws_state;     // [row * heads][n_seg][DK * DV / 4] in accumulator order: what a part starts from (read), or
+  float* ws_carry;     // its own contribution and how far it lets the state before it through (written)
+  int32_t state_only;  // the first of two passes over split time: contributions only
+  int32_t vec, vec_out;
+};
+
+template <class T, int DK, int DV> struct ScanTile {
+  static constexpr int kVec = 16 / sizeof(T);                // values of one 16-byte load
+  static constexpr int SK = DK + kVec, SV = DV + kVec;       // LDS row strides (16 bytes of padding)
+  static constexpr int SP = kChunk + kVec;
+  static constexpr int kQ = kChunk * DK / kVec / 256;        // 16-byte loads per thread and tile
+  static constexpr int kV = kChunk * DV / kVec / 256;
+  static constexpr size_t kLds = (size_t)kChunk * (2 * SK + SV + SP) * sizeof(T) + 2 * kChunk * sizeof(float);
+};
+
+__device__ inline uint32_t has_ones(uint32_t x, uint32_t e, uint32_t half) {  // any 16-bit (or the 32-bit) exponent all ones
+  const uint32_t y = x & e;
+  return half ? ((y & 0xffffu) == (e & 0xffffu)) | ((y >> 16) == (e >> 16)) : y == e;
+}
+
+template <class T, int DK, int DV> __global__ __launch_bounds__(256) void scan_chunks(Scan p, Parts parts) {
+  using M = Mma<T>;
+  using Tile = ScanTile<T, DK, DV>;
+  using frag = typename M::frag;
+  constexpr int K = M::K, kVec = Tile::kVec, SK = Tile::SK, SV = Tile::SV, SP = Tile::SP;
+  constexpr int ND = DK / 16, NV = DV / 64;  // state tiles of a wave: all keys, a quarter of the values
+  extern __shared__ __align__(16) char lds[];
+  T* qs = (T*)lds;
+  T* ks = qs + kChunk * SK;
+  T* vs = ks + kChunk * SK;
+  T* ps = vs + kChunk * SV;
+  float* w_up = (float*)(ps + kChunk * SP);
+  int* odd = (int*)(w_up + kChunk);  // a key or value of this chunk is not finite
+
+  const int64_t rh = blockIdx.x;
+  const int64_t row = rh / p.heads;
+  const int h = (int)(rh % p.heads);
+  // (of the contributions only those are needed that a later part starts from)
+  const int seg = blockIdx.y + (parts.state_only && p.reverse ? 1 : 0);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
+  const int v0 = wave * (DV / 4);
+  const bool rev = p.reverse;
+  const float l2 = fmaxf(p.log_decay[h] * 1.44269504088896f, -1e30f);  // (decay 0: its power 0 is still 1)
+
+  const T* gq = (const T*)p.q + row * p.q_stride[1] + (h / p.q_group) * p.q_stride[2];
+  const T* gk = (const T*)p.k + row * p.k_stride[1] + (h / p.k_group) * p.k_stride[2];
+  const T* gv = (const T*)p.v + row * p.v_stride[1] + (h / p.v_group) * p.v_stride[2];
+  const uint8_t* gf = p.fresh ? p.fresh + row * p.fresh_stride[1] : nullptr;
+
+  // ---- the state the part starts from
+  f32x4 s[ND][NV];
+  f32x4* ws = parts.ws_state ? parts.ws_state + (rh * parts.n_seg + seg) * (DK * DV / 4) : nullptr;
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      s[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (parts.state_only) continue;
+      if (parts.n_seg > 1) {
+        s[i][j] = ws[((i * NV + j) * 4 + wave) * 64 + lane];
+      } else if (p.state_in) {
+        const int v = v0 + 16 * j + l16, d = 16 * i + 4 * g;
+        const float* a = p.state_in + row * p.in_stride[0] + h * p.in_stride[1] + v * p.in_stride[3];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (v < p.dv && d + r < p.dk) s[i][j][r] = a[(d + r) * p.in_stride[2]];
+      }
+    }
+  float through = 1.f;
+
+  const int64_t seg0 = seg * parts.seg_len;
+  const int64_t seg1 = seg0 + parts.seg_len < p.steps ? seg0 + parts.seg_len : p.steps;
+
+  // ---- a chunk's tiles, on their way from memory
+  uint4 rq[Tile::kQ], rk[Tile::kQ], rv[Tile::kV];
+  uint8_t rf = 0;
+  const auto load_tile = [&](uint4* r, int count, const T* base, int64_t step_stride, int width, int padded, int64_t start, int n) {
+    const int per_row = padded / kVec;
+#pragma unroll
+    for (int i = 0; i < count; ++i) {
+      const int at = i * 256 + threadIdx.x;
+      const int t = at / per_row, c = (at % per_row) * kVec;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (t < n && c < width) {
+        const T* a = base + (start + t) * step_stride + c;
+        if (parts.vec) {
+          x = *(const uint4*)a;
+        } else {
+          union { uint4 u; T e[kVec]; } b;
+          b.u = x;
+#pragma unroll
+          for (int e = 0; e < kVec; ++e)
+            if (c + e < width) b.e[e] = a[e];
+          x = b.u;
+        }
+      }
+      r[i] = x;
+    }
+  };
+  const auto load = [&](int64_t start, int n) {
+    if (!parts.state_only) load_tile(rq, Tile::kQ, gq, p.q_stride[0], p.dk, DK, start, n);
+    load_tile(rk, Tile::kQ, gk, p.k_stride[0], p.dk, DK, start, n);
+    load_tile(rv, Tile::kV, gv, p.v_stride[0], p.dv, DV, start, n);
+    rf = gf && lane < n ? gf[(start + lane) * p.fresh_stride[0]] : 0;
+  };
+  const auto put_tile = [&](const uint4* r, int count, T* tile, int padded, int stride) {
+    uint32_t bad = 0;
+    const int per_row = padded / kVec;
+#pragma unroll
+    for (int i = 0; i < count; ++i) {
+      const int at = i * 256 + threadIdx.x;
+      *(uint4*)(tile + (at / per_row) * stride + (at % per_row) * kVec) = r[i];
+      constexpr uint32_t e = M::kExp, half = sizeof(T) == 2;
+      bad |= has_ones(r[i].x, e, half) | has_ones(r[i].y, e, half) | has_ones(r[i].z, e, half) | has_ones(r[i].w, e, half);
+    }
+    return bad;
+  };
+
+  int64_t start = rev ? seg1 - (seg1 - seg0 < kChunk ? seg1 - seg0 : kChunk) : seg0;
+  int n = (int)(seg1 - seg0 < kChunk ? seg1 - seg0 : kChunk);
+  if (threadIdx.x == 0) *odd = 0;
+  if (n > 0) load(start, n);
+  while (n > 0) {
+    __syncthreads();  // (the tiles of the chunk before have been read)
+    if (!parts.state_only) put_tile(rq, Tile::kQ, qs, DK, SK);
+    const uint32_t bad = put_tile(rk, Tile::kQ, ks, DK, SK) | put_tile(rv, Tile::kV, vs, DV, SV);
+    uint64_t starts = __ballot(rf != 0);  // bit t: step t starts an episode
+    if (bad && starts) *odd = 1;
+    __syncthreads();
+    if (starts && *odd) {
+      // 0 * inf would carry what is not finite across the start of an episode: such a chunk ends there
+      // (its outer episode first), and the rest is a chunk of its own
+      __syncthreads();
+      if (threadIdx.x == 0) *odd = 0;
+      int from = 0, to = n;
+      if (rev) from = 63 - __clzll(starts);
+      else if ((starts & ~1ull) != 0) to = __ffsll((unsigned long long)(starts & ~1ull)) - 1;
+      start += from;
+      n = to - from;
+      load(start, n);
+      if (!parts.state_only) put_tile(rq, Tile::kQ, qs, DK, SK);
+      put_tile(rk, Tile::kQ, ks, DK, SK);
+      put_tile(rv, Tile::kV, vs, DV, SV);
+      starts = __ballot(rf != 0);
+      __syncthreads();
+    }
+    // the next chunk's loads run under this one's products
+    const int64_t left = rev ? start - seg0 : seg1 - (start + n);
+    const int n_next = (int)(left < kChunk ? left : kChunk);
+    const int64_t start_next = rev ? start - n_next : start + n;
+    const int n_now = n;
+    const int64_t start_now = start;
+    if (n_next > 0) load(start_next, n_next);
+
+    if (threadIdx.x < kChunk) {  // weights of the steps in the state that leaves the chunk
+      const int t = threadIdx.x;
+      const uint64_t between = rev ? starts & ((2ull << t) - 1) : (t < 63 ? starts >> (t + 1) : 0);
+      w_up[t] = t < n_now && between == 0 ? __builtin_amdgcn_exp2f(l2 * (rev ? t + 1 : n_now - 1 - t)) * p.inc_scale : 0.f;
+    }
+    if (!parts.state_only) {
+      // ---- scores of 16 query steps per wave
+      const int t = 16 * wave + l16;
+      int lo, hi;  // the steps that reach step t
+      if (rev) {
+        const uint64_t later = t < 63 ? starts >> (t + 1) : 0;
+        lo = t;
+        hi = later ? t + __ffsll((unsigned long long)later) - 1 : kChunk - 1;
+      } else {
+        const uint64_t until = starts & ((2ull << t) - 1);
+        lo = until ? 63 - __clzll(until) : 0;
+        hi = t;
+      }
+      frag q[DK / K];
+#pragma unroll
+      for (int k = 0; k < DK / K; ++k) q[k] = M::row(qs, SK, 16 * wave, k * K);
+      const int i0 = rev ? (16 * wave) / K * K / 16 : 0, i1 = rev ? kChunk / 16 : ((16 * wave) / K + 1) * K / 16;
+      for (int i = i0; i < i1; ++i) {
+        f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (rev ? i >= wave : i <= wave) {
+#pragma unroll
+          for (int k = 0; k < DK / K; ++k) a = M::mul(M::row(ks, SK, 16 * i, k * K), q[k], a);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int u = 16 * i + 4 * g + r;
+            const float w = __builtin_amdgcn_exp2f(l2 * (float)(rev ? u - t : t - u)) * (p.inc_scale * p.out_scale);
+            a[r] = u >= lo && u <= hi ? a[r] * w : 0.f;
+          }
+        }
+        M::put4(ps + t * SP + 16 * i + 4 * g, a);
+      }
+    }
+    __syncthreads();
+    const float carry = starts ? 0.f : __builtin_amdgcn_exp2f(l2 * n_now);
+    through *= carry;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      frag vf[kChunk / K];
+#pragma unroll
+      for (int k = 0; k < kChunk / K; ++k) vf[k] = M::col(vs, SV, k * K, v0 + 16 * j);
+      if (!parts.state_only) {
+        frag sf[DK / K];
+#pragma unroll
+        for (int k = 0; k < DK / K; ++k) {
+          if constexpr (sizeof(T) == 2) sf[k] = M::from_acc(s[2 * k][j], s[2 * k + 1][j]);
+          else sf[k] = s[k][j];
+        }
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < DK / K; ++k) a = M::mul(sf[k], M::row_as_acc(qs, SK, 16 * b, k * K), a);
+          const int t = 16 * b + l16;
+          const uint64_t cut = rev ? (t < 63 ? starts >> (t + 1) : 0) : starts & ((2ull << t) - 1);
+          const float w = __builtin_amdgcn_exp2f(l2 * (float)(rev ? n_now - 1 - t : t + 1)) * p.out_scale;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) a[r] = cut == 0 && t < n_now ? a[r] * w : 0.f;
+#pragma unroll
+          for (int k = 0; k < kChunk / K; ++k)
+            if (rev ? (k + 1) * K > 16 * b : k * K <= 16 * b) a = M::mul(vf[k], M::row(ps, SP, 16 * b, k * K), a);
+          if (t < n_now) {
+            const int v = v0 + 16 * j + 4 * g;
+            const int64_t at = (start_now + t) * p.out_stride[0] + row * p.out_stride[1] + h * p.out_stride[2] + v;
+            if (p.out_f32) {
+              float* o = (float*)p.out + at;
+              if (parts.vec_out && v + 4 <= p.dv) *(f32x4*)o = a;
+              else
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  if (v + r < p.dv) o[r] = a[r];
+            } else {
+              T* o = (T*)p.out + at;
+              if (parts.vec_out && v + 4 <= p.dv) M::put4(o, a);
+              else
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  if (v + r < p.dv) o[r] = (T)a[r];
+            }
+          }
+        }
+      }
+      // ---- the state: keys as rows, weighted values as columns
+      if (rev && (starts & 1)) {  // nothing of this chunk leaves it (and 0 * inf must not)
+#pragma unroll
+        for (int i = 0; i < ND; ++i) s[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        continue;
+      }
+#pragma unroll
+      for (int k = 0; k < kChunk / K; ++k) vf[k] = M::weighted(vf[k], w_up + k * K + (K / 4) * g);
+#pragma unroll
+      for (int i = 0; i < ND; ++i) {
+        f32x4 a;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) a[r] = carry != 0.f ? s[i][j][r] * carry : 0.f;
+#pragma unroll
+        for (int k = 0; k < kChunk / K; ++k) a = M::mul(M::col(ks, SK, k * K, 16 * i), vf[k], a);
+        s[i][j] = a;
+      }
+    }
+    start = start_next;
+    n = n_next;
+  }
+
+  // ---- the state the part ends with
+  if (parts.state_only) {
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) ws[((i * NV + j) * 4 + wave) * 64 + lane] = s[i][j];
+    if (threadIdx.x == 0) parts.ws_carry[rh * parts.n_seg + seg] = through;
+    return;
+  }
+  const bool last = rev ? seg == 0 : seg == parts.n_seg - 1;
+  if (!last || !p.state_out) return;
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int v = v0 + 16 * j + l16, d = 16 * i + 4 * g;
+      float* a = p.state_out + row * p.outs_stride[0] + h * p.outs_stride[1] + v * p.outs_stride[3];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (v < p.dv && d + r < p.dk) a[(d + r) * p.outs_stride[2]] = s[i][j][r];
+    }
+}
+
+// Turns the parts' own contributions into what each part starts from, in time's direction: one thread per 4
+// values of a state.
+template <int DK, int DV> __global__ __launch_bounds__(256) void join_parts(Scan p, Parts parts) {
+  const int64_t rh = blockIdx.x;
+  const int at = blockIdx.y * 256 + threadIdx.x;  // in accumulator order
+  const int lane = at & 63, wave = (at >> 6) & 3, tile = at >> 8;
+  const int i = tile / (DV / 64), j = tile % (DV / 64);
+  const int v = wave * (DV / 4) + 16 * j + (lane & 15), d = 16 * i + 4 * (lane >> 4);
+  const int64_t row = rh / p.heads;
+  const int h = (int)(rh % p.heads);
+  f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (p.state_in) {
+    const float* a = p.state_in + row * p.in_stride[0] + h * p.in_stride[1] + v * p.in_stride[3];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (v < p.dv && d + r < p.dk) s[r] = a[(d + r) * p.in_stride[2]];
+  }
+  f32x4* ws = parts.ws_state + rh * parts.n_seg * (DK * DV / 4) + at;
+  for (int n = 0; n < parts.n_seg; ++n) {
+    const int seg = p.reverse ? parts.n_seg - 1 - n : n;
+    f32x4* a = ws + (int64_t)seg * (DK * DV / 4);
+    const bool last = n + 1 == parts.n_seg;
+    const f32x4 own = last ? s : *a;
+    *a = s;
+    if (last) break;
+    const float carry = parts.ws_carry[rh * parts.n_seg + seg];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[r] = (carry != 0.f ? s[r] * carry : 0.f) + own[r];
+  }
+}
+
+}  // namespace epm

@@ -322,7 +322,7 @@ SCANS = [
   # steps, rows, heads, kv heads, key dim, value dim, fresh, state
   (1, 1, 1, 1, 1, 1, 0.0, False), (1, 5, 2, 2, 64, 64, 0.5, True), (7, 3, 2, 1, 16, 24, 0.3, True), (63, 2, 1, 1, 32, 32, 0.0, True),
   (64, 2, 2, 2, 64, 64, 0.02, True), (65, 2, 3, 3, 40, 72, 0.05, False), (130, 3, 4, 2, 64, 128, 0.02, True), (200, 1, 2, 2, 128, 128, 0.0, True),
-  (257, 2, 3, 1, 80, 112, 0.01, True), (96, 1, 1, 1, 128, 5, 0.9, True), (1000, 1, 2, 2, 33, 64, 0.003, True),
+  (257, 2, 3, 1, 80, 112, 0.01, True), (700, 3, 2, 2, 72, 16, 0.004, True), (96, 1, 1, 1, 128, 5, 0.9, True), (1000, 1, 2, 2, 33, 64, 0.003, True),
 ]
 
 
@@ -378,6 +378,46 @@ def test_memory_scan_and_its_gradients(case, dtype):
       tol = _tol(s, w, dtype, t, max(dk, dv), extra=group)
     err = (x.cpu().double() - w).abs()
     assert (err <= tol).all(), (name, float((err - tol).max()), float(err.max()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_memory_scan_keeps_what_is_not_finite_inside_its_episode(dtype):
+  """An env whose keys or values overflowed: the next episode, and the one before in the gradients, are as if
+  those steps had been zero."""
+  from envpool_amd import policy
+  t, n, h, dk, dv = 150, 4, 2, 40, 24
+  q, k, v, decay, _, state, do, ds = _scan_problem((t, n, h, h, dk, dv, 0.0, True), dtype)
+  fresh = torch.zeros(t, n, dtype=torch.bool)
+  fresh[[0, 20, 33, 70, 140], 0] = True   # several episodes inside a chunk
+  fresh[[63, 64, 65], 1] = True
+  fresh[100, 2] = True
+  bad = torch.zeros(t, n, dtype=torch.bool)
+  bad[25, 0] = bad[64, 1] = bad[99, 2] = True
+  ep = fresh.int().cumsum(0)
+  sick = torch.zeros(t, n, dtype=torch.bool)  # steps of an episode with a bad step
+  for b in range(n):
+    for e in ep[bad[:, b], b].tolist():
+      sick[:, b] |= ep[:, b] == e
+
+  def run(filler):
+    kk, vv, dd = k.clone(), v.clone(), do.clone()
+    kk[bad], vv[bad], dd[bad] = filler, filler, filler
+    leaves = [x.to(DEV).requires_grad_() for x in (q, kk, vv, state)]
+    out, final = policy.memory_scan(*leaves[:3], decay.to(DEV), fresh=fresh.to(DEV), state=leaves[3])
+    grads = torch.autograd.grad([out, final], leaves, [dd.to(DEV), ds.to(DEV)])
+    return [x.detach().cpu() for x in (out, final, *grads)]
+
+  clean = run(0.0)
+  for filler in (math.inf, math.nan):
+    got = run(filler)
+    for name, x, w in zip(("out", "grad_q", "grad_k", "grad_v"), (got[0], *got[2:5]), (clean[0], *clean[2:5])):
+      ok = ~sick
+      # the same values, chunks cut differently: two results of one formula, each within the bound of the other tests
+      assert torch.isfinite(x[ok]).all(), name
+      assert torch.allclose(x[ok].float(), w[ok].float(), rtol=16 * ref.HALF[dtype], atol=16 * ref.HALF[dtype] * float(w.abs().max())), name
+    live = [b for b in range(n) if not sick[t - 1, b]]
+    assert torch.isfinite(got[1][live]).all()
+    assert torch.isfinite(got[5][[1, 3]]).all()
 
 
 def test_memory_scan_layouts_and_missing_pieces():
