@@ -35,9 +35,9 @@ int64_t step_workspace(const ep_memory_step_args* a) {
   return a->env_id && a->rows > kLookThrough ? a->num_envs * 4 : 0;
 }
 
-template <class T, int DK, int DV> int scan_tile(const epm::Scan& k, epm::Parts parts, unsigned states, hipStream_t stream) {
+template <class T, int DK, int DV, bool kAligned> int scan_tile(const epm::Scan& k, epm::Parts parts, unsigned states, hipStream_t stream) {
   constexpr size_t lds = epm::ScanTile<T, DK, DV>::kLds;
-  const auto fn = epm::scan_chunks<T, DK, DV>;
+  const auto fn = epm::scan_chunks<T, DK, DV, kAligned>;
   if (lds > 65536) HIP_TRY(hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
   if (parts.n_seg > 1) {
     parts.state_only = 1;
@@ -47,6 +47,12 @@ template <class T, int DK, int DV> int scan_tile(const epm::Scan& k, epm::Parts 
   }
   hipLaunchKernelGGL(fn, dim3(states, (unsigned)parts.n_seg), dim3(256), lds, stream, k, parts);
   return EP_OK;
+}
+
+template <class T, bool kAligned> int scan_sizes(const epm::Scan& k, const epm::Parts& parts, unsigned states, hipStream_t stream) {
+  if (k.dk <= 64)
+    return k.dv <= 64 ? scan_tile<T, 64, 64, kAligned>(k, parts, states, stream) : scan_tile<T, 64, 128, kAligned>(k, parts, states, stream);
+  return k.dv <= 64 ? scan_tile<T, 128, 64, kAligned>(k, parts, states, stream) : scan_tile<T, 128, 128, kAligned>(k, parts, states, stream);
 }
 
 int padded(int dim) { return dim <= 64 ? 64 : 128; }
@@ -75,22 +81,20 @@ int scan_launch(const ep_memory_scan_args* a, const epm::Scan& k, hipStream_t st
     parts.ws_state = (epm::f32x4*)a->workspace;
     parts.ws_carry = (float*)((char*)a->workspace + a->rows * a->heads * parts.n_seg * ((int64_t)padded(a->key_dim) * padded(a->value_dim) * 4));
   }
-  const int64_t size = size_of(a->dtype), vec = 16 / size;
+  const int64_t size = size_of(a->dtype), per_load = 16 / size;
   const auto aligned = [&](const void* ptr, const int64_t* stride, int64_t unit, int64_t bytes) {
     return (uintptr_t)ptr % unit == 0 && stride[0] * bytes % unit == 0 && stride[1] * bytes % unit == 0 && stride[2] * bytes % unit == 0;
   };
-  parts.vec = aligned(a->q, a->q_stride, 16, size) && aligned(a->k, a->k_stride, 16, size) && aligned(a->v, a->v_stride, 16, size) &&
-              a->key_dim % vec == 0 && a->value_dim % vec == 0;
   const int64_t out_size = size_of(a->out_dtype);
-  parts.vec_out = aligned(a->out, a->out_stride, 4 * out_size, out_size);
+  // operands and results in 16-byte (results: 4-value) pieces, or value by value
+  const bool vec = aligned(a->q, a->q_stride, 16, size) && aligned(a->k, a->k_stride, 16, size) && aligned(a->v, a->v_stride, 16, size) &&
+                   aligned(a->out, a->out_stride, 4 * out_size, out_size) && a->key_dim % per_load == 0 && a->value_dim % per_load == 0;
   const int64_t states = a->rows * a->heads;
   if (states > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld states", (long long)states);
   int rc = EP_OK;
   with_type(a->dtype, [&](auto t) {
     using T = decltype(t);
-    const unsigned n = (unsigned)states;
-    if (a->key_dim <= 64) rc = a->value_dim <= 64 ? scan_tile<T, 64, 64>(k, parts, n, stream) : scan_tile<T, 64, 128>(k, parts, n, stream);
-    else rc = a->value_dim <= 64 ? scan_tile<T, 128, 64>(k, parts, n, stream) : scan_tile<T, 128, 128>(k, parts, n, stream);
+    rc = vec ? scan_sizes<T, true>(k, parts, (unsigned)states, stream) : scan_sizes<T, false>(k, parts, (unsigned)states, stream);
   });
   return rc;
 }

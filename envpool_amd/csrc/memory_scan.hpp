@@ -109,7 +109,6 @@ struct Parts {
   f32x4* ws_state;     // [row * heads][n_seg][DK * DV / 4] in accumulator order: what a part starts from (read), or
   float* ws_carry;     // its own contribution and how far it lets the state before it through (written)
   int32_t state_only;  // the first of two passes over split time: contributions only
-  int32_t vec, vec_out;
 };
 
 template <class T, int DK, int DV> struct ScanTile {
@@ -118,6 +117,8 @@ template <class T, int DK, int DV> struct ScanTile {
   static constexpr int SP = kChunk + kVec;
   static constexpr int kQ = kChunk * DK / kVec / 256;        // 16-byte loads per thread and tile
   static constexpr int kV = kChunk * DV / kVec / 256;
+  // workgroups (one wave per SIMD each) that LDS lets a CU hold: the registers are kept to as many
+  static constexpr int kPerCu = 163840 / (int)((size_t)kChunk * (2 * SK + SV + SP) * sizeof(T) + 2 * kChunk * sizeof(float));
   static constexpr size_t kLds = (size_t)kChunk * (2 * SK + SV + SP) * sizeof(T) + 2 * kChunk * sizeof(float);
 };
 
@@ -126,7 +127,8 @@ __device__ inline uint32_t has_ones(uint32_t x, uint32_t e, uint32_t half) {  //
   return half ? ((y & 0xffffu) == (e & 0xffffu)) | ((y >> 16) == (e >> 16)) : y == e;
 }
 
-template <class T, int DK, int DV> __global__ __launch_bounds__(256) void scan_chunks(Scan p, Parts parts) {
+template <class T, int DK, int DV, bool kAligned>
+__global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kPerCu)) void scan_chunks(Scan p, Parts parts) {
   using M = Mma<T>;
   using Tile = ScanTile<T, DK, DV>;
   using frag = typename M::frag;
@@ -191,7 +193,7 @@ template <class T, int DK, int DV> __global__ __launch_bounds__(256) void scan_c
       uint4 x = make_uint4(0, 0, 0, 0);
       if (t < n && c < width) {
         const T* a = base + (start + t) * step_stride + c;
-        if (parts.vec) {
+        if (kAligned) {
           x = *(const uint4*)a;
         } else {
           union { uint4 u; T e[kVec]; } b;
@@ -330,14 +332,14 @@ template <class T, int DK, int DV> __global__ __launch_bounds__(256) void scan_c
             const int64_t at = (start_now + t) * p.out_stride[0] + row * p.out_stride[1] + h * p.out_stride[2] + v;
             if (p.out_f32) {
               float* o = (float*)p.out + at;
-              if (parts.vec_out && v + 4 <= p.dv) *(f32x4*)o = a;
+              if (kAligned && v + 4 <= p.dv) *(f32x4*)o = a;
               else
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                   if (v + r < p.dv) o[r] = a[r];
             } else {
               T* o = (T*)p.out + at;
-              if (parts.vec_out && v + 4 <= p.dv) M::put4(o, a);
+              if (kAligned && v + 4 <= p.dv) M::put4(o, a);
               else
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
