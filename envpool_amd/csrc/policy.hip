@@ -92,12 +92,44 @@ template <class F> void with_type(int32_t dtype, F f) {
   else f(epp::bf16{});
 }
 
-// rows of the gradient kernel are split so that about this many workgroups stand on the chip (8 a CU)
-constexpr int64_t kGradBlocks = 2048;
+// How rows map to the chip. Up to 2048 options a row is held by 1 to 64 neighbouring lanes (8 options a lane and
+// piece, 1 or 4 pieces): enough lanes for the options, and for a long history at least a lane per 16 entries
+// of it. Longer rows are walked by workgroups, 2048 options at a time; with few rows each is cut into parts so
+// that about kFill workgroups stand on the chip.
+constexpr int64_t kGroupOptions = 64 * epp::kPer * 4;
+constexpr int64_t kFill = 2048;
 
+struct Width {
+  int log, pieces;
+  unsigned blocks;  // workgroups for all rows
+  size_t lds;
+};
+Width group_width(const epp::Rows& k) {
+  Width w{0, k.options <= 64 * epp::kPer ? 1 : 4, 0, 0};
+  const int64_t lanes = (k.options + epp::kPer * w.pieces - 1) / (epp::kPer * w.pieces);
+  const int64_t want = std::max<int64_t>(lanes, k.history ? std::min<int64_t>(64, (k.history_len + 15) / 16) : 1);
+  while ((1 << w.log) < want) ++w.log;
+  const int64_t per = epp::kThreads >> w.log;
+  w.blocks = (unsigned)((k.rows + per - 1) / per);
+  w.lds = (size_t)epp::kThreads * epp::kPer * w.pieces * 4;
+  return w;
+}
+
+struct Cut {
+  int pieces, parts;  // pieces per part, parts per row
+};
+Cut cut_rows(int64_t rows, int64_t options) {
+  const int64_t all = (options + epp::kPiece - 1) / epp::kPiece;
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(all, (kFill + rows - 1) / std::max<int64_t>(rows, 1)));
+  const int64_t pieces = (all + want - 1) / want;
+  return {(int)pieces, (int)((all + pieces - 1) / pieces)};
+}
+
+// partial sums of a shared bias' gradient: one row of them per workgroup that walks down rows
+int64_t grad_group_blocks(const Width& w) { return std::min<int64_t>(w.blocks, 1024); }
 int64_t grad_row_blocks(int64_t rows, int64_t options) {
   const int64_t pieces = (options + epp::kPiece - 1) / epp::kPiece;
-  const int64_t blocks = std::min<int64_t>(std::min<int64_t>(rows, 65535), std::max<int64_t>(1, kGradBlocks / pieces));
+  const int64_t blocks = std::min<int64_t>(std::min<int64_t>(rows, 65535), std::max<int64_t>(1, kFill / pieces));
   const int64_t per = (rows + blocks - 1) / std::max<int64_t>(blocks, 1);
   return per > 0 ? (rows + per - 1) / per : 0;
 }
@@ -106,7 +138,10 @@ int64_t grad_row_blocks(int64_t rows, int64_t options) {
 
 extern "C" {
 
-int64_t ep_policy_choose_workspace(const ep_policy_rows*) { return 0; }
+int64_t ep_policy_choose_workspace(const ep_policy_rows* r) {
+  if (!r || r->rows <= 0 || r->options <= kGroupOptions) return 0;
+  return r->rows * cut_rows(r->rows, r->options).parts * (int64_t)sizeof(epp::Stat<double>);
+}
 
 int ep_policy_choose(const ep_policy_rows* r, const void* u, int32_t u_dtype, int32_t* action, float* log_prob, float* entropy) {
   epp::Rows k;
@@ -117,16 +152,34 @@ int ep_policy_choose(const ep_policy_rows* r, const void* u, int32_t u_dtype, in
   if (int rc = check_workspace(r, ep_policy_choose_workspace(r))) return rc;
   if (r->rows == 0) return EP_OK;
   EP_ENTER_DEVICE(r->device_id);
-  const unsigned grid = (unsigned)std::min<int64_t>(r->rows, 1 << 20);
-  with_type(r->dtype, [&](auto t) {
-    hipLaunchKernelGGL(epp::choose_row<decltype(t)>, dim3(grid), dim3(epp::kThreads), 0, (hipStream_t)r->stream, k, u, u_dtype == EP_F64, action,
-                       log_prob, entropy);
-  });
+  const hipStream_t stream = (hipStream_t)r->stream;
+  const epp::ChooseOut out{action, log_prob, entropy};
+  const int u_f64 = u_dtype == EP_F64;
+  if (r->options <= kGroupOptions) {
+    const Width w = group_width(k);
+    const size_t lds = k.history ? w.lds : 0;
+    with_type(r->dtype, [&](auto t) {
+      if (w.pieces == 1) hipLaunchKernelGGL((epp::choose_group<decltype(t), 1>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, u, u_f64, out);
+      else hipLaunchKernelGGL((epp::choose_group<decltype(t), 4>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, u, u_f64, out);
+    });
+  } else {
+    const Cut cut = cut_rows(r->rows, r->options);
+    if (r->rows * cut.parts > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld rows of %lld options", (long long)r->rows, (long long)r->options);
+    auto* parts = (epp::Stat<double>*)r->workspace;
+    with_type(r->dtype, [&](auto t) {
+      hipLaunchKernelGGL(epp::choose_parts<decltype(t)>, dim3((unsigned)(r->rows * cut.parts)), dim3(epp::kThreads), 0, stream, k, cut.pieces, cut.parts, parts);
+      hipLaunchKernelGGL(epp::choose_join<decltype(t)>, dim3((unsigned)r->rows), dim3(epp::kThreads), 0, stream, k, cut.pieces, cut.parts, parts, u, u_f64, out);
+    });
+  }
   HIP_TRY(hipGetLastError());
   return EP_OK;
 }
 
-int64_t ep_policy_evaluate_workspace(const ep_policy_rows*) { return 0; }
+int64_t ep_policy_evaluate_workspace(const ep_policy_rows* r) {
+  if (!r || r->rows <= 0 || r->options <= kGroupOptions) return 0;
+  const Cut cut = cut_rows(r->rows, r->options);
+  return cut.parts == 1 ? 0 : r->rows * cut.parts * (int64_t)sizeof(epp::EvaluatePart);
+}
 
 int ep_policy_evaluate(const ep_policy_rows* r, const int32_t* action, float* log_prob, float* entropy, float* stats) {
   epp::Rows k;
@@ -135,17 +188,35 @@ int ep_policy_evaluate(const ep_policy_rows* r, const int32_t* action, float* lo
   if (int rc = check_workspace(r, ep_policy_evaluate_workspace(r))) return rc;
   if (r->rows == 0) return EP_OK;
   EP_ENTER_DEVICE(r->device_id);
-  const unsigned grid = (unsigned)std::min<int64_t>(r->rows, 1 << 20);
-  with_type(r->dtype, [&](auto t) {
-    hipLaunchKernelGGL(epp::evaluate_row<decltype(t)>, dim3(grid), dim3(epp::kThreads), 0, (hipStream_t)r->stream, k, action, log_prob, entropy, stats);
-  });
+  const hipStream_t stream = (hipStream_t)r->stream;
+  const epp::EvaluateOut out{action, log_prob, entropy, stats};
+  if (r->options <= kGroupOptions) {
+    const Width w = group_width(k);
+    const size_t lds = k.history ? w.lds : 0;
+    with_type(r->dtype, [&](auto t) {
+      if (w.pieces == 1) hipLaunchKernelGGL((epp::evaluate_group<decltype(t), 1>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, out);
+      else hipLaunchKernelGGL((epp::evaluate_group<decltype(t), 4>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, out);
+    });
+  } else {
+    const Cut cut = cut_rows(r->rows, r->options);
+    if (r->rows * cut.parts > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld rows of %lld options", (long long)r->rows, (long long)r->options);
+    auto* parts = (epp::EvaluatePart*)r->workspace;
+    with_type(r->dtype, [&](auto t) {
+      hipLaunchKernelGGL(epp::evaluate_parts<decltype(t)>, dim3((unsigned)(r->rows * cut.parts)), dim3(epp::kThreads), 0, stream, k, cut.pieces, cut.parts, parts, out);
+    });
+    if (cut.parts > 1)
+      hipLaunchKernelGGL(epp::evaluate_join, dim3((unsigned)((r->rows + 3) / 4)), dim3(epp::kThreads), 0, stream, k, cut.parts, parts, out);
+  }
   HIP_TRY(hipGetLastError());
   return EP_OK;
 }
 
 int64_t ep_policy_evaluate_grad_workspace(const ep_policy_rows* r, int32_t with_bias) {
   if (!r || !with_bias || !r->bias || r->bias_stride != 0 || r->rows <= 0 || r->options < 1) return 0;
-  return grad_row_blocks(r->rows, r->options) * r->options * 4;
+  if (r->options > kGroupOptions) return grad_row_blocks(r->rows, r->options) * r->options * 4;
+  epp::Rows k{};
+  k.rows = r->rows, k.options = r->options, k.history = r->history_len > 0 ? r->history : nullptr, k.history_len = r->history_len;
+  return grad_group_blocks(group_width(k)) * r->options * 4;
 }
 
 int ep_policy_evaluate_grad(const ep_policy_rows* r, const int32_t* action, const float* entropy, const float* stats,
@@ -166,7 +237,9 @@ int ep_policy_evaluate_grad(const ep_policy_rows* r, const int32_t* action, cons
   EP_ENTER_DEVICE(r->device_id);
   const hipStream_t stream = (hipStream_t)r->stream;
   const int64_t pieces = (r->options + epp::kPiece - 1) / epp::kPiece;
-  const int64_t blocks = grad_row_blocks(r->rows, r->options);
+  const bool group = r->options <= kGroupOptions;
+  const Width w = group ? group_width(k) : Width{};
+  const int64_t blocks = group ? grad_group_blocks(w) : grad_row_blocks(r->rows, r->options);
   float* partial = shared ? (float*)r->workspace : nullptr;
   if (r->rows > 0) {
     epp::GradArgs g{action, entropy, stats, grad_log_prob, grad_entropy, grad_logits, grad_logits_stride, shared ? nullptr : grad_bias, grad_bias_stride,
@@ -174,6 +247,12 @@ int ep_policy_evaluate_grad(const ep_policy_rows* r, const int32_t* action, cons
     g.vec_out = (uintptr_t)grad_logits % 16 == 0 && (r->rows <= 1 || (grad_logits_stride * (int64_t)size_of(r->dtype)) % 16 == 0);
     const int64_t per = (r->rows + blocks - 1) / blocks;
     with_type(r->dtype, [&](auto t) {
+      const size_t lds = k.history || shared ? w.lds : 0;
+      if (group && w.pieces == 1)
+        hipLaunchKernelGGL((epp::evaluate_grad_group<decltype(t), 1>), dim3((unsigned)blocks), dim3(epp::kThreads), lds, stream, k, g, w.log, (int64_t)w.blocks);
+      else if (group)
+        hipLaunchKernelGGL((epp::evaluate_grad_group<decltype(t), 4>), dim3((unsigned)blocks), dim3(epp::kThreads), lds, stream, k, g, w.log, (int64_t)w.blocks);
+      else
       hipLaunchKernelGGL(epp::evaluate_grad_piece<decltype(t)>, dim3((unsigned)pieces, (unsigned)blocks), dim3(epp::kThreads), 0, stream, k, g, per);
     });
     HIP_TRY(hipGetLastError());

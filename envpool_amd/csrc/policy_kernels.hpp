@@ -169,7 +169,28 @@ __device__ inline uint32_t load_z(const Rows& p, const RowConst<R>& c, int64_t r
   return legal;
 }
 
-__device__ inline double exp_of(double x) { return exp(x); }
+// exp of x <= 0 in 64 bits: x = n ln 2 + r, |r| <= ln 2 / 2, the series of exp r to r^11 (the first term left
+// out is below 7e-15), times 2^n. About two thirds of the library function's instructions: there are no
+// overflows or positive arguments to look after, and what is below e^-745 is 0.
+__device__ inline double exp_of(double x) {
+  x = fmax(x, -800.0);
+  const double n = rint(x * 1.4426950408889634);
+  double r = fma(n, -0.6931471805599453, x);  // ln 2 to 53 bits, then what it lacks
+  r = fma(n, -2.3190468138462996e-17, r);
+  double p = 1.0 / 39916800;
+  p = fma(p, r, 1.0 / 3628800);
+  p = fma(p, r, 1.0 / 362880);
+  p = fma(p, r, 1.0 / 40320);
+  p = fma(p, r, 1.0 / 5040);
+  p = fma(p, r, 1.0 / 720);
+  p = fma(p, r, 1.0 / 120);
+  p = fma(p, r, 1.0 / 24);
+  p = fma(p, r, 1.0 / 6);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return __builtin_amdgcn_ldexp(p, (int)n);
+}
 __device__ inline float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896f); }
 
 // running statistics of a row, or of a part of it
@@ -194,13 +215,6 @@ template <class R> __device__ inline void stat_rebase(Stat<R>& a, R m, R inv_t) 
   }
   a.m = m;
 }
-template <class R> __device__ inline Stat<R> stat_join(Stat<R> a, Stat<R> b, R inv_t) {
-  const R m = a.m > b.m ? a.m : b.m;
-  const int64_t best = a.m > b.m ? a.best : (b.m > a.m ? b.best : (a.best < b.best ? a.best : b.best));
-  stat_rebase(a, m, inv_t);
-  stat_rebase(b, m, inv_t);
-  return {m, a.s + b.s, a.e + b.e, best, a.bad | b.bad};
-}
 // adds the options j0 .. j0+7
 template <class R> __device__ inline void stat_add(Stat<R>& a, const R (&z)[kPer], int64_t j0, R inv_t) {
   R m = neg_inf<R>();
@@ -223,24 +237,52 @@ template <class R> __device__ inline void stat_add(Stat<R>& a, const R (&z)[kPer
   }
 }
 
-template <class R> __device__ inline R shfl_xor_of(R v, int lane_mask) { return __shfl_xor(v, lane_mask, 64); }
-template <class R> __device__ inline Stat<R> stat_shfl(const Stat<R>& a, int lane_mask) {
-  return {shfl_xor_of(a.m, lane_mask), shfl_xor_of(a.s, lane_mask), shfl_xor_of(a.e, lane_mask),
-          (int64_t)__shfl_xor((long long)a.best, lane_mask, 64), __shfl_xor(a.bad, lane_mask, 64)};
-}
-// over the block; the result is the same in every thread
-template <class R> __device__ inline Stat<R> stat_block(Stat<R> a, R inv_t, Stat<R>* lds) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const Stat<R> b = stat_shfl(a, o);
-    // the same order of the two in both lanes, so that both get the same bits
-    a = (threadIdx.x & o) ? stat_join(b, a, inv_t) : stat_join(a, b, inv_t);
+// over `width` neighbouring lanes (a power of two up to 64), the same result in all of them
+template <class V> __device__ inline V lanes_max(V v, int width) {
+  for (int o = 1; o < width; o <<= 1) {
+    const V b = __shfl_xor(v, o, 64);
+    v = v > b ? v : b;
   }
+  return v;
+}
+template <class V> __device__ inline V lanes_min(V v, int width) { return -lanes_max(-v, width); }
+template <class V> __device__ inline V lanes_sum(V v, int width) {
+  for (int o = 1; o < width; o <<= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+// sum over the lanes up to and including this one, of `width`
+template <class V> __device__ inline V lanes_scan(V v, int width) {
+  const int at = threadIdx.x & (width - 1);
+  for (int o = 1; o < width; o <<= 1) {
+    const V b = __shfl_up(v, o, 64);
+    if (at >= o) v += b;
+  }
+  return v;
+}
+
+// over the workgroup, the same result in every thread: the maximum first, then every thread moves its own
+// sums to it (one exponential each) and they are added
+template <class R> __device__ inline Stat<R> stat_block(Stat<R> a, R inv_t, Stat<R>* lds) {
+  constexpr int kWaves = kThreads / 64;
+  const int wave = threadIdx.x >> 6;
+  const R m_wave = lanes_max(a.m, 64);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
+  if ((threadIdx.x & 63) == 0) lds[wave].m = m_wave;
+  __syncthreads();
+  R m = lds[0].m;
+  for (int i = 1; i < kWaves; ++i) m = m > lds[i].m ? m : lds[i].m;
+  const int64_t best = lanes_min((long long)(a.m == m ? a.best : INT64_MAX), 64);
+  stat_rebase(a, m, inv_t);
+  const R sum = lanes_sum(a.s, 64), e = lanes_sum(a.e, 64);
+  const int bad = __any(a.bad);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[wave] = {m, sum, e, best, bad};
   __syncthreads();
   Stat<R> r = lds[0];
-  for (int i = 1; i < kThreads / 64; ++i) r = stat_join(r, lds[i], inv_t);
+  for (int i = 1; i < kWaves; ++i) {
+    r.s += lds[i].s, r.e += lds[i].e, r.bad |= lds[i].bad;
+    if (lds[i].best < r.best) r.best = lds[i].best;
+  }
   return r;
 }
 
@@ -259,137 +301,357 @@ __device__ inline void count_piece(const Rows& p, int64_t row, int64_t j0, uint3
 
 template <class R> __device__ inline R quiet_nan() { return (R)__builtin_nanf(""); }
 
-// ---- one workgroup per row --------------------------------------------------------------------------
-template <class T>
-__global__ __launch_bounds__(kThreads) void choose_row(Rows p, const void* u, int u_f64, int32_t* action, float* log_prob,
-                                                       float* entropy) {
-  __shared__ uint32_t counts[kPiece];
-  __shared__ Stat<double> red[kThreads / 64];
-  __shared__ double wave_sum[kThreads / 64];
-  __shared__ int64_t found;
-  __shared__ double found_z;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    const RowConst<double> c = row_const<double>(p, row);
-    Stat<double> a = stat_zero<double>();
-    for (int64_t j0 = 0; j0 < c.n_legal; j0 += kPiece) {
-      if (p.history) count_piece(p, row, j0, counts);
-      const int64_t j = j0 + threadIdx.x * kPer;
-      double z[kPer];
-      load_z<T, double>(p, c, row, j, p.history ? counts + threadIdx.x * kPer : nullptr, z);
-      stat_add(a, z, j, c.inv_t);
-    }
-    a = stat_block(a, c.inv_t, red);
-    const bool bad = a.bad || c.bad;
-    const bool empty = !bad && a.m == neg_inf<double>();
-    int64_t pick = a.best;
-    double z_pick = a.m;
-    if (u && !bad && !empty) {
-      const double target = (u_f64 ? ((const double*)u)[row] : (double)((const float*)u)[row]) * a.s;
-      if (threadIdx.x == 0) found = INT64_MAX;
-      double before = 0;
-      int64_t last = -1;  // the last option with any weight: where a sum that rounding left short ends
-      double last_z = 0;
-      for (int64_t j0 = 0; j0 < c.n_legal; j0 += kPiece) {
-        if (p.history) count_piece(p, row, j0, counts);
-        const int64_t j = j0 + threadIdx.x * kPer;
-        double z[kPer], w[kPer], sum = 0;
-        load_z<T, double>(p, c, row, j, p.history ? counts + threadIdx.x * kPer : nullptr, z);
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          w[i] = exp_of((z[i] - a.m) * c.inv_t);
-          sum += w[i];
-          if (w[i] > 0) last = j + i, last_z = z[i];
-        }
-        double incl = sum;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const double t = __shfl_up(incl, o, 64);
-          if ((int)(threadIdx.x & 63) >= o) incl += t;
-        }
-        __syncthreads();
-        if ((threadIdx.x & 63) == 63) wave_sum[threadIdx.x >> 6] = incl;
-        __syncthreads();
-        double base = before;
-        for (int i = 0; i < (int)(threadIdx.x >> 6); ++i) base += wave_sum[i];
-        double cum = base + incl - sum;
-        int64_t hit = INT64_MAX;
-        double hit_z = 0;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          cum += w[i];
-          if (hit == INT64_MAX && w[i] > 0 && cum > target) hit = j + i, hit_z = z[i];
-        }
-        if (hit != INT64_MAX) atomicMin((unsigned long long*)&found, (unsigned long long)hit);
-        __syncthreads();
-        if (hit != INT64_MAX && hit == found) found_z = hit_z;
-        __syncthreads();
-        if (found != INT64_MAX) break;
-        for (int i = 0; i < kThreads / 64; ++i) before += wave_sum[i];
-      }
-      if (found == INT64_MAX) {
-        __syncthreads();
-        if (threadIdx.x == 0) found = -1;
-        __syncthreads();
-        atomicMax((long long*)&found, (long long)last);
-        __syncthreads();
-        if (last == found) found_z = last_z;
-        __syncthreads();
-      }
-      pick = found;
-      z_pick = found_z;
-      __syncthreads();
-    }
-    if (threadIdx.x == 0) {
-      const double log_s = log(a.s);
-      action[row] = bad || empty ? -1 : (int32_t)pick;
-      log_prob[row] = bad ? quiet_nan<float>() : empty ? 0.f : (float)((z_pick - a.m) * c.inv_t - log_s);
-      entropy[row] = bad ? quiet_nan<float>() : empty ? 0.f : (float)(log_s - a.e / a.s);
-    }
-  }
+// ---- results ------------------------------------------------------------------------------------------
+struct ChooseOut {
+  int32_t* action;
+  float *log_prob, *entropy;
+};
+__device__ inline void finish_choose(const ChooseOut& o, int64_t row, const Stat<double>& a, bool bad_row, double inv_t, int64_t pick, double z_pick) {
+  const bool bad = a.bad || bad_row;
+  const bool empty = !bad && a.m == neg_inf<double>();
+  const double log_s = log(a.s);
+  o.action[row] = bad || empty ? -1 : (int32_t)pick;
+  o.log_prob[row] = bad ? quiet_nan<float>() : empty ? 0.f : (float)((z_pick - a.m) * inv_t - log_s);
+  o.entropy[row] = bad ? quiet_nan<float>() : empty ? 0.f : (float)(log_s - a.e / a.s);
 }
 
-// results of one row of ep_policy_evaluate, from its statistics
-__device__ inline void finish_evaluate(int64_t row, const Rows& p, const RowConst<float>& c, const Stat<float>& a, int32_t act,
-                                       float z_act, float* log_prob, float* entropy, float* stats) {
-  const bool bad = a.bad || c.bad;
+struct EvaluateOut {
+  const int32_t* action;
+  float *log_prob, *entropy, *stats;
+};
+__device__ inline void finish_evaluate(const EvaluateOut& o, int64_t row, int64_t options, const Stat<float>& a, bool bad_row, float inv_t, int32_t act,
+                                       float z_act) {
+  const bool bad = a.bad || bad_row;
   const bool empty = !bad && a.m == -INFINITY;
   const float log_s = logf(a.s);
   float lp;
   if (act == -1) lp = 0.f;
-  else if (act < 0 || act >= p.options) lp = quiet_nan<float>();
+  else if (act < 0 || act >= options) lp = quiet_nan<float>();
   else if (empty || z_act == -INFINITY) lp = -INFINITY;
-  else lp = (z_act - a.m) * c.inv_t - log_s;
-  log_prob[row] = bad ? quiet_nan<float>() : lp;
-  entropy[row] = bad ? quiet_nan<float>() : empty ? 0.f : log_s - a.e / a.s;
-  stats[2 * row] = bad ? quiet_nan<float>() : a.m;
-  stats[2 * row + 1] = bad ? quiet_nan<float>() : empty ? 0.f : log_s;
+  else lp = (z_act - a.m) * inv_t - log_s;
+  o.log_prob[row] = bad ? quiet_nan<float>() : lp;
+  o.entropy[row] = bad ? quiet_nan<float>() : empty ? 0.f : log_s - a.e / a.s;
+  o.stats[2 * row] = bad ? quiet_nan<float>() : a.m;
+  o.stats[2 * row + 1] = bad ? quiet_nan<float>() : empty ? 0.f : log_s;
 }
 
+// ---- rows of up to 64 * 8 * NP options: `width` lanes per row, a lane's options in registers -----------
+// Option j of a row sits in lane (j / 8) % width, piece j / 8 / width. Neighbouring rows are neighbouring lanes,
+// so that a wave reads one contiguous stretch however short the rows are.
+struct Group {
+  int64_t row;
+  int lane, width;
+  bool there;
+  __device__ int64_t j(int piece) const { return ((int64_t)piece * width + lane) * kPer; }
+};
+__device__ inline Group group_of(const Rows& p, int64_t block, int width_log) {
+  Group g;
+  g.width = 1 << width_log;
+  g.lane = threadIdx.x & (g.width - 1);
+  g.row = block * (kThreads >> width_log) + (threadIdx.x >> width_log);
+  g.there = g.row < p.rows;
+  if (!g.there) g.row = 0;
+  return g;
+}
+// the histories of a workgroup's rows, counted; returns this row's counts
+template <int NP> __device__ inline const uint32_t* count_groups(const Rows& p, const Group& g, uint32_t* counts) {
+  if (!p.history) return nullptr;
+  uint32_t* mine = counts + (threadIdx.x - g.lane) * kPer * NP;
+  __syncthreads();
+  for (int i = threadIdx.x; i < kThreads * kPer * NP; i += kThreads) counts[i] = 0;
+  __syncthreads();
+  const int32_t* h = p.history + g.row * p.history_stride;
+  for (int64_t i = g.lane; i < p.history_len; i += g.width) {
+    const int32_t j = h[i];
+    if (j >= 0 && j < p.options) atomicAdd(&mine[j], 1u);
+  }
+  __syncthreads();
+  return mine;
+}
+
+template <class T, int NP>
+__global__ __launch_bounds__(kThreads) void choose_group(Rows p, int width_log, const void* u, int u_f64, ChooseOut out) {
+  extern __shared__ uint32_t counts[];
+  const Group g = group_of(p, blockIdx.x, width_log);
+  const RowConst<double> c = row_const<double>(p, g.row);
+  const uint32_t* n = count_groups<NP>(p, g, counts);
+  double z[NP][kPer];
+  Stat<double> a = stat_zero<double>();
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    load_z<T, double>(p, c, g.row, g.j(k), n ? n + g.j(k) : nullptr, z[k]);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (!(z[k][i] < (double)INFINITY)) a.bad = 1;
+      if (z[k][i] > a.m) a.m = z[k][i], a.best = g.j(k) + i;
+    }
+  }
+  const double m = lanes_max(a.m, g.width);
+  int32_t best = a.m == m && a.best < INT32_MAX ? (int32_t)a.best : INT32_MAX;
+  a.m = m;
+  a.best = lanes_min(best, g.width);
+  a.bad = lanes_max(a.bad, g.width);
+  double w[NP][kPer];
+#pragma unroll
+  for (int k = 0; k < NP; ++k)
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const double d = (z[k][i] - m) * c.inv_t;
+      w[k][i] = exp_of(d);
+      a.s += w[k][i];
+      if (w[k][i] > 0) a.e += w[k][i] * d;
+    }
+  a.s = lanes_sum(a.s, g.width);
+  a.e = lanes_sum(a.e, g.width);
+  int32_t pick = (int32_t)a.best;
+  double z_pick = m;
+  if (u) {
+    const double target = (u_f64 ? ((const double*)u)[g.row] : (double)((const float*)u)[g.row]) * a.s;
+    double before = 0;
+    int32_t hit = INT32_MAX, last = -1;
+    double hit_z = 0, last_z = 0;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      double sum = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) sum += w[k][i];
+      const double incl = lanes_scan(sum, g.width);
+      double cum = before + incl - sum;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        cum += w[k][i];
+        if (w[k][i] > 0) {
+          last = (int32_t)g.j(k) + i, last_z = z[k][i];
+          if (hit == INT32_MAX && cum > target) hit = last, hit_z = last_z;
+        }
+      }
+      before += __shfl(incl, (threadIdx.x & 63) | (g.width - 1), 64);
+    }
+    pick = lanes_min(hit, g.width);
+    if (pick == INT32_MAX) {  // (a sum that rounding left short of the target: the last option with any weight)
+      pick = lanes_max(last, g.width);
+      hit = last, hit_z = last_z;
+    }
+    z_pick = lanes_max(hit == pick ? hit_z : neg_inf<double>(), g.width);
+  }
+  if (g.lane == 0 && g.there) finish_choose(out, g.row, a, c.bad, c.inv_t, pick, z_pick);
+}
+
+template <class T, int NP> __global__ __launch_bounds__(kThreads) void evaluate_group(Rows p, int width_log, EvaluateOut out) {
+  extern __shared__ uint32_t counts[];
+  const Group g = group_of(p, blockIdx.x, width_log);
+  const RowConst<float> c = row_const<float>(p, g.row);
+  const uint32_t* n = count_groups<NP>(p, g, counts);
+  const int32_t act = out.action[g.row];
+  float z[NP][kPer];
+  Stat<float> a = stat_zero<float>();
+  float z_act = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    load_z<T, float>(p, c, g.row, g.j(k), n ? n + g.j(k) : nullptr, z[k]);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (!(z[k][i] < INFINITY)) a.bad = 1;
+      a.m = fmaxf(a.m, z[k][i]);
+      if (act == g.j(k) + i) z_act = z[k][i];
+    }
+  }
+  a.m = lanes_max(a.m, g.width);
+  a.bad = lanes_max(a.bad, g.width);
+  z_act = lanes_max(z_act, g.width);
+#pragma unroll
+  for (int k = 0; k < NP; ++k)
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const float d = (z[k][i] - a.m) * c.inv_t;
+      const float w = exp_of(d);
+      if (w > 0.f) a.s += w, a.e += w * d;
+    }
+  a.s = lanes_sum(a.s, g.width);
+  a.e = lanes_sum(a.e, g.width);
+  if (g.lane == 0 && g.there) finish_evaluate(out, g.row, p.options, a, c.bad, c.inv_t, act, z_act);
+}
+
+// ---- longer rows: a workgroup per part of a row (`pieces` pieces of kPiece options), parts joined after ---
 template <class T>
-__global__ __launch_bounds__(kThreads) void evaluate_row(Rows p, const int32_t* action, float* log_prob, float* entropy, float* stats) {
+__global__ __launch_bounds__(kThreads) void choose_parts(Rows p, int pieces, int n_parts, Stat<double>* parts) {
+  __shared__ uint32_t counts[kPiece];
+  __shared__ Stat<double> red[kThreads / 64];
+  const int64_t row = blockIdx.x / n_parts, part = blockIdx.x % n_parts;
+  const RowConst<double> c = row_const<double>(p, row);
+  Stat<double> a = stat_zero<double>();
+  const int64_t j_end = min((part + 1) * pieces * (int64_t)kPiece, c.n_legal);
+  for (int64_t j0 = part * pieces * (int64_t)kPiece; j0 < j_end; j0 += kPiece) {
+    if (p.history) count_piece(p, row, j0, counts);
+    const int64_t j = j0 + threadIdx.x * kPer;
+    double z[kPer];
+    load_z<T, double>(p, c, row, j, p.history ? counts + threadIdx.x * kPer : nullptr, z);
+    stat_add(a, z, j, c.inv_t);
+  }
+  a = stat_block(a, c.inv_t, red);
+  if (threadIdx.x == 0) parts[blockIdx.x] = a;
+}
+
+// joins a row's parts, and finds the option that u falls on by walking down the one part it lies in
+template <class T>
+__global__ __launch_bounds__(kThreads) void choose_join(Rows p, int pieces, int n_parts, const Stat<double>* all_parts, const void* u, int u_f64, ChooseOut out) {
+  __shared__ uint32_t counts[kPiece];
+  __shared__ Stat<double> red[kThreads / 64];
+  __shared__ double wave_sum[kThreads / 64];
+  __shared__ long long found;
+  __shared__ double found_z, part_before;
+  __shared__ int part_at;
+  const int64_t row = blockIdx.x;
+  const Stat<double>* parts = all_parts + row * n_parts;
+  const RowConst<double> c = row_const<double>(p, row);
+  Stat<double> a = stat_zero<double>();
+  for (int i = threadIdx.x; i < n_parts; i += kThreads) {
+    Stat<double> b = parts[i];
+    const double m = a.m > b.m ? a.m : b.m;
+    const int64_t best = a.m > b.m ? a.best : (b.m > a.m ? b.best : min(a.best, b.best));
+    stat_rebase(a, m, c.inv_t);
+    stat_rebase(b, m, c.inv_t);
+    a = {m, a.s + b.s, a.e + b.e, best, a.bad | b.bad};
+  }
+  a = stat_block(a, c.inv_t, red);
+  const bool bad = a.bad || c.bad, empty = !bad && a.m == neg_inf<double>();
+  int64_t pick = a.best;
+  double z_pick = a.m;
+  if (u && !bad && !empty) {
+    const double target = (u_f64 ? ((const double*)u)[row] : (double)((const float*)u)[row]) * a.s;
+    // the part: its weights, moved to the row's maximum, cumulated 64 parts at a time by one wave
+    if (threadIdx.x < 64) {
+      double before = 0;
+      int at = -1, last = 0;
+      double at_before = 0, last_before = 0;
+      for (int i0 = 0; i0 < n_parts && at < 0; i0 += 64) {
+        double w = 0;
+        if (i0 + (int)threadIdx.x < n_parts) {
+          Stat<double> b = parts[i0 + threadIdx.x];
+          stat_rebase(b, a.m, c.inv_t);
+          w = b.s;
+        }
+        const double incl = before + lanes_scan(w, 64);
+        const uint64_t over = __ballot(incl > target && w > 0), any = __ballot(w > 0);
+        if (over) {
+          const int k = __ffsll((unsigned long long)over) - 1;
+          at = i0 + k;
+          at_before = __shfl(incl - w, k, 64);
+        }
+        if (any) {
+          const int k = 63 - __clzll(any);
+          last = i0 + k;
+          last_before = __shfl(incl - w, k, 64);
+        }
+        before = __shfl(incl, 63, 64);
+      }
+      if (threadIdx.x == 0) part_at = at >= 0 ? at : last, part_before = at >= 0 ? at_before : last_before, found = INT64_MAX;
+    }
+    __syncthreads();
+    double before = part_before;
+    int64_t last = -1;
+    double last_z = 0;
+    const int64_t j_first = part_at * (int64_t)pieces * kPiece, j_end = min(j_first + pieces * (int64_t)kPiece, c.n_legal);
+    for (int64_t j0 = j_first; j0 < j_end; j0 += kPiece) {
+      if (p.history) count_piece(p, row, j0, counts);
+      const int64_t j = j0 + threadIdx.x * kPer;
+      double z[kPer], w[kPer], sum = 0;
+      load_z<T, double>(p, c, row, j, p.history ? counts + threadIdx.x * kPer : nullptr, z);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        w[i] = exp_of((z[i] - a.m) * c.inv_t);
+        sum += w[i];
+        if (w[i] > 0) last = j + i, last_z = z[i];
+      }
+      const double incl = lanes_scan(sum, 64);
+      __syncthreads();
+      if ((threadIdx.x & 63) == 63) wave_sum[threadIdx.x >> 6] = incl;
+      __syncthreads();
+      double cum = before + incl - sum;
+      for (int i = 0; i < (int)(threadIdx.x >> 6); ++i) cum += wave_sum[i];
+      int64_t hit = INT64_MAX;
+      double hit_z = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        cum += w[i];
+        if (hit == INT64_MAX && w[i] > 0 && cum > target) hit = j + i, hit_z = z[i];
+      }
+      if (hit != INT64_MAX) atomicMin(&found, (long long)hit);
+      __syncthreads();
+      if (hit != INT64_MAX && hit == found) found_z = hit_z;
+      if (found != INT64_MAX) break;
+      for (int i = 0; i < kThreads / 64; ++i) before += wave_sum[i];
+    }
+    __syncthreads();
+    if (found == INT64_MAX) {  // rounding: the last option of the part with any weight
+      __syncthreads();
+      if (threadIdx.x == 0) found = -1;
+      __syncthreads();
+      atomicMax(&found, (long long)last);
+      __syncthreads();
+      if (last == found) found_z = last_z;
+      __syncthreads();
+    }
+    pick = found;
+    z_pick = found_z;
+  }
+  if (threadIdx.x == 0) finish_choose(out, row, a, c.bad, c.inv_t, pick, z_pick);
+}
+
+// The same walk in 32 bits. One part: the row's results at once; several: partial sums, with the logit of the
+// action from the part that holds it.
+struct EvaluatePart {
+  Stat<float> stat;
+  float z_act;
+};
+template <class T>
+__global__ __launch_bounds__(kThreads) void evaluate_parts(Rows p, int pieces, int n_parts, EvaluatePart* parts, EvaluateOut out) {
   __shared__ uint32_t counts[kPiece];
   __shared__ Stat<float> red[kThreads / 64];
   __shared__ float z_act;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
-    const RowConst<float> c = row_const<float>(p, row);
-    const int32_t act = action[row];
-    Stat<float> a = stat_zero<float>();
-    __syncthreads();
-    if (threadIdx.x == 0) z_act = -INFINITY;
-    __syncthreads();
-    for (int64_t j0 = 0; j0 < c.n_legal; j0 += kPiece) {
-      if (p.history) count_piece(p, row, j0, counts);
-      const int64_t j = j0 + threadIdx.x * kPer;
-      float z[kPer];
-      load_z<T, float>(p, c, row, j, p.history ? counts + threadIdx.x * kPer : nullptr, z);
-      stat_add(a, z, j, c.inv_t);
+  const int64_t row = blockIdx.x / n_parts, part = blockIdx.x % n_parts;
+  const RowConst<float> c = row_const<float>(p, row);
+  const int32_t act = out.action[row];
+  Stat<float> a = stat_zero<float>();
+  if (threadIdx.x == 0) z_act = -INFINITY;
+  __syncthreads();
+  const int64_t j_end = min((part + 1) * pieces * (int64_t)kPiece, c.n_legal);
+  for (int64_t j0 = part * pieces * (int64_t)kPiece; j0 < j_end; j0 += kPiece) {
+    if (p.history) count_piece(p, row, j0, counts);
+    const int64_t j = j0 + threadIdx.x * kPer;
+    float z[kPer];
+    load_z<T, float>(p, c, row, j, p.history ? counts + threadIdx.x * kPer : nullptr, z);
+    stat_add(a, z, j, c.inv_t);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        if (act == j + i) z_act = z[i];
-    }
-    a = stat_block(a, c.inv_t, red);
-    if (threadIdx.x == 0) finish_evaluate(row, p, c, a, act, z_act, log_prob, entropy, stats);
+    for (int i = 0; i < kPer; ++i)
+      if (act == j + i) z_act = z[i];
   }
+  a = stat_block(a, c.inv_t, red);
+  if (threadIdx.x != 0) return;
+  if (n_parts == 1) finish_evaluate(out, row, p.options, a, c.bad, c.inv_t, act, z_act);
+  else parts[blockIdx.x] = {a, z_act};
+}
+__global__ __launch_bounds__(kThreads) inline void evaluate_join(Rows p, int n_parts, const EvaluatePart* all_parts, EvaluateOut out) {
+  // one wave per row
+  const int64_t row = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  if (row >= p.rows) return;
+  const RowConst<float> c = row_const<float>(p, row);
+  const EvaluatePart* parts = all_parts + row * n_parts;
+  Stat<float> a = stat_zero<float>();
+  float z_act = -INFINITY;
+  for (int i = threadIdx.x & 63; i < n_parts; i += 64) {
+    EvaluatePart b = parts[i];
+    const float m = fmaxf(a.m, b.stat.m);
+    stat_rebase(a, m, c.inv_t);
+    stat_rebase(b.stat, m, c.inv_t);
+    a.s += b.stat.s, a.e += b.stat.e, a.bad |= b.stat.bad;
+    z_act = fmaxf(z_act, b.z_act);
+  }
+  const float m = lanes_max(a.m, 64);
+  stat_rebase(a, m, c.inv_t);
+  a.s = lanes_sum(a.s, 64), a.e = lanes_sum(a.e, 64), a.bad = lanes_max(a.bad, 64);
+  z_act = lanes_max(z_act, 64);
+  if ((threadIdx.x & 63) == 0) finish_evaluate(out, row, p.options, a, c.bad, c.inv_t, out.action[row], z_act);
 }
 
 struct GradArgs {
@@ -438,6 +700,59 @@ template <class T> __device__ inline void store8(T* out, const float (&v)[kPer],
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
       if (j + i < options) out[i] = (T)v[i];
+  }
+}
+
+// short rows: the lanes of evaluate_group, walking down the rows; a shared bias' gradient is summed per lane, then
+// over the workgroup's row slots
+template <class T, int NP> __global__ __launch_bounds__(kThreads) void evaluate_grad_group(Rows p, GradArgs g, int width_log, int64_t blocks_of_rows) {
+  extern __shared__ uint32_t counts[];  // (as floats for the sums afterwards)
+  float sum[NP][kPer];
+#pragma unroll
+  for (int k = 0; k < NP; ++k)
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) sum[k][i] = 0.f;
+  for (int64_t b = blockIdx.x; b < blocks_of_rows; b += gridDim.x) {
+    const Group at = group_of(p, b, width_log);
+    const uint32_t* n = count_groups<NP>(p, at, counts);
+    if (!at.there) continue;
+    const RowConst<float> c = row_const<float>(p, at.row);
+    const GradRow r = grad_row(g, at.row);
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      const int64_t j = at.j(k);
+      if (j >= p.options) continue;
+      float z[kPer], slope[kPer], dx[kPer], db[kPer];
+      const uint32_t legal = load_z<T, float>(p, c, at.row, j, n ? n + j : nullptr, z, slope);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const bool ok = (legal >> i) & 1;
+        db[i] = grad_y(r, z[i], ok, r.act == j + i, c.inv_t) * c.inv_t;
+        dx[i] = ok ? db[i] * slope[i] : 0.f;
+        sum[k][i] += db[i];
+      }
+      if (g.grad_logits) store8<T>((T*)g.grad_logits + at.row * g.grad_logits_stride + j, dx, j, p.options, g.vec_out);
+      if (g.grad_bias) {
+        const int64_t to = at.row * g.grad_bias_stride + j;
+        if (p.bias_f32) store8<float>((float*)g.grad_bias + to, db, j, p.options, false);
+        else store8<T>((T*)g.grad_bias + to, db, j, p.options, false);
+      }
+    }
+  }
+  if (!g.partial) return;
+  float* sums = (float*)counts;
+  const int width = 1 << width_log, per_row = width * kPer * NP;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < NP; ++k)
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      sums[(threadIdx.x >> width_log) * per_row + (k * width + (threadIdx.x & (width - 1))) * kPer + i] = sum[k][i];
+  __syncthreads();
+  for (int64_t j = threadIdx.x; j < p.options; j += kThreads) {
+    float s = 0.f;
+    for (int i = 0; i < (kThreads >> width_log); ++i) s += sums[i * per_row + j];
+    g.partial[blockIdx.x * p.options + j] = s;
   }
 }
 
