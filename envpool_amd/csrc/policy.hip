@@ -1,6 +1,7 @@
 // policy.hip - ep_policy_choose / ep_policy_evaluate / ep_policy_evaluate_grad: checks and launches.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "../../include/envpool_amd_policy.h"
 #include "common.hpp"
@@ -91,6 +92,12 @@ template <class F> void with_type(int32_t dtype, F f) {
   else if (dtype == EP_F16) f(epp::f16{});
   else f(epp::bf16{});
 }
+template <class F> void with_kernel(int32_t dtype, bool history, F f) {
+  with_type(dtype, [&](auto t) {
+    if (history) f(t, std::true_type{});
+    else f(t, std::false_type{});
+  });
+}
 
 // How rows map to the chip. Up to 2048 options a row is held by 1 to 64 neighbouring lanes (8 options a lane and
 // piece, 1 or 4 pieces): enough lanes for the options, and for a long history at least a lane per 16 entries
@@ -158,17 +165,18 @@ int ep_policy_choose(const ep_policy_rows* r, const void* u, int32_t u_dtype, in
   if (r->options <= kGroupOptions) {
     const Width w = group_width(k);
     const size_t lds = k.history ? w.lds : 0;
-    with_type(r->dtype, [&](auto t) {
-      if (w.pieces == 1) hipLaunchKernelGGL((epp::choose_group<decltype(t), 1>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, u, u_f64, out);
-      else hipLaunchKernelGGL((epp::choose_group<decltype(t), 4>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, u, u_f64, out);
+    with_kernel(r->dtype, k.history, [&](auto t, auto h) {
+      if (w.pieces == 1) hipLaunchKernelGGL((epp::choose_group<decltype(t), 1, h.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, u, u_f64, out);
+      else hipLaunchKernelGGL((epp::choose_group<decltype(t), 4, h.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, u, u_f64, out);
     });
   } else {
     const Cut cut = cut_rows(r->rows, r->options);
     if (r->rows * cut.parts > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld rows of %lld options", (long long)r->rows, (long long)r->options);
     auto* parts = (epp::Stat<double>*)r->workspace;
-    with_type(r->dtype, [&](auto t) {
-      hipLaunchKernelGGL(epp::choose_parts<decltype(t)>, dim3((unsigned)(r->rows * cut.parts)), dim3(epp::kThreads), 0, stream, k, cut.pieces, cut.parts, parts);
-      hipLaunchKernelGGL(epp::choose_join<decltype(t)>, dim3((unsigned)r->rows), dim3(epp::kThreads), 0, stream, k, cut.pieces, cut.parts, parts, u, u_f64, out);
+    with_kernel(r->dtype, k.history, [&](auto t, auto h) {
+      const auto stats = u ? epp::choose_parts<decltype(t), h.value, false> : epp::choose_parts<decltype(t), h.value, true>;
+      hipLaunchKernelGGL(stats, dim3((unsigned)(r->rows * cut.parts)), dim3(epp::kThreads), 0, stream, k, cut.pieces, cut.parts, parts);
+      hipLaunchKernelGGL((epp::choose_join<decltype(t), h.value>), dim3((unsigned)r->rows), dim3(epp::kThreads), 0, stream, k, cut.pieces, cut.parts, parts, u, u_f64, out);
     });
   }
   HIP_TRY(hipGetLastError());
@@ -193,16 +201,16 @@ int ep_policy_evaluate(const ep_policy_rows* r, const int32_t* action, float* lo
   if (r->options <= kGroupOptions) {
     const Width w = group_width(k);
     const size_t lds = k.history ? w.lds : 0;
-    with_type(r->dtype, [&](auto t) {
-      if (w.pieces == 1) hipLaunchKernelGGL((epp::evaluate_group<decltype(t), 1>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, out);
-      else hipLaunchKernelGGL((epp::evaluate_group<decltype(t), 4>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, out);
+    with_kernel(r->dtype, k.history, [&](auto t, auto h) {
+      if (w.pieces == 1) hipLaunchKernelGGL((epp::evaluate_group<decltype(t), 1, h.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, out);
+      else hipLaunchKernelGGL((epp::evaluate_group<decltype(t), 4, h.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, out);
     });
   } else {
     const Cut cut = cut_rows(r->rows, r->options);
     if (r->rows * cut.parts > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld rows of %lld options", (long long)r->rows, (long long)r->options);
     auto* parts = (epp::EvaluatePart*)r->workspace;
-    with_type(r->dtype, [&](auto t) {
-      hipLaunchKernelGGL(epp::evaluate_parts<decltype(t)>, dim3((unsigned)(r->rows * cut.parts)), dim3(epp::kThreads), 0, stream, k, cut.pieces, cut.parts, parts, out);
+    with_kernel(r->dtype, k.history, [&](auto t, auto h) {
+      hipLaunchKernelGGL((epp::evaluate_parts<decltype(t), h.value>), dim3((unsigned)(r->rows * cut.parts)), dim3(epp::kThreads), 0, stream, k, cut.pieces, cut.parts, parts, out);
     });
     if (cut.parts > 1)
       hipLaunchKernelGGL(epp::evaluate_join, dim3((unsigned)((r->rows + 3) / 4)), dim3(epp::kThreads), 0, stream, k, cut.parts, parts, out);
@@ -246,14 +254,14 @@ int ep_policy_evaluate_grad(const ep_policy_rows* r, const int32_t* action, cons
                     partial, 0};
     g.vec_out = (uintptr_t)grad_logits % 16 == 0 && (r->rows <= 1 || (grad_logits_stride * (int64_t)size_of(r->dtype)) % 16 == 0);
     const int64_t per = (r->rows + blocks - 1) / blocks;
-    with_type(r->dtype, [&](auto t) {
+    with_kernel(r->dtype, k.history, [&](auto t, auto h) {
       const size_t lds = k.history || shared ? w.lds : 0;
       if (group && w.pieces == 1)
-        hipLaunchKernelGGL((epp::evaluate_grad_group<decltype(t), 1>), dim3((unsigned)blocks), dim3(epp::kThreads), lds, stream, k, g, w.log, (int64_t)w.blocks);
+        hipLaunchKernelGGL((epp::evaluate_grad_group<decltype(t), 1, h.value>), dim3((unsigned)blocks), dim3(epp::kThreads), lds, stream, k, g, w.log, (int64_t)w.blocks);
       else if (group)
-        hipLaunchKernelGGL((epp::evaluate_grad_group<decltype(t), 4>), dim3((unsigned)blocks), dim3(epp::kThreads), lds, stream, k, g, w.log, (int64_t)w.blocks);
+        hipLaunchKernelGGL((epp::evaluate_grad_group<decltype(t), 4, h.value>), dim3((unsigned)blocks), dim3(epp::kThreads), lds, stream, k, g, w.log, (int64_t)w.blocks);
       else
-      hipLaunchKernelGGL(epp::evaluate_grad_piece<decltype(t)>, dim3((unsigned)pieces, (unsigned)blocks), dim3(epp::kThreads), 0, stream, k, g, per);
+        hipLaunchKernelGGL((epp::evaluate_grad_piece<decltype(t), h.value>), dim3((unsigned)pieces, (unsigned)blocks), dim3(epp::kThreads), 0, stream, k, g, per);
     });
     HIP_TRY(hipGetLastError());
   }

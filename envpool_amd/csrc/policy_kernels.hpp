@@ -38,23 +38,71 @@ constexpr int kThreads = 256;
 constexpr int kPer = 8;                      // options per thread and piece
 constexpr int kPiece = kThreads * kPer;      // options per piece of a row
 
-template <class R> __device__ inline R neg_inf() { return -(R)INFINITY; }
+// What stands for "no weight" among the y: illegal options, and legal ones that are -inf. In 64 bits no legal
+// value comes near it. In 32 bits a legal value is held one step above (HoldRange), so that an option masked
+// with the type's lowest value keeps its (vanishing) weight and a row of nothing else is uniform.
+template <class R> struct Num;
+template <> struct Num<double> {
+  static constexpr double kNone = -1.7976931348623157e308;
+  static constexpr double kUnit = 1.0;        // weights are exp(d kUnit): natural units
+  static constexpr double kFloor = -800.0;    // exp of this and less is 0
+};
+template <> struct Num<float> {
+  static constexpr float kNone = -3.40282347e38f;
+  static constexpr float kLow = -3.40282326e38f, kHigh = 3.40282326e38f;
+  static constexpr float kUnit = 0.693147181f;  // d counts octaves: the hardware's exponential is 2^d
+  static constexpr float kFloor = -10000.f;
+};
+
+// exp of x in [-800, 0] in 64 bits: x = n ln 2 + r, |r| <= ln 2 / 2, the series of exp r to r^11 (the first term
+// left out is below 7e-15), times 2^n. About two thirds of the library function's instructions: there are no
+// overflows or positive arguments to look after.
+__device__ inline double weight(double x) {
+  const double n = rint(x * 1.4426950408889634);
+  double r = fma(n, -0.6931471805599453, x);  // ln 2 to 53 bits, then what it lacks
+  r = fma(n, -2.3190468138462996e-17, r);
+  double p = 1.0 / 39916800;
+  p = fma(p, r, 1.0 / 3628800);
+  p = fma(p, r, 1.0 / 362880);
+  p = fma(p, r, 1.0 / 40320);
+  p = fma(p, r, 1.0 / 5040);
+  p = fma(p, r, 1.0 / 720);
+  p = fma(p, r, 1.0 / 120);
+  p = fma(p, r, 1.0 / 24);
+  p = fma(p, r, 1.0 / 6);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return __builtin_amdgcn_ldexp(p, (int)n);
+}
+__device__ inline float weight(float x) { return __builtin_amdgcn_exp2f(x); }
+// (maximum without the NaN rules of fmax's library form: the operands are numbers, or a NaN that must not win)
+__device__ inline double larger(double a, double b) { return __builtin_fmax(a, b); }
+__device__ inline float larger(float a, float b) { return __builtin_fmaxf(a, b); }
+
+__device__ inline double mul_add(double a, double b, double c) { return __builtin_fma(a, b, c); }
+__device__ inline float mul_add(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 
 // what is the same for all options of a row
 template <class R> struct RowConst {
   R rep, freq, pres, inv_t;
+  R k;              // (z - m) * k is a weight's exponent
   int64_t n_legal;  // options below this are legal as far as num_options goes
   bool bad;
 };
 
-template <class R> __device__ inline RowConst<R> row_const(const Rows& p, int64_t row) {
-  RowConst<R> c;
+template <class R, bool kHist> __device__ inline RowConst<R> row_const(const Rows& p, int64_t row) {
+  RowConst<R> c{};
   const R t = p.temperature ? (R)p.temperature[row] : (R)p.temperature_all;
-  c.rep = p.repetition ? (R)p.repetition[row] : (R)p.repetition_all;
-  c.freq = p.frequency ? (R)p.frequency[row] : (R)p.frequency_all;
-  c.pres = p.presence ? (R)p.presence[row] : (R)p.presence_all;
   c.inv_t = (R)1 / t;
-  c.bad = !(t > (R)0) || !(t < (R)INFINITY) || !(c.inv_t < (R)INFINITY) || (p.history && !(c.rep > (R)0));
+  c.k = c.inv_t / Num<R>::kUnit;
+  c.bad = !(t > (R)0) || !(t < (R)INFINITY) || !(c.k < (R)INFINITY);
+  if (kHist) {
+    c.rep = p.repetition ? (R)p.repetition[row] : (R)p.repetition_all;
+    c.freq = p.frequency ? (R)p.frequency[row] : (R)p.frequency_all;
+    c.pres = p.presence ? (R)p.presence[row] : (R)p.presence_all;
+    c.bad = c.bad || !(c.rep > (R)0);
+  }
   int64_t n = p.options;
   if (p.num_options) {
     const int64_t k = p.num_options[row];
@@ -77,163 +125,179 @@ template <class R> __device__ inline R penalized(R x, uint32_t count, const RowC
   return x;
 }
 
-// finite inputs whose 32-bit sum leaves the range stay at its end: a mask of the type's lowest value
-// plus a negative bias is still a (vanishing) weight and not an illegal option
-__device__ inline float hold_range(float z, float x, float b) {
-  if (fabsf(z) == INFINITY && fabsf(x) < INFINITY && fabsf(b) < INFINITY) return z > 0 ? 3.402823466e38f : -3.402823466e38f;
-  return z;
-}
-__device__ inline double hold_range(double z, double, double) { return z; }
-
 template <class T> struct Vec8 {
   alignas(16) T v[8];
 };
 
-template <class T> __device__ inline bool legal_at(const Rows& p, int64_t row, int64_t j) {
-  if (!p.mask) return true;
-  if (p.mask_bits) return (((const uint32_t*)p.mask)[row * p.mask_stride + (j >> 5)] >> (j & 31)) & 1u;
-  return ((const uint8_t*)p.mask)[row * p.mask_stride + j] != 0;
-}
-
-// z of options j0 .. j0+7 (j0 a multiple of 8): logits after penalties and bias, before the temperature;
-// -inf where illegal. legal: bit i = option j0 + i is legal. slope: d z / d logit, for the gradient.
-template <class T, class R>
-__device__ inline uint32_t load_z(const Rows& p, const RowConst<R>& c, int64_t row, int64_t j0, const uint32_t* counts,
-                                  R (&z)[kPer], R* slope = nullptr) {
-  uint32_t legal = 0;
+// Options j0 .. j0+7 of a row (j0 a multiple of 8, below the row's end): y before the temperature, as they
+// come. Returns which are legal (bit i = option j0 + i); the y of the others are unspecified.
+// slope: d y / d logit.
+template <class T, class R, bool kHist>
+__device__ inline uint32_t load_y(const Rows& p, const RowConst<R>& c, int64_t row, int64_t j0, const uint32_t* counts, R (&y)[kPer],
+                                  R* slope = nullptr) {
   const int64_t left = c.n_legal - j0;
-  if (left <= 0) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) z[i] = neg_inf<R>();
-    return 0;
-  }
-  legal = left >= kPer ? 0xffu : (1u << left) - 1u;
+  uint32_t legal = left >= kPer ? 0xffu : left > 0 ? (1u << left) - 1u : 0u;
+  const bool whole = j0 + kPer <= p.options;
   if (p.mask) {
     if (p.mask_bits) {
       legal &= ((const uint32_t*)p.mask)[row * p.mask_stride + (j0 >> 5)] >> (j0 & 31);
     } else {
       const uint8_t* m = (const uint8_t*)p.mask + row * p.mask_stride + j0;
-      if (((uintptr_t)m & 7) == 0 && j0 + kPer <= p.options) {
-        const uint64_t w = *(const uint64_t*)m;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-          if (!((w >> (8 * i)) & 0xff)) legal &= ~(1u << i);
+      uint64_t w = 0;
+      if (whole && ((uintptr_t)m & 7) == 0) {
+        w = *(const uint64_t*)m;
       } else {
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
-          if (j0 + i < p.options && !m[i]) legal &= ~(1u << i);
+          if (j0 + i < p.options) w |= (uint64_t)m[i] << (8 * i);
       }
+      // nonzero bytes to bits: every byte folded onto its lowest bit, the eight of them gathered by a product
+      w |= w >> 4;
+      w |= w >> 2;
+      w |= w >> 1;
+      w &= 0x0101010101010101ull;
+      legal &= (uint32_t)((w * 0x0102040810204080ull) >> 56);
     }
   }
   const T* x = (const T*)p.logits + row * p.logits_stride + j0;
   T xv[kPer];
-  if (p.vec && j0 + kPer <= p.options) {
+  if (p.vec && whole) {
     *(Vec8<T>*)xv = *(const Vec8<T>*)x;
   } else {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) xv[i] = j0 + i < p.options ? x[i] : (T)0.f;
   }
-  float bv[kPer];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) bv[i] = 0.f;
+  for (int i = 0; i < kPer; ++i) y[i] = (R)(float)xv[i];
+  if (kHist) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t n = counts[i];
+      if (slope) slope[i] = n ? (y[i] > (R)0 ? (R)1 / c.rep : c.rep) : (R)1;
+      y[i] = penalized<R>(y[i], n, c);
+    }
+  }
   if (p.bias) {
     const int64_t b0 = row * p.bias_stride + j0;
     if (p.bias_f32) {
       const float* b = (const float*)p.bias + b0;
-      if (p.vec && j0 + kPer <= p.options) {
-        *(Vec8<float>*)bv = *(const Vec8<float>*)b;
+      if (p.vec && whole) {
+        const Vec8<float> v = *(const Vec8<float>*)b;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) y[i] += (R)v.v[i];
       } else {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) bv[i] = j0 + i < p.options ? b[i] : 0.f;
+        for (int i = 0; i < kPer; ++i) y[i] += j0 + i < p.options ? (R)b[i] : (R)0;
       }
     } else {
       const T* b = (const T*)p.bias + b0;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) bv[i] = j0 + i < p.options ? (float)b[i] : 0.f;
+      for (int i = 0; i < kPer; ++i) y[i] += j0 + i < p.options ? (R)(float)b[i] : (R)0;
     }
-  }
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const R x0 = (R)(float)xv[i];
-    R y = x0;
-    if (counts) {
-      const uint32_t n = counts[i];
-      y = penalized<R>(x0, n, c);
-      if (slope) slope[i] = n ? (x0 > (R)0 ? (R)1 / c.rep : c.rep) : (R)1;
-    } else if (slope) {
-      slope[i] = (R)1;
-    }
-    const R b = (R)bv[i];
-    z[i] = (legal >> i) & 1 ? hold_range(y + b, x0, b) : neg_inf<R>();
   }
   return legal;
 }
 
-// exp of x <= 0 in 64 bits: x = n ln 2 + r, |r| <= ln 2 / 2, the series of exp r to r^11 (the first term left
-// out is below 7e-15), times 2^n. About two thirds of the library function's instructions: there are no
-// overflows or positive arguments to look after, and what is below e^-745 is 0.
-__device__ inline double exp_of(double x) {
-  x = fmax(x, -800.0);
-  const double n = rint(x * 1.4426950408889634);
-  double r = fma(n, -0.6931471805599453, x);  // ln 2 to 53 bits, then what it lacks
-  r = fma(n, -2.3190468138462996e-17, r);
-  double p = 1.0 / 39916800;
-  p = fma(p, r, 1.0 / 3628800);
-  p = fma(p, r, 1.0 / 362880);
-  p = fma(p, r, 1.0 / 40320);
-  p = fma(p, r, 1.0 / 5040);
-  p = fma(p, r, 1.0 / 720);
-  p = fma(p, r, 1.0 / 120);
-  p = fma(p, r, 1.0 / 24);
-  p = fma(p, r, 1.0 / 6);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  return __builtin_amdgcn_ldexp(p, (int)n);
+__device__ inline bool bit(uint32_t bits, int i) { return (bits >> i) & 1u; }
+
+// The y of `legal` made ready for sums: kNone where there is no weight. Returns whether one of them is NaN or
+// +inf. Nearly always all are finite, which one product with 0 per option shows (0 * inf and 0 * NaN are NaN).
+template <class R> __device__ inline bool ready_y(uint32_t legal, R (&y)[kPer]) {
+  R odd = (R)0;
+  R m = Num<R>::kNone;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    y[i] = bit(legal, i) ? y[i] : Num<R>::kNone;
+    odd = mul_add(y[i], (R)0, odd);
+    m = larger(m, y[i]);
+  }
+  if (odd == (R)0 && (m > Num<R>::kNone || !legal)) return false;
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (!bit(legal, i)) continue;
+    if (!(y[i] < (R)INFINITY)) bad = true;
+    if constexpr (sizeof(R) == 4) y[i] = y[i] == -INFINITY ? Num<R>::kNone : larger(y[i], Num<R>::kLow);
+    else if (y[i] == -(R)INFINITY) y[i] = Num<R>::kNone;
+  }
+  return bad;
 }
-__device__ inline float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896f); }
+
+// In 32 bits the sum of finite values may leave the range: the end of it stands for the sum then, so that it
+// is not taken for a logit that was infinite.
+template <class T, bool kHist>
+__device__ inline void hold_range(const Rows& p, const RowConst<float>& c, int64_t row, int64_t j0, uint32_t legal, float (&y)[kPer]) {
+  float odd = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) odd = mul_add(bit(legal, i) ? y[i] : 0.f, 0.f, odd);
+  if (odd == 0.f || !(p.bias || kHist)) return;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (!bit(legal, i) || fabsf(y[i]) != INFINITY) continue;
+    const float x = (float)((const T*)p.logits)[row * p.logits_stride + j0 + i];
+    float b = 0.f;
+    if (p.bias) {
+      const int64_t at = row * p.bias_stride + j0 + i;
+      b = p.bias_f32 ? ((const float*)p.bias)[at] : (float)((const T*)p.bias)[at];
+    }
+    if (fabsf(x) < INFINITY && fabsf(b) < INFINITY) y[i] = y[i] > 0.f ? Num<float>::kHigh : Num<float>::kLow;
+  }
+}
+template <class T, bool kHist>
+__device__ inline void hold_range(const Rows&, const RowConst<double>&, int64_t, int64_t, uint32_t, double (&)[kPer]) {}
+
+// load_y, hold_range and ready_y in one
+template <class T, class R, bool kHist>
+__device__ inline bool load_ready(const Rows& p, const RowConst<R>& c, int64_t row, int64_t j0, const uint32_t* counts, R (&y)[kPer]) {
+  if (j0 >= c.n_legal) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) y[i] = Num<R>::kNone;
+    return false;
+  }
+  const uint32_t legal = load_y<T, R, kHist>(p, c, row, j0, counts, y);
+  hold_range<T, kHist>(p, c, row, j0, legal, y);
+  return ready_y(legal, y);
+}
 
 // running statistics of a row, or of a part of it
 template <class R> struct Stat {
-  R m;       // largest z
-  R s, e;    // sum w, sum w (y - ym) with w = exp((z - m) / t); in units of 1/t: y - ym = (z - m) / t
-  int64_t best;  // lowest index with z == m
+  R m;           // largest y
+  R s, e;        // sum w, sum w d with d = (y - m) k, w = exp(d kUnit)
+  int64_t best;  // lowest index with y == m
   int32_t bad;
 };
-template <class R> __device__ inline Stat<R> stat_zero() { return {neg_inf<R>(), (R)0, (R)0, INT64_MAX, 0}; }
+template <class R> __device__ inline Stat<R> stat_zero() { return {Num<R>::kNone, (R)0, (R)0, INT64_MAX, 0}; }
+template <class R> __device__ inline R exponent(R y, R m, R k) { return larger((y - m) * k, Num<R>::kFloor); }
 
 // brings s, e from reference a.m to reference m >= a.m
-template <class R> __device__ inline void stat_rebase(Stat<R>& a, R m, R inv_t) {
-  if (a.m == m) return;
-  if (a.m == neg_inf<R>()) {
-    a.s = a.e = (R)0;
-  } else {
-    const R d = (a.m - m) * inv_t;
-    const R f = exp_of(d);
-    a.e = f > (R)0 ? f * (a.e + a.s * d) : (R)0;
-    a.s = f * a.s;
-  }
+template <class R> __device__ inline void stat_rebase(Stat<R>& a, R m, R k) {
+  const R d = exponent(a.m, m, k);
+  const R f = weight(d);
+  a.e = f * mul_add(a.s, d, a.e);
+  a.s = f * a.s;
   a.m = m;
 }
-// adds the options j0 .. j0+7
-template <class R> __device__ inline void stat_add(Stat<R>& a, const R (&z)[kPer], int64_t j0, R inv_t) {
-  R m = neg_inf<R>();
-  int at = 0;
+// adds the options j0 .. j0+7 (kBest: and notes where the largest is)
+template <class R, bool kBest> __device__ inline void stat_add(Stat<R>& a, const R (&y)[kPer], int64_t j0, R k) {
+  R m = y[0];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    if (!(z[i] < (R)INFINITY)) a.bad = 1;
-    if (z[i] > m) m = z[i], at = i;
-  }
-  if (m == neg_inf<R>()) return;
+  for (int i = 1; i < kPer; ++i) m = larger(m, y[i]);
+  if (m == Num<R>::kNone) return;
   if (m > a.m) {
-    a.best = j0 + at;
-    stat_rebase(a, m, inv_t);
+    if (kBest) {
+      int at = 0;
+#pragma unroll
+      for (int i = kPer - 1; i >= 0; --i) at = y[i] == m ? i : at;
+      a.best = j0 + at;
+    }
+    stat_rebase(a, m, k);
   }
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const R d = (z[i] - a.m) * inv_t;
-    const R w = exp_of(d);
-    if (w > (R)0) a.s += w, a.e += w * d;
+    const R d = exponent(y[i], a.m, k);
+    const R w = weight(d);
+    a.s += w;
+    a.e = mul_add(w, d, a.e);
   }
 }
 
@@ -262,7 +326,7 @@ template <class V> __device__ inline V lanes_scan(V v, int width) {
 
 // over the workgroup, the same result in every thread: the maximum first, then every thread moves its own
 // sums to it (one exponential each) and they are added
-template <class R> __device__ inline Stat<R> stat_block(Stat<R> a, R inv_t, Stat<R>* lds) {
+template <class R> __device__ inline Stat<R> stat_block(Stat<R> a, R k, Stat<R>* lds) {
   constexpr int kWaves = kThreads / 64;
   const int wave = threadIdx.x >> 6;
   const R m_wave = lanes_max(a.m, 64);
@@ -270,9 +334,9 @@ template <class R> __device__ inline Stat<R> stat_block(Stat<R> a, R inv_t, Stat
   if ((threadIdx.x & 63) == 0) lds[wave].m = m_wave;
   __syncthreads();
   R m = lds[0].m;
-  for (int i = 1; i < kWaves; ++i) m = m > lds[i].m ? m : lds[i].m;
+  for (int i = 1; i < kWaves; ++i) m = larger(m, lds[i].m);
   const int64_t best = lanes_min((long long)(a.m == m ? a.best : INT64_MAX), 64);
-  stat_rebase(a, m, inv_t);
+  stat_rebase(a, m, k);
   const R sum = lanes_sum(a.s, 64), e = lanes_sum(a.e, 64);
   const int bad = __any(a.bad);
   __syncthreads();
@@ -306,32 +370,32 @@ struct ChooseOut {
   int32_t* action;
   float *log_prob, *entropy;
 };
-__device__ inline void finish_choose(const ChooseOut& o, int64_t row, const Stat<double>& a, bool bad_row, double inv_t, int64_t pick, double z_pick) {
-  const bool bad = a.bad || bad_row;
-  const bool empty = !bad && a.m == neg_inf<double>();
+__device__ inline void finish_choose(const ChooseOut& o, int64_t row, const Stat<double>& a, const RowConst<double>& c, int64_t pick, double y_pick) {
+  const bool bad = a.bad || c.bad;
+  const bool empty = !bad && a.m == Num<double>::kNone;
   const double log_s = log(a.s);
   o.action[row] = bad || empty ? -1 : (int32_t)pick;
-  o.log_prob[row] = bad ? quiet_nan<float>() : empty ? 0.f : (float)((z_pick - a.m) * inv_t - log_s);
+  o.log_prob[row] = bad ? quiet_nan<float>() : empty ? 0.f : (float)((y_pick - a.m) * c.k - log_s);
   o.entropy[row] = bad ? quiet_nan<float>() : empty ? 0.f : (float)(log_s - a.e / a.s);
 }
 
 struct EvaluateOut {
   const int32_t* action;
-  float *log_prob, *entropy, *stats;
+  float *log_prob, *entropy, *stats;  // stats: {largest y, log2 of the sum of weights}; {-inf, 0}: EMPTY; {NaN, NaN}: BAD
 };
-__device__ inline void finish_evaluate(const EvaluateOut& o, int64_t row, int64_t options, const Stat<float>& a, bool bad_row, float inv_t, int32_t act,
-                                       float z_act) {
-  const bool bad = a.bad || bad_row;
-  const bool empty = !bad && a.m == -INFINITY;
-  const float log_s = logf(a.s);
+__device__ inline void finish_evaluate(const EvaluateOut& o, int64_t row, int64_t options, const Stat<float>& a, const RowConst<float>& c, int32_t act,
+                                       float y_act) {
+  const bool bad = a.bad || c.bad;
+  const bool empty = !bad && a.m == Num<float>::kNone;
+  const float log_s = __builtin_amdgcn_logf(a.s);
   float lp;
   if (act == -1) lp = 0.f;
   else if (act < 0 || act >= options) lp = quiet_nan<float>();
-  else if (empty || z_act == -INFINITY) lp = -INFINITY;
-  else lp = (z_act - a.m) * inv_t - log_s;
+  else if (empty || y_act == Num<float>::kNone) lp = -INFINITY;
+  else lp = ((y_act - a.m) * c.k - log_s) * Num<float>::kUnit;
   o.log_prob[row] = bad ? quiet_nan<float>() : lp;
-  o.entropy[row] = bad ? quiet_nan<float>() : empty ? 0.f : log_s - a.e / a.s;
-  o.stats[2 * row] = bad ? quiet_nan<float>() : a.m;
+  o.entropy[row] = bad ? quiet_nan<float>() : empty ? 0.f : (log_s - a.e / a.s) * Num<float>::kUnit;
+  o.stats[2 * row] = bad ? quiet_nan<float>() : empty ? -INFINITY : a.m;
   o.stats[2 * row + 1] = bad ? quiet_nan<float>() : empty ? 0.f : log_s;
 }
 
@@ -355,7 +419,6 @@ __device__ inline Group group_of(const Rows& p, int64_t block, int width_log) {
 }
 // the histories of a workgroup's rows, counted; returns this row's counts
 template <int NP> __device__ inline const uint32_t* count_groups(const Rows& p, const Group& g, uint32_t* counts) {
-  if (!p.history) return nullptr;
   uint32_t* mine = counts + (threadIdx.x - g.lane) * kPer * NP;
   __syncthreads();
   for (int i = threadIdx.x; i < kThreads * kPer * NP; i += kThreads) counts[i] = 0;
@@ -369,155 +432,165 @@ template <int NP> __device__ inline const uint32_t* count_groups(const Rows& p, 
   return mine;
 }
 
-template <class T, int NP>
+template <class T, int NP, bool kHist>
 __global__ __launch_bounds__(kThreads) void choose_group(Rows p, int width_log, const void* u, int u_f64, ChooseOut out) {
   extern __shared__ uint32_t counts[];
   const Group g = group_of(p, blockIdx.x, width_log);
-  const RowConst<double> c = row_const<double>(p, g.row);
-  const uint32_t* n = count_groups<NP>(p, g, counts);
-  double z[NP][kPer];
+  const RowConst<double> c = row_const<double, kHist>(p, g.row);
+  const uint32_t* n = kHist ? count_groups<NP>(p, g, counts) : nullptr;
+  double y[NP][kPer];
   Stat<double> a = stat_zero<double>();
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    load_z<T, double>(p, c, g.row, g.j(k), n ? n + g.j(k) : nullptr, z[k]);
+    a.bad |= load_ready<T, double, kHist>(p, c, g.row, g.j(k), kHist ? n + g.j(k) : nullptr, y[k]);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      if (!(z[k][i] < (double)INFINITY)) a.bad = 1;
-      if (z[k][i] > a.m) a.m = z[k][i], a.best = g.j(k) + i;
-    }
+    for (int i = 0; i < kPer; ++i) a.m = larger(a.m, y[k][i]);
   }
-  const double m = lanes_max(a.m, g.width);
-  int32_t best = a.m == m && a.best < INT32_MAX ? (int32_t)a.best : INT32_MAX;
-  a.m = m;
-  a.best = lanes_min(best, g.width);
+  a.m = lanes_max(a.m, g.width);
   a.bad = lanes_max(a.bad, g.width);
   double w[NP][kPer];
 #pragma unroll
   for (int k = 0; k < NP; ++k)
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const double d = (z[k][i] - m) * c.inv_t;
-      w[k][i] = exp_of(d);
+      const double d = exponent(y[k][i], a.m, c.k);
+      w[k][i] = weight(d);
       a.s += w[k][i];
-      if (w[k][i] > 0) a.e += w[k][i] * d;
+      a.e = fma(w[k][i], d, a.e);
     }
-  a.s = lanes_sum(a.s, g.width);
   a.e = lanes_sum(a.e, g.width);
-  int32_t pick = (int32_t)a.best;
-  double z_pick = m;
-  if (u) {
-    const double target = (u_f64 ? ((const double*)u)[g.row] : (double)((const float*)u)[g.row]) * a.s;
-    double before = 0;
-    int32_t hit = INT32_MAX, last = -1;
-    double hit_z = 0, last_z = 0;
+  int32_t pick;
+  double y_pick = a.m;
+  if (!u) {
+    a.s = lanes_sum(a.s, g.width);
+    int32_t best = INT32_MAX;
+#pragma unroll
+    for (int k = NP - 1; k >= 0; --k)
+#pragma unroll
+      for (int i = kPer - 1; i >= 0; --i) best = y[k][i] == a.m ? (int32_t)g.j(k) + i : best;
+    pick = lanes_min(best, g.width);
+  } else {
+    // cumulated from option 0 on: piece by piece, lane by lane
+    double sum[NP], incl[NP], before = 0;
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-      double sum = 0;
+      sum[k] = 0;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) sum += w[k][i];
-      const double incl = lanes_scan(sum, g.width);
-      double cum = before + incl - sum;
+      for (int i = 0; i < kPer; ++i) sum[k] += w[k][i];
+      incl[k] = lanes_scan(sum[k], g.width) + before;
+      before = __shfl(incl[k], (threadIdx.x & 63) | (g.width - 1), 64);
+    }
+    a.s = before;
+    const double target = (u_f64 ? ((const double*)u)[g.row] : (double)((const float*)u)[g.row]) * a.s;
+    int32_t hit = INT32_MAX;
+    double hit_y = Num<double>::kNone;
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        cum += w[k][i];
-        if (w[k][i] > 0) {
-          last = (int32_t)g.j(k) + i, last_z = z[k][i];
-          if (hit == INT32_MAX && cum > target) hit = last, hit_z = last_z;
-        }
+    for (int k = NP - 1; k >= 0; --k) {
+      // from the lane's end: the lowest option whose sum is above the target stays
+      double cum = incl[k];
+#pragma unroll
+      for (int i = kPer - 1; i >= 0; --i) {
+        const bool is = cum > target && w[k][i] > 0;
+        hit = is ? (int32_t)g.j(k) + i : hit;
+        hit_y = is ? y[k][i] : hit_y;
+        cum = i ? cum - w[k][i] : cum;
       }
-      before += __shfl(incl, (threadIdx.x & 63) | (g.width - 1), 64);
     }
     pick = lanes_min(hit, g.width);
-    if (pick == INT32_MAX) {  // (a sum that rounding left short of the target: the last option with any weight)
-      pick = lanes_max(last, g.width);
-      hit = last, hit_z = last_z;
+    if (pick == INT32_MAX) {  // (u at the upper end: the last option with any weight)
+      hit = -1;
+#pragma unroll
+      for (int k = 0; k < NP; ++k)
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          if (w[k][i] > 0) hit = (int32_t)g.j(k) + i, hit_y = y[k][i];
+      pick = lanes_max(hit, g.width);
     }
-    z_pick = lanes_max(hit == pick ? hit_z : neg_inf<double>(), g.width);
+    y_pick = lanes_max(hit == pick ? hit_y : Num<double>::kNone, g.width);
   }
-  if (g.lane == 0 && g.there) finish_choose(out, g.row, a, c.bad, c.inv_t, pick, z_pick);
+  if (g.lane == 0 && g.there) finish_choose(out, g.row, a, c, pick, y_pick);
 }
 
-template <class T, int NP> __global__ __launch_bounds__(kThreads) void evaluate_group(Rows p, int width_log, EvaluateOut out) {
+template <class T, int NP, bool kHist> __global__ __launch_bounds__(kThreads) void evaluate_group(Rows p, int width_log, EvaluateOut out) {
   extern __shared__ uint32_t counts[];
   const Group g = group_of(p, blockIdx.x, width_log);
-  const RowConst<float> c = row_const<float>(p, g.row);
-  const uint32_t* n = count_groups<NP>(p, g, counts);
+  const RowConst<float> c = row_const<float, kHist>(p, g.row);
+  const uint32_t* n = kHist ? count_groups<NP>(p, g, counts) : nullptr;
   const int32_t act = out.action[g.row];
-  float z[NP][kPer];
+  float y[NP][kPer];
   Stat<float> a = stat_zero<float>();
-  float z_act = -INFINITY;
+  float y_act = Num<float>::kNone;
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    load_z<T, float>(p, c, g.row, g.j(k), n ? n + g.j(k) : nullptr, z[k]);
+    a.bad |= load_ready<T, float, kHist>(p, c, g.row, g.j(k), kHist ? n + g.j(k) : nullptr, y[k]);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      if (!(z[k][i] < INFINITY)) a.bad = 1;
-      a.m = fmaxf(a.m, z[k][i]);
-      if (act == g.j(k) + i) z_act = z[k][i];
+      a.m = larger(a.m, y[k][i]);
+      y_act = act == g.j(k) + i ? y[k][i] : y_act;
     }
   }
   a.m = lanes_max(a.m, g.width);
   a.bad = lanes_max(a.bad, g.width);
-  z_act = lanes_max(z_act, g.width);
+  y_act = lanes_max(y_act, g.width);
 #pragma unroll
   for (int k = 0; k < NP; ++k)
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const float d = (z[k][i] - a.m) * c.inv_t;
-      const float w = exp_of(d);
-      if (w > 0.f) a.s += w, a.e += w * d;
+      const float d = exponent(y[k][i], a.m, c.k);
+      const float w = weight(d);
+      a.s += w;
+      a.e = fmaf(w, d, a.e);
     }
   a.s = lanes_sum(a.s, g.width);
   a.e = lanes_sum(a.e, g.width);
-  if (g.lane == 0 && g.there) finish_evaluate(out, g.row, p.options, a, c.bad, c.inv_t, act, z_act);
+  if (g.lane == 0 && g.there) finish_evaluate(out, g.row, p.options, a, c, act, y_act);
 }
 
 // ---- longer rows: a workgroup per part of a row (`pieces` pieces of kPiece options), parts joined after ---
-template <class T>
+template <class T, bool kHist, bool kBest>
 __global__ __launch_bounds__(kThreads) void choose_parts(Rows p, int pieces, int n_parts, Stat<double>* parts) {
-  __shared__ uint32_t counts[kPiece];
+  __shared__ uint32_t counts[kHist ? kPiece : 1];
   __shared__ Stat<double> red[kThreads / 64];
   const int64_t row = blockIdx.x / n_parts, part = blockIdx.x % n_parts;
-  const RowConst<double> c = row_const<double>(p, row);
+  const RowConst<double> c = row_const<double, kHist>(p, row);
   Stat<double> a = stat_zero<double>();
   const int64_t j_end = min((part + 1) * pieces * (int64_t)kPiece, c.n_legal);
   for (int64_t j0 = part * pieces * (int64_t)kPiece; j0 < j_end; j0 += kPiece) {
-    if (p.history) count_piece(p, row, j0, counts);
+    if (kHist) count_piece(p, row, j0, counts);
     const int64_t j = j0 + threadIdx.x * kPer;
-    double z[kPer];
-    load_z<T, double>(p, c, row, j, p.history ? counts + threadIdx.x * kPer : nullptr, z);
-    stat_add(a, z, j, c.inv_t);
+    double y[kPer];
+    a.bad |= load_ready<T, double, kHist>(p, c, row, j, kHist ? counts + threadIdx.x * kPer : nullptr, y);
+    stat_add<double, kBest>(a, y, j, c.k);
   }
-  a = stat_block(a, c.inv_t, red);
+  a = stat_block(a, c.k, red);
   if (threadIdx.x == 0) parts[blockIdx.x] = a;
 }
 
 // joins a row's parts, and finds the option that u falls on by walking down the one part it lies in
-template <class T>
+template <class T, bool kHist>
 __global__ __launch_bounds__(kThreads) void choose_join(Rows p, int pieces, int n_parts, const Stat<double>* all_parts, const void* u, int u_f64, ChooseOut out) {
-  __shared__ uint32_t counts[kPiece];
+  __shared__ uint32_t counts[kHist ? kPiece : 1];
   __shared__ Stat<double> red[kThreads / 64];
   __shared__ double wave_sum[kThreads / 64];
   __shared__ long long found;
-  __shared__ double found_z, part_before;
+  __shared__ double found_y, part_before;
   __shared__ int part_at;
   const int64_t row = blockIdx.x;
   const Stat<double>* parts = all_parts + row * n_parts;
-  const RowConst<double> c = row_const<double>(p, row);
+  const RowConst<double> c = row_const<double, kHist>(p, row);
   Stat<double> a = stat_zero<double>();
   for (int i = threadIdx.x; i < n_parts; i += kThreads) {
     Stat<double> b = parts[i];
-    const double m = a.m > b.m ? a.m : b.m;
+    const double m = larger(a.m, b.m);
     const int64_t best = a.m > b.m ? a.best : (b.m > a.m ? b.best : min(a.best, b.best));
-    stat_rebase(a, m, c.inv_t);
-    stat_rebase(b, m, c.inv_t);
+    stat_rebase(a, m, c.k);
+    stat_rebase(b, m, c.k);
     a = {m, a.s + b.s, a.e + b.e, best, a.bad | b.bad};
   }
-  a = stat_block(a, c.inv_t, red);
-  const bool bad = a.bad || c.bad, empty = !bad && a.m == neg_inf<double>();
+  a = stat_block(a, c.k, red);
   int64_t pick = a.best;
-  double z_pick = a.m;
-  if (u && !bad && !empty) {
+  double y_pick = a.m;
+  if (u && !a.bad && !c.bad && a.m != Num<double>::kNone) {
     const double target = (u_f64 ? ((const double*)u)[row] : (double)((const float*)u)[row]) * a.s;
     // the part: its weights, moved to the row's maximum, cumulated 64 parts at a time by one wave
     if (threadIdx.x < 64) {
@@ -528,7 +601,7 @@ __global__ __launch_bounds__(kThreads) void choose_join(Rows p, int pieces, int 
         double w = 0;
         if (i0 + (int)threadIdx.x < n_parts) {
           Stat<double> b = parts[i0 + threadIdx.x];
-          stat_rebase(b, a.m, c.inv_t);
+          stat_rebase(b, a.m, c.k);
           w = b.s;
         }
         const double incl = before + lanes_scan(w, 64);
@@ -550,18 +623,18 @@ __global__ __launch_bounds__(kThreads) void choose_join(Rows p, int pieces, int 
     __syncthreads();
     double before = part_before;
     int64_t last = -1;
-    double last_z = 0;
+    double last_y = 0;
     const int64_t j_first = part_at * (int64_t)pieces * kPiece, j_end = min(j_first + pieces * (int64_t)kPiece, c.n_legal);
     for (int64_t j0 = j_first; j0 < j_end; j0 += kPiece) {
-      if (p.history) count_piece(p, row, j0, counts);
+      if (kHist) count_piece(p, row, j0, counts);
       const int64_t j = j0 + threadIdx.x * kPer;
-      double z[kPer], w[kPer], sum = 0;
-      load_z<T, double>(p, c, row, j, p.history ? counts + threadIdx.x * kPer : nullptr, z);
+      double y[kPer], w[kPer], sum = 0;
+      (void)load_ready<T, double, kHist>(p, c, row, j, kHist ? counts + threadIdx.x * kPer : nullptr, y);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        w[i] = exp_of((z[i] - a.m) * c.inv_t);
+        w[i] = weight(exponent(y[i], a.m, c.k));
         sum += w[i];
-        if (w[i] > 0) last = j + i, last_z = z[i];
+        if (w[i] > 0) last = j + i, last_y = y[i];
       }
       const double incl = lanes_scan(sum, 64);
       __syncthreads();
@@ -570,15 +643,15 @@ __global__ __launch_bounds__(kThreads) void choose_join(Rows p, int pieces, int 
       double cum = before + incl - sum;
       for (int i = 0; i < (int)(threadIdx.x >> 6); ++i) cum += wave_sum[i];
       int64_t hit = INT64_MAX;
-      double hit_z = 0;
+      double hit_y = 0;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         cum += w[i];
-        if (hit == INT64_MAX && w[i] > 0 && cum > target) hit = j + i, hit_z = z[i];
+        if (hit == INT64_MAX && w[i] > 0 && cum > target) hit = j + i, hit_y = y[i];
       }
       if (hit != INT64_MAX) atomicMin(&found, (long long)hit);
       __syncthreads();
-      if (hit != INT64_MAX && hit == found) found_z = hit_z;
+      if (hit != INT64_MAX && hit == found) found_y = hit_y;
       if (found != INT64_MAX) break;
       for (int i = 0; i < kThreads / 64; ++i) before += wave_sum[i];
     }
@@ -589,69 +662,71 @@ __global__ __launch_bounds__(kThreads) void choose_join(Rows p, int pieces, int 
       __syncthreads();
       atomicMax(&found, (long long)last);
       __syncthreads();
-      if (last == found) found_z = last_z;
+      if (last == found) found_y = last_y;
       __syncthreads();
     }
     pick = found;
-    z_pick = found_z;
+    y_pick = found_y;
   }
-  if (threadIdx.x == 0) finish_choose(out, row, a, c.bad, c.inv_t, pick, z_pick);
+  if (threadIdx.x == 0) finish_choose(out, row, a, c, pick, y_pick);
 }
 
 // The same walk in 32 bits. One part: the row's results at once; several: partial sums, with the logit of the
 // action from the part that holds it.
 struct EvaluatePart {
   Stat<float> stat;
-  float z_act;
+  float y_act;
 };
-template <class T>
+template <class T, bool kHist>
 __global__ __launch_bounds__(kThreads) void evaluate_parts(Rows p, int pieces, int n_parts, EvaluatePart* parts, EvaluateOut out) {
-  __shared__ uint32_t counts[kPiece];
+  __shared__ uint32_t counts[kHist ? kPiece : 1];
   __shared__ Stat<float> red[kThreads / 64];
-  __shared__ float z_act;
+  __shared__ float y_act;
   const int64_t row = blockIdx.x / n_parts, part = blockIdx.x % n_parts;
-  const RowConst<float> c = row_const<float>(p, row);
+  const RowConst<float> c = row_const<float, kHist>(p, row);
   const int32_t act = out.action[row];
   Stat<float> a = stat_zero<float>();
-  if (threadIdx.x == 0) z_act = -INFINITY;
+  if (threadIdx.x == 0) y_act = Num<float>::kNone;
   __syncthreads();
   const int64_t j_end = min((part + 1) * pieces * (int64_t)kPiece, c.n_legal);
   for (int64_t j0 = part * pieces * (int64_t)kPiece; j0 < j_end; j0 += kPiece) {
-    if (p.history) count_piece(p, row, j0, counts);
+    if (kHist) count_piece(p, row, j0, counts);
     const int64_t j = j0 + threadIdx.x * kPer;
-    float z[kPer];
-    load_z<T, float>(p, c, row, j, p.history ? counts + threadIdx.x * kPer : nullptr, z);
-    stat_add(a, z, j, c.inv_t);
+    float y[kPer];
+    a.bad |= load_ready<T, float, kHist>(p, c, row, j, kHist ? counts + threadIdx.x * kPer : nullptr, y);
+    stat_add<float, false>(a, y, j, c.k);
+    if ((uint64_t)(act - j) < kPer) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (act == j + i) z_act = z[i];
+      for (int i = 0; i < kPer; ++i)
+        if (act == j + i) y_act = y[i];
+    }
   }
-  a = stat_block(a, c.inv_t, red);
+  a = stat_block(a, c.k, red);
   if (threadIdx.x != 0) return;
-  if (n_parts == 1) finish_evaluate(out, row, p.options, a, c.bad, c.inv_t, act, z_act);
-  else parts[blockIdx.x] = {a, z_act};
+  if (n_parts == 1) finish_evaluate(out, row, p.options, a, c, act, y_act);
+  else parts[blockIdx.x] = {a, y_act};
 }
 __global__ __launch_bounds__(kThreads) inline void evaluate_join(Rows p, int n_parts, const EvaluatePart* all_parts, EvaluateOut out) {
   // one wave per row
   const int64_t row = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
   if (row >= p.rows) return;
-  const RowConst<float> c = row_const<float>(p, row);
+  const RowConst<float> c = p.history ? row_const<float, true>(p, row) : row_const<float, false>(p, row);
   const EvaluatePart* parts = all_parts + row * n_parts;
   Stat<float> a = stat_zero<float>();
-  float z_act = -INFINITY;
+  float y_act = Num<float>::kNone;
   for (int i = threadIdx.x & 63; i < n_parts; i += 64) {
     EvaluatePart b = parts[i];
-    const float m = fmaxf(a.m, b.stat.m);
-    stat_rebase(a, m, c.inv_t);
-    stat_rebase(b.stat, m, c.inv_t);
+    const float m = larger(a.m, b.stat.m);
+    stat_rebase(a, m, c.k);
+    stat_rebase(b.stat, m, c.k);
     a.s += b.stat.s, a.e += b.stat.e, a.bad |= b.stat.bad;
-    z_act = fmaxf(z_act, b.z_act);
+    y_act = larger(y_act, b.y_act);
   }
   const float m = lanes_max(a.m, 64);
-  stat_rebase(a, m, c.inv_t);
+  stat_rebase(a, m, c.k);
   a.s = lanes_sum(a.s, 64), a.e = lanes_sum(a.e, 64), a.bad = lanes_max(a.bad, 64);
-  z_act = lanes_max(z_act, 64);
-  if ((threadIdx.x & 63) == 0) finish_evaluate(out, row, p.options, a, c.bad, c.inv_t, out.action[row], z_act);
+  y_act = lanes_max(y_act, 64);
+  if ((threadIdx.x & 63) == 0) finish_evaluate(out, row, p.options, a, c, out.action[row], y_act);
 }
 
 struct GradArgs {
@@ -665,29 +740,43 @@ struct GradArgs {
   int32_t vec_out;
 };
 
-// per-row factors of the gradient
+// What the gradient of a row needs, all scaled by 1 / temperature: with d = log2 p_j,
+// d/dy_j = [j = act] g1 - p_j (g1 + g2 (H + ln p_j)).
 struct GradRow {
-  float m, log_s, h, g1, g2;
+  float m, k, log_s;
+  float flat, lean;  // g1 + g2 H, g2 ln 2
+  float g1;
   int32_t act;
+  bool empty;
 };
-__device__ inline GradRow grad_row(const GradArgs& g, int64_t row) {
+template <bool kHist> __device__ inline GradRow grad_row(const GradArgs& g, const RowConst<float>& c, int64_t row) {
   GradRow r;
   r.m = g.stats[2 * row];
   r.log_s = g.stats[2 * row + 1];
-  r.h = g.entropy[row];
-  r.g1 = g.g_lp ? g.g_lp[row] : 0.f;
-  r.g2 = g.g_h ? g.g_h[row] : 0.f;
+  r.k = c.k;
   r.act = g.action[row];
-  if (r.act == -1) r.g1 = 0.f;
+  const float g1 = r.act != -1 && g.g_lp ? g.g_lp[row] : 0.f, g2 = g.g_h ? g.g_h[row] : 0.f;
+  r.empty = r.m == -INFINITY;
+  const float nan = r.m != r.m ? r.m : 0.f;  // a BAD row: its gradient is NaN where legal
+  r.g1 = g1 * c.inv_t;
+  r.flat = (g1 + g2 * g.entropy[row]) * c.inv_t + nan;
+  r.lean = g2 * Num<float>::kUnit * c.inv_t;
   return r;
 }
-// d/dy of g1 log p[act] + g2 H for one option
-__device__ inline float grad_y(const GradRow& r, float z, bool legal, bool is_act, float inv_t) {
-  if (!legal || r.m == -INFINITY) return 0.f;
-  const float d = (z - r.m) * inv_t - r.log_s;
-  const float pr = exp_of(d);
-  const float ent = pr > 0.f ? r.g2 * pr * (d + r.h) : 0.f;
-  return r.g1 * ((is_act ? 1.f : 0.f) - pr) - ent + (pr != pr ? pr : 0.f);
+// the gradient with respect to y / temperature's argument for options j .. j+7; 0 where illegal
+__device__ inline void grad_y(const GradRow& r, const float (&y)[kPer], uint32_t legal, int64_t j, float (&out)[kPer]) {
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const float z = __builtin_amdgcn_fmed3f(y[i], Num<float>::kLow, Num<float>::kHigh);
+    const float d = larger((z - r.m) * r.k - r.log_s, Num<float>::kFloor);
+    const float v = -weight(d) * fmaf(r.lean, d, r.flat);
+    out[i] = bit(legal, i) ? v : 0.f;
+  }
+  if ((uint64_t)(r.act - j) < kPer) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (r.act == j + i && bit(legal, i)) out[i] += r.g1;
+  }
 }
 
 template <class T> __device__ inline void store8(T* out, const float (&v)[kPer], int64_t j, int64_t options, bool vec) {
@@ -705,7 +794,7 @@ template <class T> __device__ inline void store8(T* out, const float (&v)[kPer],
 
 // short rows: the lanes of evaluate_group, walking down the rows; a shared bias' gradient is summed per lane, then
 // over the workgroup's row slots
-template <class T, int NP> __global__ __launch_bounds__(kThreads) void evaluate_grad_group(Rows p, GradArgs g, int width_log, int64_t blocks_of_rows) {
+template <class T, int NP, bool kHist> __global__ __launch_bounds__(kThreads) void evaluate_grad_group(Rows p, GradArgs g, int width_log, int64_t blocks_of_rows) {
   extern __shared__ uint32_t counts[];  // (as floats for the sums afterwards)
   float sum[NP][kPer];
 #pragma unroll
@@ -714,21 +803,20 @@ template <class T, int NP> __global__ __launch_bounds__(kThreads) void evaluate_
     for (int i = 0; i < kPer; ++i) sum[k][i] = 0.f;
   for (int64_t b = blockIdx.x; b < blocks_of_rows; b += gridDim.x) {
     const Group at = group_of(p, b, width_log);
-    const uint32_t* n = count_groups<NP>(p, at, counts);
+    const uint32_t* n = kHist ? count_groups<NP>(p, at, counts) : nullptr;
     if (!at.there) continue;
-    const RowConst<float> c = row_const<float>(p, at.row);
-    const GradRow r = grad_row(g, at.row);
+    const RowConst<float> c = row_const<float, kHist>(p, at.row);
+    const GradRow r = grad_row<kHist>(g, c, at.row);
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
       const int64_t j = at.j(k);
       if (j >= p.options) continue;
-      float z[kPer], slope[kPer], dx[kPer], db[kPer];
-      const uint32_t legal = load_z<T, float>(p, c, at.row, j, n ? n + j : nullptr, z, slope);
+      float y[kPer], slope[kPer], dx[kPer], db[kPer];
+      const uint32_t legal = load_y<T, float, kHist>(p, c, at.row, j, kHist ? n + j : nullptr, y, slope);
+      grad_y(r, y, r.empty ? 0u : legal, j, db);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const bool ok = (legal >> i) & 1;
-        db[i] = grad_y(r, z[i], ok, r.act == j + i, c.inv_t) * c.inv_t;
-        dx[i] = ok ? db[i] * slope[i] : 0.f;
+        dx[i] = kHist ? db[i] * slope[i] : db[i];
         sum[k][i] += db[i];
       }
       if (g.grad_logits) store8<T>((T*)g.grad_logits + at.row * g.grad_logits_stride + j, dx, j, p.options, g.vec_out);
@@ -757,9 +845,9 @@ template <class T, int NP> __global__ __launch_bounds__(kThreads) void evaluate_
 }
 
 // a workgroup owns kPiece columns and walks down its rows: the sum of a shared bias' gradient stays in registers
-template <class T>
+template <class T, bool kHist>
 __global__ __launch_bounds__(kThreads) void evaluate_grad_piece(Rows p, GradArgs g, int64_t rows_per_block) {
-  __shared__ uint32_t counts[kPiece];
+  __shared__ uint32_t counts[kHist ? kPiece : 1];
   const int64_t j0 = (int64_t)blockIdx.x * kPiece;
   const int64_t j = j0 + threadIdx.x * kPer;
   const int64_t r0 = (int64_t)blockIdx.y * rows_per_block;
@@ -768,17 +856,16 @@ __global__ __launch_bounds__(kThreads) void evaluate_grad_piece(Rows p, GradArgs
 #pragma unroll
   for (int i = 0; i < kPer; ++i) sum[i] = 0.f;
   for (int64_t row = r0; row < r1; ++row) {
-    const RowConst<float> c = row_const<float>(p, row);
-    const GradRow r = grad_row(g, row);
-    if (p.history) count_piece(p, row, j0, counts);
+    const RowConst<float> c = row_const<float, kHist>(p, row);
+    const GradRow r = grad_row<kHist>(g, c, row);
+    if (kHist) count_piece(p, row, j0, counts);
     if (j >= p.options) continue;
-    float z[kPer], slope[kPer], dx[kPer], db[kPer];
-    const uint32_t legal = load_z<T, float>(p, c, row, j, p.history ? counts + threadIdx.x * kPer : nullptr, z, slope);
+    float y[kPer], slope[kPer], dx[kPer], db[kPer];
+    const uint32_t legal = load_y<T, float, kHist>(p, c, row, j, kHist ? counts + threadIdx.x * kPer : nullptr, y, slope);
+    grad_y(r, y, r.empty ? 0u : legal, j, db);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const bool ok = (legal >> i) & 1;
-      db[i] = grad_y(r, z[i], ok, r.act == j + i, c.inv_t) * c.inv_t;
-      dx[i] = ok ? db[i] * slope[i] : 0.f;
+      dx[i] = kHist ? db[i] * slope[i] : db[i];
       sum[i] += db[i];
     }
     if (g.grad_logits) store8<T>((T*)g.grad_logits + row * g.grad_logits_stride + j, dx, j, p.options, g.vec_out);
