@@ -75,7 +75,8 @@ int check_rows(const ep_policy_rows* r, epp::Rows* k) {
     return (uintptr_t)ptr % 16 == 0 && (r->rows <= 1 || (stride * (int64_t)size) % 16 == 0);
   };
   k->vec = rows16(r->logits, r->logits_stride, size_of(r->dtype)) &&
-           (!r->bias || r->bias_dtype != EP_F32 || rows16(r->bias, r->bias_stride, 4));
+           (!r->bias || r->bias_dtype != EP_F32 || rows16(r->bias, r->bias_stride, 4)) &&
+           (!r->mask || r->mask_dtype == EP_I32 || ((uintptr_t)r->mask % 8 == 0 && (r->rows <= 1 || r->mask_stride % 8 == 0)));
   return EP_OK;
 }
 
@@ -105,6 +106,7 @@ template <class F> void with_kernel(int32_t dtype, bool history, F f) {
 // that about kFill workgroups stand on the chip.
 constexpr int64_t kGroupOptions = 64 * epp::kPer * 4;
 constexpr int64_t kFill = 2048;
+constexpr int64_t kManyOctets = 262144;
 
 struct Width {
   int log, pieces;
@@ -112,8 +114,11 @@ struct Width {
   size_t lds;
 };
 Width group_width(const epp::Rows& k) {
-  Width w{0, k.options <= 64 * epp::kPer ? 1 : 4, 0, 0};
-  const int64_t lanes = (k.options + epp::kPer * w.pieces - 1) / (epp::kPer * w.pieces);
+  const int64_t octets = (k.options + epp::kPer - 1) / epp::kPer;
+  // More pieces a lane mean fewer lanes a row and less work that every lane repeats (one lane for 16 options: no
+  // exchange at all), at half the lanes in flight: for rows that fill the chip anyway
+  Width w{0, octets > 128 ? 4 : octets > 64 || (octets > 1 && k.rows * octets >= kManyOctets) ? 2 : 1, 0, 0};
+  const int64_t lanes = (octets + w.pieces - 1) / w.pieces;
   const int64_t want = std::max<int64_t>(lanes, k.history ? std::min<int64_t>(64, (k.history_len + 15) / 16) : 1);
   while ((1 << w.log) < want) ++w.log;
   const int64_t per = epp::kThreads >> w.log;
@@ -167,6 +172,7 @@ int ep_policy_choose(const ep_policy_rows* r, const void* u, int32_t u_dtype, in
     const size_t lds = k.history ? w.lds : 0;
     with_kernel(r->dtype, k.history, [&](auto t, auto h) {
       if (w.pieces == 1) hipLaunchKernelGGL((epp::choose_group<decltype(t), 1, h.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, u, u_f64, out);
+      else if (w.pieces == 2) hipLaunchKernelGGL((epp::choose_group<decltype(t), 2, h.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, u, u_f64, out);
       else hipLaunchKernelGGL((epp::choose_group<decltype(t), 4, h.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, u, u_f64, out);
     });
   } else {
@@ -203,6 +209,7 @@ int ep_policy_evaluate(const ep_policy_rows* r, const int32_t* action, float* lo
     const size_t lds = k.history ? w.lds : 0;
     with_kernel(r->dtype, k.history, [&](auto t, auto h) {
       if (w.pieces == 1) hipLaunchKernelGGL((epp::evaluate_group<decltype(t), 1, h.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, out);
+      else if (w.pieces == 2) hipLaunchKernelGGL((epp::evaluate_group<decltype(t), 2, h.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, out);
       else hipLaunchKernelGGL((epp::evaluate_group<decltype(t), 4, h.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, out);
     });
   } else {
@@ -258,6 +265,8 @@ int ep_policy_evaluate_grad(const ep_policy_rows* r, const int32_t* action, cons
       const size_t lds = k.history || shared ? w.lds : 0;
       if (group && w.pieces == 1)
         hipLaunchKernelGGL((epp::evaluate_grad_group<decltype(t), 1, h.value>), dim3((unsigned)blocks), dim3(epp::kThreads), lds, stream, k, g, w.log, (int64_t)w.blocks);
+      else if (group && w.pieces == 2)
+        hipLaunchKernelGGL((epp::evaluate_grad_group<decltype(t), 2, h.value>), dim3((unsigned)blocks), dim3(epp::kThreads), lds, stream, k, g, w.log, (int64_t)w.blocks);
       else if (group)
         hipLaunchKernelGGL((epp::evaluate_grad_group<decltype(t), 4, h.value>), dim3((unsigned)blocks), dim3(epp::kThreads), lds, stream, k, g, w.log, (int64_t)w.blocks);
       else
@@ -267,8 +276,13 @@ int ep_policy_evaluate_grad(const ep_policy_rows* r, const int32_t* action, cons
   }
   if (shared) {
     with_type(r->bias_dtype, [&](auto t) {
-      hipLaunchKernelGGL(epp::sum_partials<decltype(t)>, dim3((unsigned)((r->options + 15) / 16)), dim3(epp::kThreads), 0, stream, partial,
-                         r->rows > 0 ? blocks : 0, r->options, (decltype(t)*)grad_bias);
+      // few columns: four a workgroup, so that 64 threads go down each; many: a cache line of them
+      if (r->options <= 1024)
+        hipLaunchKernelGGL((epp::sum_partials<decltype(t), 4>), dim3((unsigned)((r->options + 3) / 4)), dim3(epp::kThreads), 0, stream, partial,
+                           r->rows > 0 ? blocks : 0, r->options, (decltype(t)*)grad_bias);
+      else
+        hipLaunchKernelGGL((epp::sum_partials<decltype(t), 32>), dim3((unsigned)((r->options + 31) / 32)), dim3(epp::kThreads), 0, stream, partial,
+                           r->rows > 0 ? blocks : 0, r->options, (decltype(t)*)grad_bias);
     });
     HIP_TRY(hipGetLastError());
   }

@@ -31,7 +31,7 @@ struct Rows {
   int64_t history_len, history_stride;
   const float *repetition, *frequency, *presence, *temperature;
   double repetition_all, frequency_all, presence_all, temperature_all;
-  int32_t vec;  // logits rows (and biases, if any) start on 8-element boundaries: load 8 at a time
+  int32_t vec;  // rows of logits, 32-bit biases and byte masks start on boundaries of their 8-option loads
 };
 
 constexpr int kThreads = 256;
@@ -44,34 +44,34 @@ constexpr int kPiece = kThreads * kPer;      // options per piece of a row
 template <class R> struct Num;
 template <> struct Num<double> {
   static constexpr double kNone = -1.7976931348623157e308;
-  static constexpr double kUnit = 1.0;        // weights are exp(d kUnit): natural units
-  static constexpr double kFloor = -800.0;    // exp of this and less is 0
+  static constexpr double kUnit = 0.6931471805599453;
+  static constexpr double kFloor = -1100.0;  // 2^d of this and less is 0
 };
 template <> struct Num<float> {
   static constexpr float kNone = -3.40282347e38f;
   static constexpr float kLow = -3.40282326e38f, kHigh = 3.40282326e38f;
-  static constexpr float kUnit = 0.693147181f;  // d counts octaves: the hardware's exponential is 2^d
+  static constexpr float kUnit = 0.693147181f;  // exponents d count octaves, weights are 2^d
   static constexpr float kFloor = -10000.f;
 };
 
-// exp of x in [-800, 0] in 64 bits: x = n ln 2 + r, |r| <= ln 2 / 2, the series of exp r to r^11 (the first term
-// left out is below 7e-15), times 2^n. About two thirds of the library function's instructions: there are no
-// overflows or positive arguments to look after.
-__device__ inline double weight(double x) {
-  const double n = rint(x * 1.4426950408889634);
-  double r = fma(n, -0.6931471805599453, x);  // ln 2 to 53 bits, then what it lacks
-  r = fma(n, -2.3190468138462996e-17, r);
-  double p = 1.0 / 39916800;
-  p = fma(p, r, 1.0 / 3628800);
-  p = fma(p, r, 1.0 / 362880);
-  p = fma(p, r, 1.0 / 40320);
-  p = fma(p, r, 1.0 / 5040);
-  p = fma(p, r, 1.0 / 720);
-  p = fma(p, r, 1.0 / 120);
-  p = fma(p, r, 1.0 / 24);
-  p = fma(p, r, 1.0 / 6);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
+// 2^d for d in [-1100, 0] in 64 bits: d = n + r, |r| <= 1/2, the series of exp(r ln 2) to the 11th power (the first
+// term left out is below 7e-15), times 2^n. Half the library function's instructions: there are no
+// overflows or positive arguments to look after, and the octaves come for free with the factor 1 / t.
+__device__ inline double weight(double d) {
+  constexpr double l = 0.6931471805599453;
+  constexpr double c2 = l * l / 2, c3 = c2 * l / 3, c4 = c3 * l / 4, c5 = c4 * l / 5, c6 = c5 * l / 6, c7 = c6 * l / 7, c8 = c7 * l / 8,
+                   c9 = c8 * l / 9, c10 = c9 * l / 10, c11 = c10 * l / 11;
+  const double n = rint(d), r = d - n;
+  double p = fma(c11, r, c10);
+  p = fma(p, r, c9);
+  p = fma(p, r, c8);
+  p = fma(p, r, c7);
+  p = fma(p, r, c6);
+  p = fma(p, r, c5);
+  p = fma(p, r, c4);
+  p = fma(p, r, c3);
+  p = fma(p, r, c2);
+  p = fma(p, r, l);
   p = fma(p, r, 1.0);
   return __builtin_amdgcn_ldexp(p, (int)n);
 }
@@ -85,7 +85,7 @@ __device__ inline float mul_add(float a, float b, float c) { return __builtin_fm
 
 // what is the same for all options of a row
 template <class R> struct RowConst {
-  R rep, freq, pres, inv_t;
+  R rep, inv_rep, freq, pres, inv_t;
   R k;              // (z - m) * k is a weight's exponent
   int64_t n_legal;  // options below this are legal as far as num_options goes
   bool bad;
@@ -99,6 +99,7 @@ template <class R, bool kHist> __device__ inline RowConst<R> row_const(const Row
   c.bad = !(t > (R)0) || !(t < (R)INFINITY) || !(c.k < (R)INFINITY);
   if (kHist) {
     c.rep = p.repetition ? (R)p.repetition[row] : (R)p.repetition_all;
+    c.inv_rep = (R)1 / c.rep;
     c.freq = p.frequency ? (R)p.frequency[row] : (R)p.frequency_all;
     c.pres = p.presence ? (R)p.presence[row] : (R)p.presence_all;
     c.bad = c.bad || !(c.rep > (R)0);
@@ -129,39 +130,48 @@ template <class T> struct Vec8 {
   alignas(16) T v[8];
 };
 
+// The penalized logits of a row's options that stand in its history: `count` per option, `value` where it is
+// not 0. (A long row's workgroup computes them once per entry: of 2048 options a few dozen have any.)
+template <class R> struct Seen {
+  const uint32_t* count = nullptr;
+  const R* value = nullptr;  // NULL: computed per option from the count
+  __device__ Seen at(int64_t i) const { return {count + i, value ? value + i : nullptr}; }
+};
+
+__device__ inline bool bit(uint32_t bits, int i) { return (bits >> i) & 1u; }
+
 // Options j0 .. j0+7 of a row (j0 a multiple of 8, below the row's end): y before the temperature, as they
 // come. Returns which are legal (bit i = option j0 + i); the y of the others are unspecified.
-// slope: d y / d logit.
+// whole: all eight exist and every operand can be read eight at a time. slope: d y / d logit.
 template <class T, class R, bool kHist>
-__device__ inline uint32_t load_y(const Rows& p, const RowConst<R>& c, int64_t row, int64_t j0, const uint32_t* counts, R (&y)[kPer],
+__device__ inline uint32_t load_y(const Rows& p, const RowConst<R>& c, int64_t row, int64_t j0, bool whole, const Seen<R>& seen, R (&y)[kPer],
                                   R* slope = nullptr) {
   const int64_t left = c.n_legal - j0;
   uint32_t legal = left >= kPer ? 0xffu : left > 0 ? (1u << left) - 1u : 0u;
-  const bool whole = j0 + kPer <= p.options;
   if (p.mask) {
     if (p.mask_bits) {
       legal &= ((const uint32_t*)p.mask)[row * p.mask_stride + (j0 >> 5)] >> (j0 & 31);
     } else {
       const uint8_t* m = (const uint8_t*)p.mask + row * p.mask_stride + j0;
       uint64_t w = 0;
-      if (whole && ((uintptr_t)m & 7) == 0) {
+      if (whole) {
         w = *(const uint64_t*)m;
       } else {
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
           if (j0 + i < p.options) w |= (uint64_t)m[i] << (8 * i);
       }
-      // nonzero bytes to bits: every byte folded onto its lowest bit, the eight of them gathered by a product
+      // nonzero bytes to bits: every byte folded onto its lowest bit, four of them gathered by a product
       w |= w >> 4;
       w |= w >> 2;
       w |= w >> 1;
-      w &= 0x0101010101010101ull;
-      legal &= (uint32_t)((w * 0x0102040810204080ull) >> 56);
+      const uint32_t lo = (uint32_t)w & 0x01010101u, hi = (uint32_t)(w >> 32) & 0x01010101u;
+      legal &= ((lo * 0x01020408u) >> 24) | (((hi * 0x01020408u) >> 24) << 4);
     }
   }
   const T* x = (const T*)p.logits + row * p.logits_stride + j0;
   T xv[kPer];
-  if (p.vec && whole) {
+  if (whole) {
     *(Vec8<T>*)xv = *(const Vec8<T>*)x;
   } else {
 #pragma unroll
@@ -172,16 +182,17 @@ __device__ inline uint32_t load_y(const Rows& p, const RowConst<R>& c, int64_t r
   if (kHist) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const uint32_t n = counts[i];
-      if (slope) slope[i] = n ? (y[i] > (R)0 ? (R)1 / c.rep : c.rep) : (R)1;
-      y[i] = penalized<R>(y[i], n, c);
+      const uint32_t n = seen.count[i];
+      if (slope) slope[i] = n ? (y[i] > (R)0 ? c.inv_rep : c.rep) : (R)1;
+      if (seen.value) y[i] = n ? seen.value[i] : y[i];
+      else y[i] = penalized<R>(y[i], n, c);
     }
   }
   if (p.bias) {
     const int64_t b0 = row * p.bias_stride + j0;
     if (p.bias_f32) {
       const float* b = (const float*)p.bias + b0;
-      if (p.vec && whole) {
+      if (whole) {
         const Vec8<float> v = *(const Vec8<float>*)b;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) y[i] += (R)v.v[i];
@@ -198,11 +209,29 @@ __device__ inline uint32_t load_y(const Rows& p, const RowConst<R>& c, int64_t r
   return legal;
 }
 
-__device__ inline bool bit(uint32_t bits, int i) { return (bits >> i) & 1u; }
+// In 32 bits the sum of finite values may leave the range: the end of it stands for the sum then, so that it
+// is not taken for a logit that was infinite.
+template <class T> __device__ inline float hold_range(const Rows& p, int64_t row, int64_t j, float y) {
+  if (fabsf(y) != INFINITY) return y;
+  const float x = (float)((const T*)p.logits)[row * p.logits_stride + j];
+  float b = 0.f;
+  if (p.bias) {
+    const int64_t at = row * p.bias_stride + j;
+    b = p.bias_f32 ? ((const float*)p.bias)[at] : (float)((const T*)p.bias)[at];
+  }
+  return fabsf(x) < INFINITY && fabsf(b) < INFINITY ? (y > 0.f ? Num<float>::kHigh : Num<float>::kLow) : y;
+}
 
-// The y of `legal` made ready for sums: kNone where there is no weight. Returns whether one of them is NaN or
-// +inf. Nearly always all are finite, which one product with 0 per option shows (0 * inf and 0 * NaN are NaN).
-template <class R> __device__ inline bool ready_y(uint32_t legal, R (&y)[kPer]) {
+// load_y made ready for sums: kNone where there is no weight. Returns whether a legal one is NaN or +inf. Nearly
+// always all are finite, which one product with 0 per option shows (0 * inf and 0 * NaN are NaN).
+template <class T, class R, bool kHist>
+__device__ inline bool load_ready(const Rows& p, const RowConst<R>& c, int64_t row, int64_t j0, bool whole, const Seen<R>& seen, R (&y)[kPer]) {
+  if (j0 >= c.n_legal) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) y[i] = Num<R>::kNone;
+    return false;
+  }
+  const uint32_t legal = load_y<T, R, kHist>(p, c, row, j0, whole, seen, y);
   R odd = (R)0;
   R m = Num<R>::kNone;
 #pragma unroll
@@ -216,47 +245,12 @@ template <class R> __device__ inline bool ready_y(uint32_t legal, R (&y)[kPer]) 
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     if (!bit(legal, i)) continue;
+    if constexpr (sizeof(R) == 4) y[i] = hold_range<T>(p, row, j0 + i, y[i]);
     if (!(y[i] < (R)INFINITY)) bad = true;
-    if constexpr (sizeof(R) == 4) y[i] = y[i] == -INFINITY ? Num<R>::kNone : larger(y[i], Num<R>::kLow);
-    else if (y[i] == -(R)INFINITY) y[i] = Num<R>::kNone;
+    if (y[i] == -(R)INFINITY) y[i] = Num<R>::kNone;
+    else if constexpr (sizeof(R) == 4) y[i] = larger(y[i], Num<float>::kLow);
   }
   return bad;
-}
-
-// In 32 bits the sum of finite values may leave the range: the end of it stands for the sum then, so that it
-// is not taken for a logit that was infinite.
-template <class T, bool kHist>
-__device__ inline void hold_range(const Rows& p, const RowConst<float>& c, int64_t row, int64_t j0, uint32_t legal, float (&y)[kPer]) {
-  float odd = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) odd = mul_add(bit(legal, i) ? y[i] : 0.f, 0.f, odd);
-  if (odd == 0.f || !(p.bias || kHist)) return;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    if (!bit(legal, i) || fabsf(y[i]) != INFINITY) continue;
-    const float x = (float)((const T*)p.logits)[row * p.logits_stride + j0 + i];
-    float b = 0.f;
-    if (p.bias) {
-      const int64_t at = row * p.bias_stride + j0 + i;
-      b = p.bias_f32 ? ((const float*)p.bias)[at] : (float)((const T*)p.bias)[at];
-    }
-    if (fabsf(x) < INFINITY && fabsf(b) < INFINITY) y[i] = y[i] > 0.f ? Num<float>::kHigh : Num<float>::kLow;
-  }
-}
-template <class T, bool kHist>
-__device__ inline void hold_range(const Rows&, const RowConst<double>&, int64_t, int64_t, uint32_t, double (&)[kPer]) {}
-
-// load_y, hold_range and ready_y in one
-template <class T, class R, bool kHist>
-__device__ inline bool load_ready(const Rows& p, const RowConst<R>& c, int64_t row, int64_t j0, const uint32_t* counts, R (&y)[kPer]) {
-  if (j0 >= c.n_legal) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) y[i] = Num<R>::kNone;
-    return false;
-  }
-  const uint32_t legal = load_y<T, R, kHist>(p, c, row, j0, counts, y);
-  hold_range<T, kHist>(p, c, row, j0, legal, y);
-  return ready_y(legal, y);
 }
 
 // running statistics of a row, or of a part of it
@@ -350,18 +344,40 @@ template <class R> __device__ inline Stat<R> stat_block(Stat<R> a, R k, Stat<R>*
   return r;
 }
 
-// how often each option of [j0, j0 + kPiece) stands in the row's history
-__device__ inline void count_piece(const Rows& p, int64_t row, int64_t j0, uint32_t* counts) {
+// the options [j0, j0 + kPiece) of a row that stand in its history: counts and penalized logits
+template <class T, class R> struct SeenPiece {
+  uint32_t count[kPiece];
+  R value[kPiece];
+  uint16_t list[kPiece];
+  int n;
+};
+template <class T, class R>
+__device__ inline Seen<R> count_piece(const Rows& p, const RowConst<R>& c, int64_t row, int64_t j0, SeenPiece<T, R>& s) {
   __syncthreads();
-  for (int i = threadIdx.x; i < kPiece; i += kThreads) counts[i] = 0;
+  for (int i = threadIdx.x; i < kPiece; i += kThreads) s.count[i] = 0;
+  if (threadIdx.x == 0) s.n = 0;
   __syncthreads();
   const int32_t* h = p.history + row * p.history_stride;
+  const uint32_t size = (uint32_t)min((int64_t)kPiece, p.options - j0);
   for (int64_t i = threadIdx.x; i < p.history_len; i += kThreads) {
-    const int64_t j = h[i];
-    if (j >= j0 && j < j0 + kPiece && j < p.options) atomicAdd(&counts[j - j0], 1u);
+    const uint32_t j = (uint32_t)h[i] - (uint32_t)j0;
+    if (j < size && atomicAdd(&s.count[j], 1u) == 0) s.list[atomicAdd(&s.n, 1)] = (uint16_t)j;
   }
   __syncthreads();
+  for (int i = threadIdx.x; i < s.n; i += kThreads) {
+    const int j = s.list[i];
+    s.value[j] = penalized<R>((R)(float)((const T*)p.logits)[row * p.logits_stride + j0 + j], s.count[j], c);
+  }
+  __syncthreads();
+  return {s.count, s.value};
 }
+template <class T, class R, bool kHist> struct PieceMemory {
+  SeenPiece<T, R> s;
+  __device__ Seen<R> count(const Rows& p, const RowConst<R>& c, int64_t row, int64_t j0) { return count_piece<T, R>(p, c, row, j0, s).at(threadIdx.x * kPer); }
+};
+template <class T, class R> struct PieceMemory<T, R, false> {
+  __device__ Seen<R> count(const Rows&, const RowConst<R>&, int64_t, int64_t) { return {}; }
+};
 
 template <class R> __device__ inline R quiet_nan() { return (R)__builtin_nanf(""); }
 
@@ -375,8 +391,8 @@ __device__ inline void finish_choose(const ChooseOut& o, int64_t row, const Stat
   const bool empty = !bad && a.m == Num<double>::kNone;
   const double log_s = log(a.s);
   o.action[row] = bad || empty ? -1 : (int32_t)pick;
-  o.log_prob[row] = bad ? quiet_nan<float>() : empty ? 0.f : (float)((y_pick - a.m) * c.k - log_s);
-  o.entropy[row] = bad ? quiet_nan<float>() : empty ? 0.f : (float)(log_s - a.e / a.s);
+  o.log_prob[row] = bad ? quiet_nan<float>() : empty ? 0.f : (float)((y_pick - a.m) * c.inv_t - log_s);
+  o.entropy[row] = bad ? quiet_nan<float>() : empty ? 0.f : (float)(log_s - a.e / a.s * Num<double>::kUnit);
 }
 
 struct EvaluateOut {
@@ -438,11 +454,12 @@ __global__ __launch_bounds__(kThreads) void choose_group(Rows p, int width_log, 
   const Group g = group_of(p, blockIdx.x, width_log);
   const RowConst<double> c = row_const<double, kHist>(p, g.row);
   const uint32_t* n = kHist ? count_groups<NP>(p, g, counts) : nullptr;
+  const bool whole = p.vec && p.options % kPer == 0;
   double y[NP][kPer];
   Stat<double> a = stat_zero<double>();
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    a.bad |= load_ready<T, double, kHist>(p, c, g.row, g.j(k), kHist ? n + g.j(k) : nullptr, y[k]);
+    a.bad |= load_ready<T, double, kHist>(p, c, g.row, g.j(k), whole, Seen<double>{n}.at(kHist ? g.j(k) : 0), y[k]);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) a.m = larger(a.m, y[k][i]);
   }
@@ -516,13 +533,14 @@ template <class T, int NP, bool kHist> __global__ __launch_bounds__(kThreads) vo
   const Group g = group_of(p, blockIdx.x, width_log);
   const RowConst<float> c = row_const<float, kHist>(p, g.row);
   const uint32_t* n = kHist ? count_groups<NP>(p, g, counts) : nullptr;
+  const bool whole = p.vec && p.options % kPer == 0;
   const int32_t act = out.action[g.row];
   float y[NP][kPer];
   Stat<float> a = stat_zero<float>();
   float y_act = Num<float>::kNone;
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    a.bad |= load_ready<T, float, kHist>(p, c, g.row, g.j(k), kHist ? n + g.j(k) : nullptr, y[k]);
+    a.bad |= load_ready<T, float, kHist>(p, c, g.row, g.j(k), whole, Seen<float>{n}.at(kHist ? g.j(k) : 0), y[k]);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       a.m = larger(a.m, y[k][i]);
@@ -549,17 +567,17 @@ template <class T, int NP, bool kHist> __global__ __launch_bounds__(kThreads) vo
 // ---- longer rows: a workgroup per part of a row (`pieces` pieces of kPiece options), parts joined after ---
 template <class T, bool kHist, bool kBest>
 __global__ __launch_bounds__(kThreads) void choose_parts(Rows p, int pieces, int n_parts, Stat<double>* parts) {
-  __shared__ uint32_t counts[kHist ? kPiece : 1];
+  __shared__ PieceMemory<T, double, kHist> mem;
   __shared__ Stat<double> red[kThreads / 64];
   const int64_t row = blockIdx.x / n_parts, part = blockIdx.x % n_parts;
   const RowConst<double> c = row_const<double, kHist>(p, row);
   Stat<double> a = stat_zero<double>();
   const int64_t j_end = min((part + 1) * pieces * (int64_t)kPiece, c.n_legal);
   for (int64_t j0 = part * pieces * (int64_t)kPiece; j0 < j_end; j0 += kPiece) {
-    if (kHist) count_piece(p, row, j0, counts);
+    const auto seen = mem.count(p, c, row, j0);
     const int64_t j = j0 + threadIdx.x * kPer;
     double y[kPer];
-    a.bad |= load_ready<T, double, kHist>(p, c, row, j, kHist ? counts + threadIdx.x * kPer : nullptr, y);
+    a.bad |= load_ready<T, double, kHist>(p, c, row, j, p.vec && j0 + kPiece <= p.options, seen, y);
     stat_add<double, kBest>(a, y, j, c.k);
   }
   a = stat_block(a, c.k, red);
@@ -569,7 +587,7 @@ __global__ __launch_bounds__(kThreads) void choose_parts(Rows p, int pieces, int
 // joins a row's parts, and finds the option that u falls on by walking down the one part it lies in
 template <class T, bool kHist>
 __global__ __launch_bounds__(kThreads) void choose_join(Rows p, int pieces, int n_parts, const Stat<double>* all_parts, const void* u, int u_f64, ChooseOut out) {
-  __shared__ uint32_t counts[kHist ? kPiece : 1];
+  __shared__ PieceMemory<T, double, kHist> mem;
   __shared__ Stat<double> red[kThreads / 64];
   __shared__ double wave_sum[kThreads / 64];
   __shared__ long long found;
@@ -626,10 +644,10 @@ __global__ __launch_bounds__(kThreads) void choose_join(Rows p, int pieces, int 
     double last_y = 0;
     const int64_t j_first = part_at * (int64_t)pieces * kPiece, j_end = min(j_first + pieces * (int64_t)kPiece, c.n_legal);
     for (int64_t j0 = j_first; j0 < j_end; j0 += kPiece) {
-      if (kHist) count_piece(p, row, j0, counts);
+      const auto seen = mem.count(p, c, row, j0);
       const int64_t j = j0 + threadIdx.x * kPer;
       double y[kPer], w[kPer], sum = 0;
-      (void)load_ready<T, double, kHist>(p, c, row, j, kHist ? counts + threadIdx.x * kPer : nullptr, y);
+      (void)load_ready<T, double, kHist>(p, c, row, j, p.vec && j0 + kPiece <= p.options, seen, y);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         w[i] = weight(exponent(y[i], a.m, c.k));
@@ -679,7 +697,7 @@ struct EvaluatePart {
 };
 template <class T, bool kHist>
 __global__ __launch_bounds__(kThreads) void evaluate_parts(Rows p, int pieces, int n_parts, EvaluatePart* parts, EvaluateOut out) {
-  __shared__ uint32_t counts[kHist ? kPiece : 1];
+  __shared__ PieceMemory<T, float, kHist> mem;
   __shared__ Stat<float> red[kThreads / 64];
   __shared__ float y_act;
   const int64_t row = blockIdx.x / n_parts, part = blockIdx.x % n_parts;
@@ -690,10 +708,10 @@ __global__ __launch_bounds__(kThreads) void evaluate_parts(Rows p, int pieces, i
   __syncthreads();
   const int64_t j_end = min((part + 1) * pieces * (int64_t)kPiece, c.n_legal);
   for (int64_t j0 = part * pieces * (int64_t)kPiece; j0 < j_end; j0 += kPiece) {
-    if (kHist) count_piece(p, row, j0, counts);
+    const auto seen = mem.count(p, c, row, j0);
     const int64_t j = j0 + threadIdx.x * kPer;
     float y[kPer];
-    a.bad |= load_ready<T, float, kHist>(p, c, row, j, kHist ? counts + threadIdx.x * kPer : nullptr, y);
+    a.bad |= load_ready<T, float, kHist>(p, c, row, j, p.vec && j0 + kPiece <= p.options, seen, y);
     stat_add<float, false>(a, y, j, c.k);
     if ((uint64_t)(act - j) < kPer) {
 #pragma unroll
@@ -804,6 +822,7 @@ template <class T, int NP, bool kHist> __global__ __launch_bounds__(kThreads) vo
   for (int64_t b = blockIdx.x; b < blocks_of_rows; b += gridDim.x) {
     const Group at = group_of(p, b, width_log);
     const uint32_t* n = kHist ? count_groups<NP>(p, at, counts) : nullptr;
+    const bool whole = p.vec && p.options % kPer == 0;
     if (!at.there) continue;
     const RowConst<float> c = row_const<float, kHist>(p, at.row);
     const GradRow r = grad_row<kHist>(g, c, at.row);
@@ -812,7 +831,7 @@ template <class T, int NP, bool kHist> __global__ __launch_bounds__(kThreads) vo
       const int64_t j = at.j(k);
       if (j >= p.options) continue;
       float y[kPer], slope[kPer], dx[kPer], db[kPer];
-      const uint32_t legal = load_y<T, float, kHist>(p, c, at.row, j, kHist ? n + j : nullptr, y, slope);
+      const uint32_t legal = load_y<T, float, kHist>(p, c, at.row, j, whole, Seen<float>{n}.at(kHist ? j : 0), y, slope);
       grad_y(r, y, r.empty ? 0u : legal, j, db);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
@@ -847,7 +866,7 @@ template <class T, int NP, bool kHist> __global__ __launch_bounds__(kThreads) vo
 // a workgroup owns kPiece columns and walks down its rows: the sum of a shared bias' gradient stays in registers
 template <class T, bool kHist>
 __global__ __launch_bounds__(kThreads) void evaluate_grad_piece(Rows p, GradArgs g, int64_t rows_per_block) {
-  __shared__ uint32_t counts[kHist ? kPiece : 1];
+  __shared__ PieceMemory<T, float, kHist> mem;
   const int64_t j0 = (int64_t)blockIdx.x * kPiece;
   const int64_t j = j0 + threadIdx.x * kPer;
   const int64_t r0 = (int64_t)blockIdx.y * rows_per_block;
@@ -858,10 +877,10 @@ __global__ __launch_bounds__(kThreads) void evaluate_grad_piece(Rows p, GradArgs
   for (int64_t row = r0; row < r1; ++row) {
     const RowConst<float> c = row_const<float, kHist>(p, row);
     const GradRow r = grad_row<kHist>(g, c, row);
-    if (kHist) count_piece(p, row, j0, counts);
+    const auto seen = mem.count(p, c, row, j0);
     if (j >= p.options) continue;
     float y[kPer], slope[kPer], dx[kPer], db[kPer];
-    const uint32_t legal = load_y<T, float, kHist>(p, c, row, j, kHist ? counts + threadIdx.x * kPer : nullptr, y, slope);
+    const uint32_t legal = load_y<T, float, kHist>(p, c, row, j, p.vec && j0 + kPiece <= p.options, seen, y, slope);
     grad_y(r, y, r.empty ? 0u : legal, j, db);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -883,21 +902,27 @@ __global__ __launch_bounds__(kThreads) void evaluate_grad_piece(Rows p, GradArgs
   }
 }
 
-// column sums of partial [n][options], in order of the rows
-template <class T>
+// column sums of partial [n][options], in a fixed order: kCols columns a workgroup, the other threads down the rows
+template <class T, int kCols>
 __global__ __launch_bounds__(kThreads) void sum_partials(const float* partial, int64_t n, int64_t options, T* out) {
   __shared__ float red[kThreads];
-  // 16 columns a workgroup, 16 threads down each
-  const int64_t j = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
-  float s = 0.f;
-  if (j < options)
-    for (int64_t i = threadIdx.x >> 4; i < n; i += kThreads / 16) s += partial[i * options + j];
-  red[threadIdx.x] = s;
-  __syncthreads();
-  if (threadIdx.x < 16 && j < options) {
-    for (int i = 1; i < kThreads / 16; ++i) s += red[threadIdx.x + 16 * i];
-    out[j] = (T)s;
+  constexpr int kDown = kThreads / kCols;
+  const int64_t j = (int64_t)blockIdx.x * kCols + threadIdx.x % kCols;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (j < options) {
+    int64_t i = threadIdx.x / kCols;
+    for (; i + 3 * kDown < n; i += 4 * kDown)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) s[q] += partial[(i + q * kDown) * options + j];
+    for (; i < n; i += kDown) s[0] += partial[i * options + j];
   }
+  red[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  for (int o = kDown / 2; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o * kCols) red[threadIdx.x] += red[threadIdx.x + o * kCols];
+    __syncthreads();
+  }
+  if (threadIdx.x < kCols && j < options) out[j] = (T)red[threadIdx.x];
 }
 
 }  // namespace epp
