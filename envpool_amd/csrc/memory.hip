@@ -127,6 +127,7 @@ int ep_memory_step(const ep_memory_step_args* a) {
     if ((uintptr_t)ptr % 4) return fail(EP_ERR_INVALID, "an array of 4-byte values is not aligned to 4 bytes");
   if (int rc = check_workspace(a->workspace, a->workspace_bytes, step_workspace(a))) return rc;
   if (a->rows == 0) return EP_OK;
+  if (a->rows * a->heads > 4 * (int64_t)INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld rows of %d heads", (long long)a->rows, a->heads);
   EP_ENTER_DEVICE(a->device_id);
   const hipStream_t stream = (hipStream_t)a->stream;
   epm::Step k{};
@@ -145,8 +146,11 @@ int ep_memory_step(const ep_memory_step_args* a) {
     hipLaunchKernelGGL(epm::count_claims, grid, dim3(256), 0, stream, k);
     HIP_TRY(hipGetLastError());
   }
+  const int64_t blocks = (a->rows * a->heads + 3) / 4;
+  const bool four = a->value_dim % 4 == 0 && (uintptr_t)a->state % 16 == 0;  // states in 16-byte pieces
   with_type(a->dtype, [&](auto t) {
-    hipLaunchKernelGGL(epm::step_row<decltype(t)>, dim3((unsigned)std::min<int64_t>(a->rows, 1 << 20), (unsigned)a->heads), dim3(256), 0, stream, k);
+    if (four) hipLaunchKernelGGL((epm::step_rows<decltype(t), 4>), dim3((unsigned)blocks), dim3(256), 0, stream, k);
+    else hipLaunchKernelGGL((epm::step_rows<decltype(t), 1>), dim3((unsigned)blocks), dim3(256), 0, stream, k);
   });
   HIP_TRY(hipGetLastError());
   return EP_OK;

@@ -45,67 +45,122 @@ __global__ __launch_bounds__(256) void count_claims(Step p) {
   if (e >= 0 && e < p.num_envs) atomicAdd(&p.claims[e], 1);
 }
 
-// One workgroup per (row, head): thread = (value column, key part). Rows of one env are stepped by the
-// workgroup of the first of them, in order.
-template <class T> __global__ __launch_bounds__(256) void step_row(Step p) {
-  __shared__ float qs[256], ks[256];
-  __shared__ float part[256];
-  __shared__ int earlier, again;
-  const int h = blockIdx.y;
-  const float decay = expf(p.log_decay[h]);
-  for (int64_t row0 = blockIdx.x; row0 < p.rows; row0 += gridDim.x) {
-    const int64_t id = p.env_id ? p.env_id[row0] : row0 + p.env_id_offset;
-    const int64_t e = id - p.env_id_offset;
-    if (e < 0 || e >= p.num_envs) {
-      if (threadIdx.x == 0 && h == 0 && p.error) *p.error = 1;
-      for (int j = threadIdx.x; j < p.dv; j += 256)
-        ((T*)p.out)[row0 * p.out_stride[0] + h * p.out_stride[1] + j] = (T)__builtin_nanf("");
-      continue;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) earlier = again = 0;
-    __syncthreads();
-    if (p.env_id && (!p.claims || p.claims[e] > 1)) {
-      for (int64_t r = threadIdx.x; r < p.rows; r += 256)
-        if (r != row0 && p.env_id[r] == id) {
-          if (r < row0) earlier = 1;
-          else again = 1;
-        }
-    }
-    __syncthreads();
-    if (earlier) continue;
-    float* s = p.state + (e * p.heads + h) * (int64_t)p.dk * p.dv;
-    const bool repeats = again != 0;
-    for (int64_t row = row0; row < p.rows; ++row) {
-      if (row > row0 && p.env_id[row] != id) continue;
-      const float keep = starts(p, row) ? 0.f : decay;
-      const T* q = (const T*)p.q + row * p.q_stride[0] + h * p.q_stride[1];
-      const T* k = (const T*)p.k + row * p.k_stride[0] + (h / p.kv_group) * p.k_stride[1];
-      const T* v = (const T*)p.v + row * p.v_stride[0] + (h / p.kv_group) * p.v_stride[1];
-      __syncthreads();
-      for (int i = threadIdx.x; i < p.dk; i += 256) qs[i] = (float)q[i], ks[i] = (float)k[i];
-      __syncthreads();
-      for (int j0 = 0; j0 < p.dv; j0 += 64) {
-        const int j = j0 + (threadIdx.x & 63);
-        float acc = 0.f;
-        if (j < p.dv) {
-          const float vj = (float)v[j];
-          for (int i = threadIdx.x >> 6; i < p.dk; i += 4) {
-            const float old = s[i * p.dv + j];
-            const float now = (keep == 0.f ? 0.f : keep * old) + ks[i] * vj;
-            s[i * p.dv + j] = now;
-            acc += qs[i] * now;
-          }
-        }
-        __syncthreads();
-        part[threadIdx.x] = acc;
-        __syncthreads();
-        if (threadIdx.x < 64 && j < p.dv)
-          ((T*)p.out)[row * p.out_stride[0] + h * p.out_stride[1] + j] =
-              (T)(p.scale * (part[threadIdx.x] + part[threadIdx.x + 64] + part[threadIdx.x + 128] + part[threadIdx.x + 192]));
+// One wave per (row, head) streams the state through its registers: a lane holds kVec neighbouring value columns
+// and walks down the keys, 64 / (lanes per key row) keys an instruction, so that a load instruction of the wave
+// is one contiguous stretch. Nothing is read twice; HBM bounds it (8 bytes moved per 5 flops), so what matters
+// is bytes in flight: kAhead loads per lane before the first is used. State loads and stores bypass the caches'
+// retention (a step touches each value once).
+constexpr int kAhead = 8;
+// orders a wave's LDS accesses across its lanes (the hardware keeps them in order; this tells the compiler)
+__device__ inline void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+template <int kVec> struct Piece {
+  typedef float type __attribute__((ext_vector_type(kVec)));
+};
+template <> struct Piece<1> {
+  typedef float type;
+};
+
+template <class T, int kVec> __device__ inline void step_one(const Step& p, int64_t row, int64_t e, int h, float decay, float* qs, float* ks, float* red) {
+  using V = typename Piece<kVec>::type;
+  const int lane = threadIdx.x & 63;
+  const bool drop = starts(p, row);
+  const T* q = (const T*)p.q + row * p.q_stride[0] + h * p.q_stride[1];
+  const T* k = (const T*)p.k + row * p.k_stride[0] + (h / p.kv_group) * p.k_stride[1];
+  const T* v = (const T*)p.v + row * p.v_stride[0] + (h / p.kv_group) * p.v_stride[1];
+  T* out = (T*)p.out + row * p.out_stride[0] + h * p.out_stride[1];
+  float* state = p.state + (e * p.heads + h) * (int64_t)p.dk * p.dv;
+  wave_sync();
+  for (int i = lane; i < p.dk; i += 64) qs[i] = (float)q[i] * p.scale, ks[i] = (float)k[i];
+  wave_sync();
+  const int columns = (p.dv + kVec - 1) / kVec;  // of kVec values (dv is a multiple of it)
+  for (int c0 = 0; c0 < columns; c0 += 64) {
+    const int width = columns - c0 < 64 ? columns - c0 : 64;
+    const int down = 64 / width;  // keys per instruction
+    const int c = c0 + lane % width, d0 = lane / width;
+    const bool on = d0 < down;
+    float* s = state + c * kVec;
+    V vv;
+    if constexpr (kVec == 1) vv = on ? (float)v[c] : 0.f;
+    else
+#pragma unroll
+      for (int r = 0; r < kVec; ++r) vv[r] = on ? (float)v[c * kVec + r] : 0.f;
+    V acc = (V)0.f;
+    for (int i0 = on ? d0 : p.dk; i0 < p.dk; i0 += down * kAhead) {
+      V old[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int d = i0 + i * down;
+        old[i] = (V)0.f;
+        if (d < p.dk && !drop) old[i] = __builtin_nontemporal_load((const V*)(s + (int64_t)d * p.dv));
       }
-      __syncthreads();
-      if (!repeats) break;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int d = i0 + i * down;
+        if (d < p.dk) {
+          const V now = old[i] * decay + ks[d] * vv;
+          __builtin_nontemporal_store(now, (V*)(s + (int64_t)d * p.dv));
+          acc += qs[d] * now;
+        }
+      }
+    }
+    // the sums over the keys: `down` lanes apart by `width`
+    wave_sync();
+#pragma unroll
+    for (int r = 0; r < kVec; ++r) {
+      if constexpr (kVec == 1) red[lane] = acc;
+      else red[r * 64 + lane] = acc[r];
+    }
+    wave_sync();
+    if (lane < width) {
+#pragma unroll
+      for (int r = 0; r < kVec; ++r) {
+        float sum = 0.f;
+        for (int i = 0; i < down; ++i) sum += red[r * 64 + i * width + lane];
+        out[c * kVec + r] = (T)sum;
+      }
+    }
+  }
+}
+
+// Rows of one env are stepped by the wave of the first of them, in order.
+template <class T, int kVec> __global__ __launch_bounds__(256) void step_rows(Step p) {
+  __shared__ float lds[4][256 + 256 + 64 * kVec];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float *qs = lds[wave], *ks = qs + 256, *red = ks + 256;  // a wave's own: its LDS operations are in order
+  const int64_t item = (int64_t)blockIdx.x * 4 + wave;
+  if (item >= p.rows * p.heads) return;
+  const int64_t row0 = item / p.heads;
+  const int h = (int)(item % p.heads);
+  const float decay = expf(p.log_decay[h]);
+  const int64_t id = p.env_id ? p.env_id[row0] : row0 + p.env_id_offset;
+  const int64_t e = id - p.env_id_offset;
+  if (e < 0 || e >= p.num_envs) {
+    if (lane == 0 && h == 0 && p.error) *p.error = 1;
+    for (int j = lane; j < p.dv; j += 64) ((T*)p.out)[row0 * p.out_stride[0] + h * p.out_stride[1] + j] = (T)__builtin_nanf("");
+    return;
+  }
+  int again = 0;
+  if (p.env_id && (!p.claims || p.claims[e] > 1)) {
+    int earlier = 0;
+    for (int64_t r = lane; r < p.rows; r += 64)
+      if (p.env_id[r] == id) {
+        if (r < row0) earlier = 1;
+        if (r > row0) again = 1;
+      }
+    if (__any(earlier)) return;
+    again = __any(again);
+  }
+  step_one<T, kVec>(p, row0, e, h, decay, qs, ks, red);
+  if (!again) return;
+  for (int64_t base = row0 / 64 * 64; base < p.rows; base += 64) {
+    uint64_t hits = __ballot(base + lane < p.rows && base + lane > row0 && p.env_id[base + lane] == id);
+    for (; hits; hits &= hits - 1) {
+      __threadfence_block();  // (the state written for the row before is read again)
+      step_one<T, kVec>(p, base + __ffsll((unsigned long long)hits) - 1, e, h, decay, qs, ks, red);
     }
   }
 }

@@ -164,6 +164,12 @@ def choose(logits, u=None, *, num_options=None, mask=None, bias=None, history=No
     return Choice(action, log_prob, entropy)
 
 
+def _run_backward(plain, once, ctx, *grads):
+  """A backward pass whose results are not differentiable again: torch's wrapper that says so costs more than
+  a small pass and is only needed where a graph of the backward pass is asked for."""
+  return once(ctx, *grads) if torch.is_grad_enabled() else plain(ctx, *grads)
+
+
 def _evaluate_forward(p, action):
   log_prob = torch.empty(p.n, dtype=torch.float32, device=p.dev)
   entropy = torch.empty(p.n, dtype=torch.float32, device=p.dev)
@@ -171,6 +177,26 @@ def _evaluate_forward(p, action):
   ws, ws_ptr, ws_bytes = _scratch(p.native.evaluate_workspace(), p.dev)
   p.native.evaluate(action.data_ptr(), log_prob.data_ptr(), entropy.data_ptr(), stats.data_ptr(), ws_ptr, ws_bytes)
   return log_prob, entropy, stats
+
+
+def _evaluate_backward(ctx, g_lp, g_h):
+  p = ctx.p
+  logits, bias, action, entropy, stats = ctx.saved_tensors[:5]  # (unpacking checks the versions of all that were saved)
+  want_x, want_b = ctx.needs_input_grad[:2]
+  if g_lp is None and g_h is None:
+    return None, None, None, None
+  g_lp = None if g_lp is None else g_lp.contiguous()
+  g_h = None if g_h is None else g_h.contiguous()
+  grad_x = torch.empty_like(logits, memory_format=torch.contiguous_format) if want_x else None
+  grad_b, stride = None, 0
+  if want_b:
+    grad_b = torch.empty(p.bias.shape if p.bias_stride else (p.options,), dtype=bias.dtype, device=p.dev)
+    stride = p.options if p.bias_stride else 0
+  ws, ws_ptr, ws_bytes = _scratch(p.native.grad_workspace(want_b), p.dev)
+  p.native.evaluate_grad(action.data_ptr(), entropy.data_ptr(), stats.data_ptr(), 0 if g_lp is None else g_lp.data_ptr(),
+                         0 if g_h is None else g_h.data_ptr(), 0 if grad_x is None else grad_x.data_ptr(), p.options,
+                         0 if grad_b is None else grad_b.data_ptr(), stride, ws_ptr, ws_bytes, current_stream_handle(p.dev))
+  return grad_x, None if grad_b is None else grad_b.view(bias.shape), None, None
 
 
 class _Evaluate(torch.autograd.Function):
@@ -181,30 +207,16 @@ class _Evaluate(torch.autograd.Function):
     ctx.set_materialize_grads(False)
     # (the native struct holds addresses: every tensor behind it is saved, so that torch notices one that was
     # changed in place before the backward pass)
-    ctx.save_for_backward(logits, bias, action, entropy, stats, p.logits, p.bias, *p.keep)
+    ctx.save_for_backward(logits, bias, action, entropy, stats, *[t for t in (p.logits, p.bias, *p.keep) if t is not None])
     ctx.p = p
     return log_prob, entropy
 
   @staticmethod
-  @torch.autograd.function.once_differentiable
   def backward(ctx, g_lp, g_h):
-    p = ctx.p
-    logits, bias, action, entropy, stats = ctx.saved_tensors[:5]
-    want_x, want_b = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-    if g_lp is None and g_h is None:
-      return None, None, None, None
-    g_lp = None if g_lp is None else g_lp.contiguous()
-    g_h = None if g_h is None else g_h.contiguous()
-    grad_x = torch.empty(p.n, p.options, dtype=logits.dtype, device=p.dev) if want_x else None
-    grad_b, stride = None, 0
-    if want_b:
-      grad_b = torch.empty(p.bias.shape if p.bias_stride else (p.options,), dtype=bias.dtype, device=p.dev)
-      stride = p.options if p.bias_stride else 0
-    ws, ws_ptr, ws_bytes = _scratch(p.native.grad_workspace(want_b), p.dev)
-    p.native.evaluate_grad(action.data_ptr(), entropy.data_ptr(), stats.data_ptr(), 0 if g_lp is None else g_lp.data_ptr(),
-                           0 if g_h is None else g_h.data_ptr(), 0 if grad_x is None else grad_x.data_ptr(), p.options,
-                           0 if grad_b is None else grad_b.data_ptr(), stride, ws_ptr, ws_bytes, current_stream_handle(p.dev))
-    return grad_x, None if grad_b is None else grad_b.view(bias.shape), None, None
+    return _run_backward(_evaluate_backward, _evaluate_backward_once, ctx, g_lp, g_h)
+
+
+_evaluate_backward_once = torch.autograd.function.once_differentiable(_evaluate_backward)
 
 
 def evaluate(logits, action, *, num_options=None, mask=None, bias=None, history=None, repetition=1.0, frequency=0.0, presence=0.0, temperature=1.0):
@@ -356,6 +368,45 @@ def _scan_forward(q, k, v, state, log_decay, fresh, scale):
   return out, final
 
 
+def _scan_backward(ctx, g_out, g_final):
+  q, k, v, state, log_decay, fresh = ctx.saved_tensors
+  t, n, h, dk = q.shape
+  dv, hk = v.shape[3], k.shape[2]
+  group, scale = h // hk, ctx.scale
+  if g_out is None and g_final is None:
+    return (None,) * 7
+  g_out = torch.zeros(t, n, h, dv, dtype=q.dtype, device=q.device) if g_out is None else _dense_last(g_out)
+  want_q, want_k, want_v, want_s = ctx.needs_input_grad[:4]
+  grad_q = grad_k = grad_v = grad_s = None
+  if want_q:
+    grad_q = torch.empty(t, n, h, dk, dtype=q.dtype, device=q.device)
+    _scan_call((t, n, h, dv, dk), log_decay, fresh, g_out, 1, v, group, k, group, grad_q, state, None, 1.0, scale, False, True)
+
+  def per_head(dim):  # heads that share keys and values: their gradients in 32 bits first, then summed
+    return torch.empty(t, n, h, dim, dtype=q.dtype if group == 1 else torch.float32, device=q.device)
+
+  def summed(x, dim):
+    if group == 1:
+      return x
+    y = torch.empty(t, n, hk, dim, dtype=q.dtype, device=q.device)
+    _native.sum_heads(q.device.index, x.data_ptr(), t * n, hk, group, dim, y.data_ptr(), _FLOATS[q.dtype], current_stream_handle(q.device))
+    return y
+
+  if want_k:
+    grad_k = per_head(dk)
+    _scan_call((t, n, h, dv, dk), log_decay, fresh, v, group, g_out, 1, q, 1, grad_k, g_final, None, scale, 1.0, True, True)
+    grad_k = summed(grad_k, dk)
+  if want_v or want_s:
+    grad_v = per_head(dv) if want_v else None
+    grad_s = torch.empty(n, h, dk, dv, dtype=torch.float32, device=q.device) if want_s else None
+    _scan_call((t, n, h, dk, dv), log_decay, fresh, k, group, q, 1, g_out, 1, grad_v, g_final, grad_s, scale, 1.0, True, False)
+    grad_v = summed(grad_v, dv) if want_v else None
+  return grad_q, grad_k, grad_v, grad_s, None, None, None
+
+
+_scan_backward_once = torch.autograd.function.once_differentiable(_scan_backward)
+
+
 class _MemoryScan(torch.autograd.Function):
 
   @staticmethod
@@ -366,41 +417,8 @@ class _MemoryScan(torch.autograd.Function):
     return _scan_forward(q, k, v, state, log_decay, fresh, scale)
 
   @staticmethod
-  @torch.autograd.function.once_differentiable
   def backward(ctx, g_out, g_final):
-    q, k, v, state, log_decay, fresh = ctx.saved_tensors
-    t, n, h, dk = q.shape
-    dv, hk = v.shape[3], k.shape[2]
-    group, scale = h // hk, ctx.scale
-    if g_out is None and g_final is None:
-      return (None,) * 7
-    g_out = torch.zeros(t, n, h, dv, dtype=q.dtype, device=q.device) if g_out is None else _dense_last(g_out)
-    want_q, want_k, want_v, want_s = ctx.needs_input_grad[:4]
-    grad_q = grad_k = grad_v = grad_s = None
-    if want_q:
-      grad_q = torch.empty(t, n, h, dk, dtype=q.dtype, device=q.device)
-      _scan_call((t, n, h, dv, dk), log_decay, fresh, g_out, 1, v, group, k, group, grad_q, state, None, 1.0, scale, False, True)
-
-    def per_head(dim):  # heads that share keys and values: their gradients in 32 bits first, then summed
-      return torch.empty(t, n, h, dim, dtype=q.dtype if group == 1 else torch.float32, device=q.device)
-
-    def summed(x, dim):
-      if group == 1:
-        return x
-      y = torch.empty(t, n, hk, dim, dtype=q.dtype, device=q.device)
-      _native.sum_heads(q.device.index, x.data_ptr(), t * n, hk, group, dim, y.data_ptr(), _FLOATS[q.dtype], current_stream_handle(q.device))
-      return y
-
-    if want_k:
-      grad_k = per_head(dk)
-      _scan_call((t, n, h, dv, dk), log_decay, fresh, v, group, g_out, 1, q, 1, grad_k, g_final, None, scale, 1.0, True, True)
-      grad_k = summed(grad_k, dk)
-    if want_v or want_s:
-      grad_v = per_head(dv) if want_v else None
-      grad_s = torch.empty(n, h, dk, dv, dtype=torch.float32, device=q.device) if want_s else None
-      _scan_call((t, n, h, dk, dv), log_decay, fresh, k, group, q, 1, g_out, 1, grad_v, g_final, grad_s, scale, 1.0, True, False)
-      grad_v = summed(grad_v, dv) if want_v else None
-    return grad_q, grad_k, grad_v, grad_s, None, None, None
+    return _run_backward(_scan_backward, _scan_backward_once, ctx, g_out, g_final)
 
 
 def memory_scan(q, k, v, log_decay, *, fresh=None, state=None, scale: Optional[float] = None):
