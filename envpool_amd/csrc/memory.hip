@@ -57,14 +57,20 @@ template <class T, bool kAligned> int scan_sizes(const epm::Scan& k, const epm::
 
 int padded(int dim) { return dim <= 64 ? 64 : 128; }
 
-// Split of the time axis. One part per state keeps everything single-pass. With fewer states than fill the
-// chip, parts of at least two chunks are walked side by side: keys and values are then read twice (first for
-// the states between the parts).
-constexpr int64_t kFill = 1024;  // workgroups
+// Split of the time axis. One part per state keeps everything single-pass. With fewer states than the chip holds at
+// once, the axis is cut into parts that are walked side by side: keys and values are then read twice (first for the
+// states between the parts), which counts as 1.6 times the chunks plus the join.
 int64_t scan_parts(const ep_memory_scan_args* a) {
   const int64_t states = a->rows * a->heads, chunks = (a->steps + epm::kChunk - 1) / epm::kChunk;
-  if (states <= 0 || states * 2 > kFill || chunks < 4) return 1;
-  return std::min<int64_t>(std::min<int64_t>(chunks / 2, (kFill + states - 1) / states), 65535);
+  if (states <= 0 || chunks < 2) return 1;
+  const int64_t size = size_of(a->dtype), pad = 16 / size;
+  const int64_t lds = epm::kChunk * (2 * (padded(a->key_dim) + pad) + padded(a->value_dim) + pad + epm::kChunk + pad) * size + 3 * epm::kChunk * 4;
+  const int64_t slots = 256 * (163840 / lds);  // workgroups that run at once
+  if (states * 2 > slots) return 1;
+  const int64_t per = std::max<int64_t>((chunks * states + slots - 1) / slots, (chunks + 65534) / 65535);
+  const int64_t parts = (chunks + per - 1) / per;
+  const int64_t rounds = (states * parts + slots - 1) / slots;
+  return 10 * chunks > 16 * rounds * per + 20 ? parts : 1;
 }
 int64_t scan_workspace(const ep_memory_scan_args* a, int64_t n_seg) {
   if (n_seg <= 1) return 0;
@@ -82,13 +88,20 @@ int scan_launch(const ep_memory_scan_args* a, const epm::Scan& k, hipStream_t st
     parts.ws_carry = (float*)((char*)a->workspace + a->rows * a->heads * parts.n_seg * ((int64_t)padded(a->key_dim) * padded(a->value_dim) * 4));
   }
   const int64_t size = size_of(a->dtype), per_load = 16 / size;
-  const auto aligned = [&](const void* ptr, const int64_t* stride, int64_t unit, int64_t bytes) {
-    return (uintptr_t)ptr % unit == 0 && stride[0] * bytes % unit == 0 && stride[1] * bytes % unit == 0 && stride[2] * bytes % unit == 0;
-  };
   const int64_t out_size = size_of(a->out_dtype);
-  // operands and results in 16-byte (results: 4-value) pieces, or value by value
-  const bool vec = aligned(a->q, a->q_stride, 16, size) && aligned(a->k, a->k_stride, 16, size) && aligned(a->v, a->v_stride, 16, size) &&
-                   aligned(a->out, a->out_stride, 4 * out_size, out_size) && a->key_dim % per_load == 0 && a->value_dim % per_load == 0;
+  // 16-byte pieces (results: 4 values), rows that follow one another, and a chunk within 2^31 bytes
+  const auto aligned = [&](const void* ptr, const int64_t* stride, int64_t width, int64_t unit, int64_t bytes) {
+    return (uintptr_t)ptr % unit == 0 && stride[0] * bytes % unit == 0 && stride[1] * bytes % unit == 0 && stride[2] * bytes % unit == 0 &&
+           stride[0] >= width && stride[0] * bytes <= (int64_t(1) << 31) / epm::kChunk;
+  };
+  const auto state_near = [&](const void* ptr, const int64_t* stride) {
+    return !ptr || (stride[2] >= 0 && stride[3] >= 0 && stride[2] < (1 << 20) && stride[3] < (1 << 20));
+  };
+  const bool vec = aligned(a->q, a->q_stride, a->key_dim, 16, size) && aligned(a->k, a->k_stride, a->key_dim, 16, size) &&
+                   aligned(a->v, a->v_stride, a->value_dim, 16, size) && (!a->out || aligned(a->out, a->out_stride, a->value_dim, 4 * out_size, out_size)) &&
+                   state_near(a->state_in, a->state_in_stride) && state_near(a->state_out, a->state_out_stride) && a->key_dim % per_load == 0 &&
+                   a->value_dim % per_load == 0;
+  parts.state_vec = (uintptr_t)a->state_in % 16 == 0 && a->state_in_stride[0] % 4 == 0 && a->state_in_stride[1] % 4 == 0 && a->state_in_stride[3] % 4 == 0;
   const int64_t states = a->rows * a->heads;
   if (states > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld states", (long long)states);
   int rc = EP_OK;

@@ -54,7 +54,7 @@ template <class T, class V8, class V4> struct Mma16 {
   static __device__ frag weighted(frag f, const float* w) {  // element e times w[e], e = 0 .. 7
     frag o;
 #pragma unroll
-    for (int r = 0; r < 8; ++r) o[r] = (T)(w[r] != 0.f ? (float)f[r] * w[r] : 0.f);
+    for (int r = 0; r < 8; ++r) o[r] = (T)((float)f[r] * w[r]);
     return o;
   }
   static __device__ void put4(T* p, f32x4 a) {
@@ -69,17 +69,17 @@ typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 typedef f16 f16x4 __attribute__((ext_vector_type(4)));
 template <> struct Mma<bf16> : Mma16<bf16, bf16x8, bf16x4> {
-  static constexpr uint32_t kExp = 0x7f807f80u;
+  static constexpr uint32_t kInf = 0x7f80;
   static __device__ f32x4 mul(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct Mma<f16> : Mma16<f16, f16x8, f16x4> {
-  static constexpr uint32_t kExp = 0x7c007c00u;
+  static constexpr uint32_t kInf = 0x7c00;
   static __device__ f32x4 mul(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct Mma<float> {
   using frag = f32x4;
   static constexpr int K = 16;  // four products of 4: lane group g holds 4g + r in step r
-  static constexpr uint32_t kExp = 0x7f800000u;
+  static constexpr uint32_t kInf = 0x7f800000u;
   static __device__ frag row(const float* tile, int stride, int r0, int k0) {
     return *(const f32x4*)(tile + (r0 + (threadIdx.x & 15)) * stride + k0 + 4 * ((threadIdx.x >> 4) & 3));
   }
@@ -91,7 +91,7 @@ template <> struct Mma<float> {
   static __device__ frag weighted(frag f, const float* w) {
     frag o;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) o[r] = w[r] != 0.f ? f[r] * w[r] : 0.f;
+    for (int r = 0; r < 4; ++r) o[r] = f[r] * w[r];
     return o;
   }
   static __device__ void put4(float* p, f32x4 a) { *(f32x4*)p = a; }
@@ -109,6 +109,7 @@ struct Parts {
   f32x4* ws_state;     // [row * heads][n_seg][DK * DV / 4] in accumulator order: what a part starts from (read), or
   float* ws_carry;     // its own contribution and how far it lets the state before it through (written)
   int32_t state_only;  // the first of two passes over split time: contributions only
+  int32_t state_vec;   // state_in's rows are 16-byte pieces when its key stride is 1
 };
 
 template <class T, int DK, int DV> struct ScanTile {
@@ -117,18 +118,45 @@ template <class T, int DK, int DV> struct ScanTile {
   static constexpr int SP = kChunk + kVec;
   static constexpr int kQ = kChunk * DK / kVec / 256;        // 16-byte loads per thread and tile
   static constexpr int kV = kChunk * DV / kVec / 256;
-  // workgroups (one wave per SIMD each) that LDS lets a CU hold: the registers are kept to as many
-  static constexpr int kPerCu = 163840 / (int)((size_t)kChunk * (2 * SK + SV + SP) * sizeof(T) + 2 * kChunk * sizeof(float));
-  static constexpr size_t kLds = (size_t)kChunk * (2 * SK + SV + SP) * sizeof(T) + 2 * kChunk * sizeof(float);
+  static constexpr size_t kLds = (size_t)kChunk * (2 * SK + SV + SP) * sizeof(T) + 3 * kChunk * sizeof(float);
+  // workgroups (one wave per SIMD each) that LDS lets a CU hold: the registers are kept to as many (value-by-value
+  // addressing needs more of them: half as many)
+  static constexpr int kPerCu = (int)(163840 / kLds);
+  static constexpr int kWaves(bool aligned) { return aligned || kPerCu == 1 ? kPerCu : kPerCu / 2; }
 };
 
-__device__ inline uint32_t has_ones(uint32_t x, uint32_t e, uint32_t half) {  // any 16-bit (or the 32-bit) exponent all ones
-  const uint32_t y = x & e;
-  return half ? ((y & 0xffffu) == (e & 0xffffu)) | ((y >> 16) == (e >> 16)) : y == e;
+// largest magnitude bits seen: of each 16-bit half, or of the word
+template <class T> __device__ inline uint32_t top_bits(uint32_t top, uint32_t x) {
+  if constexpr (sizeof(T) == 2) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    union { uint32_t u; u16x2 v; } a, b;
+    a.u = top, b.u = x & 0x7fff7fffu;
+    a.v = __builtin_elementwise_max(a.v, b.v);
+    return a.u;
+  } else {
+    const uint32_t y = x & 0x7fffffffu;
+    return top > y ? top : y;
+  }
+}
+template <class T> __device__ inline bool not_finite(uint32_t top) {
+  if constexpr (sizeof(T) == 2) return (top & 0xffffu) >= Mma<T>::kInf || (top >> 16) >= Mma<T>::kInf;
+  else return top >= Mma<T>::kInf;
 }
 
+// Buffer addressing: a 64-bit base that the whole workgroup shares plus a 32-bit byte offset per lane; loads past
+// `bytes` give 0 and stores there are dropped, so that ragged ends cost no instructions. kOutside plus anything below
+// 2^31 is past every buffer.
+constexpr uint32_t kOutside = 0x80000000u;
+__device__ inline __amdgpu_buffer_rsrc_t buffer(const void* base, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00020000);
+}
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// How a launch addresses: kAligned: every operand in 16-byte pieces through buffers (offsets below 2^31, rows that do
+// not overlap); otherwise value by value.
 template <class T, int DK, int DV, bool kAligned>
-__global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kPerCu)) void scan_chunks(Scan p, Parts parts) {
+__global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void scan_chunks(Scan p, Parts parts) {
   using M = Mma<T>;
   using Tile = ScanTile<T, DK, DV>;
   using frag = typename M::frag;
@@ -139,8 +167,9 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kPerCu)) void scan_chunk
   T* ks = qs + kChunk * SK;
   T* vs = ks + kChunk * SK;
   T* ps = vs + kChunk * SV;
-  float* w_up = (float*)(ps + kChunk * SP);
-  int* odd = (int*)(w_up + kChunk);  // a key or value of this chunk is not finite
+  float* w_up = (float*)(ps + kChunk * SP);  // weight of a step in the state that leaves the chunk
+  float* w_in = w_up + kChunk;               // and of the state that enters it in a step's output
+  int* odd = (int*)(w_in + kChunk);          // a key or value of this chunk is not finite
 
   const int64_t rh = blockIdx.x;
   const int64_t row = rh / p.heads;
@@ -148,35 +177,18 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kPerCu)) void scan_chunk
   // (of the contributions only those are needed that a later part starts from)
   const int seg = blockIdx.y + (parts.state_only && p.reverse ? 1 : 0);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
-  const int v0 = wave * (DV / 4);
+  const int v0 = 16 * wave;  // this wave's value columns: 16 of every 64
   const bool rev = p.reverse;
   const float l2 = fmaxf(p.log_decay[h] * 1.44269504088896f, -1e30f);  // (decay 0: its power 0 is still 1)
+  const float lambda = __builtin_amdgcn_exp2f(l2);
+  // tiles that the operands' sizes reach (in 32 bits the matrix cores are the bound, so padding is not multiplied)
+  constexpr bool kTrim = sizeof(T) == 4;
+  const int nk = kTrim ? (p.dk + K - 1) / K : DK / K, nd = kTrim ? (p.dk + 15) / 16 : ND;
 
   const T* gq = (const T*)p.q + row * p.q_stride[1] + (h / p.q_group) * p.q_stride[2];
   const T* gk = (const T*)p.k + row * p.k_stride[1] + (h / p.k_group) * p.k_stride[2];
   const T* gv = (const T*)p.v + row * p.v_stride[1] + (h / p.v_group) * p.v_stride[2];
   const uint8_t* gf = p.fresh ? p.fresh + row * p.fresh_stride[1] : nullptr;
-
-  // ---- the state the part starts from
-  f32x4 s[ND][NV];
-  f32x4* ws = parts.ws_state ? parts.ws_state + (rh * parts.n_seg + seg) * (DK * DV / 4) : nullptr;
-#pragma unroll
-  for (int i = 0; i < ND; ++i)
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      s[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (parts.state_only) continue;
-      if (parts.n_seg > 1) {
-        s[i][j] = ws[((i * NV + j) * 4 + wave) * 64 + lane];
-      } else if (p.state_in) {
-        const int v = v0 + 16 * j + l16, d = 16 * i + 4 * g;
-        const float* a = p.state_in + row * p.in_stride[0] + h * p.in_stride[1] + v * p.in_stride[3];
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (v < p.dv && d + r < p.dk) s[i][j][r] = a[(d + r) * p.in_stride[2]];
-      }
-    }
-  float through = 1.f;
 
   const int64_t seg0 = seg * parts.seg_len;
   const int64_t seg1 = seg0 + parts.seg_len < p.steps ? seg0 + parts.seg_len : p.steps;
@@ -186,56 +198,108 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kPerCu)) void scan_chunk
   uint8_t rf = 0;
   const auto load_tile = [&](uint4* r, int count, const T* base, int64_t step_stride, int width, int padded, int64_t start, int n) {
     const int per_row = padded / kVec;
+    if constexpr (kAligned) {
+      const auto b = buffer(base + start * step_stride, ((n - 1) * step_stride + width) * (int64_t)sizeof(T));
+      const int t = threadIdx.x / per_row, c = (threadIdx.x % per_row) * kVec;
+      const uint32_t stride = (uint32_t)step_stride * (uint32_t)sizeof(T);
+      const uint32_t at = c < width ? t * stride + c * (uint32_t)sizeof(T) : kOutside;
 #pragma unroll
-    for (int i = 0; i < count; ++i) {
-      const int at = i * 256 + threadIdx.x;
-      const int t = at / per_row, c = (at % per_row) * kVec;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (t < n && c < width) {
-        const T* a = base + (start + t) * step_stride + c;
-        if (kAligned) {
-          x = *(const uint4*)a;
-        } else {
-          union { uint4 u; T e[kVec]; } b;
-          b.u = x;
+      for (int i = 0; i < count; ++i) {
+        const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(b, at + i * (256 / per_row) * stride, 0, 0);
+        r[i] = make_uint4(x.x, x.y, x.z, x.w);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < count; ++i) {
+        const int at = i * 256 + threadIdx.x;
+        const int t = at / per_row, c = (at % per_row) * kVec;
+        union { uint4 u; T e[kVec]; } x;
+        x.u = make_uint4(0, 0, 0, 0);
+        if (t < n && c < width) {
+          const T* a = base + (start + t) * step_stride + c;
 #pragma unroll
           for (int e = 0; e < kVec; ++e)
-            if (c + e < width) b.e[e] = a[e];
-          x = b.u;
+            if (c + e < width) x.e[e] = a[e];
         }
+        r[i] = x.u;
       }
-      r[i] = x;
     }
   };
   const auto load = [&](int64_t start, int n) {
-    if (!parts.state_only) load_tile(rq, Tile::kQ, gq, p.q_stride[0], p.dk, DK, start, n);
     load_tile(rk, Tile::kQ, gk, p.k_stride[0], p.dk, DK, start, n);
     load_tile(rv, Tile::kV, gv, p.v_stride[0], p.dv, DV, start, n);
+    if (!parts.state_only) load_tile(rq, Tile::kQ, gq, p.q_stride[0], p.dk, DK, start, n);
     rf = gf && lane < n ? gf[(start + lane) * p.fresh_stride[0]] : 0;
   };
   const auto put_tile = [&](const uint4* r, int count, T* tile, int padded, int stride) {
-    uint32_t bad = 0;
     const int per_row = padded / kVec;
+    T* to = tile + (threadIdx.x / per_row) * stride + (threadIdx.x % per_row) * kVec;
+#pragma unroll
+    for (int i = 0; i < count; ++i) *(uint4*)(to + i * (256 / per_row) * stride) = r[i];
+  };
+  const auto top_of = [&](uint32_t top, const uint4* r, int count) {
 #pragma unroll
     for (int i = 0; i < count; ++i) {
-      const int at = i * 256 + threadIdx.x;
-      *(uint4*)(tile + (at / per_row) * stride + (at % per_row) * kVec) = r[i];
-      constexpr uint32_t e = M::kExp, half = sizeof(T) == 2;
-      bad |= has_ones(r[i].x, e, half) | has_ones(r[i].y, e, half) | has_ones(r[i].z, e, half) | has_ones(r[i].w, e, half);
+      top = top_bits<T>(top, r[i].x);
+      top = top_bits<T>(top, r[i].y);
+      top = top_bits<T>(top, r[i].z);
+      top = top_bits<T>(top, r[i].w);
     }
-    return bad;
+    return top;
   };
 
   int64_t start = rev ? seg1 - (seg1 - seg0 < kChunk ? seg1 - seg0 : kChunk) : seg0;
   int n = (int)(seg1 - seg0 < kChunk ? seg1 - seg0 : kChunk);
   if (threadIdx.x == 0) *odd = 0;
   if (n > 0) load(start, n);
+
+  // ---- the state the part starts from
+  f32x4 s[ND][NV];
+  f32x4* ws = parts.ws_state ? parts.ws_state + (rh * parts.n_seg + seg) * (DK * DV / 4) : nullptr;
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int j = 0; j < NV; ++j) s[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (!parts.state_only && parts.n_seg > 1) {
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) s[i][j] = ws[((i * NV + j) * 4 + wave) * 64 + lane];
+  } else if (!parts.state_only && p.state_in) {
+    const float* base = p.state_in + row * p.in_stride[0] + h * p.in_stride[1];
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int v = v0 + 64 * j + l16, d = 16 * i + 4 * g;
+        if constexpr (kAligned) {
+          const auto b = buffer(base, 0x7fffffff);
+          const uint32_t sd = (uint32_t)p.in_stride[2] * 4u, sv = (uint32_t)p.in_stride[3] * 4u;
+          const uint32_t at = v < p.dv && d < p.dk ? d * sd + v * sv : kOutside;
+          if (sd == 4 && parts.state_vec) {
+            union { u32x4 u; f32x4 f; } x;
+            x.u = __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0);
+            s[i][j] = x.f;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[i][j][r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(b, at + r * sd, 0, 0));
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (v < p.dv && d + r < p.dk) s[i][j][r] = base[(d + r) * p.in_stride[2] + v * p.in_stride[3]];
+        }
+      }
+  }
+  float through = 1.f;
+
   while (n > 0) {
     __syncthreads();  // (the tiles of the chunk before have been read)
     if (!parts.state_only) put_tile(rq, Tile::kQ, qs, DK, SK);
-    const uint32_t bad = put_tile(rk, Tile::kQ, ks, DK, SK) | put_tile(rv, Tile::kV, vs, DV, SV);
+    put_tile(rk, Tile::kQ, ks, DK, SK);
+    put_tile(rv, Tile::kV, vs, DV, SV);
     uint64_t starts = __ballot(rf != 0);  // bit t: step t starts an episode
-    if (bad && starts) *odd = 1;
+    if (starts && not_finite<T>(top_of(top_of(0, rk, Tile::kQ), rv, Tile::kV))) *odd = 1;
     __syncthreads();
     if (starts && *odd) {
       // 0 * inf would carry what is not finite across the start of an episode: such a chunk ends there
@@ -262,10 +326,12 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kPerCu)) void scan_chunk
     const int64_t start_now = start;
     if (n_next > 0) load(start_next, n_next);
 
-    if (threadIdx.x < kChunk) {  // weights of the steps in the state that leaves the chunk
-      const int t = threadIdx.x;
-      const uint64_t between = rev ? starts & ((2ull << t) - 1) : (t < 63 ? starts >> (t + 1) : 0);
-      w_up[t] = t < n_now && between == 0 ? __builtin_amdgcn_exp2f(l2 * (rev ? t + 1 : n_now - 1 - t)) * p.inc_scale : 0.f;
+    if (threadIdx.x < 2 * kChunk) {
+      const int t = threadIdx.x & 63;
+      const uint64_t until = starts & ((2ull << t) - 1), later = t < 63 ? starts >> (t + 1) : 0;
+      const float from_0 = __builtin_amdgcn_exp2f(l2 * (t + 1)), to_end = __builtin_amdgcn_exp2f(l2 * (n_now - 1 - t));
+      if (threadIdx.x < kChunk) w_up[t] = t < n_now && (rev ? until : later) == 0 ? (rev ? from_0 : to_end) * p.inc_scale : 0.f;
+      else w_in[t] = t < n_now && (rev ? later : until) == 0 ? (rev ? to_end : from_0) * p.out_scale : 0.f;
     }
     if (!parts.state_only) {
       // ---- scores of 16 query steps per wave
@@ -284,29 +350,43 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kPerCu)) void scan_chunk
 #pragma unroll
       for (int k = 0; k < DK / K; ++k) q[k] = M::row(qs, SK, 16 * wave, k * K);
       const int i0 = rev ? (16 * wave) / K * K / 16 : 0, i1 = rev ? kChunk / 16 : ((16 * wave) / K + 1) * K / 16;
+      const float scale = p.inc_scale * p.out_scale;
       for (int i = i0; i < i1; ++i) {
         f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
         if (rev ? i >= wave : i <= wave) {
 #pragma unroll
-          for (int k = 0; k < DK / K; ++k) a = M::mul(M::row(ks, SK, 16 * i, k * K), q[k], a);
+          for (int k = 0; k < DK / K; ++k)
+            if (k < nk) a = M::mul(M::row(ks, SK, 16 * i, k * K), q[k], a);
+          const int u = 16 * i + 4 * g;
+          f32x4 w;
+          if (i == wave) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int u = 16 * i + 4 * g + r;
-            const float w = __builtin_amdgcn_exp2f(l2 * (float)(rev ? u - t : t - u)) * (p.inc_scale * p.out_scale);
-            a[r] = u >= lo && u <= hi ? a[r] * w : 0.f;
+            for (int r = 0; r < 4; ++r) w[r] = __builtin_amdgcn_exp2f(l2 * (float)(rev ? u + r - t : t - u - r)) * scale;
+          } else if (rev) {  // the nearest of the four, then one decay each
+            w[0] = __builtin_amdgcn_exp2f(l2 * (float)(u - t)) * scale;
+            w[1] = w[0] * lambda, w[2] = w[1] * lambda, w[3] = w[2] * lambda;
+          } else {
+            w[3] = __builtin_amdgcn_exp2f(l2 * (float)(t - u - 3)) * scale;
+            w[2] = w[3] * lambda, w[1] = w[2] * lambda, w[0] = w[1] * lambda;
           }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) a[r] = u + r >= lo && u + r <= hi ? a[r] * w[r] : 0.f;
         }
         M::put4(ps + t * SP + 16 * i + 4 * g, a);
       }
     }
     __syncthreads();
-    const float carry = starts ? 0.f : __builtin_amdgcn_exp2f(l2 * n_now);
+    const float carry = __builtin_amdgcn_exp2f(l2 * n_now);
+    if (starts) through = 0.f;
     through *= carry;
+    const uint32_t out_size = p.out_f32 ? 4u : (uint32_t)sizeof(T);
+    const T* out_row = (const T*)((const char*)p.out + (start_now * p.out_stride[0] + row * p.out_stride[1] + h * p.out_stride[2]) * (int64_t)out_size);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
+      if (kTrim && v0 + 64 * j >= p.dv) continue;
       frag vf[kChunk / K];
 #pragma unroll
-      for (int k = 0; k < kChunk / K; ++k) vf[k] = M::col(vs, SV, k * K, v0 + 16 * j);
+      for (int k = 0; k < kChunk / K; ++k) vf[k] = M::col(vs, SV, k * K, v0 + 64 * j);
       if (!parts.state_only) {
         frag sf[DK / K];
 #pragma unroll
@@ -318,53 +398,53 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kPerCu)) void scan_chunk
         for (int b = 0; b < 4; ++b) {
           f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int k = 0; k < DK / K; ++k) a = M::mul(sf[k], M::row_as_acc(qs, SK, 16 * b, k * K), a);
+          for (int k = 0; k < DK / K; ++k)
+            if (k < nk) a = M::mul(sf[k], M::row_as_acc(qs, SK, 16 * b, k * K), a);
           const int t = 16 * b + l16;
-          const uint64_t cut = rev ? (t < 63 ? starts >> (t + 1) : 0) : starts & ((2ull << t) - 1);
-          const float w = __builtin_amdgcn_exp2f(l2 * (float)(rev ? n_now - 1 - t : t + 1)) * p.out_scale;
+          const float w = w_in[t];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) a[r] = cut == 0 && t < n_now ? a[r] * w : 0.f;
+          for (int r = 0; r < 4; ++r) a[r] = w != 0.f ? a[r] * w : 0.f;
 #pragma unroll
           for (int k = 0; k < kChunk / K; ++k)
             if (rev ? (k + 1) * K > 16 * b : k * K <= 16 * b) a = M::mul(vf[k], M::row(ps, SP, 16 * b, k * K), a);
-          if (t < n_now) {
-            const int v = v0 + 16 * j + 4 * g;
-            const int64_t at = (start_now + t) * p.out_stride[0] + row * p.out_stride[1] + h * p.out_stride[2] + v;
-            if (p.out_f32) {
-              float* o = (float*)p.out + at;
-              if (kAligned && v + 4 <= p.dv) *(f32x4*)o = a;
-              else
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  if (v + r < p.dv) o[r] = a[r];
-            } else {
-              T* o = (T*)p.out + at;
-              if (kAligned && v + 4 <= p.dv) M::put4(o, a);
-              else
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  if (v + r < p.dv) o[r] = (T)a[r];
+          const int v = v0 + 64 * j + 4 * g;
+          if constexpr (kAligned) {
+            const auto o = buffer(out_row, p.out ? ((n_now - 1) * p.out_stride[0] + p.dv) * (int64_t)out_size : 0);
+            const uint32_t at = v < p.dv ? (uint32_t)(t * (uint32_t)p.out_stride[0] + v) * out_size : kOutside;
+            if (sizeof(T) == 4 || p.out_f32) {
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, a), o, at, 0, 0);
+            } else if constexpr (sizeof(T) == 2) {
+              alignas(8) T x[4];
+              M::put4(x, a);
+              __builtin_amdgcn_raw_buffer_store_b64(*(const u32x2*)x, o, at, 0, 0);
             }
+          } else if (t < n_now && p.out) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (v + r < p.dv) {
+                if (p.out_f32) ((float*)out_row)[t * p.out_stride[0] + v + r] = a[r];
+                else ((T*)out_row)[t * p.out_stride[0] + v + r] = (T)a[r];
+              }
           }
         }
       }
       // ---- the state: keys as rows, weighted values as columns
-      if (rev && (starts & 1)) {  // nothing of this chunk leaves it (and 0 * inf must not)
+      if (starts) {  // nothing from before the chunk leaves it (and 0 * inf must not)
 #pragma unroll
         for (int i = 0; i < ND; ++i) s[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        continue;
+        if (rev && (starts & 1)) continue;  // nothing of the chunk itself
+      } else {
+#pragma unroll
+        for (int i = 0; i < ND; ++i) s[i][j] *= carry;
       }
 #pragma unroll
       for (int k = 0; k < kChunk / K; ++k) vf[k] = M::weighted(vf[k], w_up + k * K + (K / 4) * g);
 #pragma unroll
-      for (int i = 0; i < ND; ++i) {
-        f32x4 a;
+      for (int i = 0; i < ND; ++i)
+        if (i < nd) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) a[r] = carry != 0.f ? s[i][j][r] * carry : 0.f;
-#pragma unroll
-        for (int k = 0; k < kChunk / K; ++k) a = M::mul(M::col(ks, SK, k * K, 16 * i), vf[k], a);
-        s[i][j] = a;
-      }
+          for (int k = 0; k < kChunk / K; ++k) s[i][j] = M::mul(M::col(ks, SK, k * K, 16 * i), vf[k], s[i][j]);
+        }
     }
     start = start_next;
     n = n_next;
@@ -381,15 +461,23 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kPerCu)) void scan_chunk
   }
   const bool last = rev ? seg == 0 : seg == parts.n_seg - 1;
   if (!last || !p.state_out) return;
+  float* base = p.state_out + row * p.outs_stride[0] + h * p.outs_stride[1];
 #pragma unroll
   for (int i = 0; i < ND; ++i)
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int v = v0 + 16 * j + l16, d = 16 * i + 4 * g;
-      float* a = p.state_out + row * p.outs_stride[0] + h * p.outs_stride[1] + v * p.outs_stride[3];
+      const int v = v0 + 64 * j + l16, d = 16 * i + 4 * g;
+      if constexpr (kAligned) {
+        const auto b = buffer(base, 0x7fffffff);
+        const uint32_t sd = (uint32_t)p.outs_stride[2] * 4u, sv = (uint32_t)p.outs_stride[3] * 4u;
+        const uint32_t at = v < p.dv && d < p.dk ? d * sd + v * sv : kOutside;
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (v < p.dv && d + r < p.dk) a[(d + r) * p.outs_stride[2]] = s[i][j][r];
+        for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, (float)s[i][j][r]), b, at + r * sd, 0, 0);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (v < p.dv && d + r < p.dk) base[(d + r) * p.outs_stride[2] + v * p.outs_stride[3]] = s[i][j][r];
+      }
     }
 }
 
@@ -400,7 +488,7 @@ template <int DK, int DV> __global__ __launch_bounds__(256) void join_parts(Scan
   const int at = blockIdx.y * 256 + threadIdx.x;  // in accumulator order
   const int lane = at & 63, wave = (at >> 6) & 3, tile = at >> 8;
   const int i = tile / (DV / 64), j = tile % (DV / 64);
-  const int v = wave * (DV / 4) + 16 * j + (lane & 15), d = 16 * i + 4 * (lane >> 4);
+  const int v = 64 * j + 16 * wave + (lane & 15), d = 16 * i + 4 * (lane >> 4);
   const int64_t row = rh / p.heads;
   const int h = (int)(rh % p.heads);
   f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};

@@ -453,6 +453,22 @@ def test_memory_scan_layouts_and_missing_pieces():
   assert torch.allclose(first + second, both, atol=1e-4, rtol=1e-4)
 
 
+@pytest.mark.parametrize("t,dk,dv", [(70, 24, 40), (300, 128, 128), (33, 7, 5)])
+def test_memory_scan_only_what_is_asked_for(t, dk, dv):
+  """Each gradient alone (the others are not computed) is what it is among the others."""
+  from envpool_amd import policy
+  q, k, v, decay, fresh, state, do, ds = (x.to(DEV) for x in _scan_problem((t, 2, 2, 1, dk, dv, 0.02, True), torch.bfloat16))
+
+  def run(wanted):
+    leaves = [x.detach().requires_grad_(i in wanted) for i, x in enumerate((q, k, v, state))]
+    out, final = policy.memory_scan(*leaves[:3], decay, fresh=fresh, state=leaves[3])
+    return torch.autograd.grad([out, final], [leaves[i] for i in wanted], [do, ds])
+
+  every = run((0, 1, 2, 3))
+  for i in range(4):
+    assert torch.equal(run((i,))[0], every[i])
+
+
 def test_memory_scan_agrees_with_steps():
   """The acting path and the learning path are one memory: T steps of EnvMemory against one scan."""
   from envpool_amd import policy
