@@ -35,27 +35,14 @@ int64_t step_workspace(const ep_memory_step_args* a) {
   return a->env_id && a->rows > kLookThrough ? a->num_envs * 4 : 0;
 }
 
-template <class T, int DK, int DV, bool kAligned> int scan_tile(const epm::Scan& k, epm::Parts parts, unsigned states, hipStream_t stream) {
-  constexpr size_t lds = epm::ScanTile<T, DK, DV>::kLds;
-  const auto fn = epm::scan_chunks<T, DK, DV, kAligned>;
-  if (lds > 65536) HIP_TRY(hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-  if (parts.n_seg > 1) {
-    parts.state_only = 1;
-    hipLaunchKernelGGL(fn, dim3(states, (unsigned)parts.n_seg - 1), dim3(256), lds, stream, k, parts);
-    hipLaunchKernelGGL((epm::join_parts<DK, DV>), dim3(states, DK * DV / 1024), dim3(256), 0, stream, k, parts);
-    parts.state_only = 0;
-  }
-  hipLaunchKernelGGL(fn, dim3(states, (unsigned)parts.n_seg), dim3(256), lds, stream, k, parts);
-  return EP_OK;
-}
-
-template <class T, bool kAligned> int scan_sizes(const epm::Scan& k, const epm::Parts& parts, unsigned states, hipStream_t stream) {
-  if (k.dk <= 64)
-    return k.dv <= 64 ? scan_tile<T, 64, 64, kAligned>(k, parts, states, stream) : scan_tile<T, 64, 128, kAligned>(k, parts, states, stream);
-  return k.dv <= 64 ? scan_tile<T, 128, 64, kAligned>(k, parts, states, stream) : scan_tile<T, 128, 128, kAligned>(k, parts, states, stream);
-}
-
 int padded(int dim) { return dim <= 64 ? 64 : 128; }
+
+template <class T> int per_cu_of(int dk, int dv) {
+  using namespace epm;
+  return dk <= 64 ? (dv <= 64 ? ScanTile<T, 64, 64>::kPerCu : ScanTile<T, 64, 128>::kPerCu)
+                  : (dv <= 64 ? ScanTile<T, 128, 64>::kPerCu : ScanTile<T, 128, 128>::kPerCu);
+}
+int64_t per_cu(int32_t dtype, int dk, int dv) { return dtype == EP_F32 ? per_cu_of<float>(dk, dv) : per_cu_of<epm::bf16>(dk, dv); }
 
 // Split of the time axis. One part per state keeps everything single-pass. With fewer states than the chip holds at
 // once, the axis is cut into parts that are walked side by side: keys and values are then read twice (first for the
@@ -63,9 +50,7 @@ int padded(int dim) { return dim <= 64 ? 64 : 128; }
 int64_t scan_parts(const ep_memory_scan_args* a) {
   const int64_t states = a->rows * a->heads, chunks = (a->steps + epm::kChunk - 1) / epm::kChunk;
   if (states <= 0 || chunks < 2) return 1;
-  const int64_t size = size_of(a->dtype), pad = 16 / size;
-  const int64_t lds = epm::kChunk * (2 * (padded(a->key_dim) + pad) + padded(a->value_dim) + pad + epm::kChunk + pad) * size + 3 * epm::kChunk * 4;
-  const int64_t slots = 256 * (163840 / lds);  // workgroups that run at once
+  const int64_t slots = 256 * per_cu(a->dtype, a->key_dim, a->value_dim);  // workgroups that run at once
   if (states * 2 > slots) return 1;
   const int64_t per = std::max<int64_t>((chunks * states + slots - 1) / slots, (chunks + 65534) / 65535);
   const int64_t parts = (chunks + per - 1) / per;
@@ -104,12 +89,10 @@ int scan_launch(const ep_memory_scan_args* a, const epm::Scan& k, hipStream_t st
   parts.state_vec = (uintptr_t)a->state_in % 16 == 0 && a->state_in_stride[0] % 4 == 0 && a->state_in_stride[1] % 4 == 0 && a->state_in_stride[3] % 4 == 0;
   const int64_t states = a->rows * a->heads;
   if (states > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld states", (long long)states);
-  int rc = EP_OK;
-  with_type(a->dtype, [&](auto t) {
-    using T = decltype(t);
-    rc = vec ? scan_sizes<T, true>(k, parts, (unsigned)states, stream) : scan_sizes<T, false>(k, parts, (unsigned)states, stream);
-  });
-  return rc;
+  hipError_t e = hipSuccess;
+  with_type(a->dtype, [&](auto t) { e = epm::scan_run<decltype(t)>(k, parts, vec, (unsigned)states, stream); });
+  HIP_TRY(e);
+  return EP_OK;
 }
 
 }  // namespace

@@ -32,13 +32,13 @@ __device__ inline bool starts(const Step& p, int64_t row) {
 }
 
 // claims of the envs that this batch names: zeroed, then counted
-__global__ __launch_bounds__(256) void clear_claims(Step p) {
+static __global__ __launch_bounds__(256) void clear_claims(Step p) {
   const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (r >= p.rows) return;
   const int64_t e = (int64_t)p.env_id[r] - p.env_id_offset;
   if (e >= 0 && e < p.num_envs) p.claims[e] = 0;
 }
-__global__ __launch_bounds__(256) void count_claims(Step p) {
+static __global__ __launch_bounds__(256) void count_claims(Step p) {
   const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (r >= p.rows) return;
   const int64_t e = (int64_t)p.env_id[r] - p.env_id_offset;

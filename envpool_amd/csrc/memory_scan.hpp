@@ -45,18 +45,8 @@ template <class T, class V8, class V4> struct Mma16 {
     u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(p + 4 * stride));
     return u.v;
   }
-  static __device__ frag from_acc(f32x4 a, f32x4 b) {
-    frag f;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) f[r] = (T)a[r], f[r + 4] = (T)b[r];
-    return f;
-  }
-  static __device__ frag weighted(frag f, const float* w) {  // element e times w[e], e = 0 .. 7
-    frag o;
-#pragma unroll
-    for (int r = 0; r < 8; ++r) o[r] = (T)((float)f[r] * w[r]);
-    return o;
-  }
+  // the value of element e (0 .. 7) from a pair of accumulators, in row_as_acc's order
+  static __device__ float of(f32x4 a, f32x4 b, int e) { return e < 4 ? a[e] : b[e - 4]; }
   static __device__ void put4(T* p, f32x4 a) {
     V4 v;
 #pragma unroll
@@ -68,18 +58,31 @@ typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+// 32-bit values as operands of 16-bit products. Rounded once (a score next to its value) they cost half a step of
+// the type per term; where a result is kept in 32 bits they go in as several pieces whose sum is the value.
+// bf16: the pieces are plain remainders, three of them hold 24 bits, and add up in one accumulator. f16: 11 bits a
+// piece and a narrow range, so the second piece is scaled by 2^11 and has an accumulator of its own, and what may
+// be large or small as a whole is brought to the middle of the range first (kNarrow).
 template <> struct Mma<bf16> : Mma16<bf16, bf16x8, bf16x4> {
   static constexpr uint32_t kInf = 0x7f80;
+  static constexpr bool kNarrow = false;
   static __device__ f32x4 mul(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <> struct Mma<f16> : Mma16<f16, f16x8, f16x4> {
   static constexpr uint32_t kInf = 0x7c00;
+  static constexpr bool kNarrow = true;
   static __device__ f32x4 mul(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
+// the power of two that brings a largest magnitude of `top` to 2^13 .. 2^14 (1 for 0 and for what is not finite)
+__device__ inline float to_middle(float top) {
+  const int e = __builtin_amdgcn_frexp_expf(top);
+  return top > 0.f && top < INFINITY ? __builtin_amdgcn_ldexpf(1.f, max(-120, min(120, 14 - e))) : 1.f;
+}
 template <> struct Mma<float> {
   using frag = f32x4;
   static constexpr int K = 16;  // four products of 4: lane group g holds 4g + r in step r
   static constexpr uint32_t kInf = 0x7f800000u;
+  static constexpr bool kNarrow = false;
   static __device__ frag row(const float* tile, int stride, int r0, int k0) {
     return *(const f32x4*)(tile + (r0 + (threadIdx.x & 15)) * stride + k0 + 4 * ((threadIdx.x >> 4) & 3));
   }
@@ -88,12 +91,6 @@ template <> struct Mma<float> {
     const float* p = tile + (k0 + 4 * ((threadIdx.x >> 4) & 3)) * stride + c0 + (threadIdx.x & 15);
     return frag{p[0], p[stride], p[2 * stride], p[3 * stride]};
   }
-  static __device__ frag weighted(frag f, const float* w) {
-    frag o;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) o[r] = f[r] * w[r];
-    return o;
-  }
   static __device__ void put4(float* p, f32x4 a) { *(f32x4*)p = a; }
   static __device__ f32x4 mul(frag a, frag b, f32x4 c) {
 #pragma unroll
@@ -101,6 +98,21 @@ template <> struct Mma<float> {
     return c;
   }
 };
+
+// Keeps the compiler from moving a later phase's LDS reads up here: it would need registers for all of them, and
+// the waves that those registers cost hide more latency than the early reads.
+__device__ inline void keep_order() { __builtin_amdgcn_sched_barrier(0); }
+
+// After products that a wave may have skipped, or whose results it may not use, before their registers are touched: the
+// compiler counts a matrix instruction's wait states along the straight path, and has been seen to come up short
+// where the skipping path joins it from elsewhere. Sixteen are more than any of them needs.
+template <bool kSkips> __device__ inline void settle() {
+  if constexpr (kSkips) {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
 
 // how a launch's states come and go
 struct Parts {
@@ -114,11 +126,13 @@ struct Parts {
 
 template <class T, int DK, int DV> struct ScanTile {
   static constexpr int kVec = 16 / sizeof(T);                // values of one 16-byte load
-  static constexpr int SK = DK + kVec, SV = DV + kVec;       // LDS row strides (16 bytes of padding)
+  // LDS row strides. 16 bytes of padding let 16 lanes read 16 bytes of a row each without a bank twice; the
+  // transposing reads take 32 bytes of 4 rows, which 32 bytes of padding keep apart
+  static constexpr int SQ = DK + kVec, SK = DK + 32 / (int)sizeof(T), SV = DV + 32 / (int)sizeof(T);
   static constexpr int SP = kChunk + kVec;
   static constexpr int kQ = kChunk * DK / kVec / 256;        // 16-byte loads per thread and tile
   static constexpr int kV = kChunk * DV / kVec / 256;
-  static constexpr size_t kLds = (size_t)kChunk * (2 * SK + SV + SP) * sizeof(T) + 3 * kChunk * sizeof(float);
+  static constexpr size_t kLds = (size_t)kChunk * (SQ + SK + SV + SP) * sizeof(T) + 4 * kChunk * sizeof(float);
   // workgroups (one wave per SIMD each) that LDS lets a CU hold: the registers are kept to as many (value-by-value
   // addressing needs more of them: half as many)
   static constexpr int kPerCu = (int)(163840 / kLds);
@@ -155,32 +169,33 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 // How a launch addresses: kAligned: every operand in 16-byte pieces through buffers (offsets below 2^31, rows that do
 // not overlap); otherwise value by value.
-template <class T, int DK, int DV, bool kAligned>
+template <class T, int DK, int DV, bool kAligned, bool rev>
 __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void scan_chunks(Scan p, Parts parts) {
   using M = Mma<T>;
   using Tile = ScanTile<T, DK, DV>;
   using frag = typename M::frag;
-  constexpr int K = M::K, kVec = Tile::kVec, SK = Tile::SK, SV = Tile::SV, SP = Tile::SP;
+  constexpr int K = M::K, kVec = Tile::kVec, SQ = Tile::SQ, SK = Tile::SK, SV = Tile::SV, SP = Tile::SP;
   constexpr int ND = DK / 16, NV = DV / 64;  // state tiles of a wave: all keys, a quarter of the values
   extern __shared__ __align__(16) char lds[];
   T* qs = (T*)lds;
-  T* ks = qs + kChunk * SK;
+  T* ks = qs + kChunk * SQ;
   T* vs = ks + kChunk * SK;
   T* ps = vs + kChunk * SV;
   float* w_up = (float*)(ps + kChunk * SP);  // weight of a step in the state that leaves the chunk
   float* w_in = w_up + kChunk;               // and of the state that enters it in a step's output
-  int* odd = (int*)(w_in + kChunk);          // a key or value of this chunk is not finite
+  float* p_top = w_in + kChunk;              // kNarrow: what a step's scores were multiplied by
+  int* odd = (int*)(p_top + kChunk);         // a key or value of this chunk is not finite
 
   const int64_t rh = blockIdx.x;
   const int64_t row = rh / p.heads;
   const int h = (int)(rh % p.heads);
   // (of the contributions only those are needed that a later part starts from)
-  const int seg = blockIdx.y + (parts.state_only && p.reverse ? 1 : 0);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l16 = lane & 15;
+  const int seg = blockIdx.y + (parts.state_only && rev ? 1 : 0);
+  const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int v0 = 16 * wave;  // this wave's value columns: 16 of every 64
-  const bool rev = p.reverse;
-  const float l2 = fmaxf(p.log_decay[h] * 1.44269504088896f, -1e30f);  // (decay 0: its power 0 is still 1)
-  const float lambda = __builtin_amdgcn_exp2f(l2);
+  const float log2_decay = fmaxf(p.log_decay[h] * 1.44269504088896f, -1e30f);  // (decay 0: its power 0 is still 1)
+  const float lambda = __builtin_amdgcn_exp2f(log2_decay);
   // tiles that the operands' sizes reach (in 32 bits the matrix cores are the bound, so padding is not multiplied)
   constexpr bool kTrim = sizeof(T) == 4;
   const int nk = kTrim ? (p.dk + K - 1) / K : DK / K, nd = kTrim ? (p.dk + 15) / 16 : ND;
@@ -294,8 +309,11 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
   float through = 1.f;
 
   while (n > 0) {
+    // (opaque to the compiler here, or it would keep every step's powers of the decay in registers across the loop)
+    float l2 = log2_decay;
+    asm volatile("" : "+v"(l2));
     __syncthreads();  // (the tiles of the chunk before have been read)
-    if (!parts.state_only) put_tile(rq, Tile::kQ, qs, DK, SK);
+    if (!parts.state_only) put_tile(rq, Tile::kQ, qs, DK, SQ);
     put_tile(rk, Tile::kQ, ks, DK, SK);
     put_tile(rv, Tile::kV, vs, DV, SV);
     uint64_t starts = __ballot(rf != 0);  // bit t: step t starts an episode
@@ -312,7 +330,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
       start += from;
       n = to - from;
       load(start, n);
-      if (!parts.state_only) put_tile(rq, Tile::kQ, qs, DK, SK);
+      if (!parts.state_only) put_tile(rq, Tile::kQ, qs, DK, SQ);
       put_tile(rk, Tile::kQ, ks, DK, SK);
       put_tile(rv, Tile::kV, vs, DV, SV);
       starts = __ballot(rf != 0);
@@ -330,7 +348,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
       const int t = threadIdx.x & 63;
       const uint64_t until = starts & ((2ull << t) - 1), later = t < 63 ? starts >> (t + 1) : 0;
       const float from_0 = __builtin_amdgcn_exp2f(l2 * (t + 1)), to_end = __builtin_amdgcn_exp2f(l2 * (n_now - 1 - t));
-      if (threadIdx.x < kChunk) w_up[t] = t < n_now && (rev ? until : later) == 0 ? (rev ? from_0 : to_end) * p.inc_scale : 0.f;
+      if (threadIdx.x < kChunk) w_up[t] = t < n_now && (rev ? until : later) == 0 ? (rev ? from_0 : to_end) * (M::kNarrow ? 1.f : p.inc_scale) : 0.f;
       else w_in[t] = t < n_now && (rev ? later : until) == 0 ? (rev ? to_end : from_0) * p.out_scale : 0.f;
     }
     if (!parts.state_only) {
@@ -348,15 +366,20 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
       }
       frag q[DK / K];
 #pragma unroll
-      for (int k = 0; k < DK / K; ++k) q[k] = M::row(qs, SK, 16 * wave, k * K);
+      for (int k = 0; k < DK / K; ++k) q[k] = M::row(qs, SQ, 16 * wave, k * K);
+      // (all tiles of whole fragments, so that what lies across the diagonal is 0)
       const int i0 = rev ? (16 * wave) / K * K / 16 : 0, i1 = rev ? kChunk / 16 : ((16 * wave) / K + 1) * K / 16;
       const float scale = p.inc_scale * p.out_scale;
-      for (int i = i0; i < i1; ++i) {
+      f32x4 score[4];
+      float top = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
         f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
         if (rev ? i >= wave : i <= wave) {
 #pragma unroll
           for (int k = 0; k < DK / K; ++k)
             if (k < nk) a = M::mul(M::row(ks, SK, 16 * i, k * K), q[k], a);
+          settle<kTrim>();
           const int u = 16 * i + 4 * g;
           f32x4 w;
           if (i == wave) {
@@ -372,7 +395,22 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
 #pragma unroll
           for (int r = 0; r < 4; ++r) a[r] = u + r >= lo && u + r <= hi ? a[r] * w[r] : 0.f;
         }
-        M::put4(ps + t * SP + 16 * i + 4 * g, a);
+        if constexpr (M::kNarrow) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf(a[r]));
+          score[i] = a;
+        } else if (i >= i0 && i < i1) {
+          M::put4(ps + t * SP + 16 * i + 4 * g, a);
+        }
+      }
+      if constexpr (M::kNarrow) {
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float f = to_middle(top);
+        if (g == 0) p_top[t] = f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i >= i0 && i < i1) M::put4(ps + t * SP + 16 * i + 4 * g, score[i] * f);
       }
     }
     __syncthreads();
@@ -381,71 +419,163 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
     through *= carry;
     const uint32_t out_size = p.out_f32 ? 4u : (uint32_t)sizeof(T);
     const T* out_row = (const T*)((const char*)p.out + (start_now * p.out_stride[0] + row * p.out_stride[1] + h * p.out_stride[2]) * (int64_t)out_size);
+    const auto there = [&](int j) { return !kTrim || v0 + 64 * j < p.dv; };  // (the same for the whole wave)
+    if (!parts.state_only) {
+      // ---- outputs: what the entering state gives, then the chunk's own steps
+      f32x4 a[4][NV];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (kTrim && v0 + 64 * j >= p.dv) continue;
-      frag vf[kChunk / K];
+      for (int b = 0; b < 4; ++b)
 #pragma unroll
-      for (int k = 0; k < kChunk / K; ++k) vf[k] = M::col(vs, SV, k * K, v0 + 64 * j);
-      if (!parts.state_only) {
-        frag sf[DK / K];
+        for (int j = 0; j < NV; ++j) a[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      float s_scale = 1.f;
+      if constexpr (M::kNarrow) {
+        float top = 0.f;
 #pragma unroll
-        for (int k = 0; k < DK / K; ++k) {
-          if constexpr (sizeof(T) == 2) sf[k] = M::from_acc(s[2 * k][j], s[2 * k + 1][j]);
-          else sf[k] = s[k][j];
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+          for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf(s[i][j][r]));
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+        s_scale = to_middle(top);
+      }
+#pragma unroll
+      for (int k = 0; k < DK / K; ++k) {
+        if (k >= nk) continue;
+        // the state rounded, and what that left out
+        frag hi[NV], lo[NV];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float x = M::of(s[2 * k][j], s[2 * k + 1][j], e) * s_scale;
+              hi[j][e] = (T)x;
+              lo[j][e] = (T)(x - (float)hi[j][e]);
+            }
+          } else {
+            hi[j] = s[k][j];
+          }
         }
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
+          const frag qf = M::row_as_acc(qs, SQ, 16 * b, k * K);
 #pragma unroll
-          for (int k = 0; k < DK / K; ++k)
-            if (k < nk) a = M::mul(sf[k], M::row_as_acc(qs, SK, 16 * b, k * K), a);
-          const int t = 16 * b + l16;
-          const float w = w_in[t];
+          for (int j = 0; j < NV; ++j) {
+            if (!there(j)) continue;
+            a[b][j] = M::mul(hi[j], qf, a[b][j]);
+            if constexpr (sizeof(T) == 2) a[b][j] = M::mul(lo[j], qf, a[b][j]);
+          }
+        }
+        keep_order();
+      }
+      settle<kTrim>();
+      frag vf[NV][kChunk / K];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) a[r] = w != 0.f ? a[r] * w : 0.f;
+      for (int j = 0; j < NV; ++j)
 #pragma unroll
-          for (int k = 0; k < kChunk / K; ++k)
-            if (rev ? (k + 1) * K > 16 * b : k * K <= 16 * b) a = M::mul(vf[k], M::row(ps, SP, 16 * b, k * K), a);
+        for (int k = 0; k < kChunk / K; ++k) vf[j][k] = M::col(vs, SV, k * K, v0 + 64 * j);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int t = 16 * b + l16;
+        const float f = M::kNarrow ? p_top[t] : 1.f;
+        const float w = w_in[t], ws_ = w * f / s_scale;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) a[b][j][r] = w != 0.f ? a[b][j][r] * ws_ : 0.f;
+#pragma unroll
+        for (int k = 0; k < kChunk / K; ++k)
+          if (rev ? (k + 1) * K > 16 * b : k * K <= 16 * b) {
+            const frag pf = M::row(ps, SP, 16 * b, k * K);
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+              if (there(j)) a[b][j] = M::mul(vf[j][k], pf, a[b][j]);
+          }
+        settle<kTrim || !kAligned>();  // (value by value, a lane may have nothing to store)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          f32x4 x = a[b][j];
+          if constexpr (M::kNarrow) x *= 1.f / f;
           const int v = v0 + 64 * j + 4 * g;
           if constexpr (kAligned) {
             const auto o = buffer(out_row, p.out ? ((n_now - 1) * p.out_stride[0] + p.dv) * (int64_t)out_size : 0);
             const uint32_t at = v < p.dv ? (uint32_t)(t * (uint32_t)p.out_stride[0] + v) * out_size : kOutside;
             if (sizeof(T) == 4 || p.out_f32) {
-              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, a), o, at, 0, 0);
+              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), o, at, 0, 0);
             } else if constexpr (sizeof(T) == 2) {
-              alignas(8) T x[4];
-              M::put4(x, a);
-              __builtin_amdgcn_raw_buffer_store_b64(*(const u32x2*)x, o, at, 0, 0);
+              alignas(8) T y[4];
+              M::put4(y, x);
+              __builtin_amdgcn_raw_buffer_store_b64(*(const u32x2*)y, o, at, 0, 0);
             }
           } else if (t < n_now && p.out) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               if (v + r < p.dv) {
-                if (p.out_f32) ((float*)out_row)[t * p.out_stride[0] + v + r] = a[r];
-                else ((T*)out_row)[t * p.out_stride[0] + v + r] = (T)a[r];
+                if (p.out_f32) ((float*)out_row)[t * p.out_stride[0] + v + r] = x[r];
+                else ((T*)out_row)[t * p.out_stride[0] + v + r] = (T)x[r];
               }
           }
         }
+        keep_order();
       }
-      // ---- the state: keys as rows, weighted values as columns
-      if (starts) {  // nothing from before the chunk leaves it (and 0 * inf must not)
-#pragma unroll
-        for (int i = 0; i < ND; ++i) s[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (rev && (starts & 1)) continue;  // nothing of the chunk itself
-      } else {
-#pragma unroll
-        for (int i = 0; i < ND; ++i) s[i][j] *= carry;
-      }
-#pragma unroll
-      for (int k = 0; k < kChunk / K; ++k) vf[k] = M::weighted(vf[k], w_up + k * K + (K / 4) * g);
+    }
+    // ---- the state: keys as rows, weighted values as columns
+    if (starts) {  // nothing from before the chunk leaves it (and 0 * inf must not)
 #pragma unroll
       for (int i = 0; i < ND; ++i)
-        if (i < nd) {
 #pragma unroll
-          for (int k = 0; k < kChunk / K; ++k) s[i][j] = M::mul(M::col(ks, SK, k * K, 16 * i), vf[k], s[i][j]);
-        }
+        for (int j = 0; j < NV; ++j) s[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    } else {
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) s[i][j] *= carry;
     }
+    if (!(rev && (starts & 1))) {  // (else nothing of the chunk itself leaves it)
+#pragma unroll
+      for (int k = 0; k < kChunk / K; ++k) {
+        const float* w = w_up + k * K + (K / 4) * g;
+        constexpr int kPieces = sizeof(T) == 4 ? 1 : M::kNarrow ? 2 : 3;
+        frag vw[NV][kPieces];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const frag v = M::col(vs, SV, k * K, v0 + 64 * j);
+#pragma unroll
+          for (int e = 0; e < K / 4; ++e) {
+            float x = (float)v[e] * w[e];
+#pragma unroll
+            for (int c = 0; c < kPieces; ++c) {
+              vw[j][c][e] = (T)x;
+              x -= (float)vw[j][c][e];
+              if (M::kNarrow) x *= 2048.f;
+            }
+          }
+        }
+        keep_order();
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+          if (i < nd) {
+            const frag kf = M::col(ks, SK, k * K, 16 * i);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+              if (!there(j)) continue;
+              if constexpr (M::kNarrow) {
+                f32x4 x = f32x4{0.f, 0.f, 0.f, 0.f}, y = x;
+                x = M::mul(kf, vw[j][0], x);
+                y = M::mul(kf, vw[j][1], y);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[i][j][r] = fmaf(fmaf(y[r], 1.f / 2048, x[r]), p.inc_scale, s[i][j][r]);
+              } else {
+#pragma unroll
+                for (int c = 0; c < kPieces; ++c) s[i][j] = M::mul(kf, vw[j][c], s[i][j]);
+              }
+            }
+          }
+      }
+    }
+    settle<true>();  // (a whole update may have been skipped)
     start = start_next;
     n = n_next;
   }
@@ -498,18 +628,60 @@ template <int DK, int DV> __global__ __launch_bounds__(256) void join_parts(Scan
     for (int r = 0; r < 4; ++r)
       if (v < p.dv && d + r < p.dk) s[r] = a[(d + r) * p.in_stride[2]];
   }
+  // (the parts' own states do not depend on each other: eight are under way at a time)
   f32x4* ws = parts.ws_state + rh * parts.n_seg * (DK * DV / 4) + at;
-  for (int n = 0; n < parts.n_seg; ++n) {
-    const int seg = p.reverse ? parts.n_seg - 1 - n : n;
-    f32x4* a = ws + (int64_t)seg * (DK * DV / 4);
-    const bool last = n + 1 == parts.n_seg;
-    const f32x4 own = last ? s : *a;
-    *a = s;
-    if (last) break;
-    const float carry = parts.ws_carry[rh * parts.n_seg + seg];
+  constexpr int kAheadParts = 8;
+  for (int n0 = 0; n0 < parts.n_seg; n0 += kAheadParts) {
+    f32x4 own[kAheadParts];
+    float carry[kAheadParts];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s[r] = (carry != 0.f ? s[r] * carry : 0.f) + own[r];
+    for (int i = 0; i < kAheadParts; ++i) {
+      const int n = n0 + i, seg = p.reverse ? parts.n_seg - 1 - n : n;
+      if (n + 1 < parts.n_seg) {  // (nothing follows the last part)
+        own[i] = ws[(int64_t)seg * (DK * DV / 4)];
+        carry[i] = parts.ws_carry[rh * parts.n_seg + seg];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kAheadParts; ++i) {
+      const int n = n0 + i, seg = p.reverse ? parts.n_seg - 1 - n : n;
+      if (n < parts.n_seg) ws[(int64_t)seg * (DK * DV / 4)] = s;
+      if (n + 1 < parts.n_seg) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[r] = (carry[i] != 0.f ? s[r] * carry[i] : 0.f) + own[i][r];
+      }
+    }
   }
 }
+
+// The launches of one call: `parts` says how time is split.
+template <class T, int DK, int DV, bool kAligned, bool rev> hipError_t scan_tile(const Scan& k, Parts parts, unsigned states, hipStream_t stream) {
+  constexpr size_t lds = ScanTile<T, DK, DV>::kLds;
+  const auto fn = scan_chunks<T, DK, DV, kAligned, rev>;
+  if (lds > 65536) {
+    const hipError_t e = hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+  }
+  if (parts.n_seg > 1) {
+    parts.state_only = 1;
+    hipLaunchKernelGGL(fn, dim3(states, (unsigned)parts.n_seg - 1), dim3(256), lds, stream, k, parts);
+    hipLaunchKernelGGL((join_parts<DK, DV>), dim3(states, DK * DV / 1024), dim3(256), 0, stream, k, parts);
+    parts.state_only = 0;
+  }
+  hipLaunchKernelGGL(fn, dim3(states, (unsigned)parts.n_seg), dim3(256), lds, stream, k, parts);
+  return hipGetLastError();
+}
+template <class T, bool kAligned, bool rev> hipError_t scan_sizes(const Scan& k, const Parts& parts, unsigned states, hipStream_t stream) {
+  if (k.dk <= 64)
+    return k.dv <= 64 ? scan_tile<T, 64, 64, kAligned, rev>(k, parts, states, stream) : scan_tile<T, 64, 128, kAligned, rev>(k, parts, states, stream);
+  return k.dv <= 64 ? scan_tile<T, 128, 64, kAligned, rev>(k, parts, states, stream) : scan_tile<T, 128, 128, kAligned, rev>(k, parts, states, stream);
+}
+// (one source file per type holds these: memory_scan_<type>.hip)
+template <class T> hipError_t scan_run(const Scan& k, const Parts& parts, bool aligned, unsigned states, hipStream_t stream);
+#define EPM_SCAN_RUN(T)                                                                                                       \
+  template <> hipError_t scan_run<T>(const Scan& k, const Parts& parts, bool aligned, unsigned states, hipStream_t stream) { \
+    if (aligned) return k.reverse ? scan_sizes<T, true, true>(k, parts, states, stream) : scan_sizes<T, true, false>(k, parts, states, stream); \
+    return k.reverse ? scan_sizes<T, false, true>(k, parts, states, stream) : scan_sizes<T, false, false>(k, parts, states, stream);         \
+  }
 
 }  // namespace epm
