@@ -24,19 +24,19 @@ template <class T> struct Mma;
 template <class T, class V8, class V4> struct Mma16 {
   using frag = V8;
   static constexpr int K = 32;  // summed index per fragment: lane group g = lane / 16 holds 8g .. 8g+7
-  static __device__ frag row(const T* tile, int stride, int r0, int k0) {
-    return *(const V8*)(tile + (r0 + (threadIdx.x & 15)) * stride + k0 + 8 * ((threadIdx.x >> 4) & 3));
+  static __device__ frag row(const T* tile, int stride, int r0, int k0, int lane) {
+    return *(const V8*)(tile + (r0 + (lane & 15)) * stride + k0 + 8 * (lane >> 4));
   }
   // the order that a pair of accumulators has: 4g .. 4g+3, then 16 + 4g .. 16 + 4g+3
-  static __device__ frag row_as_acc(const T* tile, int stride, int r0, int k0) {
-    const T* p = tile + (r0 + (threadIdx.x & 15)) * stride + k0 + 4 * ((threadIdx.x >> 4) & 3);
+  static __device__ frag row_as_acc(const T* tile, int stride, int r0, int k0, int lane) {
+    const T* p = tile + (r0 + (lane & 15)) * stride + k0 + 4 * (lane >> 4);
     const V4 a = *(const V4*)p, b = *(const V4*)(p + 16);
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
   // column c0 + lane % 16 of rows k0 + 8g .. k0 + 8g + 7: the transposing LDS read takes 4 rows x 16 columns
   // per 16 lanes, lane i addressing 4 values of row i / 4
-  static __device__ frag col(const T* tile, int stride, int k0, int c0) {
-    const int i = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+  static __device__ frag col(const T* tile, int stride, int k0, int c0, int lane) {
+    const int i = lane & 15, g = lane >> 4;
     const T* p = tile + (k0 + 8 * g + (i >> 2)) * stride + c0 + 4 * (i & 3);
     typedef short s4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s4* lp;
@@ -83,12 +83,12 @@ template <> struct Mma<float> {
   static constexpr int K = 16;  // four products of 4: lane group g holds 4g + r in step r
   static constexpr uint32_t kInf = 0x7f800000u;
   static constexpr bool kNarrow = false;
-  static __device__ frag row(const float* tile, int stride, int r0, int k0) {
-    return *(const f32x4*)(tile + (r0 + (threadIdx.x & 15)) * stride + k0 + 4 * ((threadIdx.x >> 4) & 3));
+  static __device__ frag row(const float* tile, int stride, int r0, int k0, int lane) {
+    return *(const f32x4*)(tile + (r0 + (lane & 15)) * stride + k0 + 4 * (lane >> 4));
   }
-  static __device__ frag row_as_acc(const float* tile, int stride, int r0, int k0) { return row(tile, stride, r0, k0); }
-  static __device__ frag col(const float* tile, int stride, int k0, int c0) {
-    const float* p = tile + (k0 + 4 * ((threadIdx.x >> 4) & 3)) * stride + c0 + (threadIdx.x & 15);
+  static __device__ frag row_as_acc(const float* tile, int stride, int r0, int k0, int lane) { return row(tile, stride, r0, k0, lane); }
+  static __device__ frag col(const float* tile, int stride, int k0, int c0, int lane) {
+    const float* p = tile + (k0 + 4 * (lane >> 4)) * stride + c0 + (lane & 15);
     return frag{p[0], p[stride], p[2 * stride], p[3 * stride]};
   }
   static __device__ void put4(float* p, f32x4 a) { *(f32x4*)p = a; }
@@ -309,9 +309,12 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
   float through = 1.f;
 
   while (n > 0) {
-    // (opaque to the compiler here, or it would keep every step's powers of the decay in registers across the loop)
+    // (opaque to the compiler here, or it would keep every step's powers of the decay, and every address, in
+    // registers across the loop)
     float l2 = log2_decay;
-    asm volatile("" : "+v"(l2));
+    int ln = lane;
+    asm volatile("" : "+v"(l2), "+v"(ln));
+    const int g = ln >> 4, l16 = ln & 15;
     __syncthreads();  // (the tiles of the chunk before have been read)
     if (!parts.state_only) put_tile(rq, Tile::kQ, qs, DK, SQ);
     put_tile(rk, Tile::kQ, ks, DK, SK);
@@ -366,7 +369,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
       }
       frag q[DK / K];
 #pragma unroll
-      for (int k = 0; k < DK / K; ++k) q[k] = M::row(qs, SQ, 16 * wave, k * K);
+      for (int k = 0; k < DK / K; ++k) q[k] = M::row(qs, SQ, 16 * wave, k * K, ln);
       // (all tiles of whole fragments, so that what lies across the diagonal is 0)
       const int i0 = rev ? (16 * wave) / K * K / 16 : 0, i1 = rev ? kChunk / 16 : ((16 * wave) / K + 1) * K / 16;
       const float scale = p.inc_scale * p.out_scale;
@@ -378,7 +381,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
         if (rev ? i >= wave : i <= wave) {
 #pragma unroll
           for (int k = 0; k < DK / K; ++k)
-            if (k < nk) a = M::mul(M::row(ks, SK, 16 * i, k * K), q[k], a);
+            if (k < nk) a = M::mul(M::row(ks, SK, 16 * i, k * K, ln), q[k], a);
           settle<kTrim>();
           const int u = 16 * i + 4 * g;
           f32x4 w;
@@ -460,7 +463,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
         }
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-          const frag qf = M::row_as_acc(qs, SQ, 16 * b, k * K);
+          const frag qf = M::row_as_acc(qs, SQ, 16 * b, k * K, ln);
 #pragma unroll
           for (int j = 0; j < NV; ++j) {
             if (!there(j)) continue;
@@ -475,7 +478,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int k = 0; k < kChunk / K; ++k) vf[j][k] = M::col(vs, SV, k * K, v0 + 64 * j);
+        for (int k = 0; k < kChunk / K; ++k) vf[j][k] = M::col(vs, SV, k * K, v0 + 64 * j, ln);
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const int t = 16 * b + l16;
@@ -488,7 +491,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
 #pragma unroll
         for (int k = 0; k < kChunk / K; ++k)
           if (rev ? (k + 1) * K > 16 * b : k * K <= 16 * b) {
-            const frag pf = M::row(ps, SP, 16 * b, k * K);
+            const frag pf = M::row(ps, SP, 16 * b, k * K, ln);
 #pragma unroll
             for (int j = 0; j < NV; ++j)
               if (there(j)) a[b][j] = M::mul(vf[j][k], pf, a[b][j]);
@@ -541,7 +544,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
         frag vw[NV][kPieces];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          const frag v = M::col(vs, SV, k * K, v0 + 64 * j);
+          const frag v = M::col(vs, SV, k * K, v0 + 64 * j, ln);
 #pragma unroll
           for (int e = 0; e < K / 4; ++e) {
             float x = (float)v[e] * w[e];
@@ -557,7 +560,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
 #pragma unroll
         for (int i = 0; i < ND; ++i)
           if (i < nd) {
-            const frag kf = M::col(ks, SK, k * K, 16 * i);
+            const frag kf = M::col(ks, SK, k * K, 16 * i, ln);
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
               if (!there(j)) continue;
