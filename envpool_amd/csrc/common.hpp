@@ -55,6 +55,17 @@ struct DeviceScope {
   ::epc::DeviceScope _dev_scope;   \
   HIP_TRY(_dev_scope.enter(dev))
 
+// The same for calls that have no object of their own (their device comes with the arguments): a device that does
+// not exist is named as such.
+#define EP_ENTER_GPU(dev)                                                                                             \
+  ::epc::DeviceScope _dev_scope;                                                                                      \
+  do {                                                                                                                \
+    const hipError_t _e = _dev_scope.enter(dev);                                                                      \
+    if (_e == hipErrorNoDevice || _e == hipErrorInvalidDevice)                                                        \
+      return ::epc::fail(EP_ERR_NO_DEVICE, "device_id = %d: no such GPU (there is no CPU fallback)", (int)(dev));     \
+    HIP_TRY(_e);                                                                                                      \
+  } while (0)
+
 constexpr size_t kAlign = 256;
 inline size_t align_up(size_t x) { return (x + kAlign - 1) / kAlign * kAlign; }
 

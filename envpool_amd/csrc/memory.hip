@@ -124,7 +124,7 @@ int ep_memory_step(const ep_memory_step_args* a) {
   if (int rc = check_workspace(a->workspace, a->workspace_bytes, step_workspace(a))) return rc;
   if (a->rows == 0) return EP_OK;
   if (a->rows * a->heads > 4 * (int64_t)INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld rows of %d heads", (long long)a->rows, a->heads);
-  EP_ENTER_DEVICE(a->device_id);
+  EP_ENTER_GPU(a->device_id);
   const hipStream_t stream = (hipStream_t)a->stream;
   epm::Step k{};
   k.num_envs = a->num_envs, k.rows = a->rows;
@@ -179,7 +179,7 @@ int ep_memory_scan(const ep_memory_scan_args* a) {
     if ((uintptr_t)ptr % 4) return fail(EP_ERR_INVALID, "an array of 4-byte values is not aligned to 4 bytes");
   if (int rc = check_workspace(a->workspace, a->workspace_bytes, ep_memory_scan_workspace(a))) return rc;
   if (a->rows == 0 || (a->steps == 0 && !a->state_out)) return EP_OK;
-  EP_ENTER_DEVICE(a->device_id);
+  EP_ENTER_GPU(a->device_id);
   const hipStream_t stream = (hipStream_t)a->stream;
   epm::Scan k{};
   k.steps = a->steps, k.rows = a->rows, k.heads = a->heads;
@@ -206,7 +206,7 @@ int ep_memory_sum_heads(int32_t device_id, const float* src, int64_t n, int32_t 
   if (!src || !out) return fail(EP_ERR_INVALID, "src, out: null pointer");
   if ((uintptr_t)src % 4 || (uintptr_t)out % size_of(dtype)) return fail(EP_ERR_INVALID, "src, out: not aligned to their type");
   if ((total + 255) / 256 > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld elements", (long long)total);
-  EP_ENTER_DEVICE(device_id);
+  EP_ENTER_GPU(device_id);
   with_type(dtype, [&](auto t) {
     hipLaunchKernelGGL(epm::sum_heads<decltype(t)>, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, (hipStream_t)stream, src, total, group, dim,
                        (decltype(t)*)out);

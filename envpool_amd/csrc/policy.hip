@@ -163,7 +163,7 @@ int ep_policy_choose(const ep_policy_rows* r, const void* u, int32_t u_dtype, in
   if (r->rows > 0 && (!action || !log_prob || !entropy)) return fail(EP_ERR_INVALID, "action, log_prob, entropy: null pointer");
   if (int rc = check_workspace(r, ep_policy_choose_workspace(r))) return rc;
   if (r->rows == 0) return EP_OK;
-  EP_ENTER_DEVICE(r->device_id);
+  EP_ENTER_GPU(r->device_id);
   const hipStream_t stream = (hipStream_t)r->stream;
   const epp::ChooseOut out{action, log_prob, entropy};
   const int u_f64 = u_dtype == EP_F64;
@@ -201,7 +201,7 @@ int ep_policy_evaluate(const ep_policy_rows* r, const int32_t* action, float* lo
   if (r->rows > 0 && (!action || !log_prob || !entropy || !stats)) return fail(EP_ERR_INVALID, "action, log_prob, entropy, stats: null pointer");
   if (int rc = check_workspace(r, ep_policy_evaluate_workspace(r))) return rc;
   if (r->rows == 0) return EP_OK;
-  EP_ENTER_DEVICE(r->device_id);
+  EP_ENTER_GPU(r->device_id);
   const hipStream_t stream = (hipStream_t)r->stream;
   const epp::EvaluateOut out{action, log_prob, entropy, stats};
   if (r->options <= kGroupOptions) {
@@ -249,7 +249,7 @@ int ep_policy_evaluate_grad(const ep_policy_rows* r, const int32_t* action, cons
     return fail(EP_ERR_INVALID, "grad_bias_stride = %lld is less than options", (long long)grad_bias_stride);
   if (grad_bias && (uintptr_t)grad_bias % size_of(r->bias_dtype)) return fail(EP_ERR_INVALID, "grad_bias: not aligned to its type");
   if (int rc = check_workspace(r, ep_policy_evaluate_grad_workspace(r, grad_bias != nullptr))) return rc;
-  EP_ENTER_DEVICE(r->device_id);
+  EP_ENTER_GPU(r->device_id);
   const hipStream_t stream = (hipStream_t)r->stream;
   const int64_t pieces = (r->options + epp::kPiece - 1) / epp::kPiece;
   const bool group = r->options <= kGroupOptions;

@@ -164,6 +164,39 @@ def choose(logits, u=None, *, num_options=None, mask=None, bias=None, history=No
     return Choice(action, log_prob, entropy)
 
 
+_CAPTURE = None  # a token that lasts from one capture's first differentiable call to the next eager one
+
+
+def _guard_capture(*inputs):
+  """Refuses a differentiable call inside a graph capture where a leaf among its inputs is still part of a graph
+  recorded outside it: torch would make that graph's stream wait inside the capture, which ends the process
+  when the capture ends. (Whether somebody holds a leaf's accumulation node shows in a mark left on it: with no
+  other holder the node goes, and the mark with it.) Returns the nodes, to be held until the call is recorded."""
+  global _CAPTURE
+  if not torch.cuda.is_current_stream_capturing():
+    _CAPTURE = None
+    return ()
+  if _CAPTURE is None:
+    _CAPTURE = object()
+  nodes = []
+  for t in inputs:
+    if t is None or not t.requires_grad or not t.is_leaf:
+      continue
+    node = torch.autograd.graph.get_gradient_edge(t).node
+    if node.metadata.get("envpool_amd_capture") is _CAPTURE:
+      continue
+    node.metadata["envpool_amd_probe"] = True
+    del node
+    node = torch.autograd.graph.get_gradient_edge(t).node
+    if "envpool_amd_probe" in node.metadata:
+      del node.metadata["envpool_amd_probe"]
+      raise RuntimeError("graph capture: a leaf input still belongs to an autograd graph recorded outside this capture; "
+                         "drop that graph (its outputs) before capturing, or capture over other leaves")
+    node.metadata["envpool_amd_capture"] = _CAPTURE
+    nodes.append(node)
+  return nodes
+
+
 def _run_backward(plain, once, ctx, *grads):
   """A backward pass whose results are not differentiable again: torch's wrapper that says so costs more than
   a small pass and is only needed where a graph of the backward pass is asked for."""
@@ -236,6 +269,7 @@ def evaluate(logits, action, *, num_options=None, mask=None, bias=None, history=
     action = action.contiguous()
   if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
     p.logits, p.bias = p.logits.detach(), None if p.bias is None else p.bias.detach()
+    nodes = _guard_capture(logits, bias)  # noqa: F841
     return _Evaluate.apply(logits, bias, action, p)
   return _evaluate_forward(p, action)[:2]
 
@@ -455,5 +489,6 @@ def memory_scan(q, k, v, log_decay, *, fresh=None, state=None, scale: Optional[f
   q, k, v, log_decay = _dense_last(q), _dense_last(k), _dense_last(v), log_decay.contiguous()
   scale = dk ** -0.5 if scale is None else float(scale)
   if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, state)):
+    nodes = _guard_capture(q, k, v, state)  # noqa: F841
     return _MemoryScan.apply(q, k, v, state, log_decay, fresh, scale)
   return _scan_forward(q, k, v, state, log_decay, fresh, scale)

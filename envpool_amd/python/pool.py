@@ -407,6 +407,35 @@ class EnvPoolFrontEnd:
     refresh_terminated(ents, [h] * T)
     return [fresh(e[0]) for e in ents]
 
+  # ---- additive: what a policy on the GPU needs next to the batches (envpool_amd/policy.py) -------------
+  def memory_torch(self, num_heads: int, key_dim: int, value_dim: int, log_decay, state=None):
+    """An `envpool_amd.policy.EnvMemory` over this pool's envs: `memory.step(q, k, v, env_id=info["env_id"],
+    elapsed_step=info["elapsed_step"])` moves the rows of a batch (`step_torch` / `recv_torch`) one step on, in
+    whatever order they came, and starts envs anew where their episode does. `log_decay` is a float32 tensor
+    `[num_heads]` on the pool's GPU."""
+    from ..policy import EnvMemory
+    return EnvMemory(self._cfg["num_envs"], num_heads, key_dim, value_dim, log_decay, state=state, env_id_offset=int(self.all_env_ids[0]))
+
+  def choose_torch(self, logits, u=None, **options):
+    """`envpool_amd.policy.choose` under the legal-action mask of the batch that `recv_torch` handed out last:
+    `logits` has a row per env of that batch and a column per option. `options`: what `choose` takes besides
+    the mask. Send the answer with `send_choice`."""
+    mask = getattr(self, "last_action_mask", None)
+    if mask is None or not isinstance(mask, tuple):
+      raise RuntimeError(f"choose_torch: {type(self).__name__} has handed out no batch with a legal-action mask on the GPU (recv_torch)")
+    if "mask" in options:
+      raise ValueError("choose_torch: the mask is the pool's; use envpool_amd.policy.choose for another one")
+    from ..policy import choose
+    return choose(logits, u, mask=self._torch_view(mask), **options)
+
+  def send_choice(self, choice) -> None:
+    """Sends the actions of a `Choice` (`choose_torch`) to the envs of the batch received last. The actions
+    cross to the host (the duel engine is there): this waits for them. A row without a legal option (-1: an
+    ended duel, which is reset whatever it is sent) sends 0."""
+    if not hasattr(self, "last_env_ids"):
+      raise RuntimeError(f"send_choice: {type(self).__name__} does not note the env ids of the last batch")
+    self.send(choice.action.clamp_min(0), self.last_env_ids)
+
   def __repr__(self) -> str:
     cfg = ", ".join(f"{k}={pprint.pformat(v)}" for k, v in self.config.items())
     return f"{type(self).__name__}({cfg})"

@@ -554,6 +554,16 @@ class ShardedTorchMixin:
     parts = self._gather_parts(lambda r: self._shards[r]._try_recv_device())
     return self._result([self._shard_out(r, got[0], reset) for r, got in parts], [r for r, _ in parts])
 
+  def memory_torch(self, *args, **kwargs):
+    raise RuntimeError("memory_torch: a sharded pool's rows are on several GPUs; make one envpool_amd.policy.EnvMemory per shard "
+                       "(env_id_offset = the shard's first env id) and step it with that shard's part of the batch")
+
+  def choose_torch(self, *args, **kwargs):
+    raise RuntimeError("choose_torch: a sharded pool's rows are on several GPUs; use envpool_amd.policy.choose with each part's info")
+
+  def send_choice(self, *args, **kwargs):
+    raise RuntimeError("send_choice: a sharded pool's rows are on several GPUs; use send with the parts' actions and env ids")
+
   def _shard_action(self, r, adict, n_rows):
     """(ptrs, dims, keep) of one shard's action arrays, converted only where dtype / layout / device differ."""
     import torch

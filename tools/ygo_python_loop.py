@@ -50,6 +50,15 @@ def main():
           ts.append(time.perf_counter() - t0)
         torch.cuda.synchronize()
         print(f"sync  {N} envs  send + recv_torch (device views out):    {med(ts[20:]):7.1f} us per step", flush=True)
+        # the same loop with the actions chosen on the GPU, under the batch's legal-action mask
+        logits = torch.randn(N, 16, device="cuda")
+        ts = []
+        for i in range(220):
+          t0 = time.perf_counter()
+          env.send_choice(env.choose_torch(logits, torch.rand(N, device="cuda")))
+          env.recv_torch()
+          ts.append(time.perf_counter() - t0)
+        print(f"sync  {N} envs  choose_torch + send_choice + recv_torch: {med(ts[20:]):7.1f} us per step", flush=True)
       else:
         env.async_reset()
         ts = []
