@@ -60,10 +60,10 @@ struct DeviceScope {
 #define EP_ENTER_GPU(dev)                                                                                             \
   ::epc::DeviceScope _dev_scope;                                                                                      \
   do {                                                                                                                \
-    const hipError_t _e = _dev_scope.enter(dev);                                                                      \
-    if (_e == hipErrorNoDevice || _e == hipErrorInvalidDevice)                                                        \
+    const hipError_t _entered = _dev_scope.enter(dev);                                                                   \
+    if (_entered == hipErrorNoDevice || _entered == hipErrorInvalidDevice)                                                      \
       return ::epc::fail(EP_ERR_NO_DEVICE, "device_id = %d: no such GPU (there is no CPU fallback)", (int)(dev));     \
-    HIP_TRY(_e);                                                                                                      \
+    HIP_TRY(_entered);                                                                                                \
   } while (0)
 
 constexpr size_t kAlign = 256;

@@ -95,7 +95,7 @@ template <class R, bool kHist> __device__ inline RowConst<R> row_const(const Row
   RowConst<R> c{};
   const R t = p.temperature ? (R)p.temperature[row] : (R)p.temperature_all;
   c.inv_t = (R)1 / t;
-  c.k = c.inv_t / Num<R>::kUnit;
+  c.k = c.inv_t * ((R)1 / Num<R>::kUnit);
   c.bad = !(t > (R)0) || !(t < (R)INFINITY) || !(c.k < (R)INFINITY);
   if (kHist) {
     c.rep = p.repetition ? (R)p.repetition[row] : (R)p.repetition_all;
@@ -139,6 +139,19 @@ template <class R> struct Seen {
 };
 
 __device__ inline bool bit(uint32_t bits, int i) { return (bits >> i) & 1u; }
+// v where bit i is set, else other: two instructions (the bit spread over a word, a bitwise choice)
+__device__ inline uint32_t pick(uint32_t bits, int i, uint32_t v, uint32_t other) {
+  const uint32_t all = (uint32_t)__builtin_amdgcn_sbfe((int)bits, i, 1);
+  return (v & all) | (other & ~all);
+}
+__device__ inline float pick(uint32_t bits, int i, float v, float other) {
+  return __builtin_bit_cast(float, pick(bits, i, __builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, other)));
+}
+__device__ inline double pick(uint32_t bits, int i, double v, double other) {
+  const uint64_t a = __builtin_bit_cast(uint64_t, v), b = __builtin_bit_cast(uint64_t, other);
+  const uint32_t lo = pick(bits, i, (uint32_t)a, (uint32_t)b), hi = pick(bits, i, (uint32_t)(a >> 32), (uint32_t)(b >> 32));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 
 // Options j0 .. j0+7 of a row (j0 a multiple of 8, below the row's end): y before the temperature, as they
 // come. Returns which are legal (bit i = option j0 + i); the y of the others are unspecified.
@@ -222,10 +235,11 @@ template <class T> __device__ inline float hold_range(const Rows& p, int64_t row
   return fabsf(x) < INFINITY && fabsf(b) < INFINITY ? (y > 0.f ? Num<float>::kHigh : Num<float>::kLow) : y;
 }
 
-// load_y made ready for sums: kNone where there is no weight. Returns whether a legal one is NaN or +inf. Nearly
+// load_y made ready for sums: kNone where there is no weight, m the largest. Returns whether a legal one is NaN or +inf. Nearly
 // always all are finite, which one product with 0 per option shows (0 * inf and 0 * NaN are NaN).
 template <class T, class R, bool kHist>
-__device__ inline bool load_ready(const Rows& p, const RowConst<R>& c, int64_t row, int64_t j0, bool whole, const Seen<R>& seen, R (&y)[kPer]) {
+__device__ inline bool load_ready(const Rows& p, const RowConst<R>& c, int64_t row, int64_t j0, bool whole, const Seen<R>& seen, R (&y)[kPer], R& m) {
+  m = Num<R>::kNone;
   if (j0 >= c.n_legal) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) y[i] = Num<R>::kNone;
@@ -233,10 +247,9 @@ __device__ inline bool load_ready(const Rows& p, const RowConst<R>& c, int64_t r
   }
   const uint32_t legal = load_y<T, R, kHist>(p, c, row, j0, whole, seen, y);
   R odd = (R)0;
-  R m = Num<R>::kNone;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    y[i] = bit(legal, i) ? y[i] : Num<R>::kNone;
+    y[i] = pick(legal, i, y[i], Num<R>::kNone);
     odd = mul_add(y[i], (R)0, odd);
     m = larger(m, y[i]);
   }
@@ -249,6 +262,7 @@ __device__ inline bool load_ready(const Rows& p, const RowConst<R>& c, int64_t r
     if (!(y[i] < (R)INFINITY)) bad = true;
     if (y[i] == -(R)INFINITY) y[i] = Num<R>::kNone;
     else if constexpr (sizeof(R) == 4) y[i] = larger(y[i], Num<float>::kLow);
+    m = larger(m, y[i]);
   }
   return bad;
 }
@@ -271,11 +285,8 @@ template <class R> __device__ inline void stat_rebase(Stat<R>& a, R m, R k) {
   a.s = f * a.s;
   a.m = m;
 }
-// adds the options j0 .. j0+7 (kBest: and notes where the largest is)
-template <class R, bool kBest> __device__ inline void stat_add(Stat<R>& a, const R (&y)[kPer], int64_t j0, R k) {
-  R m = y[0];
-#pragma unroll
-  for (int i = 1; i < kPer; ++i) m = larger(m, y[i]);
+// adds the options j0 .. j0+7, m the largest of them (kBest: and notes where the largest is)
+template <class R, bool kBest> __device__ inline void stat_add(Stat<R>& a, const R (&y)[kPer], R m, int64_t j0, R k) {
   if (m == Num<R>::kNone) return;
   if (m > a.m) {
     if (kBest) {
@@ -459,9 +470,9 @@ __global__ __launch_bounds__(kThreads) void choose_group(Rows p, int width_log, 
   Stat<double> a = stat_zero<double>();
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    a.bad |= load_ready<T, double, kHist>(p, c, g.row, g.j(k), whole, Seen<double>{n}.at(kHist ? g.j(k) : 0), y[k]);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) a.m = larger(a.m, y[k][i]);
+    double m;
+    a.bad |= load_ready<T, double, kHist>(p, c, g.row, g.j(k), whole, Seen<double>{n}.at(kHist ? g.j(k) : 0), y[k], m);
+    a.m = larger(a.m, m);
   }
   a.m = lanes_max(a.m, g.width);
   a.bad = lanes_max(a.bad, g.width);
@@ -540,10 +551,11 @@ template <class T, int NP, bool kHist> __global__ __launch_bounds__(kThreads) vo
   float y_act = Num<float>::kNone;
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    a.bad |= load_ready<T, float, kHist>(p, c, g.row, g.j(k), whole, Seen<float>{n}.at(kHist ? g.j(k) : 0), y[k]);
+    float m;
+    a.bad |= load_ready<T, float, kHist>(p, c, g.row, g.j(k), whole, Seen<float>{n}.at(kHist ? g.j(k) : 0), y[k], m);
+    a.m = larger(a.m, m);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      a.m = larger(a.m, y[k][i]);
       y_act = act == g.j(k) + i ? y[k][i] : y_act;
     }
   }
@@ -576,9 +588,9 @@ __global__ __launch_bounds__(kThreads) void choose_parts(Rows p, int pieces, int
   for (int64_t j0 = part * pieces * (int64_t)kPiece; j0 < j_end; j0 += kPiece) {
     const auto seen = mem.count(p, c, row, j0);
     const int64_t j = j0 + threadIdx.x * kPer;
-    double y[kPer];
-    a.bad |= load_ready<T, double, kHist>(p, c, row, j, p.vec && j0 + kPiece <= p.options, seen, y);
-    stat_add<double, kBest>(a, y, j, c.k);
+    double y[kPer], m;
+    a.bad |= load_ready<T, double, kHist>(p, c, row, j, p.vec && j0 + kPiece <= p.options, seen, y, m);
+    stat_add<double, kBest>(a, y, m, j, c.k);
   }
   a = stat_block(a, c.k, red);
   if (threadIdx.x == 0) parts[blockIdx.x] = a;
@@ -646,8 +658,8 @@ __global__ __launch_bounds__(kThreads) void choose_join(Rows p, int pieces, int 
     for (int64_t j0 = j_first; j0 < j_end; j0 += kPiece) {
       const auto seen = mem.count(p, c, row, j0);
       const int64_t j = j0 + threadIdx.x * kPer;
-      double y[kPer], w[kPer], sum = 0;
-      (void)load_ready<T, double, kHist>(p, c, row, j, p.vec && j0 + kPiece <= p.options, seen, y);
+      double y[kPer], w[kPer], m, sum = 0;
+      (void)load_ready<T, double, kHist>(p, c, row, j, p.vec && j0 + kPiece <= p.options, seen, y, m);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         w[i] = weight(exponent(y[i], a.m, c.k));
@@ -710,9 +722,9 @@ __global__ __launch_bounds__(kThreads) void evaluate_parts(Rows p, int pieces, i
   for (int64_t j0 = part * pieces * (int64_t)kPiece; j0 < j_end; j0 += kPiece) {
     const auto seen = mem.count(p, c, row, j0);
     const int64_t j = j0 + threadIdx.x * kPer;
-    float y[kPer];
-    a.bad |= load_ready<T, float, kHist>(p, c, row, j, p.vec && j0 + kPiece <= p.options, seen, y);
-    stat_add<float, false>(a, y, j, c.k);
+    float y[kPer], m;
+    a.bad |= load_ready<T, float, kHist>(p, c, row, j, p.vec && j0 + kPiece <= p.options, seen, y, m);
+    stat_add<float, false>(a, y, m, j, c.k);
     if ((uint64_t)(act - j) < kPer) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
@@ -785,10 +797,9 @@ template <bool kHist> __device__ inline GradRow grad_row(const GradArgs& g, cons
 __device__ inline void grad_y(const GradRow& r, const float (&y)[kPer], uint32_t legal, int64_t j, float (&out)[kPer]) {
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const float z = __builtin_amdgcn_fmed3f(y[i], Num<float>::kLow, Num<float>::kHigh);
-    const float d = larger((z - r.m) * r.k - r.log_s, Num<float>::kFloor);
-    const float v = -weight(d) * fmaf(r.lean, d, r.flat);
-    out[i] = bit(legal, i) ? v : 0.f;
+    // (no probability is above 1: a sum that left the range of 32 bits upwards counts as the row's largest)
+    const float d = __builtin_amdgcn_fmed3f(fmaf(y[i] - r.m, r.k, -r.log_s), Num<float>::kFloor, 0.f);
+    out[i] = pick(legal, i, -weight(d) * fmaf(r.lean, d, r.flat), 0.f);
   }
   if ((uint64_t)(r.act - j) < kPer) {
 #pragma unroll
