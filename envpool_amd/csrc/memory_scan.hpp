@@ -67,11 +67,41 @@ template <> struct Mma<bf16> : Mma16<bf16, bf16x8, bf16x4> {
   static constexpr uint32_t kInf = 0x7f80;
   static constexpr bool kNarrow = false;
   static __device__ f32x4 mul(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+  // two values a conversion, and back by shift and mask
+  template <int N> static __device__ void pieces(const float (&v)[8], frag (&out)[N]) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    union { uint32_t w[4]; frag f; } u[N];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f32x2 x = {v[2 * e], v[2 * e + 1]};
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        const uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
+        u[c].w[e] = w;
+        x[0] -= __builtin_bit_cast(float, w << 16);
+        x[1] -= __builtin_bit_cast(float, w & 0xffff0000u);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < N; ++c) out[c] = u[c].f;
+  }
 };
 template <> struct Mma<f16> : Mma16<f16, f16x8, f16x4> {
   static constexpr uint32_t kInf = 0x7c00;
   static constexpr bool kNarrow = true;
   static __device__ f32x4 mul(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  template <int N> static __device__ void pieces(const float (&v)[8], frag (&out)[N], float step = 1.f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float x = v[e];
+#pragma unroll
+      for (int c = 0; c < N; ++c) {
+        out[c][e] = (f16)x;
+        x = (x - (float)out[c][e]) * step;
+      }
+    }
+  }
 };
 // the power of two that brings a largest magnitude of `top` to 2^13 .. 2^14 (1 for 0 and for what is not finite)
 __device__ inline float to_middle(float top) {
@@ -447,18 +477,16 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
       for (int k = 0; k < DK / K; ++k) {
         if (k >= nk) continue;
         // the state rounded, and what that left out
-        frag hi[NV], lo[NV];
+        frag sf[NV][2];
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           if constexpr (sizeof(T) == 2) {
+            float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float x = M::of(s[2 * k][j], s[2 * k + 1][j], e) * s_scale;
-              hi[j][e] = (T)x;
-              lo[j][e] = (T)(x - (float)hi[j][e]);
-            }
+            for (int e = 0; e < 8; ++e) x[e] = M::of(s[2 * k][j], s[2 * k + 1][j], e) * s_scale;
+            M::pieces(x, sf[j]);
           } else {
-            hi[j] = s[k][j];
+            sf[j][0] = s[k][j];
           }
         }
 #pragma unroll
@@ -467,8 +495,8 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
 #pragma unroll
           for (int j = 0; j < NV; ++j) {
             if (!there(j)) continue;
-            a[b][j] = M::mul(hi[j], qf, a[b][j]);
-            if constexpr (sizeof(T) == 2) a[b][j] = M::mul(lo[j], qf, a[b][j]);
+            a[b][j] = M::mul(sf[j][0], qf, a[b][j]);
+            if constexpr (sizeof(T) == 2) a[b][j] = M::mul(sf[j][1], qf, a[b][j]);
           }
         }
         keep_order();
@@ -545,16 +573,12 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           const frag v = M::col(vs, SV, k * K, v0 + 64 * j, ln);
+          float x[K / 4];
 #pragma unroll
-          for (int e = 0; e < K / 4; ++e) {
-            float x = (float)v[e] * w[e];
-#pragma unroll
-            for (int c = 0; c < kPieces; ++c) {
-              vw[j][c][e] = (T)x;
-              x -= (float)vw[j][c][e];
-              if (M::kNarrow) x *= 2048.f;
-            }
-          }
+          for (int e = 0; e < K / 4; ++e) x[e] = (float)v[e] * w[e];
+          if constexpr (M::kNarrow) M::pieces(x, vw[j], 2048.f);
+          else if constexpr (sizeof(T) == 2) M::pieces(x, vw[j]);
+          else vw[j][0] = frag{x[0], x[1], x[2], x[3]};
         }
         keep_order();
 #pragma unroll
