@@ -42,13 +42,14 @@ template <class T> int per_cu_of(int dk, int dv) {
   return dk <= 64 ? (dv <= 64 ? ScanTile<T, 64, 64>::kPerCu : ScanTile<T, 64, 128>::kPerCu)
                   : (dv <= 64 ? ScanTile<T, 128, 64>::kPerCu : ScanTile<T, 128, 128>::kPerCu);
 }
+int64_t chunk_steps(int32_t dtype) { return dtype == EP_F32 ? epm::ChunkOf<float>::value : epm::ChunkOf<epm::bf16>::value; }
 int64_t per_cu(int32_t dtype, int dk, int dv) { return dtype == EP_F32 ? per_cu_of<float>(dk, dv) : per_cu_of<epm::bf16>(dk, dv); }
 
 // Split of the time axis. One part per state keeps everything single-pass. With fewer states than the chip holds at
 // once, the axis is cut into parts that are walked side by side: keys and values are then read twice (first for the
 // states between the parts), which counts as 1.6 times the chunks plus the join.
 int64_t scan_parts(const ep_memory_scan_args* a) {
-  const int64_t states = a->rows * a->heads, chunks = (a->steps + epm::kChunk - 1) / epm::kChunk;
+  const int64_t states = a->rows * a->heads, chunk = chunk_steps(a->dtype), chunks = (a->steps + chunk - 1) / chunk;
   if (states <= 0 || chunks < 2) return 1;
   const int64_t slots = 256 * per_cu(a->dtype, a->key_dim, a->value_dim);  // workgroups that run at once
   if (states * 2 > slots) return 1;
@@ -64,9 +65,9 @@ int64_t scan_workspace(const ep_memory_scan_args* a, int64_t n_seg) {
 
 int scan_launch(const ep_memory_scan_args* a, const epm::Scan& k, hipStream_t stream) {
   epm::Parts parts{};
-  const int64_t chunks = std::max<int64_t>(1, (a->steps + epm::kChunk - 1) / epm::kChunk);
+  const int64_t chunk = chunk_steps(a->dtype), chunks = std::max<int64_t>(1, (a->steps + chunk - 1) / chunk);
   const int64_t want = scan_parts(a), per = (chunks + want - 1) / want;
-  parts.seg_len = per * epm::kChunk;
+  parts.seg_len = per * chunk;
   parts.n_seg = (int32_t)((chunks + per - 1) / per);
   if (parts.n_seg > 1) {
     parts.ws_state = (epm::f32x4*)a->workspace;
@@ -77,7 +78,7 @@ int scan_launch(const ep_memory_scan_args* a, const epm::Scan& k, hipStream_t st
   // 16-byte pieces (results: 4 values), rows that follow one another, and a chunk within 2^31 bytes
   const auto aligned = [&](const void* ptr, const int64_t* stride, int64_t width, int64_t unit, int64_t bytes) {
     return (uintptr_t)ptr % unit == 0 && stride[0] * bytes % unit == 0 && stride[1] * bytes % unit == 0 && stride[2] * bytes % unit == 0 &&
-           stride[0] >= width && stride[0] * bytes <= (int64_t(1) << 31) / epm::kChunk;
+           stride[0] >= width && stride[0] * bytes <= (int64_t(1) << 31) / 64;
   };
   const auto state_near = [&](const void* ptr, const int64_t* stride) {
     return !ptr || (stride[2] >= 0 && stride[3] >= 0 && stride[2] < (1 << 20) && stride[3] < (1 << 20));

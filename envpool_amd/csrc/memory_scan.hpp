@@ -1,14 +1,14 @@
 // memory_scan.hpp - the chunked form of the memory on matrix cores.
 //
-// A workgroup of four waves owns one state (row, head) and walks along time in chunks of 64 steps. Inside a
-// chunk, with D[t, s] = decay^|t-s| where s reaches t (no episode starts between them), else 0:
-//   P = (Q K^T) * D                       scores, 64 x 64
+// A workgroup of four waves owns one state (row, head) and walks along time in chunks of 32 or 64 steps. Inside
+// a chunk, with D[t, s] = decay^|t-s| where s reaches t (no episode starts between them), else 0:
+//   P = (Q K^T) * D                       scores, steps x steps
 //   O = w_in[t] * (Q S) + P V             S: the state the chunk starts from
 //   S = carry * S + (K * w_up[s])^T V
 // Everything is computed transposed (scores as [s, t], outputs as [v, t]): the accumulators of one product are
 // then laid out as an operand of the next up to a permutation of the summed index, which is applied to the
 // other operand as well. So the state never leaves its registers (32 bits; a copy rounded to the operands' type
-// feeds Q S), scores cross LDS once because each wave computes 16 of the 64 query columns and needs all of
+// feeds Q S), scores cross LDS once because each wave computes 16 of the query columns and needs all of
 // them for its quarter of the value columns, and an output row is written 4 values a lane.
 // Time backwards (for gradients) is the same chunk with the triangle and the weights mirrored.
 #pragma once
@@ -17,7 +17,11 @@
 namespace epm {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-constexpr int kChunk = 64;
+// Steps per chunk. In 32 bits the matrix cores are the bound and half the chunk halves the work inside it (and lets
+// two workgroups share a CU); in 16 bits memory is, and the longer chunk moves the state less often.
+template <class T> struct ChunkOf {
+  static constexpr int value = sizeof(T) == 4 ? 32 : 64;
+};
 
 template <class T> struct Mma;
 
@@ -146,7 +150,7 @@ template <bool kSkips> __device__ inline void settle() {
 
 // how a launch's states come and go
 struct Parts {
-  int64_t seg_len;     // steps per part of the time axis (a multiple of 64), blockIdx.y counts parts in time
+  int64_t seg_len;     // steps per part of the time axis (whole chunks), blockIdx.y counts parts in time
   int32_t n_seg;
   f32x4* ws_state;     // [row * heads][n_seg][DK * DV / 4] in accumulator order: what a part starts from (read), or
   float* ws_carry;     // its own contribution and how far it lets the state before it through (written)
@@ -155,6 +159,7 @@ struct Parts {
 };
 
 template <class T, int DK, int DV> struct ScanTile {
+  static constexpr int kChunk = ChunkOf<T>::value;
   static constexpr int kVec = 16 / sizeof(T);                // values of one 16-byte load
   // LDS row strides. 16 bytes of padding let 16 lanes read 16 bytes of a row each without a bank twice; the
   // transposing reads take 32 bytes of 4 rows, which 32 bytes of padding keep apart
@@ -163,9 +168,9 @@ template <class T, int DK, int DV> struct ScanTile {
   static constexpr int kQ = kChunk * DK / kVec / 256;        // 16-byte loads per thread and tile
   static constexpr int kV = kChunk * DV / kVec / 256;
   static constexpr size_t kLds = (size_t)kChunk * (SQ + SK + SV + SP) * sizeof(T) + 4 * kChunk * sizeof(float);
-  // workgroups (one wave per SIMD each) that LDS lets a CU hold: the registers are kept to as many (value-by-value
-  // addressing needs more of them: half as many)
-  static constexpr int kPerCu = (int)(163840 / kLds);
+  // workgroups (one wave per SIMD each) that LDS lets a CU hold, three at most in 32 bits (whose operands take twice
+  // the registers): the registers are kept to as many (value-by-value addressing needs more of them: half as many)
+  static constexpr int kFit = (int)(163840 / kLds), kPerCu = sizeof(T) == 4 && kFit > 3 ? 3 : kFit;
   static constexpr int kWaves(bool aligned) { return aligned || kPerCu == 1 ? kPerCu : kPerCu / 2; }
 };
 
@@ -204,6 +209,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
   using M = Mma<T>;
   using Tile = ScanTile<T, DK, DV>;
   using frag = typename M::frag;
+  constexpr int kChunk = Tile::kChunk, kBlocks = kChunk / 16;
   constexpr int K = M::K, kVec = Tile::kVec, SQ = Tile::SQ, SK = Tile::SK, SV = Tile::SV, SP = Tile::SP;
   constexpr int ND = DK / 16, NV = DV / 64;  // state tiles of a wave: all keys, a quarter of the values
   extern __shared__ __align__(16) char lds[];
@@ -378,15 +384,17 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
     if (n_next > 0) load(start_next, n_next);
 
     if (threadIdx.x < 2 * kChunk) {
-      const int t = threadIdx.x & 63;
+      const int t = threadIdx.x % kChunk;
       const uint64_t until = starts & ((2ull << t) - 1), later = t < 63 ? starts >> (t + 1) : 0;
       const float from_0 = __builtin_amdgcn_exp2f(l2 * (t + 1)), to_end = __builtin_amdgcn_exp2f(l2 * (n_now - 1 - t));
       if (threadIdx.x < kChunk) w_up[t] = t < n_now && (rev ? until : later) == 0 ? (rev ? from_0 : to_end) * (M::kNarrow ? 1.f : p.inc_scale) : 0.f;
       else w_in[t] = t < n_now && (rev ? later : until) == 0 ? (rev ? to_end : from_0) * p.out_scale : 0.f;
     }
     if (!parts.state_only) {
-      // ---- scores of 16 query steps per wave
-      const int t = 16 * wave + l16;
+      // ---- scores: 16 query steps per wave, or per two that take every other tile of them
+      constexpr int kShare = 4 / kBlocks;
+      static_assert(kShare == 1 || !M::kNarrow, "a step's largest score is found within one wave");
+      const int strip = wave % kBlocks, t = 16 * strip + l16;
       int lo, hi;  // the steps that reach step t
       if (rev) {
         const uint64_t later = t < 63 ? starts >> (t + 1) : 0;
@@ -399,23 +407,24 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
       }
       frag q[DK / K];
 #pragma unroll
-      for (int k = 0; k < DK / K; ++k) q[k] = M::row(qs, SQ, 16 * wave, k * K, ln);
+      for (int k = 0; k < DK / K; ++k) q[k] = M::row(qs, SQ, 16 * strip, k * K, ln);
       // (all tiles of whole fragments, so that what lies across the diagonal is 0)
-      const int i0 = rev ? (16 * wave) / K * K / 16 : 0, i1 = rev ? kChunk / 16 : ((16 * wave) / K + 1) * K / 16;
+      const int i0 = rev ? (16 * strip) / K * K / 16 : 0, i1 = rev ? kChunk / 16 : ((16 * strip) / K + 1) * K / 16;
       const float scale = p.inc_scale * p.out_scale;
-      f32x4 score[4];
+      f32x4 score[kBlocks];
       float top = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < kBlocks; ++i) {
+        if (kShare > 1 && i % kShare != wave / kBlocks) continue;
         f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (rev ? i >= wave : i <= wave) {
+        if (rev ? i >= strip : i <= strip) {
 #pragma unroll
           for (int k = 0; k < DK / K; ++k)
             if (k < nk) a = M::mul(M::row(ks, SK, 16 * i, k * K, ln), q[k], a);
           settle<kTrim>();
           const int u = 16 * i + 4 * g;
           f32x4 w;
-          if (i == wave) {
+          if (i == strip) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) w[r] = __builtin_amdgcn_exp2f(l2 * (float)(rev ? u + r - t : t - u - r)) * scale;
           } else if (rev) {  // the nearest of the four, then one decay each
@@ -442,7 +451,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
         const float f = to_middle(top);
         if (g == 0) p_top[t] = f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < kBlocks; ++i)
           if (i >= i0 && i < i1) M::put4(ps + t * SP + 16 * i + 4 * g, score[i] * f);
       }
     }
@@ -455,9 +464,9 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
     const auto there = [&](int j) { return !kTrim || v0 + 64 * j < p.dv; };  // (the same for the whole wave)
     if (!parts.state_only) {
       // ---- outputs: what the entering state gives, then the chunk's own steps
-      f32x4 a[4][NV];
+      f32x4 a[kBlocks][NV];
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
+      for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
         for (int j = 0; j < NV; ++j) a[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
       float s_scale = 1.f;
@@ -490,7 +499,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
           }
         }
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
+        for (int b = 0; b < kBlocks; ++b) {
           const frag qf = M::row_as_acc(qs, SQ, 16 * b, k * K, ln);
 #pragma unroll
           for (int j = 0; j < NV; ++j) {
@@ -508,7 +517,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
 #pragma unroll
         for (int k = 0; k < kChunk / K; ++k) vf[j][k] = M::col(vs, SV, k * K, v0 + 64 * j, ln);
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
+      for (int b = 0; b < kBlocks; ++b) {
         const int t = 16 * b + l16;
         const float f = M::kNarrow ? p_top[t] : 1.f;
         const float w = w_in[t], ws_ = w * f / s_scale;
