@@ -35,15 +35,23 @@ int64_t step_workspace(const ep_memory_step_args* a) {
   return a->env_id && a->rows > kLookThrough ? a->num_envs * 4 : 0;
 }
 
-int padded(int dim) { return dim <= 64 ? 64 : 128; }
+// the sizes of the kernel that a call's sizes run in (epm::scan_sizes chooses the same)
+struct Padded {
+  int dk, dv;
+  int64_t state() const { return (int64_t)dk * dv; }
+};
+Padded padded(const ep_memory_scan_args* a) {
+  const int dk = a->key_dim <= 64 ? 64 : 128;
+  return {dk, a->value_dim <= 64 && (dk == 64 || a->dtype != EP_F32) ? 64 : 128};
+}
 
-template <class T> int per_cu_of(int dk, int dv) {
+template <class T> int per_cu_of(Padded d) {
   using namespace epm;
-  return dk <= 64 ? (dv <= 64 ? ScanTile<T, 64, 64>::kPerCu : ScanTile<T, 64, 128>::kPerCu)
-                  : (dv <= 64 ? ScanTile<T, 128, 64>::kPerCu : ScanTile<T, 128, 128>::kPerCu);
+  return d.dk == 64 ? (d.dv == 64 ? ScanTile<T, 64, 64>::kPerCu : ScanTile<T, 64, 128>::kPerCu)
+                    : (d.dv == 64 ? ScanTile<T, 128, 64>::kPerCu : ScanTile<T, 128, 128>::kPerCu);
 }
 int64_t chunk_steps(int32_t dtype) { return dtype == EP_F32 ? epm::ChunkOf<float>::value : epm::ChunkOf<epm::bf16>::value; }
-int64_t per_cu(int32_t dtype, int dk, int dv) { return dtype == EP_F32 ? per_cu_of<float>(dk, dv) : per_cu_of<epm::bf16>(dk, dv); }
+int64_t per_cu(const ep_memory_scan_args* a) { return a->dtype == EP_F32 ? per_cu_of<float>(padded(a)) : per_cu_of<epm::bf16>(padded(a)); }
 
 // Split of the time axis. One part per state keeps everything single-pass. With fewer states than the chip holds at
 // once, the axis is cut into parts that are walked side by side: keys and values are then read twice (first for the
@@ -51,7 +59,7 @@ int64_t per_cu(int32_t dtype, int dk, int dv) { return dtype == EP_F32 ? per_cu_
 int64_t scan_parts(const ep_memory_scan_args* a) {
   const int64_t states = a->rows * a->heads, chunk = chunk_steps(a->dtype), chunks = (a->steps + chunk - 1) / chunk;
   if (states <= 0 || chunks < 2) return 1;
-  const int64_t slots = 256 * per_cu(a->dtype, a->key_dim, a->value_dim);  // workgroups that run at once
+  const int64_t slots = 256 * per_cu(a);  // workgroups that run at once
   if (states * 2 > slots) return 1;
   const int64_t per = std::max<int64_t>((chunks * states + slots - 1) / slots, (chunks + 65534) / 65535);
   const int64_t parts = (chunks + per - 1) / per;
@@ -60,7 +68,7 @@ int64_t scan_parts(const ep_memory_scan_args* a) {
 }
 int64_t scan_workspace(const ep_memory_scan_args* a, int64_t n_seg) {
   if (n_seg <= 1) return 0;
-  return a->rows * a->heads * n_seg * ((int64_t)padded(a->key_dim) * padded(a->value_dim) * 4 + 4);
+  return a->rows * a->heads * n_seg * (padded(a).state() * 4 + 4);
 }
 
 int scan_launch(const ep_memory_scan_args* a, const epm::Scan& k, hipStream_t stream) {
@@ -71,7 +79,7 @@ int scan_launch(const ep_memory_scan_args* a, const epm::Scan& k, hipStream_t st
   parts.n_seg = (int32_t)((chunks + per - 1) / per);
   if (parts.n_seg > 1) {
     parts.ws_state = (epm::f32x4*)a->workspace;
-    parts.ws_carry = (float*)((char*)a->workspace + a->rows * a->heads * parts.n_seg * ((int64_t)padded(a->key_dim) * padded(a->value_dim) * 4));
+    parts.ws_carry = (float*)((char*)a->workspace + a->rows * a->heads * parts.n_seg * (padded(a).state() * 4));
   }
   const int64_t size = size_of(a->dtype), per_load = 16 / size;
   const int64_t out_size = size_of(a->out_dtype);

@@ -107,10 +107,12 @@ template <> struct Mma<f16> : Mma16<f16, f16x8, f16x4> {
     }
   }
 };
-// the power of two that brings a largest magnitude of `top` to 2^13 .. 2^14 (1 for 0 and for what is not finite)
+// the power of two that brings a largest magnitude of `top` to 2^13 .. 2^14 (1 for 0 and for what is not finite; not
+// beyond 2^40 or below 2^-60, so that two of them against each other stay in the range of 32 bits: what is that
+// small is 0 in a float16 result, what is that large infinite)
 __device__ inline float to_middle(float top) {
   const int e = __builtin_amdgcn_frexp_expf(top);
-  return top > 0.f && top < INFINITY ? __builtin_amdgcn_ldexpf(1.f, max(-120, min(120, 14 - e))) : 1.f;
+  return top > 0.f && top < INFINITY ? __builtin_amdgcn_ldexpf(1.f, max(-60, min(40, 14 - e))) : 1.f;
 }
 template <> struct Mma<float> {
   using frag = f32x4;
@@ -202,52 +204,40 @@ __device__ inline __amdgpu_buffer_rsrc_t buffer(const void* base, int64_t bytes)
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-// How a launch addresses: kAligned: every operand in 16-byte pieces through buffers (offsets below 2^31, rows that do
-// not overlap); otherwise value by value.
-template <class T, int DK, int DV, bool kAligned, bool rev>
-__global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void scan_chunks(Scan p, Parts parts) {
+// What the workgroup knows about the chunk it is at.
+struct Now {
+  uint64_t starts;  // bit t: step t starts an episode
+  int64_t start;    // its first step
+  int n;            // its steps
+  float l2;         // log2 of the decay
+  float lambda;
+  int ln, wave;     // lane and wave
+  float *w_up, *w_in, *p_top;
+};
+
+// The pieces of a walk in one direction. kAligned: every operand in 16-byte pieces through buffers (offsets below
+// 2^31, rows that do not overlap); otherwise value by value.
+template <class T, int DK, int DV, bool kAligned, bool rev> struct Walk {
   using M = Mma<T>;
   using Tile = ScanTile<T, DK, DV>;
   using frag = typename M::frag;
-  constexpr int kChunk = Tile::kChunk, kBlocks = kChunk / 16;
-  constexpr int K = M::K, kVec = Tile::kVec, SQ = Tile::SQ, SK = Tile::SK, SV = Tile::SV, SP = Tile::SP;
-  constexpr int ND = DK / 16, NV = DV / 64;  // state tiles of a wave: all keys, a quarter of the values
-  extern __shared__ __align__(16) char lds[];
-  T* qs = (T*)lds;
-  T* ks = qs + kChunk * SQ;
-  T* vs = ks + kChunk * SK;
-  T* ps = vs + kChunk * SV;
-  float* w_up = (float*)(ps + kChunk * SP);  // weight of a step in the state that leaves the chunk
-  float* w_in = w_up + kChunk;               // and of the state that enters it in a step's output
-  float* p_top = w_in + kChunk;              // kNarrow: what a step's scores were multiplied by
-  int* odd = (int*)(p_top + kChunk);         // a key or value of this chunk is not finite
-
-  const int64_t rh = blockIdx.x;
-  const int64_t row = rh / p.heads;
-  const int h = (int)(rh % p.heads);
-  // (of the contributions only those are needed that a later part starts from)
-  const int seg = blockIdx.y + (parts.state_only && rev ? 1 : 0);
-  const int lane = threadIdx.x & 63, g = lane >> 4, l16 = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int v0 = 16 * wave;  // this wave's value columns: 16 of every 64
-  const float log2_decay = fmaxf(p.log_decay[h] * 1.44269504088896f, -1e30f);  // (decay 0: its power 0 is still 1)
-  const float lambda = __builtin_amdgcn_exp2f(log2_decay);
+  static constexpr int kChunk = Tile::kChunk, kBlocks = kChunk / 16;
+  static constexpr int K = M::K, kVec = Tile::kVec, SP = Tile::SP;
+  static constexpr int ND = DK / 16, NV = DV / 64;  // state tiles of a wave: all keys, 16 of every 64 value columns
   // tiles that the operands' sizes reach (in 32 bits the matrix cores are the bound, so padding is not multiplied)
-  constexpr bool kTrim = sizeof(T) == 4;
-  const int nk = kTrim ? (p.dk + K - 1) / K : DK / K, nd = kTrim ? (p.dk + 15) / 16 : ND;
+  static constexpr bool kTrim = sizeof(T) == 4 && kAligned;
+  // (opaque, or the compiler makes a copy of everything that follows for every number of tiles)
+  static __device__ int tiles(int dim, int unit, int all) {
+    if constexpr (!kTrim) return all;
+    int n = (dim + unit - 1) / unit;
+    asm volatile("" : "+s"(n));
+    return n;
+  }
+  static __device__ int nk(const Scan& p) { return tiles(p.dk, K, DK / K); }
+  static __device__ int nd(const Scan& p) { return tiles(p.dk, 16, ND); }
+  using State = f32x4[ND][NV];
 
-  const T* gq = (const T*)p.q + row * p.q_stride[1] + (h / p.q_group) * p.q_stride[2];
-  const T* gk = (const T*)p.k + row * p.k_stride[1] + (h / p.k_group) * p.k_stride[2];
-  const T* gv = (const T*)p.v + row * p.v_stride[1] + (h / p.v_group) * p.v_stride[2];
-  const uint8_t* gf = p.fresh ? p.fresh + row * p.fresh_stride[1] : nullptr;
-
-  const int64_t seg0 = seg * parts.seg_len;
-  const int64_t seg1 = seg0 + parts.seg_len < p.steps ? seg0 + parts.seg_len : p.steps;
-
-  // ---- a chunk's tiles, on their way from memory
-  uint4 rq[Tile::kQ], rk[Tile::kQ], rv[Tile::kV];
-  uint8_t rf = 0;
-  const auto load_tile = [&](uint4* r, int count, const T* base, int64_t step_stride, int width, int padded, int64_t start, int n) {
+  static __device__ void load_tile(uint4* r, int count, const T* base, int64_t step_stride, int width, int padded, int64_t start, int n) {
     const int per_row = padded / kVec;
     if constexpr (kAligned) {
       const auto b = buffer(base + start * step_stride, ((n - 1) * step_stride + width) * (int64_t)sizeof(T));
@@ -275,20 +265,14 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
         r[i] = x.u;
       }
     }
-  };
-  const auto load = [&](int64_t start, int n) {
-    load_tile(rk, Tile::kQ, gk, p.k_stride[0], p.dk, DK, start, n);
-    load_tile(rv, Tile::kV, gv, p.v_stride[0], p.dv, DV, start, n);
-    if (!parts.state_only) load_tile(rq, Tile::kQ, gq, p.q_stride[0], p.dk, DK, start, n);
-    rf = gf && lane < n ? gf[(start + lane) * p.fresh_stride[0]] : 0;
-  };
-  const auto put_tile = [&](const uint4* r, int count, T* tile, int padded, int stride) {
+  }
+  static __device__ void put_tile(const uint4* r, int count, T* tile, int padded, int stride) {
     const int per_row = padded / kVec;
     T* to = tile + (threadIdx.x / per_row) * stride + (threadIdx.x % per_row) * kVec;
 #pragma unroll
     for (int i = 0; i < count; ++i) *(uint4*)(to + i * (256 / per_row) * stride) = r[i];
-  };
-  const auto top_of = [&](uint32_t top, const uint4* r, int count) {
+  }
+  static __device__ uint32_t top_of(uint32_t top, const uint4* r, int count) {
 #pragma unroll
     for (int i = 0; i < count; ++i) {
       top = top_bits<T>(top, r[i].x);
@@ -297,26 +281,10 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
       top = top_bits<T>(top, r[i].w);
     }
     return top;
-  };
+  }
 
-  int64_t start = rev ? seg1 - (seg1 - seg0 < kChunk ? seg1 - seg0 : kChunk) : seg0;
-  int n = (int)(seg1 - seg0 < kChunk ? seg1 - seg0 : kChunk);
-  if (threadIdx.x == 0) *odd = 0;
-  if (n > 0) load(start, n);
-
-  // ---- the state the part starts from
-  f32x4 s[ND][NV];
-  f32x4* ws = parts.ws_state ? parts.ws_state + (rh * parts.n_seg + seg) * (DK * DV / 4) : nullptr;
-#pragma unroll
-  for (int i = 0; i < ND; ++i)
-#pragma unroll
-    for (int j = 0; j < NV; ++j) s[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (!parts.state_only && parts.n_seg > 1) {
-#pragma unroll
-    for (int i = 0; i < ND; ++i)
-#pragma unroll
-      for (int j = 0; j < NV; ++j) s[i][j] = ws[((i * NV + j) * 4 + wave) * 64 + lane];
-  } else if (!parts.state_only && p.state_in) {
+  static __device__ void load_state(const Scan& p, bool state_vec, int64_t row, int h, int lane, int wave, State& s) {
+    const int v0 = 16 * wave, g = lane >> 4, l16 = lane & 15;
     const float* base = p.state_in + row * p.in_stride[0] + h * p.in_stride[1];
 #pragma unroll
     for (int i = 0; i < ND; ++i)
@@ -327,7 +295,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
           const auto b = buffer(base, 0x7fffffff);
           const uint32_t sd = (uint32_t)p.in_stride[2] * 4u, sv = (uint32_t)p.in_stride[3] * 4u;
           const uint32_t at = v < p.dv && d < p.dk ? d * sd + v * sv : kOutside;
-          if (sd == 4 && parts.state_vec) {
+          if (sd == 4 && state_vec) {
             union { u32x4 u; f32x4 f; } x;
             x.u = __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0);
             s[i][j] = x.f;
@@ -342,226 +310,221 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
         }
       }
   }
-  float through = 1.f;
+  static __device__ void store_state(const Scan& p, int64_t row, int h, int lane, int wave, const State& s) {
+    const int v0 = 16 * wave, g = lane >> 4, l16 = lane & 15;
+    float* base = p.state_out + row * p.outs_stride[0] + h * p.outs_stride[1];
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int v = v0 + 64 * j + l16, d = 16 * i + 4 * g;
+        if constexpr (kAligned) {
+          const auto b = buffer(base, 0x7fffffff);
+          const uint32_t sd = (uint32_t)p.outs_stride[2] * 4u, sv = (uint32_t)p.outs_stride[3] * 4u;
+          const uint32_t at = v < p.dv && d < p.dk ? d * sd + v * sv : kOutside;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, (float)s[i][j][r]), b, at + r * sd, 0, 0);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (v < p.dv && d + r < p.dk) base[(d + r) * p.outs_stride[2] + v * p.outs_stride[3]] = s[i][j][r];
+        }
+      }
+  }
 
-  while (n > 0) {
-    // (opaque to the compiler here, or it would keep every step's powers of the decay, and every address, in
-    // registers across the loop)
-    float l2 = log2_decay;
-    int ln = lane;
-    asm volatile("" : "+v"(l2), "+v"(ln));
-    const int g = ln >> 4, l16 = ln & 15;
-    __syncthreads();  // (the tiles of the chunk before have been read)
-    if (!parts.state_only) put_tile(rq, Tile::kQ, qs, DK, SQ);
-    put_tile(rk, Tile::kQ, ks, DK, SK);
-    put_tile(rv, Tile::kV, vs, DV, SV);
-    uint64_t starts = __ballot(rf != 0);  // bit t: step t starts an episode
-    if (starts && not_finite<T>(top_of(top_of(0, rk, Tile::kQ), rv, Tile::kV))) *odd = 1;
-    __syncthreads();
-    if (starts && *odd) {
-      // 0 * inf would carry what is not finite across the start of an episode: such a chunk ends there
-      // (its outer episode first), and the rest is a chunk of its own
-      __syncthreads();
-      if (threadIdx.x == 0) *odd = 0;
-      int from = 0, to = n;
-      if (rev) from = 63 - __clzll(starts);
-      else if ((starts & ~1ull) != 0) to = __ffsll((unsigned long long)(starts & ~1ull)) - 1;
-      start += from;
-      n = to - from;
-      load(start, n);
-      if (!parts.state_only) put_tile(rq, Tile::kQ, qs, DK, SQ);
-      put_tile(rk, Tile::kQ, ks, DK, SK);
-      put_tile(rv, Tile::kV, vs, DV, SV);
-      starts = __ballot(rf != 0);
-      __syncthreads();
-    }
-    // the next chunk's loads run under this one's products
-    const int64_t left = rev ? start - seg0 : seg1 - (start + n);
-    const int n_next = (int)(left < kChunk ? left : kChunk);
-    const int64_t start_next = rev ? start - n_next : start + n;
-    const int n_now = n;
-    const int64_t start_now = start;
-    if (n_next > 0) load(start_next, n_next);
-
+  // the weights of the chunk's steps: in the state that leaves it, and of the state that enters it in their outputs
+  static __device__ void weights(const Scan& p, const Now& c) {
     if (threadIdx.x < 2 * kChunk) {
       const int t = threadIdx.x % kChunk;
-      const uint64_t until = starts & ((2ull << t) - 1), later = t < 63 ? starts >> (t + 1) : 0;
-      const float from_0 = __builtin_amdgcn_exp2f(l2 * (t + 1)), to_end = __builtin_amdgcn_exp2f(l2 * (n_now - 1 - t));
-      if (threadIdx.x < kChunk) w_up[t] = t < n_now && (rev ? until : later) == 0 ? (rev ? from_0 : to_end) * (M::kNarrow ? 1.f : p.inc_scale) : 0.f;
-      else w_in[t] = t < n_now && (rev ? later : until) == 0 ? (rev ? to_end : from_0) * p.out_scale : 0.f;
+      const uint64_t until = c.starts & ((2ull << t) - 1), later = t < 63 ? c.starts >> (t + 1) : 0;
+      const float from_0 = __builtin_amdgcn_exp2f(c.l2 * (t + 1)), to_end = __builtin_amdgcn_exp2f(c.l2 * (c.n - 1 - t));
+      if (threadIdx.x < kChunk) c.w_up[t] = t < c.n && (rev ? until : later) == 0 ? (rev ? from_0 : to_end) * (M::kNarrow ? 1.f : p.inc_scale) : 0.f;
+      else c.w_in[t] = t < c.n && (rev ? later : until) == 0 ? (rev ? to_end : from_0) * p.out_scale : 0.f;
     }
-    if (!parts.state_only) {
-      // ---- scores: 16 query steps per wave, or per two that take every other tile of them
-      constexpr int kShare = 4 / kBlocks;
-      static_assert(kShare == 1 || !M::kNarrow, "a step's largest score is found within one wave");
-      const int strip = wave % kBlocks, t = 16 * strip + l16;
-      int lo, hi;  // the steps that reach step t
-      if (rev) {
-        const uint64_t later = t < 63 ? starts >> (t + 1) : 0;
-        lo = t;
-        hi = later ? t + __ffsll((unsigned long long)later) - 1 : kChunk - 1;
-      } else {
-        const uint64_t until = starts & ((2ull << t) - 1);
-        lo = until ? 63 - __clzll(until) : 0;
-        hi = t;
-      }
-      frag q[DK / K];
+  }
+
+  // scores of 16 query steps per wave, or per two waves that take every other tile of them
+  static __device__ void scores(const Scan& p, const Now& c, const T* qs, int SQ, const T* ks, int SK, T* ps) {
+    const int wave = c.wave, ln = c.ln, g = ln >> 4, l16 = ln & 15, nk = Walk::nk(p);
+    const uint64_t starts = c.starts;
+    const float l2 = c.l2, lambda = c.lambda;
+    float* p_top = c.p_top;
+    constexpr int kShare = 4 / kBlocks;
+    static_assert(kShare == 1 || !M::kNarrow, "a step's largest score is found within one wave");
+    const int strip = wave % kBlocks, t = 16 * strip + l16;
+    int lo, hi;  // the steps that reach step t
+    if (rev) {
+      const uint64_t later = t < 63 ? starts >> (t + 1) : 0;
+      lo = t;
+      hi = later ? t + __ffsll((unsigned long long)later) - 1 : kChunk - 1;
+    } else {
+      const uint64_t until = starts & ((2ull << t) - 1);
+      lo = until ? 63 - __clzll(until) : 0;
+      hi = t;
+    }
+    frag q[DK / K];
 #pragma unroll
-      for (int k = 0; k < DK / K; ++k) q[k] = M::row(qs, SQ, 16 * strip, k * K, ln);
-      // (all tiles of whole fragments, so that what lies across the diagonal is 0)
-      const int i0 = rev ? (16 * strip) / K * K / 16 : 0, i1 = rev ? kChunk / 16 : ((16 * strip) / K + 1) * K / 16;
-      const float scale = p.inc_scale * p.out_scale;
-      f32x4 score[kBlocks];
+    for (int k = 0; k < DK / K; ++k) q[k] = M::row(qs, SQ, 16 * strip, k * K, ln);
+    // (all tiles of whole fragments, so that what lies across the diagonal is 0)
+    const int i0 = rev ? (16 * strip) / K * K / 16 : 0, i1 = rev ? kChunk / 16 : ((16 * strip) / K + 1) * K / 16;
+    const float scale = p.inc_scale * p.out_scale;
+    f32x4 score[kBlocks];
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < kBlocks; ++i) {
+      if (kShare > 1 && i % kShare != wave / kBlocks) continue;
+      f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (rev ? i >= strip : i <= strip) {
+#pragma unroll
+        for (int k = 0; k < DK / K; ++k)
+          if (k < nk) a = M::mul(M::row(ks, SK, 16 * i, k * K, ln), q[k], a);
+        settle<kTrim>();
+        const int u = 16 * i + 4 * g;
+        f32x4 w;
+        if (i == strip) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) w[r] = __builtin_amdgcn_exp2f(l2 * (float)(rev ? u + r - t : t - u - r)) * scale;
+        } else if (rev) {  // the nearest of the four, then one decay each
+          w[0] = __builtin_amdgcn_exp2f(l2 * (float)(u - t)) * scale;
+          w[1] = w[0] * lambda, w[2] = w[1] * lambda, w[3] = w[2] * lambda;
+        } else {
+          w[3] = __builtin_amdgcn_exp2f(l2 * (float)(t - u - 3)) * scale;
+          w[2] = w[3] * lambda, w[1] = w[2] * lambda, w[0] = w[1] * lambda;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) a[r] = u + r >= lo && u + r <= hi ? a[r] * w[r] : 0.f;
+      }
+      if constexpr (M::kNarrow) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf(a[r]));
+        score[i] = a;
+      } else if (i >= i0 && i < i1) {
+        M::put4(ps + t * SP + 16 * i + 4 * g, a);
+      }
+    }
+    if constexpr (M::kNarrow) {
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float f = to_middle(top);
+      if (g == 0) p_top[t] = f;
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i)
+        if (i >= i0 && i < i1) M::put4(ps + t * SP + 16 * i + 4 * g, score[i] * f);
+    }
+  }
+
+  // outputs: what the entering state gives, then the chunk's own steps
+  static __device__ void outputs(const Scan& p, const Now& c, int64_t row, int h, const State& s, const T* qs, int SQ, const T* vs, int SV, const T* ps) {
+    const int wave = c.wave, ln = c.ln, g = ln >> 4, l16 = ln & 15, v0 = 16 * wave, nk = Walk::nk(p), n_now = c.n;
+    const float *w_in = c.w_in, *p_top = c.p_top;
+    const uint32_t out_size = p.out_f32 ? 4u : (uint32_t)sizeof(T);
+    const T* out_row = (const T*)((const char*)p.out + (c.start * p.out_stride[0] + row * p.out_stride[1] + h * p.out_stride[2]) * (int64_t)out_size);
+    const auto there = [&](int j) { return !kTrim || j == 0 || v0 + 64 * j < p.dv; };  // (the same for the whole wave)
+    f32x4 a[kBlocks][NV];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) a[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float s_scale = 1.f;
+    if constexpr (M::kNarrow) {
       float top = 0.f;
 #pragma unroll
-      for (int i = 0; i < kBlocks; ++i) {
-        if (kShare > 1 && i % kShare != wave / kBlocks) continue;
-        f32x4 a = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (rev ? i >= strip : i <= strip) {
-#pragma unroll
-          for (int k = 0; k < DK / K; ++k)
-            if (k < nk) a = M::mul(M::row(ks, SK, 16 * i, k * K, ln), q[k], a);
-          settle<kTrim>();
-          const int u = 16 * i + 4 * g;
-          f32x4 w;
-          if (i == strip) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) w[r] = __builtin_amdgcn_exp2f(l2 * (float)(rev ? u + r - t : t - u - r)) * scale;
-          } else if (rev) {  // the nearest of the four, then one decay each
-            w[0] = __builtin_amdgcn_exp2f(l2 * (float)(u - t)) * scale;
-            w[1] = w[0] * lambda, w[2] = w[1] * lambda, w[3] = w[2] * lambda;
-          } else {
-            w[3] = __builtin_amdgcn_exp2f(l2 * (float)(t - u - 3)) * scale;
-            w[2] = w[3] * lambda, w[1] = w[2] * lambda, w[0] = w[1] * lambda;
-          }
-#pragma unroll
-          for (int r = 0; r < 4; ++r) a[r] = u + r >= lo && u + r <= hi ? a[r] * w[r] : 0.f;
-        }
-        if constexpr (M::kNarrow) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf(a[r]));
-          score[i] = a;
-        } else if (i >= i0 && i < i1) {
-          M::put4(ps + t * SP + 16 * i + 4 * g, a);
-        }
-      }
-      if constexpr (M::kNarrow) {
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float f = to_middle(top);
-        if (g == 0) p_top[t] = f;
-#pragma unroll
-        for (int i = 0; i < kBlocks; ++i)
-          if (i >= i0 && i < i1) M::put4(ps + t * SP + 16 * i + 4 * g, score[i] * f);
-      }
-    }
-    __syncthreads();
-    const float carry = __builtin_amdgcn_exp2f(l2 * n_now);
-    if (starts) through = 0.f;
-    through *= carry;
-    const uint32_t out_size = p.out_f32 ? 4u : (uint32_t)sizeof(T);
-    const T* out_row = (const T*)((const char*)p.out + (start_now * p.out_stride[0] + row * p.out_stride[1] + h * p.out_stride[2]) * (int64_t)out_size);
-    const auto there = [&](int j) { return !kTrim || v0 + 64 * j < p.dv; };  // (the same for the whole wave)
-    if (!parts.state_only) {
-      // ---- outputs: what the entering state gives, then the chunk's own steps
-      f32x4 a[kBlocks][NV];
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-        for (int j = 0; j < NV; ++j) a[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      float s_scale = 1.f;
-      if constexpr (M::kNarrow) {
-        float top = 0.f;
-#pragma unroll
-        for (int i = 0; i < ND; ++i)
-#pragma unroll
-          for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf(s[i][j][r]));
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-        s_scale = to_middle(top);
-      }
-#pragma unroll
-      for (int k = 0; k < DK / K; ++k) {
-        if (k >= nk) continue;
-        // the state rounded, and what that left out
-        frag sf[NV][2];
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          if constexpr (sizeof(T) == 2) {
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = M::of(s[2 * k][j], s[2 * k + 1][j], e) * s_scale;
-            M::pieces(x, sf[j]);
-          } else {
-            sf[j][0] = s[k][j];
-          }
-        }
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-          const frag qf = M::row_as_acc(qs, SQ, 16 * b, k * K, ln);
-#pragma unroll
-          for (int j = 0; j < NV; ++j) {
-            if (!there(j)) continue;
-            a[b][j] = M::mul(sf[j][0], qf, a[b][j]);
-            if constexpr (sizeof(T) == 2) a[b][j] = M::mul(sf[j][1], qf, a[b][j]);
-          }
-        }
-        keep_order();
-      }
-      settle<kTrim>();
-      frag vf[NV][kChunk / K];
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int k = 0; k < kChunk / K; ++k) vf[j][k] = M::col(vs, SV, k * K, v0 + 64 * j, ln);
-#pragma unroll
-      for (int b = 0; b < kBlocks; ++b) {
-        const int t = 16 * b + l16;
-        const float f = M::kNarrow ? p_top[t] : 1.f;
-        const float w = w_in[t], ws_ = w * f / s_scale;
+      for (int i = 0; i < ND; ++i)
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) a[b][j][r] = w != 0.f ? a[b][j][r] * ws_ : 0.f;
+          for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf(s[i][j][r]));
 #pragma unroll
-        for (int k = 0; k < kChunk / K; ++k)
-          if (rev ? (k + 1) * K > 16 * b : k * K <= 16 * b) {
-            const frag pf = M::row(ps, SP, 16 * b, k * K, ln);
+      for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+      s_scale = to_middle(top);
+    }
 #pragma unroll
-            for (int j = 0; j < NV; ++j)
-              if (there(j)) a[b][j] = M::mul(vf[j][k], pf, a[b][j]);
-          }
-        settle<kTrim || !kAligned>();  // (value by value, a lane may have nothing to store)
+    for (int k = 0; k < DK / K; ++k) {
+      if (k >= nk) continue;
+      // the state rounded, and what that left out
+      frag sf[NV][2];
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if constexpr (sizeof(T) == 2) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = M::of(s[2 * k][j], s[2 * k + 1][j], e) * s_scale;
+          M::pieces(x, sf[j]);
+        } else {
+          sf[j][0] = s[k][j];
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        const frag qf = M::row_as_acc(qs, SQ, 16 * b, k * K, ln);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          f32x4 x = a[b][j];
-          if constexpr (M::kNarrow) x *= 1.f / f;
-          const int v = v0 + 64 * j + 4 * g;
-          if constexpr (kAligned) {
-            const auto o = buffer(out_row, p.out ? ((n_now - 1) * p.out_stride[0] + p.dv) * (int64_t)out_size : 0);
-            const uint32_t at = v < p.dv ? (uint32_t)(t * (uint32_t)p.out_stride[0] + v) * out_size : kOutside;
-            if (sizeof(T) == 4 || p.out_f32) {
-              __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), o, at, 0, 0);
-            } else if constexpr (sizeof(T) == 2) {
-              alignas(8) T y[4];
-              M::put4(y, x);
-              __builtin_amdgcn_raw_buffer_store_b64(*(const u32x2*)y, o, at, 0, 0);
-            }
-          } else if (t < n_now && p.out) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (v + r < p.dv) {
-                if (p.out_f32) ((float*)out_row)[t * p.out_stride[0] + v + r] = x[r];
-                else ((T*)out_row)[t * p.out_stride[0] + v + r] = (T)x[r];
-              }
-          }
+          if (!there(j)) continue;
+          a[b][j] = M::mul(sf[j][0], qf, a[b][j]);
+          if constexpr (sizeof(T) == 2) a[b][j] = M::mul(sf[j][1], qf, a[b][j]);
         }
-        keep_order();
       }
+      keep_order();
     }
-    // ---- the state: keys as rows, weighted values as columns
+    settle<kTrim>();
+    frag vf[NV][kChunk / K];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int k = 0; k < kChunk / K; ++k) vf[j][k] = M::col(vs, SV, k * K, v0 + 64 * j, ln);
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+      const int t = 16 * b + l16;
+      const float f = M::kNarrow ? p_top[t] : 1.f;
+      const float w = w_in[t], ws_ = w * f / s_scale;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) a[b][j][r] = w != 0.f ? a[b][j][r] * ws_ : 0.f;
+#pragma unroll
+      for (int k = 0; k < kChunk / K; ++k)
+        if (rev ? (k + 1) * K > 16 * b : k * K <= 16 * b) {
+          const frag pf = M::row(ps, SP, 16 * b, k * K, ln);
+#pragma unroll
+          for (int j = 0; j < NV; ++j)
+            if (there(j)) a[b][j] = M::mul(vf[j][k], pf, a[b][j]);
+        }
+      settle<true>();  // (how results are stored is a branch)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        f32x4 x = a[b][j];
+        if constexpr (M::kNarrow) x *= 1.f / f;
+        const int v = v0 + 64 * j + 4 * g;
+        if constexpr (kAligned) {
+          const auto o = buffer(out_row, p.out ? ((n_now - 1) * p.out_stride[0] + p.dv) * (int64_t)out_size : 0);
+          const uint32_t at = v < p.dv ? (uint32_t)(t * (uint32_t)p.out_stride[0] + v) * out_size : kOutside;
+          if (sizeof(T) == 4 || p.out_f32) {
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x), o, at, 0, 0);
+          } else if constexpr (sizeof(T) == 2) {
+            alignas(8) T y[4];
+            M::put4(y, x);
+            __builtin_amdgcn_raw_buffer_store_b64(*(const u32x2*)y, o, at, 0, 0);
+          }
+        } else if (t < n_now && p.out) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (v + r < p.dv) {
+              if (p.out_f32) ((float*)out_row)[t * p.out_stride[0] + v + r] = x[r];
+              else ((T*)out_row)[t * p.out_stride[0] + v + r] = (T)x[r];
+            }
+        }
+      }
+      keep_order();
+    }
+  }
+
+  // the state that leaves the chunk: keys as rows, weighted values as columns
+  static __device__ void update(const Scan& p, const Now& c, State& s, const T* ks, int SK, const T* vs, int SV) {
+    const int wave = c.wave, ln = c.ln, g = ln >> 4, v0 = 16 * wave, nd = Walk::nd(p);
+    const uint64_t starts = c.starts;
+    const float* w_up = c.w_up;
+    const float carry = __builtin_amdgcn_exp2f(c.l2 * c.n);
+    const auto there = [&](int j) { return !kTrim || j == 0 || v0 + 64 * j < p.dv; };
     if (starts) {  // nothing from before the chunk leaves it (and 0 * inf must not)
 #pragma unroll
       for (int i = 0; i < ND; ++i)
@@ -612,8 +575,123 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
       }
     }
     settle<true>();  // (a whole update may have been skipped)
-    start = start_next;
-    n = n_next;
+  }
+};
+
+// where a chunk that holds the start of an episode and something that is not finite ends: 0 * inf would carry it
+// across, so the chunk keeps its outer episode only and the rest is a chunk of its own
+template <bool rev> __device__ inline void cut_chunk(uint64_t starts, int64_t& start, int& n) {
+  int from = 0, to = n;
+  if (rev) from = 63 - __clzll(starts);
+  else if ((starts & ~1ull) != 0) to = __ffsll((unsigned long long)(starts & ~1ull)) - 1;
+  start += from;
+  n = to - from;
+}
+
+template <class T, int DK, int DV, bool kAligned, bool rev>
+__global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void scan_chunks(Scan p, Parts parts) {
+  using W = Walk<T, DK, DV, kAligned, rev>;
+  using Tile = ScanTile<T, DK, DV>;
+  constexpr int kChunk = Tile::kChunk, SQ = Tile::SQ, SK = Tile::SK, SV = Tile::SV, ND = W::ND, NV = W::NV;
+  extern __shared__ __align__(16) char lds[];
+  T* qs = (T*)lds;
+  T* ks = qs + kChunk * SQ;
+  T* vs = ks + kChunk * SK;
+  T* ps = vs + kChunk * SV;
+  Now c;
+  c.w_up = (float*)(ps + kChunk * Tile::SP);
+  c.w_in = c.w_up + kChunk;
+  c.p_top = c.w_in + kChunk;             // kNarrow: what a step's scores were multiplied by
+  int* odd = (int*)(c.p_top + kChunk);   // a key or value of this chunk is not finite
+
+  const int64_t rh = blockIdx.x;
+  const int64_t row = rh / p.heads;
+  const int h = (int)(rh % p.heads);
+  // (of the contributions only those are needed that a later part starts from)
+  const int seg = blockIdx.y + (parts.state_only && rev ? 1 : 0);
+  const int lane = threadIdx.x & 63;
+  c.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const float log2_decay = fmaxf(p.log_decay[h] * 1.44269504088896f, -1e30f);  // (decay 0: its power 0 is still 1)
+  c.lambda = __builtin_amdgcn_exp2f(log2_decay);
+
+  const T* gq = (const T*)p.q + row * p.q_stride[1] + (h / p.q_group) * p.q_stride[2];
+  const T* gk = (const T*)p.k + row * p.k_stride[1] + (h / p.k_group) * p.k_stride[2];
+  const T* gv = (const T*)p.v + row * p.v_stride[1] + (h / p.v_group) * p.v_stride[2];
+  const uint8_t* gf = p.fresh ? p.fresh + row * p.fresh_stride[1] : nullptr;
+  const int64_t seg0 = seg * parts.seg_len;
+  const int64_t seg1 = seg0 + parts.seg_len < p.steps ? seg0 + parts.seg_len : p.steps;
+
+  // ---- a chunk's tiles, on their way from memory
+  uint4 rq[Tile::kQ], rk[Tile::kQ], rv[Tile::kV];
+  uint8_t rf = 0;
+  const auto load = [&](int64_t start, int n) {
+    W::load_tile(rk, Tile::kQ, gk, p.k_stride[0], p.dk, DK, start, n);
+    W::load_tile(rv, Tile::kV, gv, p.v_stride[0], p.dv, DV, start, n);
+    if (!parts.state_only) W::load_tile(rq, Tile::kQ, gq, p.q_stride[0], p.dk, DK, start, n);
+    rf = gf && lane < n ? gf[(start + lane) * p.fresh_stride[0]] : 0;
+  };
+  const auto put = [&]() {
+    if (!parts.state_only) W::put_tile(rq, Tile::kQ, qs, DK, SQ);
+    W::put_tile(rk, Tile::kQ, ks, DK, SK);
+    W::put_tile(rv, Tile::kV, vs, DV, SV);
+  };
+
+  int64_t start = rev ? seg1 - (seg1 - seg0 < kChunk ? seg1 - seg0 : kChunk) : seg0;
+  int n = (int)(seg1 - seg0 < kChunk ? seg1 - seg0 : kChunk);
+  if (threadIdx.x == 0) *odd = 0;
+  if (n > 0) load(start, n);
+
+  // ---- the state the part starts from
+  typename W::State s;
+  f32x4* ws = parts.ws_state ? parts.ws_state + (rh * parts.n_seg + seg) * (DK * DV / 4) : nullptr;
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int j = 0; j < NV; ++j) s[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (!parts.state_only && parts.n_seg > 1) {
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) s[i][j] = ws[((i * NV + j) * 4 + c.wave) * 64 + lane];
+  } else if (!parts.state_only && p.state_in) {
+    W::load_state(p, parts.state_vec, row, h, lane, c.wave, s);
+  }
+  float through = 1.f;
+
+  while (n > 0) {
+    // (opaque to the compiler here, or it would keep every step's powers of the decay, and every address, in
+    // registers across the loop)
+    c.l2 = log2_decay;
+    c.ln = lane;
+    asm volatile("" : "+v"(c.l2), "+v"(c.ln));
+    __syncthreads();  // (the tiles of the chunk before have been read)
+    put();
+    c.starts = __ballot(rf != 0);
+    if (c.starts && not_finite<T>(W::top_of(W::top_of(0, rk, Tile::kQ), rv, Tile::kV))) *odd = 1;
+    __syncthreads();
+    if (c.starts && *odd) {
+      __syncthreads();
+      if (threadIdx.x == 0) *odd = 0;
+      cut_chunk<rev>(c.starts, start, n);
+      load(start, n);
+      put();
+      c.starts = __ballot(rf != 0);
+      __syncthreads();
+    }
+    // the next chunk's loads run under this one's products
+    c.n = n;
+    c.start = start;
+    const int64_t left = rev ? start - seg0 : seg1 - (start + n);
+    n = (int)(left < kChunk ? left : kChunk);
+    start = rev ? start - n : start + c.n;
+    if (n > 0) load(start, n);
+
+    W::weights(p, c);
+    if (!parts.state_only) W::scores(p, c, qs, SQ, ks, SK, ps);
+    __syncthreads();
+    through = c.starts ? 0.f : through * __builtin_amdgcn_exp2f(c.l2 * c.n);
+    if (!parts.state_only) W::outputs(p, c, row, h, s, qs, SQ, vs, SV, ps);
+    W::update(p, c, s, ks, SK, vs, SV);
   }
 
   // ---- the state the part ends with
@@ -621,30 +699,12 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
 #pragma unroll
     for (int i = 0; i < ND; ++i)
 #pragma unroll
-      for (int j = 0; j < NV; ++j) ws[((i * NV + j) * 4 + wave) * 64 + lane] = s[i][j];
+      for (int j = 0; j < NV; ++j) ws[((i * NV + j) * 4 + c.wave) * 64 + lane] = s[i][j];
     if (threadIdx.x == 0) parts.ws_carry[rh * parts.n_seg + seg] = through;
     return;
   }
   const bool last = rev ? seg == 0 : seg == parts.n_seg - 1;
-  if (!last || !p.state_out) return;
-  float* base = p.state_out + row * p.outs_stride[0] + h * p.outs_stride[1];
-#pragma unroll
-  for (int i = 0; i < ND; ++i)
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int v = v0 + 64 * j + l16, d = 16 * i + 4 * g;
-      if constexpr (kAligned) {
-        const auto b = buffer(base, 0x7fffffff);
-        const uint32_t sd = (uint32_t)p.outs_stride[2] * 4u, sv = (uint32_t)p.outs_stride[3] * 4u;
-        const uint32_t at = v < p.dv && d < p.dk ? d * sd + v * sv : kOutside;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, (float)s[i][j][r]), b, at + r * sd, 0, 0);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (v < p.dv && d + r < p.dk) base[(d + r) * p.outs_stride[2] + v * p.outs_stride[3]] = s[i][j][r];
-      }
-    }
+  if (last && p.state_out) W::store_state(p, row, h, lane, c.wave, s);
 }
 
 // Turns the parts' own contributions into what each part starts from, in time's direction: one thread per 4
@@ -710,7 +770,10 @@ template <class T, int DK, int DV, bool kAligned, bool rev> hipError_t scan_tile
 template <class T, bool kAligned, bool rev> hipError_t scan_sizes(const Scan& k, const Parts& parts, unsigned states, hipStream_t stream) {
   if (k.dk <= 64)
     return k.dv <= 64 ? scan_tile<T, 64, 64, kAligned, rev>(k, parts, states, stream) : scan_tile<T, 64, 128, kAligned, rev>(k, parts, states, stream);
-  return k.dv <= 64 ? scan_tile<T, 128, 64, kAligned, rev>(k, parts, states, stream) : scan_tile<T, 128, 128, kAligned, rev>(k, parts, states, stream);
+  // (in 32 bits the 128 x 128 kernel skips the upper values' tiles; one of its own was built with thousands of spills)
+  if constexpr (sizeof(T) == 2)
+    if (k.dv <= 64) return scan_tile<T, 128, 64, kAligned, rev>(k, parts, states, stream);
+  return scan_tile<T, 128, 128, kAligned, rev>(k, parts, states, stream);
 }
 // (one source file per type holds these: memory_scan_<type>.hip)
 template <class T> hipError_t scan_run(const Scan& k, const Parts& parts, bool aligned, unsigned states, hipStream_t stream);

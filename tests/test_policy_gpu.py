@@ -322,7 +322,7 @@ SCANS = [
   # steps, rows, heads, kv heads, key dim, value dim, fresh, state
   (1, 1, 1, 1, 1, 1, 0.0, False), (1, 5, 2, 2, 64, 64, 0.5, True), (7, 3, 2, 1, 16, 24, 0.3, True), (63, 2, 1, 1, 32, 32, 0.0, True),
   (64, 2, 2, 2, 64, 64, 0.02, True), (65, 2, 3, 3, 40, 72, 0.05, False), (130, 3, 4, 2, 64, 128, 0.02, True), (200, 1, 2, 2, 128, 128, 0.0, True),
-  (257, 2, 3, 1, 80, 112, 0.01, True), (700, 3, 2, 2, 72, 16, 0.004, True), (96, 1, 1, 1, 128, 5, 0.9, True), (1000, 1, 2, 2, 33, 64, 0.003, True),
+  (257, 2, 3, 1, 80, 112, 0.01, True), (700, 3, 2, 2, 72, 16, 0.004, True), (700, 2, 2, 1, 100, 60, 0.004, True), (96, 1, 1, 1, 128, 5, 0.9, True), (1000, 1, 2, 2, 33, 64, 0.003, True),
 ]
 
 
