@@ -37,6 +37,7 @@ class MemoryScanArgs(C.Structure):
 SYMBOLS = [
   "ep_policy_choose", "ep_policy_choose_workspace", "ep_policy_evaluate", "ep_policy_evaluate_workspace", "ep_policy_evaluate_grad",
   "ep_policy_evaluate_grad_workspace", "ep_memory_step", "ep_memory_step_workspace", "ep_memory_scan", "ep_memory_scan_workspace",
+  "ep_memory_scan_pair", "ep_memory_scan_pair_workspace",
   "ep_memory_sum_heads",
 ]
 
@@ -54,10 +55,11 @@ def lib():
     L.ep_policy_evaluate_grad.argtypes = [rows, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64]
     L.ep_memory_step.argtypes = [step]
     L.ep_memory_scan.argtypes = [scan]
+    L.ep_memory_scan_pair.argtypes = [scan, scan]
     L.ep_memory_sum_heads.argtypes = [_i32, _vp, _i64, _i32, _i32, _i32, _vp, _i32, _vp]
     for name, args in (("ep_policy_choose_workspace", [rows]), ("ep_policy_evaluate_workspace", [rows]),
                        ("ep_policy_evaluate_grad_workspace", [rows, _i32]), ("ep_memory_step_workspace", [step]),
-                       ("ep_memory_scan_workspace", [scan])):
+                       ("ep_memory_scan_workspace", [scan]), ("ep_memory_scan_pair_workspace", [scan, scan])):
       getattr(L, name).argtypes = args
       getattr(L, name).restype = _i64
     _bound = L

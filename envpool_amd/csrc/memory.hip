@@ -71,16 +71,52 @@ int64_t scan_workspace(const ep_memory_scan_args* a, int64_t n_seg) {
   return a->rows * a->heads * n_seg * (padded(a).state() * 4 + 4);
 }
 
-int scan_launch(const ep_memory_scan_args* a, const epm::Scan& k, hipStream_t stream) {
-  epm::Parts parts{};
-  const int64_t chunk = chunk_steps(a->dtype), chunks = std::max<int64_t>(1, (a->steps + chunk - 1) / chunk);
-  const int64_t want = scan_parts(a), per = (chunks + want - 1) / want;
-  parts.seg_len = per * chunk;
-  parts.n_seg = (int32_t)((chunks + per - 1) / per);
-  if (parts.n_seg > 1) {
-    parts.ws_state = (epm::f32x4*)a->workspace;
-    parts.ws_carry = (float*)((char*)a->workspace + a->rows * a->heads * parts.n_seg * (padded(a).state() * 4));
-  }
+// every refusal but the workspace's
+int check_scan(const ep_memory_scan_args* a) {
+  if (!a) return fail(EP_ERR_INVALID, "null argument");
+  if (!float_type(a->dtype)) return fail(EP_ERR_INVALID, "dtype = %d is none of EP_F32, EP_F16, EP_BF16", a->dtype);
+  if (a->out_dtype != a->dtype && a->out_dtype != EP_F32) return fail(EP_ERR_INVALID, "out_dtype = %d is neither dtype nor EP_F32", a->out_dtype);
+  if (a->steps < 0 || a->steps > INT32_MAX) return fail(EP_ERR_INVALID, "steps = %lld", (long long)a->steps);
+  if (a->rows < 0 || a->rows > INT32_MAX) return fail(EP_ERR_INVALID, "rows = %lld", (long long)a->rows);
+  if (a->heads < 1 || a->heads > 65535) return fail(EP_ERR_INVALID, "heads = %d is outside [1, 65535]", a->heads);
+  const int32_t groups[] = {a->q_group, a->k_group, a->v_group};
+  for (int32_t g : groups)
+    if (g < 1 || a->heads % g) return fail(EP_ERR_INVALID, "a head group of %d does not divide heads = %d", g, a->heads);
+  if (a->key_dim < 1 || a->key_dim > 128 || a->value_dim < 1 || a->value_dim > 128)
+    return fail(EP_ERR_INVALID, "key_dim = %d, value_dim = %d: not both in [1, 128]", a->key_dim, a->value_dim);
+  if (a->rows > 0 && !a->log_decay) return fail(EP_ERR_INVALID, "log_decay: null pointer");
+  if (a->rows > 0 && a->steps > 0 && (!a->q || !a->k || !a->v)) return fail(EP_ERR_INVALID, "q, k, v: null pointer");
+  if (a->rows > 0 && a->steps > 0 && !a->out && !a->state_out) return fail(EP_ERR_INVALID, "neither out nor state_out is wanted");
+  if (!std::isfinite(a->inc_scale) || !std::isfinite(a->out_scale)) return fail(EP_ERR_INVALID, "inc_scale = %g, out_scale = %g", (double)a->inc_scale, (double)a->out_scale);
+  const void* typed[] = {a->q, a->k, a->v};
+  for (const void* ptr : typed)
+    if ((uintptr_t)ptr % size_of(a->dtype)) return fail(EP_ERR_INVALID, "q, k, v: not aligned to their type");
+  if ((uintptr_t)a->out % size_of(a->out_dtype)) return fail(EP_ERR_INVALID, "out: not aligned to its type");
+  const void* words[] = {a->log_decay, a->state_in, a->state_out};
+  for (const void* ptr : words)
+    if ((uintptr_t)ptr % 4) return fail(EP_ERR_INVALID, "an array of 4-byte values is not aligned to 4 bytes");
+  if (a->rows * a->heads > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld rows of %d heads", (long long)a->rows, a->heads);
+  return EP_OK;
+}
+bool nothing_to_do(const ep_memory_scan_args* a) { return a->rows == 0 || (a->steps == 0 && !a->state_out); }
+
+epm::Scan scan_of(const ep_memory_scan_args* a) {
+  epm::Scan k{};
+  k.steps = a->steps, k.rows = a->rows, k.heads = a->heads;
+  k.q_group = a->q_group, k.k_group = a->k_group, k.v_group = a->v_group, k.dk = a->key_dim, k.dv = a->value_dim;
+  k.q = a->q, k.k = a->k, k.v = a->v, k.out = a->out, k.out_f32 = a->out_dtype == EP_F32;
+  for (int i = 0; i < 3; ++i)
+    k.q_stride[i] = a->q_stride[i], k.k_stride[i] = a->k_stride[i], k.v_stride[i] = a->v_stride[i], k.out_stride[i] = a->out_stride[i];
+  k.log_decay = a->log_decay, k.fresh = a->fresh;
+  for (int i = 0; i < 2; ++i) k.fresh_stride[i] = a->fresh_stride[i];
+  k.state_in = a->state_in, k.state_out = a->state_out;
+  for (int i = 0; i < 4; ++i) k.in_stride[i] = a->state_in_stride[i], k.outs_stride[i] = a->state_out_stride[i];
+  k.inc_scale = a->inc_scale, k.out_scale = a->out_scale, k.reverse = a->reverse;
+  return k;
+}
+
+// whether a call's operands can be addressed through buffers in 16-byte pieces (memory_scan.hpp: kAligned)
+bool buffered(const ep_memory_scan_args* a) {
   const int64_t size = size_of(a->dtype), per_load = 16 / size;
   const int64_t out_size = size_of(a->out_dtype);
   // 16-byte pieces (results: 4 values), rows that follow one another, and a chunk within 2^31 bytes
@@ -91,15 +127,39 @@ int scan_launch(const ep_memory_scan_args* a, const epm::Scan& k, hipStream_t st
   const auto state_near = [&](const void* ptr, const int64_t* stride) {
     return !ptr || (stride[2] >= 0 && stride[3] >= 0 && stride[2] < (1 << 20) && stride[3] < (1 << 20));
   };
-  const bool vec = aligned(a->q, a->q_stride, a->key_dim, 16, size) && aligned(a->k, a->k_stride, a->key_dim, 16, size) &&
+  return aligned(a->q, a->q_stride, a->key_dim, 16, size) && aligned(a->k, a->k_stride, a->key_dim, 16, size) &&
                    aligned(a->v, a->v_stride, a->value_dim, 16, size) && (!a->out || aligned(a->out, a->out_stride, a->value_dim, 4 * out_size, out_size)) &&
                    state_near(a->state_in, a->state_in_stride) && state_near(a->state_out, a->state_out_stride) && a->key_dim % per_load == 0 &&
                    a->value_dim % per_load == 0;
-  parts.state_vec = (uintptr_t)a->state_in % 16 == 0 && a->state_in_stride[0] % 4 == 0 && a->state_in_stride[1] % 4 == 0 && a->state_in_stride[3] % 4 == 0;
-  const int64_t states = a->rows * a->heads;
-  if (states > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld states", (long long)states);
+}
+bool state_vec(const ep_memory_scan_args* a) {
+  return (uintptr_t)a->state_in % 16 == 0 && a->state_in_stride[0] % 4 == 0 && a->state_in_stride[1] % 4 == 0 && a->state_in_stride[3] % 4 == 0;
+}
+
+// whether two scans are the gradients of values (a) and keys (b) of one call, in a form that one kernel covers
+bool pairs_up(const ep_memory_scan_args* a, const ep_memory_scan_args* b) {
+  const auto same = [](const int64_t* x, const int64_t* y, int n) { return std::equal(x, x + n, y); };
+  return a->reverse && b->reverse && a->dtype != EP_F32 && a->dtype == b->dtype && a->steps == b->steps && a->rows == b->rows && a->heads == b->heads &&
+         a->key_dim <= 64 && a->value_dim <= 64 && a->key_dim == b->value_dim && a->value_dim == b->key_dim && a->k == b->v && a->v == b->k &&
+         a->k_group == b->v_group && a->v_group == b->k_group && same(a->k_stride, b->v_stride, 3) && same(a->v_stride, b->k_stride, 3) &&
+         a->log_decay == b->log_decay && a->fresh == b->fresh && same(a->fresh_stride, b->fresh_stride, 2) && a->inc_scale == b->inc_scale &&
+         a->out_scale == b->out_scale && !b->state_out && a->steps > 0 && a->rows > 0 && buffered(a) && buffered(b) && scan_parts(a) == 1 && scan_parts(b) == 1;
+}
+
+int scan_launch(const ep_memory_scan_args* a, hipStream_t stream) {
+  const epm::Scan k = scan_of(a);
+  epm::Parts parts{};
+  const int64_t chunk = chunk_steps(a->dtype), chunks = std::max<int64_t>(1, (a->steps + chunk - 1) / chunk);
+  const int64_t want = scan_parts(a), per = (chunks + want - 1) / want;
+  parts.seg_len = per * chunk;
+  parts.n_seg = (int32_t)((chunks + per - 1) / per);
+  if (parts.n_seg > 1) {
+    parts.ws_state = (epm::f32x4*)a->workspace;
+    parts.ws_carry = (float*)((char*)a->workspace + a->rows * a->heads * parts.n_seg * (padded(a).state() * 4));
+  }
+  parts.state_vec = state_vec(a);
   hipError_t e = hipSuccess;
-  with_type(a->dtype, [&](auto t) { e = epm::scan_run<decltype(t)>(k, parts, vec, (unsigned)states, stream); });
+  with_type(a->dtype, [&](auto t) { e = epm::scan_run<decltype(t)>(k, parts, buffered(a), (unsigned)(a->rows * a->heads), stream); });
   HIP_TRY(e);
   return EP_OK;
 }
@@ -164,45 +224,36 @@ int ep_memory_step(const ep_memory_step_args* a) {
 int64_t ep_memory_scan_workspace(const ep_memory_scan_args* a) { return a ? scan_workspace(a, scan_parts(a)) : 0; }
 
 int ep_memory_scan(const ep_memory_scan_args* a) {
-  if (!a) return fail(EP_ERR_INVALID, "null argument");
-  if (!float_type(a->dtype)) return fail(EP_ERR_INVALID, "dtype = %d is none of EP_F32, EP_F16, EP_BF16", a->dtype);
-  if (a->out_dtype != a->dtype && a->out_dtype != EP_F32) return fail(EP_ERR_INVALID, "out_dtype = %d is neither dtype nor EP_F32", a->out_dtype);
-  if (a->steps < 0 || a->steps > INT32_MAX) return fail(EP_ERR_INVALID, "steps = %lld", (long long)a->steps);
-  if (a->rows < 0 || a->rows > INT32_MAX) return fail(EP_ERR_INVALID, "rows = %lld", (long long)a->rows);
-  if (a->heads < 1 || a->heads > 65535) return fail(EP_ERR_INVALID, "heads = %d is outside [1, 65535]", a->heads);
-  const int32_t groups[] = {a->q_group, a->k_group, a->v_group};
-  for (int32_t g : groups)
-    if (g < 1 || a->heads % g) return fail(EP_ERR_INVALID, "a head group of %d does not divide heads = %d", g, a->heads);
-  if (a->key_dim < 1 || a->key_dim > 128 || a->value_dim < 1 || a->value_dim > 128)
-    return fail(EP_ERR_INVALID, "key_dim = %d, value_dim = %d: not both in [1, 128]", a->key_dim, a->value_dim);
-  if (a->rows > 0 && !a->log_decay) return fail(EP_ERR_INVALID, "log_decay: null pointer");
-  if (a->rows > 0 && a->steps > 0 && (!a->q || !a->k || !a->v)) return fail(EP_ERR_INVALID, "q, k, v: null pointer");
-  if (a->rows > 0 && a->steps > 0 && !a->out && !a->state_out) return fail(EP_ERR_INVALID, "neither out nor state_out is wanted");
-  if (!std::isfinite(a->inc_scale) || !std::isfinite(a->out_scale)) return fail(EP_ERR_INVALID, "inc_scale = %g, out_scale = %g", (double)a->inc_scale, (double)a->out_scale);
-  const void* typed[] = {a->q, a->k, a->v};
-  for (const void* ptr : typed)
-    if ((uintptr_t)ptr % size_of(a->dtype)) return fail(EP_ERR_INVALID, "q, k, v: not aligned to their type");
-  if ((uintptr_t)a->out % size_of(a->out_dtype)) return fail(EP_ERR_INVALID, "out: not aligned to its type");
-  const void* words[] = {a->log_decay, a->state_in, a->state_out};
-  for (const void* ptr : words)
-    if ((uintptr_t)ptr % 4) return fail(EP_ERR_INVALID, "an array of 4-byte values is not aligned to 4 bytes");
+  if (int rc = check_scan(a)) return rc;
   if (int rc = check_workspace(a->workspace, a->workspace_bytes, ep_memory_scan_workspace(a))) return rc;
-  if (a->rows == 0 || (a->steps == 0 && !a->state_out)) return EP_OK;
+  if (nothing_to_do(a)) return EP_OK;
+  EP_ENTER_GPU(a->device_id);
+  return scan_launch(a, (hipStream_t)a->stream);
+}
+
+int64_t ep_memory_scan_pair_workspace(const ep_memory_scan_args* a, const ep_memory_scan_args* b) {
+  if (!a || !b || pairs_up(a, b)) return 0;
+  return std::max(ep_memory_scan_workspace(a), ep_memory_scan_workspace(b));
+}
+
+int ep_memory_scan_pair(const ep_memory_scan_args* a, const ep_memory_scan_args* b) {
+  if (int rc = check_scan(a)) return rc;
+  if (int rc = check_scan(b)) return rc;
+  if (a->device_id != b->device_id || a->stream != b->stream) return fail(EP_ERR_INVALID, "the two scans are not on one device and stream");
+  if (a->workspace != b->workspace || a->workspace_bytes != b->workspace_bytes) return fail(EP_ERR_INVALID, "the two scans do not name one workspace");
+  if (int rc = check_workspace(a->workspace, a->workspace_bytes, ep_memory_scan_pair_workspace(a, b))) return rc;
+  if (nothing_to_do(a) && nothing_to_do(b)) return EP_OK;
   EP_ENTER_GPU(a->device_id);
   const hipStream_t stream = (hipStream_t)a->stream;
-  epm::Scan k{};
-  k.steps = a->steps, k.rows = a->rows, k.heads = a->heads;
-  k.q_group = a->q_group, k.k_group = a->k_group, k.v_group = a->v_group, k.dk = a->key_dim, k.dv = a->value_dim;
-  k.q = a->q, k.k = a->k, k.v = a->v, k.out = a->out, k.out_f32 = a->out_dtype == EP_F32;
-  for (int i = 0; i < 3; ++i)
-    k.q_stride[i] = a->q_stride[i], k.k_stride[i] = a->k_stride[i], k.v_stride[i] = a->v_stride[i], k.out_stride[i] = a->out_stride[i];
-  k.log_decay = a->log_decay, k.fresh = a->fresh;
-  for (int i = 0; i < 2; ++i) k.fresh_stride[i] = a->fresh_stride[i];
-  k.state_in = a->state_in, k.state_out = a->state_out;
-  for (int i = 0; i < 4; ++i) k.in_stride[i] = a->state_in_stride[i], k.outs_stride[i] = a->state_out_stride[i];
-  k.inc_scale = a->inc_scale, k.out_scale = a->out_scale, k.reverse = a->reverse;
-  if (int rc = scan_launch(a, k, stream)) return rc;
-  HIP_TRY(hipGetLastError());
+  if (!pairs_up(a, b)) {
+    if (!nothing_to_do(a))
+      if (int rc = scan_launch(a, stream)) return rc;
+    return nothing_to_do(b) ? EP_OK : scan_launch(b, stream);
+  }
+  const epm::Scan ka = scan_of(a), kb = scan_of(b);
+  const unsigned states = (unsigned)(a->rows * a->heads);
+  HIP_TRY(a->dtype == EP_F16 ? epm::scan_run_pair<epm::f16>(ka, kb, state_vec(a), state_vec(b), states, stream)
+                             : epm::scan_run_pair<epm::bf16>(ka, kb, state_vec(a), state_vec(b), states, stream));
   return EP_OK;
 }
 

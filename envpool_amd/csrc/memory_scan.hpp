@@ -707,6 +707,105 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
   if (last && p.state_out) W::store_state(p, row, h, lane, c.wave, s);
 }
 
+// Two walks back in time over the same four tensors, for the gradients of keys and values (a: values, from keys,
+// queries and the outputs' gradients; b: keys, from values, the outputs' gradients and queries): the tiles of a chunk
+// are read once for both. 16-bit types, sizes up to 64, time not split.
+template <class T> struct PairTile {
+  using Tile = ScanTile<T, 64, 64>;
+  static constexpr size_t kLds = (size_t)Tile::kChunk * (2 * Tile::SQ + 2 * Tile::SK + Tile::SP) * sizeof(T) + 4 * Tile::kChunk * sizeof(float);
+};
+template <class T> __global__ __launch_bounds__(256, 3) void scan_pair(Scan a, Scan b, int state_vec_a, int state_vec_b) {
+  using W = Walk<T, 64, 64, true, true>;
+  using Tile = ScanTile<T, 64, 64>;
+  constexpr int kChunk = Tile::kChunk, SQ = Tile::SQ, SK = Tile::SK, N = Tile::kQ;
+  static_assert(Tile::SK == Tile::SV, "keys and values change places");
+  extern __shared__ __align__(16) char lds[];
+  T* kt = (T*)lds;             // a's queries: the keys
+  T* vt = kt + kChunk * SQ;    // b's queries: the values
+  T* qt = vt + kChunk * SQ;    // a's keys, b's values
+  T* gt = qt + kChunk * SK;    // a's values, b's keys: the outputs' gradients
+  T* ps = gt + kChunk * SK;
+  Now c;
+  c.w_up = (float*)(ps + kChunk * Tile::SP);
+  c.w_in = c.w_up + kChunk;
+  c.p_top = c.w_in + kChunk;
+  int* odd = (int*)(c.p_top + kChunk);
+
+  const int64_t row = blockIdx.x / a.heads;
+  const int h = (int)(blockIdx.x % a.heads);
+  const int lane = threadIdx.x & 63;
+  c.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const float log2_decay = fmaxf(a.log_decay[h] * 1.44269504088896f, -1e30f);
+  c.lambda = __builtin_amdgcn_exp2f(log2_decay);
+  const T* gk = (const T*)a.q + row * a.q_stride[1] + (h / a.q_group) * a.q_stride[2];
+  const T* gq = (const T*)a.k + row * a.k_stride[1] + (h / a.k_group) * a.k_stride[2];
+  const T* gg = (const T*)a.v + row * a.v_stride[1] + (h / a.v_group) * a.v_stride[2];
+  const T* gv = (const T*)b.q + row * b.q_stride[1] + (h / b.q_group) * b.q_stride[2];
+  const uint8_t* gf = a.fresh ? a.fresh + row * a.fresh_stride[1] : nullptr;
+
+  uint4 rk[N], rq[N], rg[N], rv[N];
+  uint8_t rf = 0;
+  const auto load = [&](int64_t start, int n) {
+    W::load_tile(rq, N, gq, a.k_stride[0], a.dk, 64, start, n);
+    W::load_tile(rg, N, gg, a.v_stride[0], a.dv, 64, start, n);
+    W::load_tile(rk, N, gk, a.q_stride[0], a.dk, 64, start, n);
+    W::load_tile(rv, N, gv, b.q_stride[0], a.dv, 64, start, n);
+    rf = gf && lane < n ? gf[(start + lane) * a.fresh_stride[0]] : 0;
+  };
+  const auto put = [&]() {
+    W::put_tile(rq, N, qt, 64, SK);
+    W::put_tile(rg, N, gt, 64, SK);
+    W::put_tile(rk, N, kt, 64, SQ);
+    W::put_tile(rv, N, vt, 64, SQ);
+  };
+  int n = (int)(a.steps < kChunk ? a.steps : kChunk);
+  int64_t start = a.steps - n;
+  if (threadIdx.x == 0) *odd = 0;
+  if (n > 0) load(start, n);
+  typename W::State sa, sb;
+#pragma unroll
+  for (int i = 0; i < W::ND; ++i) sa[i][0] = sb[i][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (a.state_in) W::load_state(a, state_vec_a, row, h, lane, c.wave, sa);
+  if (b.state_in) W::load_state(b, state_vec_b, row, h, lane, c.wave, sb);
+
+  while (n > 0) {
+    c.l2 = log2_decay;
+    c.ln = lane;
+    asm volatile("" : "+v"(c.l2), "+v"(c.ln));
+    __syncthreads();
+    put();
+    c.starts = __ballot(rf != 0);
+    if (c.starts && not_finite<T>(W::top_of(W::top_of(0, rq, N), rg, N))) *odd = 1;
+    __syncthreads();
+    if (c.starts && *odd) {
+      __syncthreads();
+      if (threadIdx.x == 0) *odd = 0;
+      cut_chunk<true>(c.starts, start, n);
+      load(start, n);
+      put();
+      c.starts = __ballot(rf != 0);
+      __syncthreads();
+    }
+    c.n = n;
+    c.start = start;
+    n = (int)(start < kChunk ? start : kChunk);
+    start -= n;
+    if (n > 0) load(start, n);
+
+    W::weights(a, c);
+    W::scores(a, c, kt, SQ, qt, SK, ps);
+    __syncthreads();
+    W::outputs(a, c, row, h, sa, kt, SQ, gt, SK, ps);
+    W::update(a, c, sa, qt, SK, gt, SK);
+    __syncthreads();  // (the scores have been read)
+    W::scores(b, c, vt, SQ, gt, SK, ps);
+    __syncthreads();
+    W::outputs(b, c, row, h, sb, vt, SQ, qt, SK, ps);
+    W::update(b, c, sb, gt, SK, qt, SK);
+  }
+  if (a.state_out) W::store_state(a, row, h, lane, c.wave, sa);
+}
+
 // Turns the parts' own contributions into what each part starts from, in time's direction: one thread per 4
 // values of a state.
 template <int DK, int DV> __global__ __launch_bounds__(256) void join_parts(Scan p, Parts parts) {
@@ -777,6 +876,13 @@ template <class T, bool kAligned, bool rev> hipError_t scan_sizes(const Scan& k,
 }
 // (one source file per type holds these: memory_scan_<type>.hip)
 template <class T> hipError_t scan_run(const Scan& k, const Parts& parts, bool aligned, unsigned states, hipStream_t stream);
+template <class T> hipError_t scan_run_pair(const Scan& a, const Scan& b, bool state_vec_a, bool state_vec_b, unsigned states, hipStream_t stream);
+#define EPM_SCAN_RUN_PAIR(T)                                                                                                          \
+  template <>                                                                                                                         \
+  hipError_t scan_run_pair<T>(const Scan& a, const Scan& b, bool state_vec_a, bool state_vec_b, unsigned states, hipStream_t stream) { \
+    hipLaunchKernelGGL(scan_pair<T>, dim3(states), dim3(256), PairTile<T>::kLds, stream, a, b, (int)state_vec_a, (int)state_vec_b);    \
+    return hipGetLastError();                                                                                                         \
+  }
 #define EPM_SCAN_RUN(T)                                                                                                       \
   template <> hipError_t scan_run<T>(const Scan& k, const Parts& parts, bool aligned, unsigned states, hipStream_t stream) { \
     if (aligned) return k.reverse ? scan_sizes<T, true, true>(k, parts, states, stream) : scan_sizes<T, true, false>(k, parts, states, stream); \

@@ -3,4 +3,5 @@
 
 namespace epm {
 EPM_SCAN_RUN(bf16)
+EPM_SCAN_RUN_PAIR(bf16)
 }

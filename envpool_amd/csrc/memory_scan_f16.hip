@@ -3,4 +3,5 @@
 
 namespace epm {
 EPM_SCAN_RUN(f16)
+EPM_SCAN_RUN_PAIR(f16)
 }

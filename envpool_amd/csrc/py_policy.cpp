@@ -122,8 +122,9 @@ struct Scan {
     for (int i = 0; i < 4; ++i) a.state_in_stride[i] = is[i], a.state_out_stride[i] = os[i];
   }
   int64_t workspace() const { return ep_memory_scan_workspace(&a); }
-  void run(float inc_scale, float out_scale, bool reverse, u64 workspace, int64_t workspace_bytes) {
-    a.inc_scale = inc_scale, a.out_scale = out_scale, a.reverse = reverse, a.workspace = at<void>(workspace), a.workspace_bytes = workspace_bytes;
+  void direction(float inc_scale, float out_scale, bool reverse) { a.inc_scale = inc_scale, a.out_scale = out_scale, a.reverse = reverse; }
+  void run(u64 workspace, int64_t workspace_bytes) {
+    a.workspace = at<void>(workspace), a.workspace_bytes = workspace_bytes;
     int rc;
     {
       py::gil_scoped_release rel;
@@ -156,8 +157,19 @@ PYBIND11_MODULE(policy_native, m) {
       .def("operands", &Scan::operands)
       .def("output", &Scan::output)
       .def("states", &Scan::states)
+      .def("direction", &Scan::direction)
       .def("workspace", &Scan::workspace)
       .def("run", &Scan::run);
+  m.def("scan_pair_workspace", [](const Scan& x, const Scan& y) { return ep_memory_scan_pair_workspace(&x.a, &y.a); });
+  m.def("scan_pair", [](Scan& x, Scan& y, u64 workspace, int64_t workspace_bytes) {
+    x.a.workspace = y.a.workspace = at<void>(workspace), x.a.workspace_bytes = y.a.workspace_bytes = workspace_bytes;
+    int rc;
+    {
+      py::gil_scoped_release rel;
+      rc = ep_memory_scan_pair(&x.a, &y.a);
+    }
+    epy::check(rc);
+  });
   m.def("sum_heads", [](int device, u64 src, int64_t n, int heads_out, int group, int dim, u64 out, int dtype, u64 stream) {
     int rc;
     {

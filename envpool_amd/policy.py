@@ -378,8 +378,8 @@ def _turned(stride):
   return (stride[0], stride[1], stride[3], stride[2])
 
 
-def _scan_call(dims, log_decay, fresh, q, q_group, k, k_group, v, v_group, out, state_in, state_out, inc_scale, out_scale, reverse, turn):
-  """One ep_memory_scan. `dims` (steps, rows, heads, key_dim, value_dim); `turn`: the states are stored as
+def _scan_args(dims, log_decay, fresh, q, q_group, k, k_group, v, v_group, out, state_in, state_out, inc_scale, out_scale, reverse, turn):
+  """The arguments of one ep_memory_scan. `dims` (steps, rows, heads, key_dim, value_dim); `turn`: the states are stored as
   [value_dim, key_dim] of this call."""
   dev = log_decay.device
   f = (0, 0, 0) if fresh is None else (fresh.data_ptr(), *fresh.stride())
@@ -389,8 +389,14 @@ def _scan_call(dims, log_decay, fresh, q, q_group, k, k_group, v, v_group, out, 
     s.output(out.data_ptr(), out.stride()[:3], _FLOATS[out.dtype])
   stride_of = lambda t: _NO_STRIDE if t is None else _turned(t.stride()) if turn else t.stride()  # noqa: E731
   s.states(0 if state_in is None else state_in.data_ptr(), stride_of(state_in), 0 if state_out is None else state_out.data_ptr(), stride_of(state_out))
-  ws, ws_ptr, ws_bytes = _scratch(s.workspace(), dev)
-  s.run(inc_scale, out_scale, reverse, ws_ptr, ws_bytes)
+  s.direction(inc_scale, out_scale, reverse)
+  return s
+
+
+def _scan_call(*args):
+  s = _scan_args(*args)
+  ws, ws_ptr, ws_bytes = _scratch(s.workspace(), args[1].device)
+  s.run(ws_ptr, ws_bytes)
 
 
 def _scan_forward(q, k, v, state, log_decay, fresh, scale):
@@ -426,15 +432,22 @@ def _scan_backward(ctx, g_out, g_final):
     _native.sum_heads(q.device.index, x.data_ptr(), t * n, hk, group, dim, y.data_ptr(), _FLOATS[q.dtype], current_stream_handle(q.device))
     return y
 
+  for_k = for_v = None
   if want_k:
     grad_k = per_head(dk)
-    _scan_call((t, n, h, dv, dk), log_decay, fresh, v, group, g_out, 1, q, 1, grad_k, g_final, None, scale, 1.0, True, True)
-    grad_k = summed(grad_k, dk)
+    for_k = ((t, n, h, dv, dk), log_decay, fresh, v, group, g_out, 1, q, 1, grad_k, g_final, None, scale, 1.0, True, True)
   if want_v or want_s:
     grad_v = per_head(dv) if want_v else None
     grad_s = torch.empty(n, h, dk, dv, dtype=torch.float32, device=q.device) if want_s else None
-    _scan_call((t, n, h, dk, dv), log_decay, fresh, k, group, q, 1, g_out, 1, grad_v, g_final, grad_s, scale, 1.0, True, False)
-    grad_v = summed(grad_v, dv) if want_v else None
+    for_v = ((t, n, h, dk, dv), log_decay, fresh, k, group, q, 1, g_out, 1, grad_v, g_final, grad_s, scale, 1.0, True, False)
+  if for_k and for_v:
+    x, y = _scan_args(*for_v), _scan_args(*for_k)
+    ws, ws_ptr, ws_bytes = _scratch(_native.scan_pair_workspace(x, y), q.device)
+    _native.scan_pair(x, y, ws_ptr, ws_bytes)
+  elif for_k or for_v:
+    _scan_call(*(for_k or for_v))
+  grad_k = summed(grad_k, dk) if want_k else None
+  grad_v = summed(grad_v, dv) if want_v else None
   return grad_q, grad_k, grad_v, grad_s, None, None, None
 
 

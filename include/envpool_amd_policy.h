@@ -160,6 +160,13 @@ typedef struct {
 int ep_memory_scan(const ep_memory_scan_args* args);
 int64_t ep_memory_scan_workspace(const ep_memory_scan_args* args);
 
+/* Two scans as one call, both on one device and stream and naming one workspace (the larger of the two, or what
+ * ep_memory_scan_pair_workspace says). The gradients of values (a) and keys (b) of one forward scan - reverse scans
+ * over the same tensors: a's k is b's v and the other way round - share their reads where their sizes allow it
+ * (16-bit types, dims up to 64); any other two simply follow one another. Neither's results are read by the other. */
+int ep_memory_scan_pair(const ep_memory_scan_args* a, const ep_memory_scan_args* b);
+int64_t ep_memory_scan_pair_workspace(const ep_memory_scan_args* a, const ep_memory_scan_args* b);
+
 /* out[i, j] = sum of `group` neighbouring heads of src (32 bits), rounded once to `dtype`: the gradients of
  * keys and values that several heads share. src [n][heads_out * group][dim] dense, out [n][heads_out][dim] dense. */
 int ep_memory_sum_heads(int32_t device_id, const float* src, int64_t n, int32_t heads_out, int32_t group, int32_t dim,

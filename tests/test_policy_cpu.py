@@ -151,6 +151,24 @@ def test_null_arguments_and_empty_calls():
   assert L.ep_memory_sum_heads(0, None, 0, 2, 2, 8, None, capi.EP_F32, None) == capi.EP_OK
 
 
+def test_pairs_of_scans_that_are_refused():
+  L = cp.lib()
+  pair = lambda a, b: L.ep_memory_scan_pair(C.byref(_scan(**a)), C.byref(_scan(**b)))  # noqa: E731
+  _refused(L.ep_memory_scan_pair(None, C.byref(_scan())), "null")
+  _refused(L.ep_memory_scan_pair(C.byref(_scan()), None), "null")
+  _refused(pair({}, dict(key_dim=0)), "key_dim")
+  _refused(pair(dict(heads=0), {}), "heads")
+  _refused(pair({}, dict(device_id=1)), "one device")
+  _refused(pair(dict(stream=PTR), {}), "stream")
+  _refused(pair(dict(workspace=PTR), {}), "one workspace")
+  _refused(pair({}, dict(steps=10000)), "workspace")
+  assert L.ep_memory_scan_pair(C.byref(_scan(rows=0)), C.byref(_scan(rows=0))) == capi.EP_OK
+  size = L.ep_memory_scan_pair_workspace(C.byref(_scan()), C.byref(_scan(steps=10000)))
+  assert size == L.ep_memory_scan_workspace(C.byref(_scan(steps=10000))) > 0
+  # many states leave time in one piece, so that the pair needs none
+  assert L.ep_memory_scan_pair_workspace(C.byref(_scan(rows=4096)), C.byref(_scan(rows=4096))) == 0
+
+
 def test_without_a_gpu_the_calls_fail_loudly():
   L = cp.lib()
   if L.ep_device_count() > 0:

@@ -453,6 +453,24 @@ def test_memory_scan_layouts_and_missing_pieces():
   assert torch.allclose(first + second, both, atol=1e-4, rtol=1e-4)
 
 
+@pytest.mark.parametrize("t,n,dk,dv,dtype", [(300, 260, 64, 48, torch.bfloat16), (130, 600, 16, 64, torch.float16), (1, 3, 8, 8, torch.float16)])
+def test_gradients_of_keys_and_values_together_and_alone(t, n, dk, dv, dtype):
+  """Many envs: one walk serves both gradients; each is what its own walk gives."""
+  from envpool_amd import policy
+  q, k, v, decay, fresh, state, do, ds = (x.to(DEV) for x in _scan_problem((t, n, 2, 1, dk, dv, 0.01, True), dtype))
+
+  def run(wanted, start):
+    leaves = [x.detach().requires_grad_(i in wanted) for i, x in enumerate((q, k, v, state))]
+    out, final = policy.memory_scan(*leaves[:3], decay, fresh=fresh, state=leaves[3] if start else None)
+    return torch.autograd.grad([out, final], [leaves[i] for i in wanted], [do, ds])
+
+  for start in (True, False):
+    together = run((1, 2), start)
+    assert torch.equal(together[0], run((1,), start)[0]) and torch.equal(together[1], run((2,), start)[0])
+  keys, first = run((1, 3), True)
+  assert torch.equal(keys, run((1,), True)[0]) and torch.equal(first, run((3,), True)[0])
+
+
 @pytest.mark.parametrize("t,dk,dv", [(70, 24, 40), (300, 128, 128), (33, 7, 5)])
 def test_memory_scan_only_what_is_asked_for(t, dk, dv):
   """Each gradient alone (the others are not computed) is what it is among the others."""
