@@ -71,6 +71,7 @@ int check_rows(const ep_policy_rows* r, epp::Rows* k) {
   k->frequency = r->frequency, k->frequency_all = r->frequency_all;
   k->presence = r->presence, k->presence_all = r->presence_all;
   k->temperature = r->temperature, k->temperature_all = r->temperature_all;
+  k->inv_t_all = 1.0 / r->temperature_all, k->inv_t_all_32 = 1.f / (float)r->temperature_all;
   const auto rows16 = [&](const void* ptr, int64_t stride, size_t size) {
     return (uintptr_t)ptr % 16 == 0 && (r->rows <= 1 || (stride * (int64_t)size) % 16 == 0);
   };
@@ -93,10 +94,13 @@ template <class F> void with_type(int32_t dtype, F f) {
   else if (dtype == EP_F16) f(epp::f16{});
   else f(epp::bf16{});
 }
-template <class F> void with_kernel(int32_t dtype, bool history, F f) {
+template <class F> void with_kernel(int32_t dtype, const epp::Rows& k, F f, bool vec_out = true) {
+  const bool whole = k.vec && vec_out && k.options % epp::kPer == 0;
   with_type(dtype, [&](auto t) {
-    if (history) f(t, std::true_type{});
-    else f(t, std::false_type{});
+    if (k.history && whole) f(t, std::true_type{}, std::true_type{});
+    else if (k.history) f(t, std::true_type{}, std::false_type{});
+    else if (whole) f(t, std::false_type{}, std::true_type{});
+    else f(t, std::false_type{}, std::false_type{});
   });
 }
 
@@ -130,18 +134,18 @@ Width group_width(const epp::Rows& k) {
 struct Cut {
   int pieces, parts;  // pieces per part, parts per row
 };
-Cut cut_rows(int64_t rows, int64_t options) {
+Cut cut_rows(int64_t rows, int64_t options, int64_t fill = kFill) {
   const int64_t all = (options + epp::kPiece - 1) / epp::kPiece;
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(all, (kFill + rows - 1) / std::max<int64_t>(rows, 1)));
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(all, (fill + rows - 1) / std::max<int64_t>(rows, 1)));
   const int64_t pieces = (all + want - 1) / want;
   return {(int)pieces, (int)((all + pieces - 1) / pieces)};
 }
 
 // partial sums of a shared bias' gradient: one row of them per workgroup that walks down rows
-int64_t grad_group_blocks(const Width& w) { return std::min<int64_t>(w.blocks, 1024); }
+int64_t grad_group_blocks(const Width& w) { return std::min<int64_t>(w.blocks, 256 * epp::grad_group_per_cu(w.pieces)); }
 int64_t grad_row_blocks(int64_t rows, int64_t options) {
   const int64_t pieces = (options + epp::kPiece - 1) / epp::kPiece;
-  const int64_t blocks = std::min<int64_t>(std::min<int64_t>(rows, 65535), std::max<int64_t>(1, kFill / pieces));
+  const int64_t blocks = std::min<int64_t>(std::min<int64_t>(rows, 65535), std::max<int64_t>(1, 256 * epp::kGradPieceBlocks / pieces));
   const int64_t per = (rows + blocks - 1) / std::max<int64_t>(blocks, 1);
   return per > 0 ? (rows + per - 1) / per : 0;
 }
@@ -152,7 +156,7 @@ extern "C" {
 
 int64_t ep_policy_choose_workspace(const ep_policy_rows* r) {
   if (!r || r->rows <= 0 || r->options <= kGroupOptions) return 0;
-  return r->rows * cut_rows(r->rows, r->options).parts * (int64_t)sizeof(epp::Stat<double>);
+  return r->rows * cut_rows(r->rows, r->options, 2 * kFill).parts * (int64_t)sizeof(epp::Stat<double>);
 }
 
 int ep_policy_choose(const ep_policy_rows* r, const void* u, int32_t u_dtype, int32_t* action, float* log_prob, float* entropy) {
@@ -170,19 +174,19 @@ int ep_policy_choose(const ep_policy_rows* r, const void* u, int32_t u_dtype, in
   if (r->options <= kGroupOptions) {
     const Width w = group_width(k);
     const size_t lds = k.history ? w.lds : 0;
-    with_kernel(r->dtype, k.history, [&](auto t, auto h) {
-      if (w.pieces == 1) hipLaunchKernelGGL((epp::choose_group<decltype(t), 1, h.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, u, u_f64, out);
-      else if (w.pieces == 2) hipLaunchKernelGGL((epp::choose_group<decltype(t), 2, h.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, u, u_f64, out);
-      else hipLaunchKernelGGL((epp::choose_group<decltype(t), 4, h.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, u, u_f64, out);
+    with_kernel(r->dtype, k, [&](auto t, auto h, auto whole) {
+      if (w.pieces == 1) hipLaunchKernelGGL((epp::choose_group<decltype(t), 1, h.value, whole.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, u, u_f64, out);
+      else if (w.pieces == 2) hipLaunchKernelGGL((epp::choose_group<decltype(t), 2, h.value, whole.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, u, u_f64, out);
+      else hipLaunchKernelGGL((epp::choose_group<decltype(t), 4, h.value, whole.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, u, u_f64, out);
     });
   } else {
-    const Cut cut = cut_rows(r->rows, r->options);
+    const Cut cut = cut_rows(r->rows, r->options, 2 * kFill);
     if (r->rows * cut.parts > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld rows of %lld options", (long long)r->rows, (long long)r->options);
     auto* parts = (epp::Stat<double>*)r->workspace;
-    with_kernel(r->dtype, k.history, [&](auto t, auto h) {
-      const auto stats = u ? epp::choose_parts<decltype(t), h.value, false> : epp::choose_parts<decltype(t), h.value, true>;
+    with_kernel(r->dtype, k, [&](auto t, auto h, auto whole) {
+      const auto stats = u ? epp::choose_parts<decltype(t), h.value, whole.value, false> : epp::choose_parts<decltype(t), h.value, whole.value, true>;
       hipLaunchKernelGGL(stats, dim3((unsigned)(r->rows * cut.parts)), dim3(epp::kThreads), 0, stream, k, cut.pieces, cut.parts, parts);
-      hipLaunchKernelGGL((epp::choose_join<decltype(t), h.value>), dim3((unsigned)r->rows), dim3(epp::kThreads), 0, stream, k, cut.pieces, cut.parts, parts, u, u_f64, out);
+      hipLaunchKernelGGL((epp::choose_join<decltype(t), h.value, whole.value>), dim3((unsigned)r->rows), dim3(epp::kThreads), 0, stream, k, cut.pieces, cut.parts, parts, u, u_f64, out);
     });
   }
   HIP_TRY(hipGetLastError());
@@ -207,17 +211,17 @@ int ep_policy_evaluate(const ep_policy_rows* r, const int32_t* action, float* lo
   if (r->options <= kGroupOptions) {
     const Width w = group_width(k);
     const size_t lds = k.history ? w.lds : 0;
-    with_kernel(r->dtype, k.history, [&](auto t, auto h) {
-      if (w.pieces == 1) hipLaunchKernelGGL((epp::evaluate_group<decltype(t), 1, h.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, out);
-      else if (w.pieces == 2) hipLaunchKernelGGL((epp::evaluate_group<decltype(t), 2, h.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, out);
-      else hipLaunchKernelGGL((epp::evaluate_group<decltype(t), 4, h.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, out);
+    with_kernel(r->dtype, k, [&](auto t, auto h, auto whole) {
+      if (w.pieces == 1) hipLaunchKernelGGL((epp::evaluate_group<decltype(t), 1, h.value, whole.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, out);
+      else if (w.pieces == 2) hipLaunchKernelGGL((epp::evaluate_group<decltype(t), 2, h.value, whole.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, out);
+      else hipLaunchKernelGGL((epp::evaluate_group<decltype(t), 4, h.value, whole.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, out);
     });
   } else {
     const Cut cut = cut_rows(r->rows, r->options);
     if (r->rows * cut.parts > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld rows of %lld options", (long long)r->rows, (long long)r->options);
     auto* parts = (epp::EvaluatePart*)r->workspace;
-    with_kernel(r->dtype, k.history, [&](auto t, auto h) {
-      hipLaunchKernelGGL((epp::evaluate_parts<decltype(t), h.value>), dim3((unsigned)(r->rows * cut.parts)), dim3(epp::kThreads), 0, stream, k, cut.pieces, cut.parts, parts, out);
+    with_kernel(r->dtype, k, [&](auto t, auto h, auto whole) {
+      hipLaunchKernelGGL((epp::evaluate_parts<decltype(t), h.value, whole.value>), dim3((unsigned)(r->rows * cut.parts)), dim3(epp::kThreads), 0, stream, k, cut.pieces, cut.parts, parts, out);
     });
     if (cut.parts > 1)
       hipLaunchKernelGGL(epp::evaluate_join, dim3((unsigned)((r->rows + 3) / 4)), dim3(epp::kThreads), 0, stream, k, cut.parts, parts, out);
@@ -261,17 +265,17 @@ int ep_policy_evaluate_grad(const ep_policy_rows* r, const int32_t* action, cons
                     partial, 0};
     g.vec_out = (uintptr_t)grad_logits % 16 == 0 && (r->rows <= 1 || (grad_logits_stride * (int64_t)size_of(r->dtype)) % 16 == 0);
     const int64_t per = (r->rows + blocks - 1) / blocks;
-    with_kernel(r->dtype, k.history, [&](auto t, auto h) {
+    with_kernel(r->dtype, k, [&](auto t, auto h, auto whole) {
       const size_t lds = k.history || shared ? w.lds : 0;
       if (group && w.pieces == 1)
-        hipLaunchKernelGGL((epp::evaluate_grad_group<decltype(t), 1, h.value>), dim3((unsigned)blocks), dim3(epp::kThreads), lds, stream, k, g, w.log, (int64_t)w.blocks);
+        hipLaunchKernelGGL((epp::evaluate_grad_group<decltype(t), 1, h.value, whole.value>), dim3((unsigned)blocks), dim3(epp::kThreads), lds, stream, k, g, w.log, (int64_t)w.blocks);
       else if (group && w.pieces == 2)
-        hipLaunchKernelGGL((epp::evaluate_grad_group<decltype(t), 2, h.value>), dim3((unsigned)blocks), dim3(epp::kThreads), lds, stream, k, g, w.log, (int64_t)w.blocks);
+        hipLaunchKernelGGL((epp::evaluate_grad_group<decltype(t), 2, h.value, whole.value>), dim3((unsigned)blocks), dim3(epp::kThreads), lds, stream, k, g, w.log, (int64_t)w.blocks);
       else if (group)
-        hipLaunchKernelGGL((epp::evaluate_grad_group<decltype(t), 4, h.value>), dim3((unsigned)blocks), dim3(epp::kThreads), lds, stream, k, g, w.log, (int64_t)w.blocks);
+        hipLaunchKernelGGL((epp::evaluate_grad_group<decltype(t), 4, h.value, whole.value>), dim3((unsigned)blocks), dim3(epp::kThreads), lds, stream, k, g, w.log, (int64_t)w.blocks);
       else
-        hipLaunchKernelGGL((epp::evaluate_grad_piece<decltype(t), h.value>), dim3((unsigned)pieces, (unsigned)blocks), dim3(epp::kThreads), 0, stream, k, g, per);
-    });
+        hipLaunchKernelGGL((epp::evaluate_grad_piece<decltype(t), h.value, whole.value>), dim3((unsigned)pieces, (unsigned)blocks), dim3(epp::kThreads), 0, stream, k, g, per);
+    }, g.vec_out);
     HIP_TRY(hipGetLastError());
   }
   if (shared) {

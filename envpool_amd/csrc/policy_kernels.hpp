@@ -31,7 +31,10 @@ struct Rows {
   int64_t history_len, history_stride;
   const float *repetition, *frequency, *presence, *temperature;
   double repetition_all, frequency_all, presence_all, temperature_all;
-  int32_t vec;  // rows of logits, 32-bit biases and byte masks start on boundaries of their 8-option loads
+  double inv_t_all;  // 1 / temperature_all, and the same in 32 bits
+  float inv_t_all_32;
+  int32_t vec;  // rows of logits, 32-bit biases and byte masks start on boundaries of their 8-option loads (with
+                // options a multiple of 8 too, every row is made of whole eights: kWhole)
 };
 
 constexpr int kThreads = 256;
@@ -94,7 +97,8 @@ template <class R> struct RowConst {
 template <class R, bool kHist> __device__ inline RowConst<R> row_const(const Rows& p, int64_t row) {
   RowConst<R> c{};
   const R t = p.temperature ? (R)p.temperature[row] : (R)p.temperature_all;
-  c.inv_t = (R)1 / t;
+  if (p.temperature) c.inv_t = (R)1 / t;
+  else c.inv_t = sizeof(R) == 8 ? (R)p.inv_t_all : (R)p.inv_t_all_32;
   c.k = c.inv_t * ((R)1 / Num<R>::kUnit);
   c.bad = !(t > (R)0) || !(t < (R)INFINITY) || !(c.k < (R)INFINITY);
   if (kHist) {
@@ -153,26 +157,69 @@ __device__ inline double pick(uint32_t bits, int i, double v, double other) {
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
+// The operands of options j0 .. j0+7 of a row (j0 a multiple of 8, below the row's end) as they lie in memory. With
+// kWhole every row is made of whole eights that can be read at once: all operands are then asked for before the first
+// is used, and a walk asks for its next eight before it works on these. (Ragged rows are read where they are used:
+// eight guarded loads each, in twice the registers.)
+template <class T, bool kWhole> struct Raw {
+  __device__ void ask_row(const Rows&, int64_t, int64_t) {}
+  __device__ void ask_bias(const Rows&, int64_t, int64_t) {}
+};
+template <class T> struct Raw<T, true> {
+  typedef uint32_t Words __attribute__((ext_vector_type(kPer * sizeof(T) / 4)));
+  Words x;
+  uint64_t m;  // eight mask bytes, or the word that holds the eight bits
+  float b[kPer];
+  __device__ void ask_row(const Rows& p, int64_t row, int64_t j0) {
+    if (p.mask) {
+      if (p.mask_bits) m = ((const uint32_t*)p.mask)[row * p.mask_stride + (j0 >> 5)];
+      else m = *(const uint64_t*)((const uint8_t*)p.mask + row * p.mask_stride + j0);
+    }
+    x = *(const Words*)((const T*)p.logits + row * p.logits_stride + j0);
+  }
+  __device__ void ask_bias(const Rows& p, int64_t row, int64_t j0) {
+    if (!p.bias) return;
+    const int64_t b0 = row * p.bias_stride + j0;
+    if (p.bias_f32) {
+      *(Vec8<float>*)b = *(const Vec8<float>*)((const float*)p.bias + b0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) b[i] = (float)((const T*)p.bias)[b0 + i];
+    }
+  }
+  __device__ float logit(int i) const {
+    T v[sizeof(x[0]) / sizeof(T)];
+    const uint32_t word = x[i * (int)sizeof(T) / 4];
+    __builtin_memcpy(v, &word, 4);
+    return (float)v[i % (4 / (int)sizeof(T))];
+  }
+};
+
 // Options j0 .. j0+7 of a row (j0 a multiple of 8, below the row's end): y before the temperature, as they
 // come. Returns which are legal (bit i = option j0 + i); the y of the others are unspecified.
 // whole: all eight exist and every operand can be read eight at a time. slope: d y / d logit.
-template <class T, class R, bool kHist>
-__device__ inline uint32_t load_y(const Rows& p, const RowConst<R>& c, int64_t row, int64_t j0, bool whole, const Seen<R>& seen, R (&y)[kPer],
-                                  R* slope = nullptr) {
+template <class T, class R, bool kHist, bool kWhole>
+__device__ inline uint32_t load_y(const Rows& p, const RowConst<R>& c, int64_t row, int64_t j0, bool whole, const Raw<T, kWhole>& raw, const Seen<R>& seen,
+                                  R (&y)[kPer], R* slope = nullptr) {
   const int64_t left = c.n_legal - j0;
   uint32_t legal = left >= kPer ? 0xffu : left > 0 ? (1u << left) - 1u : 0u;
   if (p.mask) {
     if (p.mask_bits) {
-      legal &= ((const uint32_t*)p.mask)[row * p.mask_stride + (j0 >> 5)] >> (j0 & 31);
+      if constexpr (kWhole) legal &= (uint32_t)raw.m >> (j0 & 31);
+      else legal &= ((const uint32_t*)p.mask)[row * p.mask_stride + (j0 >> 5)] >> (j0 & 31);
     } else {
-      const uint8_t* m = (const uint8_t*)p.mask + row * p.mask_stride + j0;
       uint64_t w = 0;
-      if (whole) {
-        w = *(const uint64_t*)m;
+      if constexpr (kWhole) {
+        w = raw.m;
       } else {
+        const uint8_t* m = (const uint8_t*)p.mask + row * p.mask_stride + j0;
+        if (whole) {
+          w = *(const uint64_t*)m;
+        } else {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i)
-          if (j0 + i < p.options) w |= (uint64_t)m[i] << (8 * i);
+          for (int i = 0; i < kPer; ++i)
+            if (j0 + i < p.options) w |= (uint64_t)m[i] << (8 * i);
+        }
       }
       // nonzero bytes to bits: every byte folded onto its lowest bit, four of them gathered by a product
       w |= w >> 4;
@@ -182,16 +229,21 @@ __device__ inline uint32_t load_y(const Rows& p, const RowConst<R>& c, int64_t r
       legal &= ((lo * 0x01020408u) >> 24) | (((hi * 0x01020408u) >> 24) << 4);
     }
   }
-  const T* x = (const T*)p.logits + row * p.logits_stride + j0;
-  T xv[kPer];
-  if (whole) {
-    *(Vec8<T>*)xv = *(const Vec8<T>*)x;
+  if constexpr (kWhole) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) y[i] = (R)raw.logit(i);
   } else {
+    const T* x = (const T*)p.logits + row * p.logits_stride + j0;
+    T xv[kPer];
+    if (whole) {
+      *(Vec8<T>*)xv = *(const Vec8<T>*)x;
+    } else {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) xv[i] = j0 + i < p.options ? x[i] : (T)0.f;
+      for (int i = 0; i < kPer; ++i) xv[i] = j0 + i < p.options ? x[i] : (T)0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) y[i] = (R)(float)xv[i];
   }
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) y[i] = (R)(float)xv[i];
   if (kHist) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -201,7 +253,12 @@ __device__ inline uint32_t load_y(const Rows& p, const RowConst<R>& c, int64_t r
       else y[i] = penalized<R>(y[i], n, c);
     }
   }
-  if (p.bias) {
+  if constexpr (kWhole) {
+    if (p.bias) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) y[i] += (R)raw.b[i];
+    }
+  } else if (p.bias) {
     const int64_t b0 = row * p.bias_stride + j0;
     if (p.bias_f32) {
       const float* b = (const float*)p.bias + b0;
@@ -237,15 +294,16 @@ template <class T> __device__ inline float hold_range(const Rows& p, int64_t row
 
 // load_y made ready for sums: kNone where there is no weight, m the largest. Returns whether a legal one is NaN or +inf. Nearly
 // always all are finite, which one product with 0 per option shows (0 * inf and 0 * NaN are NaN).
-template <class T, class R, bool kHist>
-__device__ inline bool load_ready(const Rows& p, const RowConst<R>& c, int64_t row, int64_t j0, bool whole, const Seen<R>& seen, R (&y)[kPer], R& m) {
+template <class T, class R, bool kHist, bool kWhole>
+__device__ inline bool load_ready(const Rows& p, const RowConst<R>& c, int64_t row, int64_t j0, bool whole, const Raw<T, kWhole>& raw, const Seen<R>& seen,
+                                  R (&y)[kPer], R& m) {
   m = Num<R>::kNone;
   if (j0 >= c.n_legal) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) y[i] = Num<R>::kNone;
     return false;
   }
-  const uint32_t legal = load_y<T, R, kHist>(p, c, row, j0, whole, seen, y);
+  const uint32_t legal = load_y<T, R, kHist, kWhole>(p, c, row, j0, whole, raw, seen, y);
   R odd = (R)0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
@@ -370,9 +428,15 @@ __device__ inline Seen<R> count_piece(const Rows& p, const RowConst<R>& c, int64
   __syncthreads();
   const int32_t* h = p.history + row * p.history_stride;
   const uint32_t size = (uint32_t)min((int64_t)kPiece, p.options - j0);
-  for (int64_t i = threadIdx.x; i < p.history_len; i += kThreads) {
-    const uint32_t j = (uint32_t)h[i] - (uint32_t)j0;
-    if (j < size && atomicAdd(&s.count[j], 1u) == 0) s.list[atomicAdd(&s.n, 1)] = (uint16_t)j;
+  // (eight entries under way at once: one after the other, each would wait for its load and its two additions)
+  constexpr int kAhead = 8;
+  for (int64_t i0 = threadIdx.x; i0 < p.history_len; i0 += kAhead * kThreads) {
+    uint32_t j[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) j[i] = i0 + i * kThreads < p.history_len ? (uint32_t)h[i0 + i * kThreads] - (uint32_t)j0 : size;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (j[i] < size && atomicAdd(&s.count[j[i]], 1u) == 0) s.list[atomicAdd(&s.n, 1)] = (uint16_t)j[i];
   }
   __syncthreads();
   for (int i = threadIdx.x; i < s.n; i += kThreads) {
@@ -459,19 +523,23 @@ template <int NP> __device__ inline const uint32_t* count_groups(const Rows& p, 
   return mine;
 }
 
-template <class T, int NP, bool kHist>
+template <class T, int NP, bool kHist, bool kWhole>
 __global__ __launch_bounds__(kThreads) void choose_group(Rows p, int width_log, const void* u, int u_f64, ChooseOut out) {
   extern __shared__ uint32_t counts[];
   const Group g = group_of(p, blockIdx.x, width_log);
   const RowConst<double> c = row_const<double, kHist>(p, g.row);
   const uint32_t* n = kHist ? count_groups<NP>(p, g, counts) : nullptr;
-  const bool whole = p.vec && p.options % kPer == 0;
+  constexpr bool whole = kWhole;
   double y[NP][kPer];
   Stat<double> a = stat_zero<double>();
+  Raw<T, kWhole> raw[NP];
+#pragma unroll
+  for (int k = 0; k < NP; ++k)
+    if (g.j(k) < c.n_legal) raw[k].ask_row(p, g.row, g.j(k)), raw[k].ask_bias(p, g.row, g.j(k));
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
     double m;
-    a.bad |= load_ready<T, double, kHist>(p, c, g.row, g.j(k), whole, Seen<double>{n}.at(kHist ? g.j(k) : 0), y[k], m);
+    a.bad |= load_ready<T, double, kHist, kWhole>(p, c, g.row, g.j(k), whole, raw[k], Seen<double>{n}.at(kHist ? g.j(k) : 0), y[k], m);
     a.m = larger(a.m, m);
   }
   a.m = lanes_max(a.m, g.width);
@@ -539,20 +607,24 @@ __global__ __launch_bounds__(kThreads) void choose_group(Rows p, int width_log, 
   if (g.lane == 0 && g.there) finish_choose(out, g.row, a, c, pick, y_pick);
 }
 
-template <class T, int NP, bool kHist> __global__ __launch_bounds__(kThreads) void evaluate_group(Rows p, int width_log, EvaluateOut out) {
+template <class T, int NP, bool kHist, bool kWhole> __global__ __launch_bounds__(kThreads) void evaluate_group(Rows p, int width_log, EvaluateOut out) {
   extern __shared__ uint32_t counts[];
   const Group g = group_of(p, blockIdx.x, width_log);
   const RowConst<float> c = row_const<float, kHist>(p, g.row);
   const uint32_t* n = kHist ? count_groups<NP>(p, g, counts) : nullptr;
-  const bool whole = p.vec && p.options % kPer == 0;
+  constexpr bool whole = kWhole;
   const int32_t act = out.action[g.row];
   float y[NP][kPer];
   Stat<float> a = stat_zero<float>();
   float y_act = Num<float>::kNone;
+  Raw<T, kWhole> raw[NP];
+#pragma unroll
+  for (int k = 0; k < NP; ++k)
+    if (g.j(k) < c.n_legal) raw[k].ask_row(p, g.row, g.j(k)), raw[k].ask_bias(p, g.row, g.j(k));
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
     float m;
-    a.bad |= load_ready<T, float, kHist>(p, c, g.row, g.j(k), whole, Seen<float>{n}.at(kHist ? g.j(k) : 0), y[k], m);
+    a.bad |= load_ready<T, float, kHist, kWhole>(p, c, g.row, g.j(k), whole, raw[k], Seen<float>{n}.at(kHist ? g.j(k) : 0), y[k], m);
     a.m = larger(a.m, m);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -577,7 +649,7 @@ template <class T, int NP, bool kHist> __global__ __launch_bounds__(kThreads) vo
 }
 
 // ---- longer rows: a workgroup per part of a row (`pieces` pieces of kPiece options), parts joined after ---
-template <class T, bool kHist, bool kBest>
+template <class T, bool kHist, bool kWhole, bool kBest>
 __global__ __launch_bounds__(kThreads) void choose_parts(Rows p, int pieces, int n_parts, Stat<double>* parts) {
   __shared__ PieceMemory<T, double, kHist> mem;
   __shared__ Stat<double> red[kThreads / 64];
@@ -585,11 +657,18 @@ __global__ __launch_bounds__(kThreads) void choose_parts(Rows p, int pieces, int
   const RowConst<double> c = row_const<double, kHist>(p, row);
   Stat<double> a = stat_zero<double>();
   const int64_t j_end = min((part + 1) * pieces * (int64_t)kPiece, c.n_legal);
-  for (int64_t j0 = part * pieces * (int64_t)kPiece; j0 < j_end; j0 += kPiece) {
+  const int64_t j_first = part * pieces * (int64_t)kPiece;
+  Raw<T, kWhole> raw;
+  const auto ask = [&](int64_t j) {
+    if (j < j_end) raw.ask_row(p, row, j), raw.ask_bias(p, row, j);
+  };
+  ask(j_first + threadIdx.x * kPer);
+  for (int64_t j0 = j_first; j0 < j_end; j0 += kPiece) {
     const auto seen = mem.count(p, c, row, j0);
     const int64_t j = j0 + threadIdx.x * kPer;
     double y[kPer], m;
-    a.bad |= load_ready<T, double, kHist>(p, c, row, j, p.vec && j0 + kPiece <= p.options, seen, y, m);
+    a.bad |= load_ready<T, double, kHist, kWhole>(p, c, row, j, p.vec && j0 + kPiece <= p.options, raw, seen, y, m);
+    ask(j + kPiece);
     stat_add<double, kBest>(a, y, m, j, c.k);
   }
   a = stat_block(a, c.k, red);
@@ -597,7 +676,7 @@ __global__ __launch_bounds__(kThreads) void choose_parts(Rows p, int pieces, int
 }
 
 // joins a row's parts, and finds the option that u falls on by walking down the one part it lies in
-template <class T, bool kHist>
+template <class T, bool kHist, bool kWhole>
 __global__ __launch_bounds__(kThreads) void choose_join(Rows p, int pieces, int n_parts, const Stat<double>* all_parts, const void* u, int u_f64, ChooseOut out) {
   __shared__ PieceMemory<T, double, kHist> mem;
   __shared__ Stat<double> red[kThreads / 64];
@@ -656,10 +735,12 @@ __global__ __launch_bounds__(kThreads) void choose_join(Rows p, int pieces, int 
     double last_y = 0;
     const int64_t j_first = part_at * (int64_t)pieces * kPiece, j_end = min(j_first + pieces * (int64_t)kPiece, c.n_legal);
     for (int64_t j0 = j_first; j0 < j_end; j0 += kPiece) {
-      const auto seen = mem.count(p, c, row, j0);
       const int64_t j = j0 + threadIdx.x * kPer;
+      Raw<T, kWhole> raw;
+      if (j < j_end) raw.ask_row(p, row, j), raw.ask_bias(p, row, j);
+      const auto seen = mem.count(p, c, row, j0);
       double y[kPer], w[kPer], m, sum = 0;
-      (void)load_ready<T, double, kHist>(p, c, row, j, p.vec && j0 + kPiece <= p.options, seen, y, m);
+      (void)load_ready<T, double, kHist, kWhole>(p, c, row, j, p.vec && j0 + kPiece <= p.options, raw, seen, y, m);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         w[i] = weight(exponent(y[i], a.m, c.k));
@@ -707,8 +788,8 @@ struct EvaluatePart {
   Stat<float> stat;
   float y_act;
 };
-template <class T, bool kHist>
-__global__ __launch_bounds__(kThreads) void evaluate_parts(Rows p, int pieces, int n_parts, EvaluatePart* parts, EvaluateOut out) {
+template <class T, bool kHist, bool kWhole>
+__global__ __launch_bounds__(kThreads, kHist ? 6 : 8) void evaluate_parts(Rows p, int pieces, int n_parts, EvaluatePart* parts, EvaluateOut out) {
   __shared__ PieceMemory<T, float, kHist> mem;
   __shared__ Stat<float> red[kThreads / 64];
   __shared__ float y_act;
@@ -719,11 +800,18 @@ __global__ __launch_bounds__(kThreads) void evaluate_parts(Rows p, int pieces, i
   if (threadIdx.x == 0) y_act = Num<float>::kNone;
   __syncthreads();
   const int64_t j_end = min((part + 1) * pieces * (int64_t)kPiece, c.n_legal);
-  for (int64_t j0 = part * pieces * (int64_t)kPiece; j0 < j_end; j0 += kPiece) {
+  const int64_t j_first = part * pieces * (int64_t)kPiece;
+  Raw<T, kWhole> raw;
+  const auto ask = [&](int64_t j) {
+    if (j < j_end) raw.ask_row(p, row, j), raw.ask_bias(p, row, j);
+  };
+  ask(j_first + threadIdx.x * kPer);
+  for (int64_t j0 = j_first; j0 < j_end; j0 += kPiece) {
     const auto seen = mem.count(p, c, row, j0);
     const int64_t j = j0 + threadIdx.x * kPer;
     float y[kPer], m;
-    a.bad |= load_ready<T, float, kHist>(p, c, row, j, p.vec && j0 + kPiece <= p.options, seen, y, m);
+    a.bad |= load_ready<T, float, kHist, kWhole>(p, c, row, j, p.vec && j0 + kPiece <= p.options, raw, seen, y, m);
+    ask(j + kPiece);
     stat_add<float, false>(a, y, m, j, c.k);
     if ((uint64_t)(act - j) < kPer) {
 #pragma unroll
@@ -758,6 +846,11 @@ __global__ __launch_bounds__(kThreads) inline void evaluate_join(Rows p, int n_p
   y_act = lanes_max(y_act, 64);
   if ((threadIdx.x & 63) == 0) finish_evaluate(out, row, p.options, a, c, out.action[row], y_act);
 }
+
+// workgroups of the gradients' kernels that a CU holds at once: their registers are kept to as many, and the walks
+// down the rows are cut for as many (one round of equal walks, none that waits for a place)
+constexpr int kGradPieceBlocks = 6;
+constexpr int grad_group_per_cu(int pieces) { return pieces == 4 ? 2 : 4; }
 
 struct GradArgs {
   const int32_t* action;
@@ -823,33 +916,40 @@ template <class T> __device__ inline void store8(T* out, const float (&v)[kPer],
 
 // short rows: the lanes of evaluate_group, walking down the rows; a shared bias' gradient is summed per lane, then
 // over the workgroup's row slots
-template <class T, int NP, bool kHist> __global__ __launch_bounds__(kThreads) void evaluate_grad_group(Rows p, GradArgs g, int width_log, int64_t blocks_of_rows) {
+template <class T, int NP, bool kHist, bool kWhole> __global__ __launch_bounds__(kThreads, grad_group_per_cu(NP)) void evaluate_grad_group(Rows p, GradArgs g, int width_log, int64_t blocks_of_rows) {
   extern __shared__ uint32_t counts[];  // (as floats for the sums afterwards)
   float sum[NP][kPer];
 #pragma unroll
   for (int k = 0; k < NP; ++k)
 #pragma unroll
     for (int i = 0; i < kPer; ++i) sum[k][i] = 0.f;
+  Raw<T, kWhole> raw[NP];
   for (int64_t b = blockIdx.x; b < blocks_of_rows; b += gridDim.x) {
     const Group at = group_of(p, b, width_log);
     const uint32_t* n = kHist ? count_groups<NP>(p, at, counts) : nullptr;
-    const bool whole = p.vec && p.options % kPer == 0;
+    constexpr bool whole = kWhole;
     if (!at.there) continue;
     const RowConst<float> c = row_const<float, kHist>(p, at.row);
     const GradRow r = grad_row<kHist>(g, c, at.row);
+#pragma unroll
+    for (int k = 0; k < NP; ++k)
+      if (at.j(k) < p.options) {
+        raw[k].ask_row(p, at.row, at.j(k));
+        if (p.bias_stride != 0 || b == blockIdx.x) raw[k].ask_bias(p, at.row, at.j(k));
+      }
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
       const int64_t j = at.j(k);
       if (j >= p.options) continue;
       float y[kPer], slope[kPer], dx[kPer], db[kPer];
-      const uint32_t legal = load_y<T, float, kHist>(p, c, at.row, j, whole, Seen<float>{n}.at(kHist ? j : 0), y, slope);
+      const uint32_t legal = load_y<T, float, kHist, kWhole>(p, c, at.row, j, whole, raw[k], Seen<float>{n}.at(kHist ? j : 0), y, slope);
       grad_y(r, y, r.empty ? 0u : legal, j, db);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         dx[i] = kHist ? db[i] * slope[i] : db[i];
         sum[k][i] += db[i];
       }
-      if (g.grad_logits) store8<T>((T*)g.grad_logits + at.row * g.grad_logits_stride + j, dx, j, p.options, g.vec_out);
+      if (g.grad_logits) store8<T>((T*)g.grad_logits + at.row * g.grad_logits_stride + j, dx, j, kWhole ? INT64_MAX : p.options, kWhole || g.vec_out);
       if (g.grad_bias) {
         const int64_t to = at.row * g.grad_bias_stride + j;
         if (p.bias_f32) store8<float>((float*)g.grad_bias + to, db, j, p.options, false);
@@ -875,8 +975,8 @@ template <class T, int NP, bool kHist> __global__ __launch_bounds__(kThreads) vo
 }
 
 // a workgroup owns kPiece columns and walks down its rows: the sum of a shared bias' gradient stays in registers
-template <class T, bool kHist>
-__global__ __launch_bounds__(kThreads) void evaluate_grad_piece(Rows p, GradArgs g, int64_t rows_per_block) {
+template <class T, bool kHist, bool kWhole>
+__global__ __launch_bounds__(kThreads, kGradPieceBlocks) void evaluate_grad_piece(Rows p, GradArgs g, int64_t rows_per_block) {
   __shared__ PieceMemory<T, float, kHist> mem;
   const int64_t j0 = (int64_t)blockIdx.x * kPiece;
   const int64_t j = j0 + threadIdx.x * kPer;
@@ -885,20 +985,26 @@ __global__ __launch_bounds__(kThreads) void evaluate_grad_piece(Rows p, GradArgs
   float sum[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) sum[i] = 0.f;
+  Raw<T, kWhole> raw;
+  if (r0 < r1 && j < p.options) raw.ask_row(p, r0, j), raw.ask_bias(p, r0, j);
   for (int64_t row = r0; row < r1; ++row) {
     const RowConst<float> c = row_const<float, kHist>(p, row);
     const GradRow r = grad_row<kHist>(g, c, row);
     const auto seen = mem.count(p, c, row, j0);
     if (j >= p.options) continue;
     float y[kPer], slope[kPer], dx[kPer], db[kPer];
-    const uint32_t legal = load_y<T, float, kHist>(p, c, row, j, p.vec && j0 + kPiece <= p.options, seen, y, slope);
+    const uint32_t legal = load_y<T, float, kHist, kWhole>(p, c, row, j, p.vec && j0 + kPiece <= p.options, raw, seen, y, slope);
+    if (row + 1 < r1) {
+      raw.ask_row(p, row + 1, j);
+      if (p.bias_stride != 0) raw.ask_bias(p, row + 1, j);
+    }
     grad_y(r, y, r.empty ? 0u : legal, j, db);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       dx[i] = kHist ? db[i] * slope[i] : db[i];
       sum[i] += db[i];
     }
-    if (g.grad_logits) store8<T>((T*)g.grad_logits + row * g.grad_logits_stride + j, dx, j, p.options, g.vec_out);
+    if (g.grad_logits) store8<T>((T*)g.grad_logits + row * g.grad_logits_stride + j, dx, j, kWhole ? INT64_MAX : p.options, kWhole || g.vec_out);
     if (g.grad_bias) {
       const int64_t at = row * g.grad_bias_stride + j;
       if (p.bias_f32) store8<float>((float*)g.grad_bias + at, db, j, p.options, false);
