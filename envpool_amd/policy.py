@@ -223,7 +223,7 @@ def _evaluate_backward(ctx, g_lp, g_h):
   grad_x = torch.empty_like(logits, memory_format=torch.contiguous_format) if want_x else None
   grad_b, stride = None, 0
   if want_b:
-    grad_b = torch.empty(p.bias.shape if p.bias_stride else (p.options,), dtype=bias.dtype, device=p.dev)
+    grad_b = torch.empty((p.n, p.options) if p.bias_stride else (p.options,), dtype=bias.dtype, device=p.dev)
     stride = p.options if p.bias_stride else 0
   ws, ws_ptr, ws_bytes = _scratch(p.native.grad_workspace(want_b), p.dev)
   p.native.evaluate_grad(action.data_ptr(), entropy.data_ptr(), stats.data_ptr(), 0 if g_lp is None else g_lp.data_ptr(),
@@ -239,8 +239,9 @@ class _Evaluate(torch.autograd.Function):
     log_prob, entropy, stats = _evaluate_forward(p, action)
     ctx.set_materialize_grads(False)
     # (the native struct holds addresses: every tensor behind it is saved, so that torch notices one that was
-    # changed in place before the backward pass)
+    # changed in place before the backward pass, and frees it after)
     ctx.save_for_backward(logits, bias, action, entropy, stats, *[t for t in (p.logits, p.bias, *p.keep) if t is not None])
+    p.logits = p.bias = p.keep = None
     ctx.p = p
     return log_prob, entropy
 
@@ -268,7 +269,9 @@ def evaluate(logits, action, *, num_options=None, mask=None, bias=None, history=
   if not action.is_contiguous():
     action = action.contiguous()
   if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
-    p.logits, p.bias = p.logits.detach(), None if p.bias is None else p.bias.detach()
+    # (of the two that are differentiated only the copies that the kernels read instead)
+    p.logits = None if p.logits is logits else p.logits.detach()
+    p.bias = None if p.bias is bias else p.bias.detach()
     nodes = _guard_capture(logits, bias)  # noqa: F841
     return _Evaluate.apply(logits, bias, action, p)
   return _evaluate_forward(p, action)[:2]
