@@ -55,6 +55,9 @@ struct DeviceScope {
   ::epc::DeviceScope _dev_scope;   \
   HIP_TRY(_dev_scope.enter(dev))
 
+// workgroups of 256 that one launch can have: the runtime counts its threads in 32 bits
+constexpr long long kMaxGroups256 = 0xffffffffll / 256;
+
 // The same for calls that have no object of their own (their device comes with the arguments): a device that does
 // not exist is named as such.
 #define EP_ENTER_GPU(dev)                                                                                             \

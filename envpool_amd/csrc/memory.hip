@@ -10,6 +10,7 @@
 namespace {
 
 using epc::fail;
+using epc::kMaxGroups256;
 
 bool float_type(int32_t dtype) { return dtype == EP_F32 || dtype == EP_F16 || dtype == EP_BF16; }
 size_t size_of(int32_t dtype) { return dtype == EP_F32 ? 4 : 2; }
@@ -95,7 +96,7 @@ int check_scan(const ep_memory_scan_args* a) {
   const void* words[] = {a->log_decay, a->state_in, a->state_out};
   for (const void* ptr : words)
     if ((uintptr_t)ptr % 4) return fail(EP_ERR_INVALID, "an array of 4-byte values is not aligned to 4 bytes");
-  if (a->rows * a->heads > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld rows of %d heads", (long long)a->rows, a->heads);
+  if (a->rows * a->heads > kMaxGroups256) return fail(EP_ERR_TOO_LARGE, "%lld rows of %d heads", (long long)a->rows, a->heads);
   return EP_OK;
 }
 bool nothing_to_do(const ep_memory_scan_args* a) { return a->rows == 0 || (a->steps == 0 && !a->state_out); }
@@ -192,7 +193,7 @@ int ep_memory_step(const ep_memory_step_args* a) {
     if ((uintptr_t)ptr % 4) return fail(EP_ERR_INVALID, "an array of 4-byte values is not aligned to 4 bytes");
   if (int rc = check_workspace(a->workspace, a->workspace_bytes, step_workspace(a))) return rc;
   if (a->rows == 0) return EP_OK;
-  if (a->rows * a->heads > 4 * (int64_t)INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld rows of %d heads", (long long)a->rows, a->heads);
+  if (a->rows * a->heads > 4 * kMaxGroups256) return fail(EP_ERR_TOO_LARGE, "%lld rows of %d heads", (long long)a->rows, a->heads);
   EP_ENTER_GPU(a->device_id);
   const hipStream_t stream = (hipStream_t)a->stream;
   epm::Step k{};
@@ -265,10 +266,9 @@ int ep_memory_sum_heads(int32_t device_id, const float* src, int64_t n, int32_t 
   if (total == 0) return EP_OK;
   if (!src || !out) return fail(EP_ERR_INVALID, "src, out: null pointer");
   if ((uintptr_t)src % 4 || (uintptr_t)out % size_of(dtype)) return fail(EP_ERR_INVALID, "src, out: not aligned to their type");
-  if ((total + 255) / 256 > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld elements", (long long)total);
   EP_ENTER_GPU(device_id);
   with_type(dtype, [&](auto t) {
-    hipLaunchKernelGGL(epm::sum_heads<decltype(t)>, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, (hipStream_t)stream, src, total, group, dim,
+    hipLaunchKernelGGL(epm::sum_heads<decltype(t)>, dim3((unsigned)std::min<int64_t>((total + 255) / 256, kMaxGroups256)), dim3(256), 0, (hipStream_t)stream, src, total, group, dim,
                        (decltype(t)*)out);
   });
   HIP_TRY(hipGetLastError());

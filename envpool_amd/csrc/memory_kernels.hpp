@@ -183,12 +183,13 @@ struct Scan {
 };
 
 template <class T> __global__ __launch_bounds__(256) void sum_heads(const float* src, int64_t total, int32_t group, int32_t dim, T* out) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;  // over [n][heads_out][dim]
-  if (i >= total) return;
-  const int64_t head = i / dim, d = i % dim;
-  float s = 0.f;
-  for (int g = 0; g < group; ++g) s += src[(head * group + g) * dim + d];
-  out[i] = (T)s;
+  // over [n][heads_out][dim]
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t head = i / dim, d = i % dim;
+    float s = 0.f;
+    for (int g = 0; g < group; ++g) s += src[(head * group + g) * dim + d];
+    out[i] = (T)s;
+  }
 }
 
 }  // namespace epm

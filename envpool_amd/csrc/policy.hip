@@ -10,6 +10,7 @@
 namespace {
 
 using epc::fail;
+using epc::kMaxGroups256;
 
 size_t size_of(int32_t dtype) { return dtype == EP_F32 ? 4 : 2; }
 bool float_type(int32_t dtype) { return dtype == EP_F32 || dtype == EP_F16 || dtype == EP_BF16; }
@@ -109,7 +110,7 @@ template <class F> void with_kernel(int32_t dtype, const epp::Rows& k, F f, bool
 // of it. Longer rows are walked by workgroups, 2048 options at a time; with few rows each is cut into parts so
 // that about kFill workgroups stand on the chip.
 constexpr int64_t kGroupOptions = 64 * epp::kPer * 4;
-constexpr int64_t kFill = 2048;
+constexpr int64_t kFill = 2048, kChooseFill = 2 * kFill;
 constexpr int64_t kManyOctets = 262144;
 
 struct Width {
@@ -150,13 +151,20 @@ int64_t grad_row_blocks(int64_t rows, int64_t options) {
   return per > 0 ? (rows + per - 1) / per : 0;
 }
 
+// whether one launch can hold the workgroups of a pass over the rows
+int check_groups(const ep_policy_rows* r, const epp::Rows& k, int64_t fill) {
+  const int64_t groups = r->options <= kGroupOptions ? group_width(k).blocks : r->rows * cut_rows(r->rows, r->options, fill).parts;
+  if (groups > kMaxGroups256) return fail(EP_ERR_TOO_LARGE, "%lld rows of %lld options", (long long)r->rows, (long long)r->options);
+  return EP_OK;
+}
+
 }  // namespace
 
 extern "C" {
 
 int64_t ep_policy_choose_workspace(const ep_policy_rows* r) {
   if (!r || r->rows <= 0 || r->options <= kGroupOptions) return 0;
-  return r->rows * cut_rows(r->rows, r->options, 2 * kFill).parts * (int64_t)sizeof(epp::Stat<double>);
+  return r->rows * cut_rows(r->rows, r->options, kChooseFill).parts * (int64_t)sizeof(epp::Stat<double>);
 }
 
 int ep_policy_choose(const ep_policy_rows* r, const void* u, int32_t u_dtype, int32_t* action, float* log_prob, float* entropy) {
@@ -165,8 +173,9 @@ int ep_policy_choose(const ep_policy_rows* r, const void* u, int32_t u_dtype, in
   if (u && u_dtype != EP_F32 && u_dtype != EP_F64) return fail(EP_ERR_INVALID, "u_dtype = %d is neither EP_F32 nor EP_F64", u_dtype);
   if (u && (uintptr_t)u % (u_dtype == EP_F64 ? 8 : 4)) return fail(EP_ERR_INVALID, "u: not aligned to its type");
   if (r->rows > 0 && (!action || !log_prob || !entropy)) return fail(EP_ERR_INVALID, "action, log_prob, entropy: null pointer");
-  if (int rc = check_workspace(r, ep_policy_choose_workspace(r))) return rc;
   if (r->rows == 0) return EP_OK;
+  if (int rc = check_groups(r, k, kChooseFill)) return rc;
+  if (int rc = check_workspace(r, ep_policy_choose_workspace(r))) return rc;
   EP_ENTER_GPU(r->device_id);
   const hipStream_t stream = (hipStream_t)r->stream;
   const epp::ChooseOut out{action, log_prob, entropy};
@@ -180,8 +189,7 @@ int ep_policy_choose(const ep_policy_rows* r, const void* u, int32_t u_dtype, in
       else hipLaunchKernelGGL((epp::choose_group<decltype(t), 4, h.value, whole.value>), dim3(w.blocks), dim3(epp::kThreads), lds, stream, k, w.log, u, u_f64, out);
     });
   } else {
-    const Cut cut = cut_rows(r->rows, r->options, 2 * kFill);
-    if (r->rows * cut.parts > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld rows of %lld options", (long long)r->rows, (long long)r->options);
+    const Cut cut = cut_rows(r->rows, r->options, kChooseFill);
     auto* parts = (epp::Stat<double>*)r->workspace;
     with_kernel(r->dtype, k, [&](auto t, auto h, auto whole) {
       const auto stats = u ? epp::choose_parts<decltype(t), h.value, whole.value, false> : epp::choose_parts<decltype(t), h.value, whole.value, true>;
@@ -203,8 +211,9 @@ int ep_policy_evaluate(const ep_policy_rows* r, const int32_t* action, float* lo
   epp::Rows k;
   if (int rc = check_rows(r, &k)) return rc;
   if (r->rows > 0 && (!action || !log_prob || !entropy || !stats)) return fail(EP_ERR_INVALID, "action, log_prob, entropy, stats: null pointer");
-  if (int rc = check_workspace(r, ep_policy_evaluate_workspace(r))) return rc;
   if (r->rows == 0) return EP_OK;
+  if (int rc = check_groups(r, k, kFill)) return rc;
+  if (int rc = check_workspace(r, ep_policy_evaluate_workspace(r))) return rc;
   EP_ENTER_GPU(r->device_id);
   const hipStream_t stream = (hipStream_t)r->stream;
   const epp::EvaluateOut out{action, log_prob, entropy, stats};
@@ -218,7 +227,6 @@ int ep_policy_evaluate(const ep_policy_rows* r, const int32_t* action, float* lo
     });
   } else {
     const Cut cut = cut_rows(r->rows, r->options);
-    if (r->rows * cut.parts > INT32_MAX) return fail(EP_ERR_TOO_LARGE, "%lld rows of %lld options", (long long)r->rows, (long long)r->options);
     auto* parts = (epp::EvaluatePart*)r->workspace;
     with_kernel(r->dtype, k, [&](auto t, auto h, auto whole) {
       hipLaunchKernelGGL((epp::evaluate_parts<decltype(t), h.value, whole.value>), dim3((unsigned)(r->rows * cut.parts)), dim3(epp::kThreads), 0, stream, k, cut.pieces, cut.parts, parts, out);
@@ -281,12 +289,10 @@ int ep_policy_evaluate_grad(const ep_policy_rows* r, const int32_t* action, cons
   if (shared) {
     with_type(r->bias_dtype, [&](auto t) {
       // few columns: four a workgroup, so that 64 threads go down each; many: a cache line of them
-      if (r->options <= 1024)
-        hipLaunchKernelGGL((epp::sum_partials<decltype(t), 4>), dim3((unsigned)((r->options + 3) / 4)), dim3(epp::kThreads), 0, stream, partial,
-                           r->rows > 0 ? blocks : 0, r->options, (decltype(t)*)grad_bias);
-      else
-        hipLaunchKernelGGL((epp::sum_partials<decltype(t), 32>), dim3((unsigned)((r->options + 31) / 32)), dim3(epp::kThreads), 0, stream, partial,
-                           r->rows > 0 ? blocks : 0, r->options, (decltype(t)*)grad_bias);
+      const int cols = r->options <= 1024 ? 4 : 32;
+      const unsigned groups = (unsigned)std::min<int64_t>((r->options + cols - 1) / cols, 65536);
+      const auto sum = cols == 4 ? epp::sum_partials<decltype(t), 4> : epp::sum_partials<decltype(t), 32>;
+      hipLaunchKernelGGL(sum, dim3(groups), dim3(epp::kThreads), 0, stream, partial, r->rows > 0 ? blocks : 0, r->options, (decltype(t)*)grad_bias);
     });
     HIP_TRY(hipGetLastError());
   }

@@ -166,7 +166,7 @@ template <class T, bool kWhole> struct Raw {
   __device__ void ask_bias(const Rows&, int64_t, int64_t) {}
 };
 template <class T> struct Raw<T, true> {
-  typedef uint32_t Words __attribute__((ext_vector_type(kPer * sizeof(T) / 4)));
+  typedef uint32_t Words __attribute__((ext_vector_type(kPer * sizeof(T) / 4), aligned(16)));
   Words x;
   uint64_t m;  // eight mask bytes, or the word that holds the eight bits
   float b[kPer];
@@ -1024,22 +1024,25 @@ template <class T, int kCols>
 __global__ __launch_bounds__(kThreads) void sum_partials(const float* partial, int64_t n, int64_t options, T* out) {
   __shared__ float red[kThreads];
   constexpr int kDown = kThreads / kCols;
-  const int64_t j = (int64_t)blockIdx.x * kCols + threadIdx.x % kCols;
-  float s[4] = {0.f, 0.f, 0.f, 0.f};
-  if (j < options) {
-    int64_t i = threadIdx.x / kCols;
-    for (; i + 3 * kDown < n; i += 4 * kDown)
+  for (int64_t j0 = (int64_t)blockIdx.x * kCols; j0 < options; j0 += (int64_t)gridDim.x * kCols) {
+    const int64_t j = j0 + threadIdx.x % kCols;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (j < options) {
+      int64_t i = threadIdx.x / kCols;
+      for (; i + 3 * kDown < n; i += 4 * kDown)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) s[q] += partial[(i + q * kDown) * options + j];
-    for (; i < n; i += kDown) s[0] += partial[i * options + j];
-  }
-  red[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
-  __syncthreads();
-  for (int o = kDown / 2; o > 0; o >>= 1) {
-    if ((int)threadIdx.x < o * kCols) red[threadIdx.x] += red[threadIdx.x + o * kCols];
+        for (int q = 0; q < 4; ++q) s[q] += partial[(i + q * kDown) * options + j];
+      for (; i < n; i += kDown) s[0] += partial[i * options + j];
+    }
+    red[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    for (int o = kDown / 2; o > 0; o >>= 1) {
+      if ((int)threadIdx.x < o * kCols) red[threadIdx.x] += red[threadIdx.x + o * kCols];
+      __syncthreads();
+    }
+    if (threadIdx.x < kCols && j < options) out[j] = (T)red[threadIdx.x];
     __syncthreads();
   }
-  if (threadIdx.x < kCols && j < options) out[j] = (T)red[threadIdx.x];
 }
 
 }  // namespace epp

@@ -64,6 +64,15 @@ BAD_ROWS = [
 ]
 
 
+@pytest.mark.parametrize("rows,options", [(2**25, 4096), (2**27, 2048), (2**27, 1024)])
+def test_rows_that_one_launch_cannot_hold(rows, options):
+  """A launch counts its threads in 32 bits."""
+  L = cp.lib()
+  r = C.byref(_rows(rows=rows, options=options, logits_stride=options, num_options=0, workspace=PTR, workspace_bytes=2**62))
+  for rc in (L.ep_policy_choose(r, None, 0, PTR, PTR, PTR), L.ep_policy_evaluate(r, PTR, PTR, PTR, PTR)):
+    assert rc == capi.EP_ERR_TOO_LARGE and f"{rows} rows" in L.ep_last_error().decode()
+
+
 @pytest.mark.parametrize("bad,word", BAD_ROWS, ids=lambda x: str(x))
 def test_rows_that_are_refused(bad, word):
   L = cp.lib()
@@ -149,6 +158,12 @@ def test_null_arguments_and_empty_calls():
   _refused(L.ep_memory_sum_heads(0, PTR, 4, 2, 2, 8, PTR, capi.EP_I32, None), "dtype")
   _refused(L.ep_memory_sum_heads(0, None, 4, 2, 2, 8, PTR, capi.EP_F32, None), "null")
   assert L.ep_memory_sum_heads(0, None, 0, 2, 2, 8, None, capi.EP_F32, None) == capi.EP_OK
+
+
+def test_states_that_one_launch_cannot_hold():
+  L = cp.lib()
+  for rc in (L.ep_memory_scan(C.byref(_scan(rows=2**24))), L.ep_memory_step(C.byref(_step(rows=2**27, num_envs=2**27)))):
+    assert rc == capi.EP_ERR_TOO_LARGE and "heads" in L.ep_last_error().decode()
 
 
 def test_pairs_of_scans_that_are_refused():

@@ -122,6 +122,16 @@ def test_evaluate_and_its_gradients(case, dtype):
     assert ((gb - wb).abs() <= tb + ref.HALF[b.dtype] * wb.abs() + ref.TINY[b.dtype]).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", [(1700, 2056, "bits", "shared", 0, False), (1600, 2051, "none", "rows", 5, False), (1600, 2056, "bytes", "typed", 40, True),
+                                  (150000, 24, "bytes", "shared", 0, False), (140000, 13, "count", "typed", 3, False), (1200, 1500, "count", "shared", 0, True)],
+                         ids=lambda c: "-".join(str(x) for x in c))
+def test_more_rows_than_the_chip_holds_at_once(case, dtype):
+  """Workgroups that walk down several rows, each way of reading them."""
+  test_evaluate_and_its_gradients(case, dtype)
+  test_choose(case, dtype, False)
+
+
 @pytest.mark.parametrize("a", [6, 40, 300, 5000])
 def test_rows_without_a_distribution(a):
   """Nothing legal, nothing but -inf, NaN or +inf among the legal, the type's lowest value everywhere."""
