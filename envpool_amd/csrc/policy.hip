@@ -118,11 +118,13 @@ struct Width {
   unsigned blocks;  // workgroups for all rows
   size_t lds;
 };
-Width group_width(const epp::Rows& k) {
+Width group_width(const epp::Rows& k, bool grad = false) {
   const int64_t octets = (k.options + epp::kPer - 1) / epp::kPer;
   // More pieces a lane mean fewer lanes a row and less work that every lane repeats (one lane for 16 options: no
-  // exchange at all), at half the lanes in flight: for rows that fill the chip anyway
-  Width w{0, octets > 128 ? 4 : octets > 64 || (octets > 1 && k.rows * octets >= kManyOctets) ? 2 : 1, 0, 0};
+  // exchange at all), at half the lanes in flight: for rows that fill the chip anyway (choose, 524288 x 16 bf16:
+  // 16.4 us with two pieces a lane, 22 with one; a pool's 1024 rows: 4.8 us with one, 5.4 with two). Not for the
+  // gradients, which keep a sum per option: 524288 x 24 bf16 takes 21 us with one piece a lane, 30 with two.
+  Width w{0, octets > 128 ? 4 : octets > 64 || (!grad && octets > 1 && k.rows * octets >= kManyOctets) ? 2 : 1, 0, 0};
   const int64_t lanes = (octets + w.pieces - 1) / w.pieces;
   const int64_t want = std::max<int64_t>(lanes, k.history ? std::min<int64_t>(64, (k.history_len + 15) / 16) : 1);
   while ((1 << w.log) < want) ++w.log;
@@ -243,7 +245,7 @@ int64_t ep_policy_evaluate_grad_workspace(const ep_policy_rows* r, int32_t with_
   if (r->options > kGroupOptions) return grad_row_blocks(r->rows, r->options) * r->options * 4;
   epp::Rows k{};
   k.rows = r->rows, k.options = r->options, k.history = r->history_len > 0 ? r->history : nullptr, k.history_len = r->history_len;
-  return grad_group_blocks(group_width(k)) * r->options * 4;
+  return grad_group_blocks(group_width(k, true)) * r->options * 4;
 }
 
 int ep_policy_evaluate_grad(const ep_policy_rows* r, const int32_t* action, const float* entropy, const float* stats,
@@ -265,7 +267,7 @@ int ep_policy_evaluate_grad(const ep_policy_rows* r, const int32_t* action, cons
   const hipStream_t stream = (hipStream_t)r->stream;
   const int64_t pieces = (r->options + epp::kPiece - 1) / epp::kPiece;
   const bool group = r->options <= kGroupOptions;
-  const Width w = group ? group_width(k) : Width{};
+  const Width w = group ? group_width(k, true) : Width{};
   const int64_t blocks = group ? grad_group_blocks(w) : grad_row_blocks(r->rows, r->options);
   float* partial = shared ? (float*)r->workspace : nullptr;
   if (r->rows > 0) {

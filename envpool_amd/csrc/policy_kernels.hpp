@@ -850,7 +850,7 @@ __global__ __launch_bounds__(kThreads) inline void evaluate_join(Rows p, int n_p
 // workgroups of the gradients' kernels that a CU holds at once: their registers are kept to as many, and the walks
 // down the rows are cut for as many (one round of equal walks, none that waits for a place)
 constexpr int kGradPieceBlocks = 6;
-constexpr int grad_group_per_cu(int pieces) { return pieces == 4 ? 2 : 4; }
+constexpr int grad_group_per_cu(int pieces) { return pieces == 4 ? 2 : pieces == 2 ? 4 : 5; }
 
 struct GradArgs {
   const int32_t* action;
@@ -878,11 +878,12 @@ template <bool kHist> __device__ inline GradRow grad_row(const GradArgs& g, cons
   r.log_s = g.stats[2 * row + 1];
   r.k = c.k;
   r.act = g.action[row];
-  const float g1 = r.act != -1 && g.g_lp ? g.g_lp[row] : 0.f, g2 = g.g_h ? g.g_h[row] : 0.f;
+  const float g_lp = g.g_lp ? g.g_lp[row] : 0.f, g2 = g.g_h ? g.g_h[row] : 0.f, entropy = g.entropy[row];
+  const float g1 = r.act != -1 ? g_lp : 0.f;
   r.empty = r.m == -INFINITY;
   const float nan = r.m != r.m ? r.m : 0.f;  // a BAD row: its gradient is NaN where legal
   r.g1 = g1 * c.inv_t;
-  r.flat = (g1 + g2 * g.entropy[row]) * c.inv_t + nan;
+  r.flat = (g1 + g2 * entropy) * c.inv_t + nan;
   r.lean = g2 * Num<float>::kUnit * c.inv_t;
   return r;
 }
@@ -924,6 +925,17 @@ template <class T, int NP, bool kHist, bool kWhole> __global__ __launch_bounds__
 #pragma unroll
     for (int i = 0; i < kPer; ++i) sum[k][i] = 0.f;
   Raw<T, kWhole> raw[NP];
+  const int64_t rows_on = (int64_t)gridDim.x * (kThreads >> width_log);  // from a lane's row to its next
+  const auto ask = [&](int k, int64_t j, int64_t row, bool first) {
+    if (j >= p.options || row >= p.rows) return;
+    raw[k].ask_row(p, row, j);
+    if (p.bias_stride != 0 || first) raw[k].ask_bias(p, row, j);
+  };
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    const Group at = group_of(p, blockIdx.x, width_log);
+    if (at.there) ask(k, at.j(k), at.row, true);
+  }
   for (int64_t b = blockIdx.x; b < blocks_of_rows; b += gridDim.x) {
     const Group at = group_of(p, b, width_log);
     const uint32_t* n = kHist ? count_groups<NP>(p, at, counts) : nullptr;
@@ -932,17 +944,12 @@ template <class T, int NP, bool kHist, bool kWhole> __global__ __launch_bounds__
     const RowConst<float> c = row_const<float, kHist>(p, at.row);
     const GradRow r = grad_row<kHist>(g, c, at.row);
 #pragma unroll
-    for (int k = 0; k < NP; ++k)
-      if (at.j(k) < p.options) {
-        raw[k].ask_row(p, at.row, at.j(k));
-        if (p.bias_stride != 0 || b == blockIdx.x) raw[k].ask_bias(p, at.row, at.j(k));
-      }
-#pragma unroll
     for (int k = 0; k < NP; ++k) {
       const int64_t j = at.j(k);
       if (j >= p.options) continue;
       float y[kPer], slope[kPer], dx[kPer], db[kPer];
       const uint32_t legal = load_y<T, float, kHist, kWhole>(p, c, at.row, j, whole, raw[k], Seen<float>{n}.at(kHist ? j : 0), y, slope);
+      ask(k, j, at.row + rows_on, false);
       grad_y(r, y, r.empty ? 0u : legal, j, db);
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
