@@ -29,7 +29,8 @@ int check_workspace(const void* ws, int64_t have, int64_t need) {
 }
 
 // Up to this many rows every workgroup looks the whole batch's ids through for a second row of its env
-// (a few KB out of L2); above it two small launches count the rows of each env first.
+// (a few KB out of L2); above it two small launches count the rows of each env first (9 us: at 4096 rows the step
+// takes 195 + 9 us with them and 208 without, at 65536 rows 433 + 10 and 6316).
 constexpr int64_t kLookThrough = 1024;
 
 int64_t step_workspace(const ep_memory_step_args* a) {
@@ -56,7 +57,8 @@ int64_t per_cu(const ep_memory_scan_args* a) { return a->dtype == EP_F32 ? per_c
 
 // Split of the time axis. One part per state keeps everything single-pass. With fewer states than the chip holds at
 // once, the axis is cut into parts that are walked side by side: keys and values are then read twice (first for the
-// states between the parts), which counts as 1.6 times the chunks plus the join.
+// states between the parts), which counts as 1.6 times the chunks plus the join. 32768 steps of 16 states of 128 x 128
+// in bf16: 77 + 14 + 169 us in 32 parts, 2982 in one; 777 steps of 30 states in f32: 16 + 9 + 28 us, 166 in one.
 int64_t scan_parts(const ep_memory_scan_args* a) {
   const int64_t states = a->rows * a->heads, chunk = chunk_steps(a->dtype), chunks = (a->steps + chunk - 1) / chunk;
   if (states <= 0 || chunks < 2) return 1;
@@ -137,7 +139,9 @@ bool state_vec(const ep_memory_scan_args* a) {
   return (uintptr_t)a->state_in % 16 == 0 && a->state_in_stride[0] % 4 == 0 && a->state_in_stride[1] % 4 == 0 && a->state_in_stride[3] % 4 == 0;
 }
 
-// whether two scans are the gradients of values (a) and keys (b) of one call, in a form that one kernel covers
+// whether two scans are the gradients of values (a) and keys (b) of one call, in a form that one kernel covers (128
+// steps of 4096 states of 64 x 64 in bf16: 161 us, one after the other 204). Other sizes' two states and six tiles would
+// leave a CU one workgroup, and a split axis has two walks that start from different states.
 bool pairs_up(const ep_memory_scan_args* a, const ep_memory_scan_args* b) {
   const auto same = [](const int64_t* x, const int64_t* y, int n) { return std::equal(x, x + n, y); };
   return a->reverse && b->reverse && a->dtype != EP_F32 && a->dtype == b->dtype && a->steps == b->steps && a->rows == b->rows && a->heads == b->heads &&

@@ -7,8 +7,9 @@
 //   S = carry * S + (K * w_up[s])^T V
 // Everything is computed transposed (scores as [s, t], outputs as [v, t]): the accumulators of one product are
 // then laid out as an operand of the next up to a permutation of the summed index, which is applied to the
-// other operand as well. So the state never leaves its registers (32 bits; a copy rounded to the operands' type
-// feeds Q S), scores cross LDS once because each wave computes 16 of the query columns and needs all of
+// other operand as well. So the state never leaves its registers (32 bits; in 16-bit types it enters Q S as two
+// rounded pieces and its increments leave K^T V from three, or two scaled, pieces of the weighted values, so that both
+// keep what 32 bits keep), scores cross LDS once because each wave computes 16 of the query columns and needs all of
 // them for its quarter of the value columns, and an output row is written 4 values a lane.
 // Time backwards (for gradients) is the same chunk with the triangle and the weights mirrored.
 #pragma once
@@ -588,6 +589,11 @@ template <bool rev> __device__ inline void cut_chunk(uint64_t starts, int64_t& s
   n = to - from;
 }
 
+// One walk. 128 steps of 4096 states of 64 x 64 in bf16, states in and out: 105 us = 3.8 TB/s of the 403 MB it moves,
+// 78 % of a large copy; vector and matrix instructions share the rest (half of the cycles issue vector instructions).
+// 32768 steps of 16 states of 128 x 128 in 32 parts: 169 us for 537 MB and 103 Gflop with the pieces (matrix floor 85
+// us). In f32 two chunks of 32 steps of 80 x 112 take 28 us in 390 workgroups: a CU's two workgroups need 11 us on the
+// matrix cores, the rest is the state's way in and out and loads that nothing hides.
 template <class T, int DK, int DV, bool kAligned, bool rev>
 __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void scan_chunks(Scan p, Parts parts) {
   using W = Walk<T, DK, DV, kAligned, rev>;
@@ -709,7 +715,8 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
 
 // Two walks back in time over the same four tensors, for the gradients of keys and values (a: values, from keys,
 // queries and the outputs' gradients; b: keys, from values, the outputs' gradients and queries): the tiles of a chunk
-// are read once for both. 16-bit types, sizes up to 64, time not split.
+// are read once for both. 16-bit types, sizes up to 64, time not split. 128 steps of 4096 states in bf16: 161 us for the
+// 604 MB that the two move (3.75 TB/s); three workgroups a CU (149 and 160 registers, 48 KB of LDS).
 template <class T> struct PairTile {
   using Tile = ScanTile<T, 64, 64>;
   static constexpr size_t kLds = (size_t)Tile::kChunk * (2 * Tile::SQ + 2 * Tile::SK + Tile::SP) * sizeof(T) + 4 * Tile::kChunk * sizeof(float);
@@ -807,7 +814,7 @@ template <class T> __global__ __launch_bounds__(256, 3) void scan_pair(Scan a, S
 }
 
 // Turns the parts' own contributions into what each part starts from, in time's direction: one thread per 4
-// values of a state.
+// values of a state. 16 states of 128 x 128 and 32 parts: 14 us for 67 MB (4.7 TB/s).
 template <int DK, int DV> __global__ __launch_bounds__(256) void join_parts(Scan p, Parts parts) {
   const int64_t rh = blockIdx.x;
   const int at = blockIdx.y * 256 + threadIdx.x;  // in accumulator order

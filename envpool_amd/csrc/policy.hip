@@ -108,7 +108,9 @@ template <class F> void with_kernel(int32_t dtype, const epp::Rows& k, F f, bool
 // How rows map to the chip. Up to 2048 options a row is held by 1 to 64 neighbouring lanes (8 options a lane and
 // piece, 1 or 4 pieces): enough lanes for the options, and for a long history at least a lane per 16 entries
 // of it. Longer rows are walked by workgroups, 2048 options at a time; with few rows each is cut into parts so
-// that about kFill workgroups stand on the chip.
+// that about kFill workgroups stand on the chip (eight a CU; kChooseFill: the choice walks down one part again to
+// find its option, so shorter parts pay twice: 64 x 131072 bf16 takes 31 + 13 us in parts of 2048 options, 28 + 17
+// in parts of 4096).
 constexpr int64_t kGroupOptions = 64 * epp::kPer * 4;
 constexpr int64_t kFill = 2048, kChooseFill = 2 * kFill;
 constexpr int64_t kManyOctets = 262144;
@@ -122,7 +124,8 @@ Width group_width(const epp::Rows& k, bool grad = false) {
   const int64_t octets = (k.options + epp::kPer - 1) / epp::kPer;
   // More pieces a lane mean fewer lanes a row and less work that every lane repeats (one lane for 16 options: no
   // exchange at all), at half the lanes in flight: for rows that fill the chip anyway (choose, 524288 x 16 bf16:
-  // 16.4 us with two pieces a lane, 22 with one; a pool's 1024 rows: 4.8 us with one, 5.4 with two). Not for the
+  // 18.1 us with two pieces a lane, 22.3 with one; evaluate, 524288 x 24: 15.4 and 20.5; but 4096 x 16 f32: 4.6
+  // with two, 3.9 with one). Not for the
   // gradients, which keep a sum per option: 524288 x 24 bf16 takes 21 us with one piece a lane, 30 with two.
   Width w{0, octets > 128 ? 4 : octets > 64 || (!grad && octets > 1 && k.rows * octets >= kManyOctets) ? 2 : 1, 0, 0};
   const int64_t lanes = (octets + w.pieces - 1) / w.pieces;

@@ -159,8 +159,9 @@ __device__ inline double pick(uint32_t bits, int i, double v, double other) {
 
 // The operands of options j0 .. j0+7 of a row (j0 a multiple of 8, below the row's end) as they lie in memory. With
 // kWhole every row is made of whole eights that can be read at once: all operands are then asked for before the first
-// is used, and a walk asks for its next eight before it works on these. (Ragged rows are read where they are used:
-// eight guarded loads each, in twice the registers.)
+// is used, and a walk asks for its next eight before it works on these. Ragged rows are read where they are used:
+// eight guarded loads each, in more registers (524288 x 16 bf16: choose 36 us, whole 18; 524288 x 24: evaluate 36
+// and 15, its gradients 42 and 21; 2048 x 32768: gradients 71 and 59).
 template <class T, bool kWhole> struct Raw {
   __device__ void ask_row(const Rows&, int64_t, int64_t) {}
   __device__ void ask_bias(const Rows&, int64_t, int64_t) {}
@@ -523,6 +524,9 @@ template <int NP> __device__ inline const uint32_t* count_groups(const Rows& p, 
   return mine;
 }
 
+// choose: one pass, the weights stay in registers between the sum and the choice. Bound by the 64-bit arithmetic of the
+// weights (some 25 of 57 instructions an option): 524288 x 16 bf16 with byte masks and a shared bias 18 us = 1.8 TB/s
+// of 33 MB; 1024 x 16 f32 4.8 us, which is a launch.
 template <class T, int NP, bool kHist, bool kWhole>
 __global__ __launch_bounds__(kThreads) void choose_group(Rows p, int width_log, const void* u, int u_f64, ChooseOut out) {
   extern __shared__ uint32_t counts[];
@@ -607,6 +611,8 @@ __global__ __launch_bounds__(kThreads) void choose_group(Rows p, int width_log, 
   if (g.lane == 0 && g.there) finish_choose(out, g.row, a, c, pick, y_pick);
 }
 
+// evaluate: the same in 32 bits. Bound by instructions (30 an option of a lane, whether the row has it or not: a quarter
+// of the lanes of 24 options): 524288 x 24 bf16 15.4 us = 3 TB/s of 46 MB.
 template <class T, int NP, bool kHist, bool kWhole> __global__ __launch_bounds__(kThreads) void evaluate_group(Rows p, int width_log, EvaluateOut out) {
   extern __shared__ uint32_t counts[];
   const Group g = group_of(p, blockIdx.x, width_log);
@@ -649,6 +655,9 @@ template <class T, int NP, bool kHist, bool kWhole> __global__ __launch_bounds__
 }
 
 // ---- longer rows: a workgroup per part of a row (`pieces` pieces of kPiece options), parts joined after ---
+// 64 x 131072 bf16, bit masks, a shared bias and 2048 entries of history a row: 31 us. A third of it is the history
+// (every part reads all of its row's entries), the rest the weights in 64 bits; 29 KB of LDS let five workgroups stand
+// on a CU (six, with the list inside the values' memory and the registers kept to it, took 38 us).
 template <class T, bool kHist, bool kWhole, bool kBest>
 __global__ __launch_bounds__(kThreads) void choose_parts(Rows p, int pieces, int n_parts, Stat<double>* parts) {
   __shared__ PieceMemory<T, double, kHist> mem;
@@ -675,7 +684,8 @@ __global__ __launch_bounds__(kThreads) void choose_parts(Rows p, int pieces, int
   if (threadIdx.x == 0) parts[blockIdx.x] = a;
 }
 
-// joins a row's parts, and finds the option that u falls on by walking down the one part it lies in
+// joins a row's parts, and finds the option that u falls on by walking down the one part it lies in: one workgroup a
+// row and a chain of reads that depend on each other, 13 us at 64 x 131072
 template <class T, bool kHist, bool kWhole>
 __global__ __launch_bounds__(kThreads) void choose_join(Rows p, int pieces, int n_parts, const Stat<double>* all_parts, const void* u, int u_f64, ChooseOut out) {
   __shared__ PieceMemory<T, double, kHist> mem;
@@ -783,7 +793,8 @@ __global__ __launch_bounds__(kThreads) void choose_join(Rows p, int pieces, int 
 }
 
 // The same walk in 32 bits. One part: the row's results at once; several: partial sums, with the logit of the
-// action from the part that holds it.
+// action from the part that holds it. 2048 x 32768 bf16 with bit masks: 45 us = 3.2 TB/s of 142 MB, bound by
+// instructions (20 an option: 45 us with the registers kept to eight workgroups a CU, one round of them; 60 in two).
 struct EvaluatePart {
   Stat<float> stat;
   float y_act;
@@ -848,7 +859,8 @@ __global__ __launch_bounds__(kThreads) inline void evaluate_join(Rows p, int n_p
 }
 
 // workgroups of the gradients' kernels that a CU holds at once: their registers are kept to as many, and the walks
-// down the rows are cut for as many (one round of equal walks, none that waits for a place)
+// down the rows are cut for as many (one round of equal walks, none that waits for a place). 524288 x 24 bf16, one
+// piece a lane: 21.2 us with five, 22.5 with four, 25.4 with six (registers spill)
 constexpr int kGradPieceBlocks = 6;
 constexpr int grad_group_per_cu(int pieces) { return pieces == 4 ? 2 : pieces == 2 ? 4 : 5; }
 
@@ -916,7 +928,7 @@ template <class T> __device__ inline void store8(T* out, const float (&v)[kPer],
 }
 
 // short rows: the lanes of evaluate_group, walking down the rows; a shared bias' gradient is summed per lane, then
-// over the workgroup's row slots
+// over the workgroup's row slots. 524288 x 24 bf16: 21 us = 3.4 TB/s of 73 MB
 template <class T, int NP, bool kHist, bool kWhole> __global__ __launch_bounds__(kThreads, grad_group_per_cu(NP)) void evaluate_grad_group(Rows p, GradArgs g, int width_log, int64_t blocks_of_rows) {
   extern __shared__ uint32_t counts[];  // (as floats for the sums afterwards)
   float sum[NP][kPer];
@@ -981,7 +993,9 @@ template <class T, int NP, bool kHist, bool kWhole> __global__ __launch_bounds__
   }
 }
 
-// a workgroup owns kPiece columns and walks down its rows: the sum of a shared bias' gradient stays in registers
+// a workgroup owns kPiece columns and walks down its rows: the sum of a shared bias' gradient stays in registers.
+// Reads the logits again and writes as much: 2048 x 32768 bf16 59 us = 4.7 TB/s of 276 MB, what a large copy reaches
+// (90 us in workgroups that waited for a place on the chip)
 template <class T, bool kHist, bool kWhole>
 __global__ __launch_bounds__(kThreads, kGradPieceBlocks) void evaluate_grad_piece(Rows p, GradArgs g, int64_t rows_per_block) {
   __shared__ PieceMemory<T, float, kHist> mem;
@@ -1026,7 +1040,7 @@ __global__ __launch_bounds__(kThreads, kGradPieceBlocks) void evaluate_grad_piec
   }
 }
 
-// column sums of partial [n][options], in a fixed order: kCols columns a workgroup, the other threads down the rows
+// column sums of partial [n][options] (4 us at 1280 x 24 and at 94 x 32768), in a fixed order: kCols columns a workgroup, the other threads down the rows
 template <class T, int kCols>
 __global__ __launch_bounds__(kThreads) void sum_partials(const float* partial, int64_t n, int64_t options, T* out) {
   __shared__ float red[kThreads];
