@@ -9,8 +9,9 @@
  * copied to the host or waited for, so they can be captured into a HIP graph. Scratch memory is the
  * caller's (`workspace`, at least as many bytes as the call's *_workspace function says; its contents
  * need not be kept between calls, but two calls that may run at the same time - two streams, two
- * captured graphs - need one each). Refusals are EP_ERR_INVALID with ep_last_error() naming the argument,
- * and nothing has been enqueued then. No counterpart in the reference: its policies live outside it and
+ * captured graphs - need one each). Refusals are EP_ERR_INVALID with ep_last_error() naming the argument
+ * (EP_ERR_TOO_LARGE: more rows, or states, than one launch can hold, some 16 million workgroups of 256;
+ * EP_ERR_NO_DEVICE: no such GPU), and nothing has been enqueued then. No counterpart in the reference: its policies live outside it and
  * see numpy arrays (envpool2/python/envpool.py:135-142).
  */
 #ifndef ENVPOOL_AMD_POLICY_H_
@@ -160,8 +161,8 @@ typedef struct {
 int ep_memory_scan(const ep_memory_scan_args* args);
 int64_t ep_memory_scan_workspace(const ep_memory_scan_args* args);
 
-/* Two scans as one call, both on one device and stream and naming one workspace (the larger of the two, or what
- * ep_memory_scan_pair_workspace says). The gradients of values (a) and keys (b) of one forward scan - reverse scans
+/* Two scans as one call, both on one device and stream and naming one workspace (of what
+ * ep_memory_scan_pair_workspace says, or more). The gradients of values (a) and keys (b) of one forward scan - reverse scans
  * over the same tensors: a's k is b's v and the other way round - share their reads where their sizes allow it
  * (16-bit types, dims up to 64); any other two simply follow one another. Neither's results are read by the other. */
 int ep_memory_scan_pair(const ep_memory_scan_args* a, const ep_memory_scan_args* b);
