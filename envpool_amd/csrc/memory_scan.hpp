@@ -100,6 +100,9 @@ template <> struct Mma<f16> : Mma16<f16, f16x8, f16x4> {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       float x = v[e];
+      // (opaque: where x is a product the compiler rounds it to 16 bits at once in one place and by way of 32 in the
+      // other, and at a tie the remainder is then that of a neighbouring piece)
+      asm volatile("" : "+v"(x));
 #pragma unroll
       for (int c = 0; c < N; ++c) {
         out[c][e] = (f16)x;

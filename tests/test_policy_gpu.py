@@ -430,6 +430,26 @@ def test_memory_scan_keeps_what_is_not_finite_inside_its_episode(dtype):
     assert torch.isfinite(got[5][[1, 3]]).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,n,h,dk,dv", [(16, 4, 12, 64, 64), (32, 40, 4, 16, 16), (30, 3, 2, 128, 128), (17, 5, 3, 20, 19)])
+def test_states_keep_32_bits(t, n, h, dk, dv, dtype):
+  """The final state and the first state's gradient of one chunk, whatever the type of what goes in: a term is off by
+  at most 2^-22 (two pieces of 11 bits), the decay's power by 2 half steps of its exponent (at most 32 * 0.42 octaves,
+  each worth ln 2: 19 half steps of 32 bits) and 2 of its own, the sum by one per term."""
+  from envpool_amd import policy
+  q, k, v, decay, fresh, state, do, ds = _scan_problem((t, n, h, h, dk, dv, 0.02, True), dtype)
+  args = dict(fresh=fresh, state=state, scale=1.0, grad_out=do, reverse_from=ds)
+  want, size = ref.scan(q, k, v, decay, **args), ref.scan(q, k, v, decay, absolute=True, **args)
+  leaf = state.to(DEV).requires_grad_()
+  out, final = policy.memory_scan(q.to(DEV), k.to(DEV), v.to(DEV), decay.to(DEV), fresh=fresh.to(DEV), state=leaf, scale=1.0)
+  grad, = torch.autograd.grad([out, final], leaf, [do.to(DEV), ds.to(DEV)])
+  h32 = ref.HALF[torch.float32]
+  for name, x in (("final", final.detach()), ("grad_state", grad)):
+    err = (x.cpu().double() - want[name]).abs()
+    tol = size[name] * (4 + 19 + 2 + t + 2) * h32 + h32 * want[name].abs() + 2.0**-30
+    assert (err <= tol).all(), (name, float((err - tol).max()), float((err / size[name].clamp_min(1e-30)).max()))
+
+
 def test_memory_scan_layouts_and_missing_pieces():
   """Batch-major views, expanded heads, no fresh, no state, no steps, nothing wanted from one of the outputs."""
   from envpool_amd import policy
