@@ -365,18 +365,43 @@ template <class R, bool kBest> __device__ inline void stat_add(Stat<R>& a, const
   }
 }
 
-// over `width` neighbouring lanes (a power of two up to 64), the same result in all of them
-template <class V> __device__ inline V lanes_max(V v, int width) {
-  for (int o = 1; o < width; o <<= 1) {
-    const V b = __shfl_xor(v, o, 64);
-    v = v > b ? v : b;
+// Over `width` neighbouring lanes (a power of two up to 64), the same result in all of them. Six exchanges between
+// registers (no trip through LDS): with the neighbour, the neighbouring pair, the mirrored four and eight - by then every
+// quad and octet holds one value - and the neighbouring row of 16 and half of the wave.
+template <int kDpp, class V> __device__ inline V moved(V v) {
+  union { V v; int w[sizeof(V) / 4]; } u;
+  u.v = v;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(V) / 4); ++i) u.w[i] = __builtin_amdgcn_update_dpp(u.w[i], u.w[i], kDpp, 0xf, 0xf, true);
+  return u.v;
+}
+template <int kLanes, class V, class Op> __device__ inline V across(V v, Op op) {
+  union { V v; uint32_t w[sizeof(V) / 4]; } x, y;
+  x.v = v;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(V) / 4); ++i) {
+    const auto r = kLanes == 16 ? __builtin_amdgcn_permlane16_swap(x.w[i], x.w[i], false, false) : __builtin_amdgcn_permlane32_swap(x.w[i], x.w[i], false, false);
+    x.w[i] = r[0], y.w[i] = r[1];
   }
+  return op(x.v, y.v);
+}
+template <class V, class Op> __device__ inline V lanes_reduce(V v, int width, Op op) {
+  if (width > 1) v = op(v, moved<0xb1>(v));
+  if (width > 2) v = op(v, moved<0x4e>(v));
+  if (width > 4) v = op(v, moved<0x141>(v));
+  if (width > 8) v = op(v, moved<0x140>(v));
+  if (width > 16) v = across<16>(v, op);
+  if (width > 32) v = across<32>(v, op);
   return v;
 }
-template <class V> __device__ inline V lanes_min(V v, int width) { return -lanes_max(-v, width); }
+template <class V> __device__ inline V lanes_max(V v, int width) {
+  return lanes_reduce(v, width, [](V a, V b) { return a > b ? a : b; });
+}
+template <class V> __device__ inline V lanes_min(V v, int width) {
+  return lanes_reduce(v, width, [](V a, V b) { return a < b ? a : b; });
+}
 template <class V> __device__ inline V lanes_sum(V v, int width) {
-  for (int o = 1; o < width; o <<= 1) v += __shfl_xor(v, o, 64);
-  return v;
+  return lanes_reduce(v, width, [](V a, V b) { return a + b; });
 }
 // sum over the lanes up to and including this one, of `width`
 template <class V> __device__ inline V lanes_scan(V v, int width) {
@@ -390,7 +415,7 @@ template <class V> __device__ inline V lanes_scan(V v, int width) {
 
 // over the workgroup, the same result in every thread: the maximum first, then every thread moves its own
 // sums to it (one exponential each) and they are added
-template <class R> __device__ inline Stat<R> stat_block(Stat<R> a, R k, Stat<R>* lds) {
+template <class R, bool kBest> __device__ inline Stat<R> stat_block(Stat<R> a, R k, Stat<R>* lds) {
   constexpr int kWaves = kThreads / 64;
   const int wave = threadIdx.x >> 6;
   const R m_wave = lanes_max(a.m, 64);
@@ -399,7 +424,7 @@ template <class R> __device__ inline Stat<R> stat_block(Stat<R> a, R k, Stat<R>*
   __syncthreads();
   R m = lds[0].m;
   for (int i = 1; i < kWaves; ++i) m = larger(m, lds[i].m);
-  const int64_t best = lanes_min((long long)(a.m == m ? a.best : INT64_MAX), 64);
+  const int64_t best = kBest ? lanes_min((long long)(a.m == m ? a.best : INT64_MAX), 64) : INT64_MAX;
   stat_rebase(a, m, k);
   const R sum = lanes_sum(a.s, 64), e = lanes_sum(a.e, 64);
   const int bad = __any(a.bad);
@@ -655,7 +680,7 @@ template <class T, int NP, bool kHist, bool kWhole> __global__ __launch_bounds__
 }
 
 // ---- longer rows: a workgroup per part of a row (`pieces` pieces of kPiece options), parts joined after ---
-// 64 x 131072 bf16, bit masks, a shared bias and 2048 entries of history a row: 31 us. A third of it is the history
+// 64 x 131072 bf16, bit masks, a shared bias and 2048 entries of history a row: 30 us. A third of it is the history
 // (every part reads all of its row's entries), the rest the weights in 64 bits; 29 KB of LDS let five workgroups stand
 // on a CU (six, with the list inside the values' memory and the registers kept to it, took 38 us).
 template <class T, bool kHist, bool kWhole, bool kBest>
@@ -680,12 +705,12 @@ __global__ __launch_bounds__(kThreads) void choose_parts(Rows p, int pieces, int
     ask(j + kPiece);
     stat_add<double, kBest>(a, y, m, j, c.k);
   }
-  a = stat_block(a, c.k, red);
+  a = stat_block<double, kBest>(a, c.k, red);
   if (threadIdx.x == 0) parts[blockIdx.x] = a;
 }
 
 // joins a row's parts, and finds the option that u falls on by walking down the one part it lies in: one workgroup a
-// row and a chain of reads that depend on each other, 13 us at 64 x 131072
+// row and a chain of reads that depend on each other, 12 us at 64 x 131072
 template <class T, bool kHist, bool kWhole>
 __global__ __launch_bounds__(kThreads) void choose_join(Rows p, int pieces, int n_parts, const Stat<double>* all_parts, const void* u, int u_f64, ChooseOut out) {
   __shared__ PieceMemory<T, double, kHist> mem;
@@ -706,7 +731,7 @@ __global__ __launch_bounds__(kThreads) void choose_join(Rows p, int pieces, int 
     stat_rebase(b, m, c.k);
     a = {m, a.s + b.s, a.e + b.e, best, a.bad | b.bad};
   }
-  a = stat_block(a, c.k, red);
+  a = stat_block<double, true>(a, c.k, red);
   int64_t pick = a.best;
   double y_pick = a.m;
   if (u && !a.bad && !c.bad && a.m != Num<double>::kNone) {
@@ -830,7 +855,7 @@ __global__ __launch_bounds__(kThreads, kHist ? 6 : 8) void evaluate_parts(Rows p
         if (act == j + i) y_act = y[i];
     }
   }
-  a = stat_block(a, c.k, red);
+  a = stat_block<float, false>(a, c.k, red);
   if (threadIdx.x != 0) return;
   if (n_parts == 1) finish_evaluate(out, row, p.options, a, c, act, y_act);
   else parts[blockIdx.x] = {a, y_act};
