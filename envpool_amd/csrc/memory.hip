@@ -217,10 +217,15 @@ int ep_memory_step(const ep_memory_step_args* a) {
     HIP_TRY(hipGetLastError());
   }
   const int64_t blocks = (a->rows * a->heads + 3) / 4;
-  const bool four = a->value_dim % 4 == 0 && (uintptr_t)a->state % 16 == 0;  // states in 16-byte pieces
+  // values a lane holds side by side, as wide as rows of the state are aligned (2692 states of 101 x 66: 45 us two by
+  // two, 65 one by one), and how often 64 lanes of them repeat
+  const int vec = a->value_dim % 4 == 0 && (uintptr_t)a->state % 16 == 0 ? 4 : a->value_dim % 2 == 0 && (uintptr_t)a->state % 8 == 0 ? 2 : 1;
+  const int cols = (a->value_dim + 64 * vec - 1) / (64 * vec);
   with_type(a->dtype, [&](auto t) {
-    if (four) hipLaunchKernelGGL((epm::step_rows<decltype(t), 4>), dim3((unsigned)blocks), dim3(256), 0, stream, k);
-    else hipLaunchKernelGGL((epm::step_rows<decltype(t), 1>), dim3((unsigned)blocks), dim3(256), 0, stream, k);
+    using T = decltype(t);
+    const auto kernel = vec == 4 ? epm::step_rows<T, 4, 1> : vec == 2 ? (cols == 1 ? epm::step_rows<T, 2, 1> : epm::step_rows<T, 2, 2>)
+                                  : cols == 1 ? epm::step_rows<T, 1, 1> : cols == 2 ? epm::step_rows<T, 1, 2> : epm::step_rows<T, 1, 4>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, k);
   });
   HIP_TRY(hipGetLastError());
   return EP_OK;

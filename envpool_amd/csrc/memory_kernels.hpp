@@ -45,13 +45,12 @@ static __global__ __launch_bounds__(256) void count_claims(Step p) {
   if (e >= 0 && e < p.num_envs) atomicAdd(&p.claims[e], 1);
 }
 
-// One wave per (row, head) streams the state through its registers: a lane holds kVec neighbouring value columns
-// and walks down the keys, 64 / (lanes per key row) keys an instruction, so that a load instruction of the wave
-// is one contiguous stretch. Nothing is read twice; HBM bounds it (8 bytes moved per 5 flops), so what matters
-// is bytes in flight: kAhead loads per lane before the first is used. State loads and stores bypass the caches'
+// One wave per (row, head) streams the state through its registers: a lane holds kVec neighbouring value columns (or
+// kCols such pieces, 64 apart) and walks down the keys, 64 / (lanes per key row) keys an instruction, so that the load
+// instructions of the wave are one contiguous stretch. Nothing is read twice; HBM bounds it (8 bytes moved per 5 flops), so what matters
+// is bytes in flight: 128 of every lane (32 / kVec loads) before the first is used. State loads and stores bypass the caches'
 // retention (a step touches each value once). 4096 rows x 8 heads of 64 x 64, bf16: 195 us = 5.6 TB/s; 65536 x 4
 // heads of 32 x 32: 433 us = 5.1 TB/s; a pool of 8 envs 6.6 us.
-constexpr int kAhead = 8;
 // orders a wave's LDS accesses across its lanes (the hardware keeps them in order; this tells the compiler)
 __device__ inline void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -65,7 +64,7 @@ template <> struct Piece<1> {
   typedef float type;
 };
 
-template <class T, int kVec> __device__ inline void step_one(const Step& p, int64_t row, int64_t e, int h, float decay, float* qs, float* ks, float* red) {
+template <class T, int kVec, int kCols> __device__ inline void step_one(const Step& p, int64_t row, int64_t e, int h, float decay, float* qs, float* ks, float* red) {
   using V = typename Piece<kVec>::type;
   const int lane = threadIdx.x & 63;
   const bool drop = starts(p, row);
@@ -77,58 +76,79 @@ template <class T, int kVec> __device__ inline void step_one(const Step& p, int6
   wave_sync();
   for (int i = lane; i < p.dk; i += 64) qs[i] = (float)q[i] * p.scale, ks[i] = (float)k[i];
   wave_sync();
-  const int columns = (p.dv + kVec - 1) / kVec;  // of kVec values (dv is a multiple of it)
-  for (int c0 = 0; c0 < columns; c0 += 64) {
-    const int width = columns - c0 < 64 ? columns - c0 : 64;
-    const int down = 64 / width;  // keys per instruction
-    const int c = c0 + lane % width, d0 = lane / width;
-    const bool on = d0 < down;
-    float* s = state + c * kVec;
-    V vv;
-    if constexpr (kVec == 1) vv = on ? (float)v[c] : 0.f;
+  // columns of kVec values (dv is a multiple of it): up to 64 side by side, a lane holds every 64th of more
+  const int columns = p.dv / kVec, width = columns < 64 ? columns : 64;
+  const int down = kCols == 1 ? 64 / width : 1;  // keys per instruction
+  const int c = lane % width, d0 = lane / width;
+  const bool on = d0 < down;
+  // (`on` again inside the walk keeps the loads of narrow pieces together: 2692 states of 101 x 66 take 45 us with it, 54
+  // without. Wide ones take 429 us for 262144 states of 32 x 32 without it and with five workgroups a CU, 464 with it
+  // and four)
+  const auto has = [&](int j) { return kCols == 1 ? kVec == 4 || on : c + 64 * j < columns; };
+  float* s = state + c * kVec;
+  V vv[kCols], acc[kCols];
+#pragma unroll
+  for (int j = 0; j < kCols; ++j) {
+    acc[j] = (V)0.f;
+    if constexpr (kVec == 1) vv[j] = on && has(j) ? (float)v[c + 64 * j] : 0.f;
     else
 #pragma unroll
-      for (int r = 0; r < kVec; ++r) vv[r] = on ? (float)v[c * kVec + r] : 0.f;
-    V acc = (V)0.f;
-    for (int i0 = on ? d0 : p.dk; i0 < p.dk; i0 += down * kAhead) {
-      V old[kAhead];
+      for (int r = 0; r < kVec; ++r) vv[j][r] = on && has(j) ? (float)v[(c + 64 * j) * kVec + r] : 0.f;
+  }
+  constexpr int kKeys = 32 / (kVec * kCols);
+  for (int i0 = on ? d0 : p.dk; i0 < p.dk; i0 += down * kKeys) {
+    V old[kKeys][kCols];
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
+    for (int i = 0; i < kKeys; ++i)
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) {
         const int d = i0 + i * down;
-        old[i] = (V)0.f;
-        if (d < p.dk && !drop) old[i] = __builtin_nontemporal_load((const V*)(s + (int64_t)d * p.dv));
+        old[i][j] = (V)0.f;
+        if (d < p.dk && !drop && has(j)) old[i][j] = __builtin_nontemporal_load((const V*)(s + (int64_t)d * p.dv + 64 * kVec * j));
       }
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
+    for (int i = 0; i < kKeys; ++i)
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) {
         const int d = i0 + i * down;
-        if (d < p.dk) {
-          const V now = old[i] * decay + ks[d] * vv;
-          __builtin_nontemporal_store(now, (V*)(s + (int64_t)d * p.dv));
-          acc += qs[d] * now;
+        if (d < p.dk && has(j)) {
+          const V now = old[i][j] * decay + ks[d] * vv[j];
+          __builtin_nontemporal_store(now, (V*)(s + (int64_t)d * p.dv + 64 * kVec * j));
+          acc[j] += qs[d] * now;
         }
       }
-    }
-    // the sums over the keys: `down` lanes apart by `width`
-    wave_sync();
+  }
+  if (kCols > 1) {  // (a lane has been down all keys of its columns)
+#pragma unroll
+    for (int j = 0; j < kCols; ++j)
+      if (has(j)) {
+        if constexpr (kVec == 1) out[c + 64 * j] = (T)acc[j];
+        else
+#pragma unroll
+          for (int r = 0; r < kVec; ++r) out[(c + 64 * j) * kVec + r] = (T)acc[j][r];
+      }
+    return;
+  }
+  // the sums over the keys: `down` lanes apart by `width`
+  wave_sync();
+#pragma unroll
+  for (int r = 0; r < kVec; ++r) {
+    if constexpr (kVec == 1) red[lane] = acc[0];
+    else red[r * 64 + lane] = acc[0][r];
+  }
+  wave_sync();
+  if (lane < width) {
 #pragma unroll
     for (int r = 0; r < kVec; ++r) {
-      if constexpr (kVec == 1) red[lane] = acc;
-      else red[r * 64 + lane] = acc[r];
-    }
-    wave_sync();
-    if (lane < width) {
-#pragma unroll
-      for (int r = 0; r < kVec; ++r) {
-        float sum = 0.f;
-        for (int i = 0; i < down; ++i) sum += red[r * 64 + i * width + lane];
-        out[c * kVec + r] = (T)sum;
-      }
+      float sum = 0.f;
+      for (int i = 0; i < down; ++i) sum += red[r * 64 + i * width + lane];
+      out[c * kVec + r] = (T)sum;
     }
   }
 }
 
 // Rows of one env are stepped by the wave of the first of them, in order.
-template <class T, int kVec> __global__ __launch_bounds__(256) void step_rows(Step p) {
+template <class T, int kVec, int kCols> __global__ __launch_bounds__(256, kVec == 4 ? 5 : 3) void step_rows(Step p) {
   __shared__ float lds[4][256 + 256 + 64 * kVec];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float *qs = lds[wave], *ks = qs + 256, *red = ks + 256;  // a wave's own: its LDS operations are in order
@@ -155,13 +175,13 @@ template <class T, int kVec> __global__ __launch_bounds__(256) void step_rows(St
     if (__any(earlier)) return;
     again = __any(again);
   }
-  step_one<T, kVec>(p, row0, e, h, decay, qs, ks, red);
+  step_one<T, kVec, kCols>(p, row0, e, h, decay, qs, ks, red);
   if (!again) return;
   for (int64_t base = row0 / 64 * 64; base < p.rows; base += 64) {
     uint64_t hits = __ballot(base + lane < p.rows && base + lane > row0 && p.env_id[base + lane] == id);
     for (; hits; hits &= hits - 1) {
       __threadfence_block();  // (the state written for the row before is read again)
-      step_one<T, kVec>(p, base + __ffsll((unsigned long long)hits) - 1, e, h, decay, qs, ks, red);
+      step_one<T, kVec, kCols>(p, base + __ffsll((unsigned long long)hits) - 1, e, h, decay, qs, ks, red);
     }
   }
 }

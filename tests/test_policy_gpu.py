@@ -261,6 +261,13 @@ def test_memory_step(dtype, n, h, hk, dk, dv):
     assert out.dtype == dtype and ((out.cpu().double() - want["out"][0]).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("n,h,hk,dk,dv", [(40, 3, 1, 101, 66), (6, 2, 2, 33, 67), (5, 2, 1, 64, 130), (4, 1, 1, 31, 201), (3, 2, 2, 16, 255), (3, 1, 1, 5, 254)])
+def test_memory_step_of_uneven_widths(n, h, hk, dk, dv):
+  """Rows of the state that are not made of 16-byte pieces: 8 bytes or 4 a lane, once, twice or four times."""
+  for dtype in DTYPES:
+    test_memory_step(dtype, n, h, hk, dk, dv)
+
+
 @pytest.mark.parametrize("n", [9, 1300])
 def test_memory_step_envs_named_twice_and_out_of_range(n):
   """Rows of one env are stepped in row order; a foreign id touches nothing, gives NaN and an error later."""
