@@ -139,19 +139,58 @@ bool state_vec(const ep_memory_scan_args* a) {
   return (uintptr_t)a->state_in % 16 == 0 && a->state_in_stride[0] % 4 == 0 && a->state_in_stride[1] % 4 == 0 && a->state_in_stride[3] % 4 == 0;
 }
 
+// Short segments are walked step by step (scan_few). Forward / with all gradients, us, walk of chunks against it:
+//   65536 states of 16 x 16 bf16: 4 steps 401 / 1537, 107 / 418; 16 steps 405 / 1546, 310 / 1252; 32 steps 451 / 1668, 611 / 2436
+//   65536 states of 32 x 32 bf16: 4 steps 406 / 1542, 131 / 469; 16 steps 423 / 1584, 315 / 1227; 32 steps 510 / 1845, 574 / 2273
+//   16384 states of 64 x 64 f32:  4 steps 190 / 711, 126 / 576;  8 steps 195 / 722, 148 / 676;    16 steps 203 / 740, 197 / 877
+// In 16 bits states of 64 x 64 stay with the chunks (4 steps 124 / 429, 118 / 556), whose gradients share a launch.
+constexpr int64_t kFewSteps = 16, kFewKeySteps = 128;
+// how scan_few lays a state over a wave: 2^width_log lanes of four values, `keys` keys a lane; keys 0: not its size
+struct Few {
+  int width_log, keys;
+};
+Few few_steps(const ep_memory_scan_args* a);
+
 // whether two scans are the gradients of values (a) and keys (b) of one call, in a form that one kernel covers (128
 // steps of 4096 states of 64 x 64 in bf16: 161 us, one after the other 204). Other sizes' two states and six tiles would
 // leave a CU one workgroup, and a split axis has two walks that start from different states.
 bool pairs_up(const ep_memory_scan_args* a, const ep_memory_scan_args* b) {
   const auto same = [](const int64_t* x, const int64_t* y, int n) { return std::equal(x, x + n, y); };
-  return a->reverse && b->reverse && a->dtype != EP_F32 && a->dtype == b->dtype && a->steps == b->steps && a->rows == b->rows && a->heads == b->heads &&
+  return a->reverse && b->reverse && !few_steps(a).keys && a->dtype != EP_F32 && a->dtype == b->dtype && a->steps == b->steps && a->rows == b->rows && a->heads == b->heads &&
          a->key_dim <= 64 && a->value_dim <= 64 && a->key_dim == b->value_dim && a->value_dim == b->key_dim && a->k == b->v && a->v == b->k &&
          a->k_group == b->v_group && a->v_group == b->k_group && same(a->k_stride, b->v_stride, 3) && same(a->v_stride, b->k_stride, 3) &&
          a->log_decay == b->log_decay && a->fresh == b->fresh && same(a->fresh_stride, b->fresh_stride, 2) && a->inc_scale == b->inc_scale &&
          a->out_scale == b->out_scale && !b->state_out && a->steps > 0 && a->rows > 0 && buffered(a) && buffered(b) && scan_parts(a) == 1 && scan_parts(b) == 1;
 }
 
+Few few_steps(const ep_memory_scan_args* a) {
+  if (a->steps < 1 || a->key_dim > 64 || a->value_dim > 64) return {0, 0};
+  Few f{2, 4};
+  while (4 << f.width_log < a->value_dim) ++f.width_log;
+  while ((64 >> f.width_log) * f.keys < a->key_dim) f.keys *= 2;
+  const bool few = a->steps <= kFewSteps && a->steps * f.keys <= kFewKeySteps && (f.keys <= 8 || a->dtype == EP_F32);
+  return few ? f : Few{0, 0};
+}
+
+int launch_few(const ep_memory_scan_args* a, Few f, hipStream_t stream) {
+  const epm::Scan k = scan_of(a);
+  // whether states go in 16-byte pieces along the values (rows) or the keys (cols)
+  const auto pieces = [](const void* ptr, const int64_t* stride, int along, int other, int width) {
+    return (uintptr_t)ptr % 16 == 0 && stride[along] == 1 && stride[0] % 4 == 0 && stride[1] % 4 == 0 && stride[other] % 4 == 0 && width % 4 == 0;
+  };
+  const int in_rows = pieces(a->state_in, a->state_in_stride, 3, 2, a->value_dim), in_cols = pieces(a->state_in, a->state_in_stride, 2, 3, a->key_dim);
+  const int out_rows = pieces(a->state_out, a->state_out_stride, 3, 2, a->value_dim), out_cols = pieces(a->state_out, a->state_out_stride, 2, 3, a->key_dim);
+  with_type(a->dtype, [&](auto t) {
+    using T = decltype(t);
+    const auto kernel = f.keys == 4 ? epm::scan_few<T, 4> : f.keys == 8 ? epm::scan_few<T, 8> : epm::scan_few<T, 16>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((a->rows * a->heads + 3) / 4)), dim3(256), 0, stream, k, f.width_log, in_rows, in_cols, out_rows, out_cols);
+  });
+  HIP_TRY(hipGetLastError());
+  return EP_OK;
+}
+
 int scan_launch(const ep_memory_scan_args* a, hipStream_t stream) {
+  if (const Few f = few_steps(a); f.keys) return launch_few(a, f, stream);
   const epm::Scan k = scan_of(a);
   epm::Parts parts{};
   const int64_t chunk = chunk_steps(a->dtype), chunks = std::max<int64_t>(1, (a->steps + chunk - 1) / chunk);

@@ -203,6 +203,126 @@ struct Scan {
   int32_t reverse;
 };
 
+// A scan of few steps (ep_memory_scan, either direction of time): step by step, one wave per state, which stays in the
+// wave's registers from the first step to the last. Lane (d0, c) holds kKeys keys from d0 * kKeys on and the four values
+// from 4c on; a step's q, k and v go through LDS, the next one's are on their way meanwhile. A chunk of the matrix-core
+// walk costs the same however few of its steps there are; this costs kKeys * 12 multiplications and additions a
+// step and lane, and moves nothing twice. Up to 64 x 64, any strides.
+typedef float f32x4_few __attribute__((ext_vector_type(4)));
+template <class T, int kKeys> __global__ __launch_bounds__(256) void scan_few(Scan p, int width_log, int in_rows, int in_cols, int out_rows, int out_cols) {
+  using V = f32x4_few;
+  __shared__ __align__(16) float lds[4][2][3][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t item = (int64_t)blockIdx.x * 4 + wave;
+  if (item >= p.rows * p.heads) return;
+  const int64_t row = item / p.heads;
+  const int h = (int)(item % p.heads);
+  const int width = 1 << width_log, c = lane & (width - 1), first = (lane >> width_log) * kKeys;
+  const float decay = expf(p.log_decay[h]);
+  const T* gq = (const T*)p.q + row * p.q_stride[1] + (h / p.q_group) * p.q_stride[2] + lane;
+  const T* gk = (const T*)p.k + row * p.k_stride[1] + (h / p.k_group) * p.k_stride[2] + lane;
+  const T* gv = (const T*)p.v + row * p.v_stride[1] + (h / p.v_group) * p.v_stride[2] + lane;
+  T rq = (T)0.f, rk = (T)0.f, rv = (T)0.f;
+  uint8_t rf = 0;
+  const auto ask = [&](int64_t t) {
+    if (lane < p.dk) rq = gq[t * p.q_stride[0]], rk = gk[t * p.k_stride[0]];
+    if (lane < p.dv) rv = gv[t * p.v_stride[0]];
+    if (p.fresh) rf = p.fresh[t * p.fresh_stride[0] + row * p.fresh_stride[1]];
+  };
+  ask(p.reverse ? p.steps - 1 : 0);
+
+  V s[kKeys];
+#pragma unroll
+  for (int i = 0; i < kKeys; ++i) s[i] = (V)0.f;
+  if (p.state_in) {
+    const float* a = p.state_in + row * p.in_stride[0] + h * p.in_stride[1];
+    if (in_rows) {  // a key's values follow one another, in 16-byte pieces
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i)
+        if (first + i < p.dk && 4 * c < p.dv) s[i] = *(const V*)(a + (first + i) * p.in_stride[2] + 4 * c);
+    } else if (in_cols) {  // a value's keys do
+#pragma unroll
+      for (int i = 0; i < kKeys; i += 4)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (first + i < p.dk && 4 * c + r < p.dv) {
+            const V x = *(const V*)(a + (4 * c + r) * p.in_stride[3] + first + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[i + e][r] = x[e];
+          }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (first + i < p.dk && 4 * c + r < p.dv) s[i][r] = a[(first + i) * p.in_stride[2] + (4 * c + r) * p.in_stride[3]];
+    }
+  }
+  float carry = p.reverse ? 1.f : decay;  // (back in time, what enters the last step has not decayed)
+  bool drop = false;
+  for (int64_t n = 0; n < p.steps; ++n) {
+    const int64_t t = p.reverse ? p.steps - 1 - n : n;
+    float(*now)[64] = lds[wave][n & 1];
+    now[0][lane] = (float)rq, now[1][lane] = (float)rk, now[2][lane] = (float)rv * p.inc_scale;
+    const bool fresh = rf != 0;
+    if (n + 1 < p.steps) ask(p.reverse ? t - 1 : t + 1);
+    wave_sync();
+    if (!p.reverse) drop = fresh;
+    if (drop) {  // (not a product with 0: what was there may not be finite)
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i) s[i] = (V)0.f;
+    }
+    const V v = *(const V*)&now[2][4 * c];
+    V acc = (V)0.f;
+#pragma unroll
+    for (int i = 0; i < kKeys; i += 4) {
+      const V q = *(const V*)&now[0][first + i], k = *(const V*)&now[1][first + i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[i + e] = s[i + e] * carry + k[e] * v;
+        acc += q[e] * s[i + e];
+      }
+    }
+    carry = decay, drop = fresh;
+    if (!p.out) continue;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      for (int o = 32; o >= width; o >>= 1) acc[r] += __shfl_xor(acc[r], o, 64);
+    if (first == 0) {
+      const int64_t to = t * p.out_stride[0] + row * p.out_stride[1] + h * p.out_stride[2] + 4 * c;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (4 * c + r < p.dv) {
+          if (p.out_f32) ((float*)p.out)[to + r] = acc[r] * p.out_scale;
+          else ((T*)p.out)[to + r] = (T)(acc[r] * p.out_scale);
+        }
+    }
+  }
+  if (!p.state_out) return;
+  if (p.reverse) {
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) s[i] = drop ? (V)0.f : s[i] * decay;
+  }
+  float* a = p.state_out + row * p.outs_stride[0] + h * p.outs_stride[1];
+  if (out_rows) {
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i)
+      if (first + i < p.dk && 4 * c < p.dv) *(V*)(a + (first + i) * p.outs_stride[2] + 4 * c) = s[i];
+  } else if (out_cols) {
+#pragma unroll
+    for (int i = 0; i < kKeys; i += 4)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (first + i < p.dk && 4 * c + r < p.dv) *(V*)(a + (4 * c + r) * p.outs_stride[3] + first + i) = V{s[i][r], s[i + 1][r], s[i + 2][r], s[i + 3][r]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (first + i < p.dk && 4 * c + r < p.dv) a[(first + i) * p.outs_stride[2] + (4 * c + r) * p.outs_stride[3]] = s[i][r];
+  }
+}
+
 // gradients of heads that share keys and values, summed in 32 bits and rounded once (5 us at 777 x 5 x 2 x 112)
 template <class T> __global__ __launch_bounds__(256) void sum_heads(const float* src, int64_t total, int32_t group, int32_t dim, T* out) {
   // over [n][heads_out][dim]

@@ -437,6 +437,46 @@ def test_memory_scan_keeps_what_is_not_finite_inside_its_episode(dtype):
     assert torch.isfinite(got[5][[1, 3]]).all()
 
 
+FEW = [
+  # steps, rows, heads, kv heads, key dim, value dim, P(fresh), states
+  (1, 5, 2, 2, 32, 32, 0.0, True), (2, 3, 2, 1, 7, 5, 0.3, True), (8, 70, 2, 1, 32, 32, 0.2, True), (16, 33, 1, 1, 16, 16, 0.1, False), (16, 9, 3, 3, 29, 31, 0.1, True),
+  (8, 6, 2, 2, 64, 64, 0.1, True), (5, 4, 2, 2, 64, 3, 0.2, True), (16, 7, 2, 1, 3, 64, 0.2, True), (15, 5, 2, 1, 33, 12, 0.3, True), (17, 5, 2, 1, 33, 12, 0.3, True),
+  (16, 8, 1, 1, 1, 1, 0.2, True),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", FEW, ids=lambda c: "-".join(str(x) for x in c))
+def test_segments_of_few_steps(case, dtype):
+  test_memory_scan_and_its_gradients(case, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_steps_keep_what_is_not_finite_inside_its_episode(dtype):
+  from envpool_amd import policy
+  t, n, h, dk, dv = 12, 3, 2, 32, 16
+  q, k, v, decay, _, state, do, ds = _scan_problem((t, n, h, h, dk, dv, 0.0, True), dtype)
+  fresh = torch.zeros(t, n, dtype=torch.bool)
+  fresh[[3, 7], 0] = True
+  fresh[5, 1] = True
+
+  def run(filler):
+    kk, vv, dd = k.clone(), v.clone(), do.clone()
+    for x in (kk, vv, dd):
+      x[4, 0] = x[2, 1] = filler
+    leaves = [x.to(DEV).requires_grad_() for x in (q, kk, vv, state)]
+    out, final = policy.memory_scan(*leaves[:3], decay.to(DEV), fresh=fresh.to(DEV), state=leaves[3])
+    return [x.detach().cpu() for x in (out, final, *torch.autograd.grad([out, final], leaves, [dd.to(DEV), ds.to(DEV)]))]
+
+  well = torch.ones(t, n, dtype=torch.bool)
+  well[3:7, 0] = False
+  well[:5, 1] = False
+  clean, sick = run(0.0), run(math.inf)
+  for x, w in zip((sick[0], *sick[2:5]), (clean[0], *clean[2:5])):
+    assert torch.equal(x[well], w[well])
+  assert torch.equal(sick[1], clean[1]) and torch.equal(sick[5][[0, 2]], clean[5][[0, 2]])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("t,n,h,dk,dv", [(16, 4, 12, 64, 64), (32, 40, 4, 16, 16), (30, 3, 2, 128, 128), (17, 5, 3, 20, 19)])
 def test_states_keep_32_bits(t, n, h, dk, dv, dtype):
