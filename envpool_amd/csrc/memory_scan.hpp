@@ -7,10 +7,15 @@
 //   S = carry * S + (K * w_up[s])^T V
 // Everything is computed transposed (scores as [s, t], outputs as [v, t]): the accumulators of one product are
 // then laid out as an operand of the next up to a permutation of the summed index, which is applied to the
-// other operand as well. So the state never leaves its registers (32 bits; in 16-bit types it enters Q S as two
-// rounded pieces and its increments leave K^T V from three, or two scaled, pieces of the weighted values, so that both
-// keep what 32 bits keep), scores cross LDS once because each wave computes 16 of the query columns and needs all of
-// them for its quarter of the value columns, and an output row is written 4 values a lane.
+// other operand as well. So the state never leaves its registers (32 bits), scores cross LDS once because each wave
+// computes 16 of the query columns and needs all of them for its quarter of the value columns, and an output row is
+// written 4 values a lane.
+// What 32-bit values become as operands of 16-bit products (every sum is kept in 32 bits):
+//   weighted values in K^T V   three pieces (bf16) or two scaled ones (f16): the state keeps what 32 bits keep
+//   the state in Q S           two pieces: 16 bits of it in bf16, 22 in f16
+//   scores in P V              two pieces, the same
+// so that an output is off by 2^-16 (2^-22) of its terms before it is rounded to its type once. (With the scores in one
+// piece that rounding was one of two of a size: the error of a bf16 result grew from 0.00166 to 0.0020 .. 0.0022.)
 // Time backwards (for gradients) is the same chunk with the triangle and the weights mirrored.
 #pragma once
 #include "memory_kernels.hpp"
@@ -57,6 +62,19 @@ template <class T, class V8, class V4> struct Mma16 {
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = (T)a[r];
     *(V4*)p = v;
+  }
+  // the first pieces of four values to p, the second ones returned
+  static __device__ uint2 put4_first(T* p, f32x4 a) {
+    V4 v, w;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float x = a[r];
+      asm volatile("" : "+v"(x));  // (rounded once, from 32 bits: see Mma<f16>::pieces)
+      v[r] = (T)x;
+      w[r] = (T)(x - (float)v[r]);
+    }
+    *(V4*)p = v;
+    return __builtin_bit_cast(uint2, w);
   }
 };
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -347,8 +365,10 @@ template <class T, int DK, int DV, bool kAligned, bool rev> struct Walk {
     }
   }
 
-  // scores of 16 query steps per wave, or per two waves that take every other tile of them
-  static __device__ void scores(const Scan& p, const Now& c, const T* qs, int SQ, const T* ks, int SK, T* ps) {
+  // scores of 16 query steps per wave, or per two waves that take every other tile of them; their second pieces stay in
+  // registers (16-bit types) until put_seconds
+  using Seconds = uint2[kBlocks];
+  static __device__ void scores(const Scan& p, const Now& c, const T* qs, int SQ, const T* ks, int SK, T* ps, Seconds& second) {
     const int wave = c.wave, ln = c.ln, g = ln >> 4, l16 = ln & 15, nk = Walk::nk(p);
     const uint64_t starts = c.starts;
     const float l2 = c.l2, lambda = c.lambda;
@@ -369,8 +389,7 @@ template <class T, int DK, int DV, bool kAligned, bool rev> struct Walk {
     frag q[DK / K];
 #pragma unroll
     for (int k = 0; k < DK / K; ++k) q[k] = M::row(qs, SQ, 16 * strip, k * K, ln);
-    // (all tiles of whole fragments, so that what lies across the diagonal is 0)
-    const int i0 = rev ? (16 * strip) / K * K / 16 : 0, i1 = rev ? kChunk / 16 : ((16 * strip) / K + 1) * K / 16;
+    const int i0 = first_tile(strip), i1 = last_tile(strip);
     const float scale = p.inc_scale * p.out_scale;
     f32x4 score[kBlocks];
     float top = 0.f;
@@ -403,7 +422,8 @@ template <class T, int DK, int DV, bool kAligned, bool rev> struct Walk {
         for (int r = 0; r < 4; ++r) top = fmaxf(top, fabsf(a[r]));
         score[i] = a;
       } else if (i >= i0 && i < i1) {
-        M::put4(ps + t * SP + 16 * i + 4 * g, a);
+        if constexpr (sizeof(T) == 2) second[i] = M::put4_first(ps + t * SP + 16 * i + 4 * g, a);
+        else M::put4(ps + t * SP + 16 * i + 4 * g, a);
       }
     }
     if constexpr (M::kNarrow) {
@@ -413,18 +433,26 @@ template <class T, int DK, int DV, bool kAligned, bool rev> struct Walk {
       if (g == 0) p_top[t] = f;
 #pragma unroll
       for (int i = 0; i < kBlocks; ++i)
-        if (i >= i0 && i < i1) M::put4(ps + t * SP + 16 * i + 4 * g, score[i] * f);
+        if (i >= i0 && i < i1) second[i] = M::put4_first(ps + t * SP + 16 * i + 4 * g, score[i] * f);
+    }
+  }
+  // the tiles of a strip of scores that P V reads: all of whole fragments, so that what lies across the diagonal is 0
+  static __device__ int first_tile(int strip) { return rev ? (16 * strip) / K * K / 16 : 0; }
+  static __device__ int last_tile(int strip) { return rev ? kChunk / 16 : ((16 * strip) / K + 1) * K / 16; }
+  static __device__ void put_seconds(const Now& c, const Seconds& second, T* ps2) {
+    if constexpr (sizeof(T) == 2) {
+      const int strip = c.wave % kBlocks, i0 = first_tile(strip), i1 = last_tile(strip);
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i)
+        if (i >= i0 && i < i1) *(uint2*)(ps2 + (16 * strip + (c.ln & 15)) * SP + 16 * i + 4 * (c.ln >> 4)) = second[i];
     }
   }
 
-  // outputs: what the entering state gives, then the chunk's own steps
-  static __device__ void outputs(const Scan& p, const Now& c, int64_t row, int h, const State& s, const T* qs, int SQ, const T* vs, int SV, const T* ps) {
-    const int wave = c.wave, ln = c.ln, g = ln >> 4, l16 = ln & 15, v0 = 16 * wave, nk = Walk::nk(p), n_now = c.n;
-    const float *w_in = c.w_in, *p_top = c.p_top;
-    const uint32_t out_size = p.out_f32 ? 4u : (uint32_t)sizeof(T);
-    const T* out_row = (const T*)((const char*)p.out + (c.start * p.out_stride[0] + row * p.out_stride[1] + h * p.out_stride[2]) * (int64_t)out_size);
+  // outputs: what the entering state gives (not weighted yet; returns what the state was multiplied by) ..
+  using Outs = f32x4[kBlocks][NV];
+  static __device__ float from_state(const Scan& p, const Now& c, const State& s, const T* qs, int SQ, Outs& a) {
+    const int ln = c.ln, v0 = 16 * c.wave, nk = Walk::nk(p);
     const auto there = [&](int j) { return !kTrim || j == 0 || v0 + 64 * j < p.dv; };  // (the same for the whole wave)
-    f32x4 a[kBlocks][NV];
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
@@ -471,6 +499,15 @@ template <class T, int DK, int DV, bool kAligned, bool rev> struct Walk {
       keep_order();
     }
     settle<kTrim>();
+    return s_scale;
+  }
+  // .. then the chunk's own steps
+  static __device__ void outputs(const Scan& p, const Now& c, int64_t row, int h, Outs& a, float s_scale, const T* vs, int SV, const T* ps, const T* ps2) {
+    const int wave = c.wave, ln = c.ln, g = ln >> 4, l16 = ln & 15, v0 = 16 * wave, n_now = c.n;
+    const float *w_in = c.w_in, *p_top = c.p_top;
+    const uint32_t out_size = p.out_f32 ? 4u : (uint32_t)sizeof(T);
+    const T* out_row = (const T*)((const char*)p.out + (c.start * p.out_stride[0] + row * p.out_stride[1] + h * p.out_stride[2]) * (int64_t)out_size);
+    const auto there = [&](int j) { return !kTrim || j == 0 || v0 + 64 * j < p.dv; };
     frag vf[NV][kChunk / K];
 #pragma unroll
     for (int j = 0; j < NV; ++j)
@@ -492,6 +529,11 @@ template <class T, int DK, int DV, bool kAligned, bool rev> struct Walk {
 #pragma unroll
           for (int j = 0; j < NV; ++j)
             if (there(j)) a[b][j] = M::mul(vf[j][k], pf, a[b][j]);
+          if constexpr (sizeof(T) == 2) {
+            const frag pf2 = M::row(ps2, SP, 16 * b, k * K, ln);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) a[b][j] = M::mul(vf[j][k], pf2, a[b][j]);
+          }
         }
       settle<true>();  // (how results are stored is a branch)
 #pragma unroll
@@ -696,10 +738,25 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
     if (n > 0) load(start, n);
 
     W::weights(p, c);
-    if (!parts.state_only) W::scores(p, c, qs, SQ, ks, SK, ps);
-    __syncthreads();
     through = c.starts ? 0.f : through * __builtin_amdgcn_exp2f(c.l2 * c.n);
-    if (!parts.state_only) W::outputs(p, c, row, h, s, qs, SQ, vs, SV, ps);
+    if (!parts.state_only) {
+      typename W::Outs a;
+      typename W::Seconds second;
+      // (two results that wait for each other: the smaller first, or where values outnumber keys the larger, which spills
+      // fewer registers: 128 steps of 2048 states of 64 x 128, bf16 86 us against 91, f16 100 against 101)
+      float s_scale = 1.f;
+      if constexpr (DK < DV) s_scale = W::from_state(p, c, s, qs, SQ, a);
+      W::scores(p, c, qs, SQ, ks, SK, ps, second);
+      if constexpr (DK >= DV) s_scale = W::from_state(p, c, s, qs, SQ, a);
+      __syncthreads();
+      if constexpr (sizeof(T) == 2) {  // (the queries have been read: their place holds the scores' second pieces)
+        W::put_seconds(c, second, qs);
+        __syncthreads();
+      }
+      W::outputs(p, c, row, h, a, s_scale, vs, SV, ps, qs);
+    } else {
+      __syncthreads();
+    }
     W::update(p, c, s, ks, SK, vs, SV);
   }
 
@@ -803,14 +860,21 @@ template <class T> __global__ __launch_bounds__(256, 3) void scan_pair(Scan a, S
     if (n > 0) load(start, n);
 
     W::weights(a, c);
-    W::scores(a, c, kt, SQ, qt, SK, ps);
+    typename W::Outs o;
+    typename W::Seconds second;
+    W::scores(a, c, kt, SQ, qt, SK, ps, second);
+    float s_scale = W::from_state(a, c, sa, kt, SQ, o);
     __syncthreads();
-    W::outputs(a, c, row, h, sa, kt, SQ, gt, SK, ps);
+    W::put_seconds(c, second, kt);  // (a's queries have been read, here and for b: their place is free)
+    __syncthreads();
+    W::outputs(a, c, row, h, o, s_scale, gt, SK, ps, kt);
     W::update(a, c, sa, qt, SK, gt, SK);
     __syncthreads();  // (the scores have been read)
-    W::scores(b, c, vt, SQ, gt, SK, ps);
+    W::scores(b, c, vt, SQ, gt, SK, ps, second);
+    W::put_seconds(c, second, kt);
+    s_scale = W::from_state(b, c, sb, vt, SQ, o);
     __syncthreads();
-    W::outputs(b, c, row, h, sb, vt, SQ, qt, SK, ps);
+    W::outputs(b, c, row, h, o, s_scale, qt, SK, ps, kt);
     W::update(b, c, sb, gt, SK, qt, SK);
   }
   if (a.state_out) W::store_state(a, row, h, lane, c.wave, sa);

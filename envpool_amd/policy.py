@@ -479,8 +479,10 @@ def memory_scan(q, k, v, log_decay, *, fresh=None, state=None, scale: Optional[f
   `log_decay` float32 `[H]`, values <= 0, not differentiated. `fresh` bool / uint8 `[T, B]`: steps at which an
   episode starts, so that nothing from before reaches them (None: no such step). `state` float32
   `[B, H, key_dim, value_dim]`: where the rows start (None: zero). Dimensions 1 to 128.
-  Differentiable (once) in q, k, v and state; states and sums are kept in 32 bits, gradients come in the type of
-  the tensor they belong to."""
+  Differentiable (once) in q, k, v and state; gradients come in the type of the tensor they belong to. States and sums
+  are kept in 32 bits. As operands of 16-bit products the states and the scores of a chunk enter as two pieces of the type
+  (16 bits together in bfloat16, 22 in float16), so that outputs and gradients are in effect rounded once, at the end;
+  those of heads that share keys and values are summed in 32 bits before."""
   if q.dtype not in _FLOATS or k.dtype != q.dtype or v.dtype != q.dtype:
     raise ValueError(f"q, k, v must be of one type, float32, float16 or bfloat16, got {q.dtype}, {k.dtype}, {v.dtype}")
   if q.dim() != 4 or q.shape[2] < 1:

@@ -1,0 +1,91 @@
+"""envpool_amd.policy at its edges on the GPU, against the definitions in 64 bits (tests/policy_ref.py): how many bits
+results keep, values that are not finite, hooks and checkpoints of autograd, in-place changes."""
+import math
+
+import pytest
+import torch
+
+from tests import policy_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+DEV = "cuda:0"
+H32 = ref.HALF[torch.float32]
+
+
+def _gen(seed):
+  return torch.Generator().manual_seed(seed)
+
+
+def _decay(h):
+  return torch.log1p(-torch.exp2(-2.0 - 6.0 * torch.arange(h).double() / h)).float()
+
+
+def _scan_problem(t, n, h, hk, dk, dv, p_fresh, dtype):
+  g = _gen(7 * t + dk)
+  q, k, v = torch.randn(t, n, h, dk, generator=g), torch.randn(t, n, hk, dk, generator=g) * dk**-0.5, torch.randn(t, n, hk, dv, generator=g)
+  fresh = torch.rand(t, n, generator=g) < p_fresh
+  state, ds = torch.randn(n, h, dk, dv, generator=g), torch.randn(n, h, dk, dv, generator=g)
+  do = torch.randn(t, n, h, dv, generator=g)
+  return q.to(dtype), k.to(dtype), v.to(dtype), _decay(h), fresh, state, do.to(dtype), ds
+
+
+def _scan_all(q, k, v, decay, fresh, state, do, ds):
+  """Outputs and all gradients of one scan on the GPU, by name, on the CPU."""
+  from envpool_amd import policy
+  leaves = [x.to(DEV).requires_grad_() for x in (q, k, v, state)]
+  out, final = policy.memory_scan(*leaves[:3], decay.to(DEV), fresh=None if fresh is None else fresh.to(DEV), state=leaves[3])
+  grads = torch.autograd.grad([out, final], leaves, [do.to(DEV), ds.to(DEV)])
+  names = ("out", "final", "grad_q", "grad_k", "grad_v", "grad_state")
+  return {name: x.detach().cpu() for name, x in zip(names, (out, final, *grads))}
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("case", [(130, 5, 4, 4, 64, 64, 0.02), (130, 3, 4, 1, 48, 64, 0.02), (300, 2, 2, 2, 64, 128, 0.01), (200, 2, 2, 1, 128, 64, 0.01),
+                                  (700, 1, 3, 3, 128, 128, 0.004), (260, 520, 2, 2, 64, 32, 0.01), (150, 2, 2, 2, 33, 21, 0.02)],
+                         ids=lambda c: "-".join(str(x) for x in c))
+def test_results_in_16_bits_are_rounded_once(case, dtype):
+  """Chunks, several of them, split time, the pair of gradients: an output is its value in 32 bits, rounded to its type.
+  Before that rounding a term (a score times a value, or a query's product with the state) is off by what two pieces of the
+  type leave out, half a step squared; in float16 what is below 2^-36 of a row's largest score or state is lost. The
+  rest is 32-bit arithmetic: products and sums over 64 steps and `dim` entries twice, powers of the decay (their
+  exponents off by 2^-24 of at most 27 octaves, twice), a rounding of the state per chunk, the sum of shared heads."""
+  t, n, h, hk, dk, dv, _ = case
+  q, k, v, decay, fresh, state, do, ds = _scan_problem(*case, dtype)
+  got = _scan_all(q, k, v, decay, fresh, state, do, ds)
+  rows = torch.arange(min(n, 6))  # (many rows choose the kernel; a few are looked at)
+  part = lambda x, dim: x.index_select(dim, rows)  # noqa: E731
+  args = dict(fresh=part(fresh, 1), state=part(state, 0), scale=dk**-0.5, grad_out=part(do, 1), reverse_from=part(ds, 0))
+  want = ref.scan(part(q, 1), part(k, 1), part(v, 1), decay, **args)
+  size = ref.scan(part(q, 1), part(k, 1), part(v, 1), decay, absolute=True, **args)
+  half = ref.HALF[dtype]
+  for name in ("out", "grad_q", "grad_k", "grad_v"):
+    x, w, s = part(got[name], 1).double(), want[name], size[name]
+    inner = 1.01 * half**2 + H32 * (2 * max(dk, dv) + 2 * 64 + 2 * 27 + 4 * (t / 64 + 1) + h // hk + 8)
+    tol = s * inner + half * (w.abs() + s * inner) + ref.TINY[dtype] + 2.0**-34 * float(s.max())
+    err = (x - w).abs()
+    assert got[name].dtype == dtype and (err <= tol).all(), (name, float((err - tol).max()), float((err > tol).double().mean()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", [(130, 5, 4, 4, 64, 64, 0.02), (700, 1, 3, 3, 128, 128, 0.004), (700, 1, 2, 1, 24, 80, 0.0), (400, 300, 2, 2, 32, 64, 0.01)],
+                         ids=lambda c: "-".join(str(x) for x in c))
+def test_states_keep_32_bits_over_many_chunks(case, dtype):
+  """Carried from chunk to chunk, joined over split time. In half steps of 32 bits and of the sum of magnitudes: 4 for a
+  term's two pieces, 2 * 27 ln 2 for its power of the decay, a rounding per step's sum, 3 per chunk that carries it. And of
+  the whole in the 2-norm, where t independent roundings of partial sums add up as sqrt(t): 32 for up to 700."""
+  t, n, h, hk, dk, dv, _ = case
+  q, k, v, decay, fresh, state, do, ds = _scan_problem(*case, dtype)
+  got = _scan_all(q, k, v, decay, fresh, state, do, ds)
+  rows = torch.arange(min(n, 6))
+  part = lambda x, dim: x.index_select(dim, rows)  # noqa: E731
+  args = dict(fresh=part(fresh, 1), state=part(state, 0), scale=dk**-0.5, grad_out=part(do, 1), reverse_from=part(ds, 0))
+  want = ref.scan(part(q, 1), part(k, 1), part(v, 1), decay, **args)
+  size = ref.scan(part(q, 1), part(k, 1), part(v, 1), decay, absolute=True, **args)
+  for name in ("final", "grad_state"):
+    x, w = part(got[name], 0).double(), want[name]
+    err = (x - w).abs()
+    tol = size[name] * H32 * (4 + 38 + t + 3 * (t / 32 + 1) + 4) + 2.0**-30
+    assert (err <= tol).all(), (name, float((err - tol).max()))
+    assert float((x - w).norm()) <= 32 * H32 * float(w.norm()), (name, float((x - w).norm() / w.norm()))
