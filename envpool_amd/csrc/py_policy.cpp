@@ -30,6 +30,13 @@ struct Rows : ep_policy_rows {
     temperature = at<const float>(temp), temperature_all = temp_all;
     stream = at<void>(stream_);
   }
+  // whether rows follow one another without gaps (or one serves all)
+  bool dense() const {
+    const int64_t words = mask_dtype == EP_I32 ? (options + 31) / 32 : options;
+    const auto follows = [&](int64_t stride, int64_t width) { return rows <= 1 || stride == 0 || stride == width; };
+    return (rows <= 1 || logits_stride == options) && (!mask || follows(mask_stride, words)) && (!bias || follows(bias_stride, options)) &&
+           (!history || follows(history_stride, history_len));
+  }
 };
 
 void choose(const Rows& rows, u64 u, int u_dtype, u64 action, u64 log_prob, u64 entropy, u64 workspace, int64_t workspace_bytes) {
@@ -54,15 +61,20 @@ void evaluate(const Rows& rows, u64 action, u64 log_prob, u64 entropy, u64 stats
   epy::check(rc);
 }
 
-void evaluate_grad(const Rows& rows, u64 action, u64 entropy, u64 stats, u64 g_lp, u64 g_h, u64 grad_logits, int64_t grad_logits_stride, u64 grad_bias,
+// `at_now`: where the forward pass' operands are now (logits, num_options, mask, bias, history, repetition, frequency, presence,
+// temperature; then action, entropy, stats). The addresses in `rows` are not followed, those tensors may be gone.
+void evaluate_grad(const Rows& rows, const std::array<u64, 12>& at_now, u64 g_lp, u64 g_h, u64 grad_logits, int64_t grad_logits_stride, u64 grad_bias,
                    int64_t grad_bias_stride, u64 workspace, int64_t workspace_bytes, u64 stream) {
   ep_policy_rows r = rows;
   r.workspace = at<void>(workspace), r.workspace_bytes = workspace_bytes;
+  r.logits = at<void>(at_now[0]), r.num_options = at<const int32_t>(at_now[1]), r.mask = at<void>(at_now[2]), r.bias = at<void>(at_now[3]);
+  r.history = at<const int32_t>(at_now[4]), r.repetition = at<const float>(at_now[5]), r.frequency = at<const float>(at_now[6]);
+  r.presence = at<const float>(at_now[7]), r.temperature = at<const float>(at_now[8]);
   r.stream = at<void>(stream);  // (the backward pass may run on another stream than the forward pass)
   int rc;
   {
     py::gil_scoped_release rel;
-    rc = ep_policy_evaluate_grad(&r, at<const int32_t>(action), at<const float>(entropy), at<const float>(stats), at<const float>(g_lp),
+    rc = ep_policy_evaluate_grad(&r, at<const int32_t>(at_now[9]), at<const float>(at_now[10]), at<const float>(at_now[11]), at<const float>(g_lp),
                                  at<const float>(g_h), at<void>(grad_logits), grad_logits_stride, at<void>(grad_bias), grad_bias_stride);
   }
   epy::check(rc);
@@ -147,6 +159,8 @@ PYBIND11_MODULE(policy_native, m) {
       .def("grad_workspace", [](const Rows& r, bool with_bias) { return ep_policy_evaluate_grad_workspace(&r, with_bias); })
       .def("choose", &choose)
       .def("evaluate", &evaluate)
+      .def("dense", &Rows::dense)
+      .def("bias_per_row", [](const Rows& r) { return r.bias_stride != 0; })
       .def("evaluate_grad", &evaluate_grad);
   py::class_<Step>(m, "Step")
       .def(py::init<int, int64_t, int, int, int, u64, u64, int, u64>())

@@ -56,71 +56,83 @@ def _row_operand(t, name, rows, cols):
 
 
 def _penalty(v, name, rows):
-  """A number, or a float32 `[rows]` tensor -> (tensor or None, its address, the number)."""
+  """A number, or a float32 `[rows]` tensor -> (tensor or None, the number)."""
   if isinstance(v, torch.Tensor):
     if v.dtype != torch.float32 or v.shape != (rows,):
       raise ValueError(f"{name} must be a number or a float32 tensor [{rows}], got {v.dtype} {list(v.shape)}")
-    if not v.is_contiguous():
-      v = v.contiguous()
-    return v, v.data_ptr(), 1.0
-  return None, 0, float(v)
+    return v, 1.0
+  return None, float(v)
 
 
 class _Prepared:
-  """The checked operands of one call and the native struct over them."""
-  __slots__ = ("rows", "native", "keep", "bias", "bias_stride", "logits", "dev", "n", "options")
+  """The checked operands of one call: tensors as the kernels read them, the numbers beside them, and the native struct."""
+  __slots__ = ("tensors", "numbers", "native", "dev", "n")
+
+
+# the operands in `_Prepared.tensors`: logits, num_options, mask, bias, history, repetition, frequency, presence, temperature
+_BIAS, _SLOTS = 3, 9
+
+
+def _dense(t):
+  return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _bind(p):
+  """Lays `p.tensors` (of checked types and shapes) out as the kernels read them and fills `p.native` with where they are
+  now. The backward pass does it anew where what autograd hands back is laid out otherwise than what was saved."""
+  logits, num_options, mask, bias, history, *per_row = p.tensors
+  n, a = logits.shape
+  if (a > 1 and logits.stride(1) != 1) or (n > 1 and logits.stride(0) < a):
+    logits = logits.contiguous()
+  if num_options is not None and not num_options.is_contiguous():
+    num_options = num_options.contiguous()
+  mask_ptr = mask_dt = mask_stride = bias_ptr = bias_dt = bias_stride = hist_ptr = hist_len = hist_stride = 0
+  if mask is not None:
+    mask, mask_stride = _row_operand(mask, "mask", n, (a + 31) // 32 if mask.dtype == torch.int32 else a)
+    mask_ptr, mask_dt = mask.data_ptr(), _MASKS[mask.dtype]
+  if bias is not None:
+    bias, bias_stride = _row_operand(bias, "bias", n, a)
+    bias_ptr, bias_dt = bias.data_ptr(), _FLOATS[bias.dtype]
+  if history is not None:
+    hist_len = history.shape[-1]
+    if hist_len > 0:
+      history, hist_stride = _row_operand(history, "history", n, hist_len)
+      hist_ptr = history.data_ptr()
+  rep, freq, pres, temp = per_row = [t if t is None or t.is_contiguous() else t.contiguous() for t in per_row]
+  _same_device(p.dev, num_options=num_options, mask=mask, bias=bias, history=history, repetition=rep, frequency=freq, presence=pres, temperature=temp)
+  rep_all, freq_all, pres_all, temp_all = p.numbers
+  p.tensors = (logits, num_options, mask, bias, history, *per_row)
+  p.native = _native.Rows(p.dev.index, _FLOATS[logits.dtype], n, a, logits.data_ptr(), logits.stride(0), 0 if num_options is None else num_options.data_ptr(),
+                          mask_ptr, mask_dt, mask_stride, bias_ptr, bias_dt, bias_stride, hist_ptr, hist_len, hist_stride, 0 if rep is None else rep.data_ptr(),
+                          rep_all, 0 if freq is None else freq.data_ptr(), freq_all, 0 if pres is None else pres.data_ptr(), pres_all,
+                          0 if temp is None else temp.data_ptr(), temp_all, current_stream_handle(p.dev))
 
 
 def _prepare(logits, num_options, mask, bias, history, repetition, frequency, presence, temperature):
   if logits.dim() != 2 or logits.dtype not in _FLOATS or logits.shape[1] < 1:
     raise ValueError(f"logits must be float32, float16 or bfloat16 [rows, options >= 1], got {logits.dtype} {list(logits.shape)}")
-  n, a = logits.shape
-  if (a > 1 and logits.stride(1) != 1) or (n > 1 and logits.stride(0) < a):
-    logits = logits.contiguous()
-  dev = logits.device
-  opt_ptr = 0
-  if num_options is not None:
-    if num_options.dtype != torch.int32 or num_options.shape != (n,):
-      raise ValueError(f"num_options must be int32 [{n}], got {num_options.dtype} {list(num_options.shape)}")
-    if not num_options.is_contiguous():
-      num_options = num_options.contiguous()
-    opt_ptr = num_options.data_ptr()
-  mask_ptr = mask_dt = mask_stride = 0
-  if mask is not None:
-    mask_dt = _MASKS.get(mask.dtype)
-    if mask_dt is None:
-      raise ValueError(f"mask must be bool or uint8 (one per option) or int32 (32 options a word), got {mask.dtype}")
-    mask, mask_stride = _row_operand(mask, "mask", n, (a + 31) // 32 if mask.dtype == torch.int32 else a)
-    mask_ptr = mask.data_ptr()
-  bias_ptr = bias_dt = bias_stride = 0
-  if bias is not None:
-    if bias.dtype != torch.float32 and bias.dtype != logits.dtype:
-      raise ValueError(f"bias must be float32 or of the logits' type, got {bias.dtype}")
-    bias, bias_stride = _row_operand(bias, "bias", n, a)
-    bias_ptr, bias_dt = bias.data_ptr(), _FLOATS[bias.dtype]
-  hist_ptr = hist_len = hist_stride = 0
-  if history is not None:
-    if history.dtype != torch.int32 or history.dim() not in (1, 2):
-      raise ValueError(f"history must be int32 [{n}, length] or [length], got {history.dtype} {list(history.shape)}")
-    hist_len = history.shape[-1]
-    if hist_len > 0:
-      history, hist_stride = _row_operand(history, "history", n, hist_len)
-      hist_ptr = history.data_ptr()
-  rep, rep_ptr, rep_all = _penalty(repetition, "repetition", n)
-  freq, freq_ptr, freq_all = _penalty(frequency, "frequency", n)
-  pres, pres_ptr, pres_all = _penalty(presence, "presence", n)
-  temp, temp_ptr, temp_all = _penalty(temperature, "temperature", n)
+  n, dev = logits.shape[0], logits.device
+  if num_options is not None and (num_options.dtype != torch.int32 or num_options.shape != (n,)):
+    raise ValueError(f"num_options must be int32 [{n}], got {num_options.dtype} {list(num_options.shape)}")
+  if mask is not None and mask.dtype not in _MASKS:
+    raise ValueError(f"mask must be bool or uint8 (one per option) or int32 (32 options a word), got {mask.dtype}")
+  if bias is not None and bias.dtype != torch.float32 and bias.dtype != logits.dtype:
+    raise ValueError(f"bias must be float32 or of the logits' type, got {bias.dtype}")
+  if history is not None and (history.dtype != torch.int32 or history.dim() not in (1, 2)):
+    raise ValueError(f"history must be int32 [{n}, length] or [length], got {history.dtype} {list(history.shape)}")
+  rep, rep_all = _penalty(repetition, "repetition", n)
+  freq, freq_all = _penalty(frequency, "frequency", n)
+  pres, pres_all = _penalty(presence, "presence", n)
+  temp, temp_all = _penalty(temperature, "temperature", n)
   for name, t, v, low in (("temperature", temp, temp_all, 0.0), ("repetition", rep, rep_all, 0.0), ("frequency", freq, freq_all, -math.inf),
                           ("presence", pres, pres_all, -math.inf)):
     if t is None and not low < v < math.inf:
       raise ValueError(f"{name} = {v} is not a {'positive ' if low == 0.0 else ''}number")
-  _same_device(dev, num_options=num_options, mask=mask, bias=bias, history=history, repetition=rep, frequency=freq, presence=pres, temperature=temp)
   p = _Prepared()
-  p.logits, p.bias, p.bias_stride, p.dev, p.n, p.options = logits, bias, bias_stride, dev, n, a
-  p.keep = (num_options, mask, history, rep, freq, pres, temp)
-  p.native = _native.Rows(dev.index, _FLOATS[logits.dtype], n, a, logits.data_ptr(), logits.stride(0), opt_ptr, mask_ptr, mask_dt, mask_stride, bias_ptr,
-                          bias_dt, bias_stride, hist_ptr, hist_len, hist_stride, rep_ptr, rep_all, freq_ptr, freq_all, pres_ptr, pres_all, temp_ptr,
-                          temp_all, current_stream_handle(dev))
+  p.dev, p.n = dev, n
+  p.tensors = (logits, num_options, mask, bias, history, rep, freq, pres, temp)
+  p.numbers = (rep_all, freq_all, pres_all, temp_all)
+  _bind(p)
   return p
 
 
@@ -213,23 +225,46 @@ def _evaluate_forward(p, action):
 
 
 def _evaluate_backward(ctx, g_lp, g_h):
-  p = ctx.p
-  logits, bias, action, entropy, stats = ctx.saved_tensors[:5]  # (unpacking checks the versions of all that were saved)
+  saved = ctx.saved_tensors
   want_x, want_b = ctx.needs_input_grad[:2]
   if g_lp is None and g_h is None:
     return None, None, None, None
-  g_lp = None if g_lp is None else g_lp.contiguous()
-  g_h = None if g_h is None else g_h.contiguous()
-  grad_x = torch.empty_like(logits, memory_format=torch.contiguous_format) if want_x else None
+  native, dev, where, bias_like, numbers = ctx.call
+  at, same = [], native.dense()
+  for t in saved:
+    if t is None:
+      at.append(0)
+      continue
+    at.append(t.data_ptr())
+    if t.get_device() != where:
+      raise ValueError(f"a saved tensor came back on {t.device}, the others on {dev}")
+    same = same and t.is_contiguous()
+  if not same:  # rows with gaps, or a hook handed back another layout
+    p = _Prepared()
+    p.tensors, p.numbers, p.dev = list(saved[:_SLOTS]), numbers, dev
+    if want_b and len(bias_like[0]) == 2 and bias_like[0][0] > 1:  # its gradient is one per row
+      p.tensors[_BIAS] = _dense(p.tensors[_BIAS])
+    _bind(p)
+    native, saved = p.native, (*p.tensors, *(_dense(t) for t in saved[_SLOTS:]))
+    at = [0 if t is None else t.data_ptr() for t in saved]
+  logits = saved[0]
+  n, a = logits.shape
+  if g_lp is not None and not g_lp.is_contiguous():
+    g_lp = g_lp.contiguous()
+  if g_h is not None and not g_h.is_contiguous():
+    g_h = g_h.contiguous()
+  grad_x = torch.empty((n, a), dtype=logits.dtype, device=dev) if want_x else None
   grad_b, stride = None, 0
   if want_b:
-    grad_b = torch.empty((p.n, p.options) if p.bias_stride else (p.options,), dtype=bias.dtype, device=p.dev)
-    stride = p.options if p.bias_stride else 0
-  ws, ws_ptr, ws_bytes = _scratch(p.native.grad_workspace(want_b), p.dev)
-  p.native.evaluate_grad(action.data_ptr(), entropy.data_ptr(), stats.data_ptr(), 0 if g_lp is None else g_lp.data_ptr(),
-                         0 if g_h is None else g_h.data_ptr(), 0 if grad_x is None else grad_x.data_ptr(), p.options,
-                         0 if grad_b is None else grad_b.data_ptr(), stride, ws_ptr, ws_bytes, current_stream_handle(p.dev))
-  return grad_x, None if grad_b is None else grad_b.view(bias.shape), None, None
+    stride = a if native.bias_per_row() else 0
+    grad_b = torch.empty((n, a) if stride else (a,), dtype=bias_like[1], device=dev)
+  ws, ws_ptr, ws_bytes = _scratch(native.grad_workspace(want_b), dev)
+  native.evaluate_grad(at, 0 if g_lp is None else g_lp.data_ptr(), 0 if g_h is None else g_h.data_ptr(), 0 if grad_x is None else grad_x.data_ptr(), a,
+                       0 if grad_b is None else grad_b.data_ptr(), stride, ws_ptr, ws_bytes, current_stream_handle(dev))
+  return grad_x, None if grad_b is None else grad_b.view(bias_like[0]), None, None
+
+
+_evaluate_backward_once = torch.autograd.function.once_differentiable(_evaluate_backward)
 
 
 class _Evaluate(torch.autograd.Function):
@@ -238,19 +273,16 @@ class _Evaluate(torch.autograd.Function):
   def forward(ctx, logits, bias, action, p):
     log_prob, entropy, stats = _evaluate_forward(p, action)
     ctx.set_materialize_grads(False)
-    # (the native struct holds addresses: every tensor behind it is saved, so that torch notices one that was
-    # changed in place before the backward pass, and frees it after)
-    ctx.save_for_backward(logits, bias, action, entropy, stats, *[t for t in (p.logits, p.bias, *p.keep) if t is not None])
-    p.logits = p.bias = p.keep = None
-    ctx.p = p
+    # every tensor that the backward pass reads is saved, so that torch notices one that was changed in place, hands it
+    # to its hooks (offloading, checkpoints) and frees it after. The native struct stays for its sizes; the backward
+    # pass puts the addresses of what it is handed in place of the forward pass'
+    ctx.save_for_backward(*p.tensors, action, entropy, stats)
+    ctx.call = (p.native, p.dev, action.get_device(), None if bias is None else (bias.shape, bias.dtype), p.numbers)
     return log_prob, entropy
 
   @staticmethod
   def backward(ctx, g_lp, g_h):
     return _run_backward(_evaluate_backward, _evaluate_backward_once, ctx, g_lp, g_h)
-
-
-_evaluate_backward_once = torch.autograd.function.once_differentiable(_evaluate_backward)
 
 
 def evaluate(logits, action, *, num_options=None, mask=None, bias=None, history=None, repetition=1.0, frequency=0.0, presence=0.0, temperature=1.0):
@@ -269,9 +301,9 @@ def evaluate(logits, action, *, num_options=None, mask=None, bias=None, history=
   if not action.is_contiguous():
     action = action.contiguous()
   if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
-    # (of the two that are differentiated only the copies that the kernels read instead)
-    p.logits = None if p.logits is logits else p.logits.detach()
-    p.bias = None if p.bias is bias else p.bias.detach()
+    # (copies that were laid out for the kernels are no part of the graph: the gradients are those of the originals)
+    if p.tensors[0] is not logits or p.tensors[_BIAS] is not bias:
+      p.tensors = tuple(t.detach() if i in (0, _BIAS) and t is not None else t for i, t in enumerate(p.tensors))
     nodes = _guard_capture(logits, bias)  # noqa: F841
     return _Evaluate.apply(logits, bias, action, p)
   return _evaluate_forward(p, action)[:2]

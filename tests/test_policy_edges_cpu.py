@@ -1,0 +1,101 @@
+"""CPU: edges of the policy-side operators that show without a GPU - what a stand-in for the native module is handed, what
+Python refuses before anything touches a device."""
+import types
+
+import pytest
+import torch
+
+
+class _FakeRows:
+  """Takes the native struct's place: notes the addresses that a call would follow."""
+  calls = []
+
+  def __init__(self, dev, dtype, rows, options, logits, logits_stride, num_options, mask, mask_dtype, mask_stride, bias, bias_dtype, bias_stride, history,
+               history_len, history_stride, rep, rep_all, freq, freq_all, pres, pres_all, temp, temp_all, stream):
+    self.at = {"logits": logits, "num_options": num_options, "mask": mask, "bias": bias, "history": history, "repetition": rep, "frequency": freq,
+               "presence": pres, "temperature": temp}
+    self.strides = {"logits": logits_stride, "mask": mask_stride, "bias": bias_stride, "history": history_stride}
+    self.is_dense = logits_stride == options and mask_stride in (0, options) and bias_stride in (0, options) and history_stride in (0, history_len)
+
+  def evaluate_workspace(self):
+    return 0
+
+  def grad_workspace(self, with_bias):
+    return 0
+
+  def evaluate(self, *args):
+    pass
+
+  def dense(self):
+    return self.is_dense
+
+  def bias_per_row(self):
+    return self.strides["bias"] != 0
+
+  def evaluate_grad(self, at_now, *rest):
+    names = ("logits", "num_options", "mask", "bias", "history", "repetition", "frequency", "presence", "temperature", "action", "entropy", "stats")
+    _FakeRows.calls.append((dict(zip(names, at_now)), self.strides))
+
+
+@pytest.fixture
+def stand_in(monkeypatch):
+  from envpool_amd import policy
+  monkeypatch.setattr(policy, "_same_device", lambda dev, **tensors: None)
+  monkeypatch.setattr(policy, "current_stream_handle", lambda dev: 0)
+  monkeypatch.setattr(policy, "_guard_capture", lambda *inputs: ())
+  monkeypatch.setattr(policy, "_native", types.SimpleNamespace(Rows=_FakeRows))
+  _FakeRows.calls = []
+  return policy
+
+
+def _operands(n, a):
+  g = torch.Generator().manual_seed(0)
+  return dict(num_options=torch.full((n,), a, dtype=torch.int32), mask=torch.ones(n, a, dtype=torch.bool), bias=torch.randn(n, a, generator=g).requires_grad_(),
+              history=torch.randint(0, a, (n, 4), generator=g, dtype=torch.int32), repetition=torch.full((n,), 1.2), frequency=torch.zeros(n),
+              presence=torch.zeros(n), temperature=torch.ones(n))
+
+
+@pytest.mark.parametrize("layout", ["dense", "columns"])
+def test_the_backward_pass_of_evaluate_reads_what_autograd_hands_back(stand_in, layout):
+  """Under a hook for saved tensors (checkpoints and offloading are such hooks) the forward pass' own tensors may be gone:
+  every address that the backward pass follows is that of a tensor that the hook gave back."""
+  n, a = 3, 10
+  kw = _operands(n, a)
+  leaf = torch.randn(n, a).requires_grad_()
+  logits = leaf if layout == "dense" else torch.randn(a, n).requires_grad_().t()
+  given = []
+
+  def unpack(packed):
+    given.append(packed.clone())
+    return given[-1]
+
+  with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(), unpack):
+    lp, ent = stand_in.evaluate(logits, torch.zeros(n, dtype=torch.int32), **kw)
+  (lp.sum() + ent.sum()).backward()
+  (at, strides), = _FakeRows.calls
+  alive = {t.data_ptr() for t in given}
+  assert all(ptr in alive for ptr in at.values()), {k: ptr in alive for k, ptr in at.items()}
+  assert strides == {"logits": a, "mask": a, "bias": a, "history": 4}
+
+
+def test_a_hook_may_hand_back_another_layout(stand_in):
+  n, a = 3, 10
+  kw = _operands(n, a)
+  logits = torch.randn(n, a).requires_grad_()
+  kw["mask"] = kw["mask"][:1].expand(n, a)  # one mask for all rows: comes back as a row each
+
+  def unpack(packed):
+    return packed.t().contiguous().t() if packed.dim() == 2 else packed.clone()
+
+  with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(), unpack):
+    lp, ent = stand_in.evaluate(logits, torch.zeros(n, dtype=torch.int32), **kw)
+  (lp.sum() + ent.sum()).backward()
+  (_, strides), = _FakeRows.calls
+  assert strides == {"logits": a, "mask": a, "bias": a, "history": 4}
+  # rows with gaps come back without them
+  kw["mask"] = torch.ones(n, a + 6, dtype=torch.bool)[:, 2:a + 2]
+  with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(), lambda t: t.clone()):
+    lp, ent = stand_in.evaluate(logits, torch.zeros(n, dtype=torch.int32), **kw)
+  (lp.sum() + ent.sum()).backward()
+  assert _FakeRows.calls[1][1] == {"logits": a, "mask": a, "bias": a, "history": 4}
+  assert logits.grad.shape == (n, a) and kw["bias"].grad.shape == (n, a)

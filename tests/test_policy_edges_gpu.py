@@ -89,3 +89,81 @@ def test_states_keep_32_bits_over_many_chunks(case, dtype):
     tol = size[name] * H32 * (4 + 38 + t + 3 * (t / 32 + 1) + 4) + 2.0**-30
     assert (err <= tol).all(), (name, float((err - tol).max()))
     assert float((x - w).norm()) <= 32 * H32 * float(w.norm()), (name, float((x - w).norm() / w.norm()))
+
+
+# ---- what autograd may do between the forward and the backward pass ---------------------------------
+def _clone_hooks():
+  return torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(), lambda t: t.clone())
+
+
+def _checkpointed(call):
+  from torch.utils.checkpoint import checkpoint
+  return checkpoint(call, use_reentrant=False)
+
+
+HOOKS = {
+  "clone": lambda call: _under(_clone_hooks(), call),
+  "save_on_cpu": lambda call: _under(torch.autograd.graph.save_on_cpu(), call),
+  "checkpoint": _checkpointed,
+}
+
+
+def _under(context, call):
+  with context:
+    return call()
+
+
+def _spoil():
+  """Fills the allocator's free memory, so that what was freed no longer holds what it held."""
+  spoiled = [torch.full((1 << 16,), 7, dtype=torch.int32, device=DEV) for _ in range(24)] + [torch.full((2048,), 7, dtype=torch.int32, device=DEV) for _ in range(64)]
+  torch.cuda.synchronize()
+  del spoiled
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hook", list(HOOKS))
+@pytest.mark.parametrize("a", [24, 5000])
+def test_gradients_under_hooks_for_saved_tensors(a, hook, dtype):
+  """Everything the backward pass reads comes from what was saved: the same bits as without the hook."""
+  from envpool_amd import policy
+  g = _gen(a)
+  n = 40
+  x = torch.randn(n, a, generator=g).to(dtype).to(DEV).requires_grad_()
+  b = torch.randn(n, a, generator=g).to(DEV).requires_grad_()
+  mask = torch.rand(n, a, generator=g) < 0.6
+  hist = torch.randint(0, a, (n, 9), generator=g, dtype=torch.int32)
+  rows = [(0.5 + torch.rand(n, generator=g)).to(DEV) for _ in range(4)]
+  action = mask.int().argmax(1).int()
+  g1, g2 = torch.randn(n, generator=g).to(DEV), torch.randn(n, generator=g).to(DEV)
+
+  def call():  # (operands that live only as long as the call: the saved ones are the last)
+    kw = dict(mask=mask.to(DEV), num_options=torch.full((n,), a - 1, dtype=torch.int32, device=DEV), history=hist.to(DEV), bias=b * 1.0,
+              repetition=rows[0].clone(), frequency=rows[1].clone(), presence=rows[2].clone(), temperature=rows[3].clone())
+    return policy.evaluate(x * 1.0, action.to(DEV), **kw)
+
+  def run(through):
+    lp, ent = through(call)
+    _spoil()
+    return [lp.detach(), ent.detach(), *torch.autograd.grad([lp, ent], [x, b], [g1, g2])]
+
+  want = run(lambda c: c())
+  got = run(HOOKS[hook])
+  assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("hook", list(HOOKS))
+def test_gradients_of_a_scan_under_hooks_for_saved_tensors(hook):
+  from envpool_amd import policy
+  q, k, v, decay, fresh, state, do, ds = (x.to(DEV) for x in _scan_problem(130, 3, 4, 2, 32, 48, 0.02, torch.bfloat16))
+  leaves = [x.requires_grad_() for x in (q, k, v, state)]
+
+  def call():
+    return policy.memory_scan(*(x * 1.0 for x in leaves[:3]), decay.clone(), fresh=fresh.clone(), state=leaves[3] * 1.0)
+
+  def run(through):
+    out, final = through(call)
+    _spoil()
+    return [out.detach(), final.detach(), *torch.autograd.grad([out, final], leaves, [do, ds])]
+
+  want = run(lambda c: c())
+  assert all(torch.equal(p, w) for p, w in zip(run(HOOKS[hook]), want))
