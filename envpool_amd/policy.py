@@ -320,7 +320,9 @@ class EnvMemory:
 
   `log_decay` float32 `[num_heads]` on the GPU, values <= 0 (not differentiated). `state`: an existing
   `[num_envs, num_heads, key_dim, value_dim]` float32 tensor to work on (dense); made, all zero, when None.
-  Dimensions 1 to 256. Steps of one memory are ordered by the caller (one stream)."""
+  Dimensions 1 to 256. Steps of one memory are ordered by the caller (one stream). A step changes `state` in place, and
+  autograd is told so: a `memory_scan` that starts from it and is differentiated after another step needs a copy
+  (`memory.state.clone()`), without one its backward pass raises. (Replays of a captured step go unnoticed.)"""
 
   def __init__(self, num_envs: int, num_heads: int, key_dim: int, value_dim: int, log_decay: torch.Tensor, *, state: Optional[torch.Tensor] = None,
                env_id_offset: int = 0):
@@ -403,6 +405,7 @@ class EnvMemory:
                        v.stride(1), out.data_ptr(), out.stride(0), out.stride(1), 0 if env_id is None else env_id.data_ptr(),
                        0 if first is None else first.data_ptr(), _MASKS[first.dtype] if first is not None else 0,
                        self.key_dim ** -0.5 if scale is None else float(scale), ws_ptr, ws_bytes, current_stream_handle(dev))
+      torch.autograd.graph.increment_version(self.state)  # (the kernel's writes are an in-place operation)
     return out
 
 

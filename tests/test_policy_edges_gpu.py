@@ -167,3 +167,27 @@ def test_gradients_of_a_scan_under_hooks_for_saved_tensors(hook):
 
   want = run(lambda c: c())
   assert all(torch.equal(p, w) for p, w in zip(run(HOOKS[hook]), want))
+
+
+def test_a_step_between_a_scan_and_its_backward_pass_is_noticed():
+  """The state that a scan started from has moved on: an error, not the gradients of another start."""
+  from envpool_amd import policy
+  g = _gen(3)
+  q, k, v = (torch.randn(20, 3, 2, 8, generator=g).to(DEV) for _ in range(3))
+  decay = torch.tensor([-0.1, -0.2], device=DEV)
+  table = torch.randn(3, 2, 8, 8, generator=g).to(DEV)
+  for start in ("memory", "caller"):  # the memory's own view of it, and the tensor that the caller made the memory from
+    memory = policy.EnvMemory(3, 2, 8, 8, decay, state=table)
+    leaf = q.clone().requires_grad_()
+    before = table.clone()
+    out, _ = policy.memory_scan(leaf, k, v, decay, state=memory.state if start == "memory" else table)
+    kept, _ = policy.memory_scan(leaf, k, v, decay, state=before)
+    memory.step(q[0], k[0], v[0])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+      out.sum().backward()
+    kept.sum().backward()
+    assert torch.isfinite(leaf.grad).all()
+  with torch.inference_mode():
+    memory = policy.EnvMemory(3, 2, 8, 8, decay)
+    memory.step(q[0], k[0], v[0])
+  memory.step(q[0], k[0], v[0])
