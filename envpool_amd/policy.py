@@ -17,6 +17,7 @@ import math
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from ._loader import load_library
 
@@ -42,6 +43,15 @@ def _same_device(dev, **tensors):
   for name, t in tensors.items():
     if t is not None and t.device != dev:
       raise ValueError(f"{name} is on {t.device}, the others on {dev}")
+
+
+def _no_tangents(call, **tensors):
+  """Forward-mode derivatives have no formula here: a dual number is refused rather than stripped of its tangent."""
+  if forward_ad._current_level < 0:
+    return
+  for name, t in tensors.items():
+    if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+      raise ValueError(f"{call} has no forward-mode derivative: {name} is a dual number")
 
 
 def _row_operand(t, name, rows, cols):
@@ -287,11 +297,12 @@ class _Evaluate(torch.autograd.Function):
 
 def evaluate(logits, action, *, num_options=None, mask=None, bias=None, history=None, repetition=1.0, frequency=0.0, presence=0.0, temperature=1.0):
   """(log_prob, entropy), float32 `[B]` each, of stored actions under the distribution that `choose`
-  describes, differentiable in `logits` and `bias` (once).
+  describes, differentiable in `logits` and `bias` (once, backwards: dual numbers are refused).
 
   `action` int32 `[B]`: -1 (what `choose` gives a row with nothing to choose) has log_prob 0 and no gradient, an
   illegal option -inf, a value outside [-1, A) NaN. The statistics of a row and the gradients' sums are kept in
   32 bits; gradients come in the type of the tensor they belong to."""
+  _no_tangents("evaluate", logits=logits, bias=bias, repetition=repetition, frequency=frequency, presence=presence, temperature=temperature)
   if bias is not None and bias.requires_grad and bias.dim() == 2 and bias.shape[0] > 1 and bias.stride(0) == 0:
     bias = bias.contiguous()  # one row of biases expanded by the caller: its gradient is one per row
   p = _prepare(logits, num_options, mask, bias, history, repetition, frequency, presence, temperature)
@@ -514,10 +525,11 @@ def memory_scan(q, k, v, log_decay, *, fresh=None, state=None, scale: Optional[f
   `log_decay` float32 `[H]`, values <= 0, not differentiated. `fresh` bool / uint8 `[T, B]`: steps at which an
   episode starts, so that nothing from before reaches them (None: no such step). `state` float32
   `[B, H, key_dim, value_dim]`: where the rows start (None: zero). Dimensions 1 to 128.
-  Differentiable (once) in q, k, v and state; gradients come in the type of the tensor they belong to. States and sums
+  Differentiable (once, backwards: dual numbers are refused) in q, k, v and state; gradients come in the type of the tensor they belong to. States and sums
   are kept in 32 bits. As operands of 16-bit products the states and the scores of a chunk enter as two pieces of the type
   (16 bits together in bfloat16, 22 in float16), so that outputs and gradients are in effect rounded once, at the end;
   those of heads that share keys and values are summed in 32 bits before."""
+  _no_tangents("memory_scan", q=q, k=k, v=v, log_decay=log_decay, state=state)
   if q.dtype not in _FLOATS or k.dtype != q.dtype or v.dtype != q.dtype:
     raise ValueError(f"q, k, v must be of one type, float32, float16 or bfloat16, got {q.dtype}, {k.dtype}, {v.dtype}")
   if q.dim() != 4 or q.shape[2] < 1:

@@ -99,3 +99,24 @@ def test_a_hook_may_hand_back_another_layout(stand_in):
   (lp.sum() + ent.sum()).backward()
   assert _FakeRows.calls[1][1] == {"logits": a, "mask": a, "bias": a, "history": 4}
   assert logits.grad.shape == (n, a) and kw["bias"].grad.shape == (n, a)
+
+
+def test_dual_numbers_are_refused(stand_in):
+  """Forward-mode derivatives: refused, where they were lost without a word (nothing here requires a gradient)."""
+  import torch.autograd.forward_ad as fw
+  x, act = torch.randn(3, 4), torch.zeros(3, dtype=torch.int32)
+  with fw.dual_level():
+    dual = lambda *shape: fw.make_dual(torch.randn(*shape), torch.randn(*shape))  # noqa: E731
+    for kw in (dict(logits=dual(3, 4)), dict(logits=x, bias=dual(4)), dict(logits=x, temperature=dual(3)), dict(logits=dual(3, 4).requires_grad_())):
+      with pytest.raises(ValueError, match="forward-mode"):
+        stand_in.evaluate(action=act, **kw)
+    stand_in.evaluate(x, act)
+    q = torch.randn(5, 2, 1, 4)
+    for i in range(3):
+      qkv = [dual(5, 2, 1, 4) if i == j else q for j in range(3)]
+      with pytest.raises(ValueError, match="forward-mode"):
+        stand_in.memory_scan(*qkv, torch.zeros(1))
+    with pytest.raises(ValueError, match="forward-mode.*state"):
+      stand_in.memory_scan(q, q, q, torch.zeros(1), state=dual(2, 1, 4, 4))
+    with pytest.raises(ValueError, match="forward-mode.*log_decay"):
+      stand_in.memory_scan(q, q, q, dual(1))
