@@ -70,6 +70,8 @@ def _penalty(v, name, rows):
   if isinstance(v, torch.Tensor):
     if v.dtype != torch.float32 or v.shape != (rows,):
       raise ValueError(f"{name} must be a number or a float32 tensor [{rows}], got {v.dtype} {list(v.shape)}")
+    if v.requires_grad and torch.is_grad_enabled():
+      raise ValueError(f"{name} is not differentiated: pass {name}.detach()")
     return v, 1.0
   return None, float(v)
 
@@ -297,7 +299,8 @@ class _Evaluate(torch.autograd.Function):
 
 def evaluate(logits, action, *, num_options=None, mask=None, bias=None, history=None, repetition=1.0, frequency=0.0, presence=0.0, temperature=1.0):
   """(log_prob, entropy), float32 `[B]` each, of stored actions under the distribution that `choose`
-  describes, differentiable in `logits` and `bias` (once, backwards: dual numbers are refused).
+  describes, differentiable in `logits` and `bias` (once, backwards: dual numbers are refused, and so are per-row
+  numbers that require a gradient).
 
   `action` int32 `[B]`: -1 (what `choose` gives a row with nothing to choose) has log_prob 0 and no gradient, an
   illegal option -inf, a value outside [-1, A) NaN. The statistics of a row and the gradients' sums are kept in

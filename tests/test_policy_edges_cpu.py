@@ -120,3 +120,15 @@ def test_dual_numbers_are_refused(stand_in):
       stand_in.memory_scan(q, q, q, torch.zeros(1), state=dual(2, 1, 4, 4))
     with pytest.raises(ValueError, match="forward-mode.*log_decay"):
       stand_in.memory_scan(q, q, q, dual(1))
+
+
+@pytest.mark.parametrize("name", ["repetition", "frequency", "presence", "temperature"])
+def test_per_row_numbers_that_require_a_gradient_are_refused(stand_in, name):
+  """A learned temperature would be left without its gradient, in silence."""
+  x, act = torch.randn(3, 4).requires_grad_(), torch.zeros(3, dtype=torch.int32)
+  number = torch.ones(3).requires_grad_()
+  with pytest.raises(ValueError, match=f"{name} is not differentiated"):
+    stand_in.evaluate(x, act, **{name: number})
+  stand_in.evaluate(x, act, **{name: number.detach()})
+  with torch.no_grad():
+    stand_in.evaluate(x, act, **{name: number})
