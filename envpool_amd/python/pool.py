@@ -431,10 +431,17 @@ class EnvPoolFrontEnd:
   def send_choice(self, choice) -> None:
     """Sends the actions of a `Choice` (`choose_torch`) to the envs of the batch received last. The actions
     cross to the host (the duel engine is there): this waits for them. A row without a legal option (-1: an
-    ended duel, which is reset whatever it is sent) sends 0."""
+    ended duel, which is reset whatever it is sent) sends 0. A row whose logits were NaN or infinite (-1 with a
+    log_prob that is NaN) raises, and nothing is sent."""
     if not hasattr(self, "last_env_ids"):
       raise RuntimeError(f"send_choice: {type(self).__name__} does not note the env ids of the last batch")
-    self.send(choice.action.clamp_min(0), self.last_env_ids)
+    env_ids = self.last_env_ids
+    action = choice.action.masked_fill(choice.log_prob.isnan(), -2).cpu().numpy()  # (one crossing for both)
+    bad = np.flatnonzero(action == -2)
+    if len(bad):
+      raise RuntimeError(f"send_choice: {len(bad)} rows have no distribution, their logits hold NaN or +inf (first: row {bad[0]}, "
+                         f"env {env_ids[bad[0]]})")
+    self.send(np.maximum(action, 0), env_ids)
 
   def __repr__(self) -> str:
     cfg = ", ".join(f"{k}={pprint.pformat(v)}" for k, v in self.config.items())

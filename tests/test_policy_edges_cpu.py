@@ -132,3 +132,28 @@ def test_per_row_numbers_that_require_a_gradient_are_refused(stand_in, name):
   stand_in.evaluate(x, act, **{name: number.detach()})
   with torch.no_grad():
     stand_in.evaluate(x, act, **{name: number})
+
+
+def test_send_choice_tells_rows_without_options_from_rows_without_a_distribution():
+  """-1 with log_prob 0 is an ended duel and sends 0; -1 with a NaN is a policy that has diverged, and sends nothing."""
+  import numpy as np
+
+  from envpool_amd.policy import Choice
+  from envpool_amd.python.pool import EnvPoolFrontEnd
+
+  class Pool(EnvPoolFrontEnd):
+    last_env_ids = np.array([7, 3, 5], np.int32)
+
+    def __init__(self):
+      self.sent = []
+
+    def send(self, action, env_id=None):
+      self.sent.append((np.asarray(action).tolist(), np.asarray(env_id).tolist()))
+
+  pool = Pool()
+  action = torch.tensor([2, -1, 4], dtype=torch.int32)
+  pool.send_choice(Choice(action, torch.tensor([-0.5, 0.0, -1.0]), torch.zeros(3)))
+  assert pool.sent == [([2, 0, 4], [7, 3, 5])]
+  with pytest.raises(RuntimeError, match="1 rows.*row 1, env 3"):
+    pool.send_choice(Choice(action, torch.tensor([-0.5, float("nan"), -1.0]), torch.zeros(3)))
+  assert len(pool.sent) == 1
