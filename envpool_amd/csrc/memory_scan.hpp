@@ -177,7 +177,7 @@ struct Parts {
   int64_t seg_len;     // steps per part of the time axis (whole chunks), blockIdx.y counts parts in time
   int32_t n_seg;
   f32x4* ws_state;     // [row * heads][n_seg][DK * DV / 4] in accumulator order: what a part starts from (read), or
-  float* ws_carry;     // its own contribution and how far it lets the state before it through (written)
+  float* ws_carry;     // its own contribution and how far it lets the state before it through, -1: not at all (written)
   int32_t state_only;  // the first of two passes over split time: contributions only
   int32_t state_vec;   // state_in's rows are 16-byte pieces when its key stride is 1
 };
@@ -211,6 +211,16 @@ template <class T> __device__ inline uint32_t top_bits(uint32_t top, uint32_t x)
     return top > y ? top : y;
   }
 }
+// `odd` plus 0 times every value of x: 0, or NaN where one is not finite. One instruction a word, whose products are exact
+__device__ inline float plus_nothing(float odd, uint32_t x, bf16) {
+  typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, x), bf16x2{(bf16)0.f, (bf16)0.f}, odd, false);
+}
+__device__ inline float plus_nothing(float odd, uint32_t x, f16) {
+  typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, x), f16x2{(f16)0.f, (f16)0.f}, odd, false);
+}
+__device__ inline float plus_nothing(float odd, uint32_t x, float) { return __builtin_fmaf(__builtin_bit_cast(float, x), 0.f, odd); }
 template <class T> __device__ inline bool not_finite(uint32_t top) {
   if constexpr (sizeof(T) == 2) return (top & 0xffffu) >= Mma<T>::kInf || (top >> 16) >= Mma<T>::kInf;
   else return top >= Mma<T>::kInf;
@@ -294,15 +304,36 @@ template <class T, int DK, int DV, bool kAligned, bool rev> struct Walk {
 #pragma unroll
     for (int i = 0; i < count; ++i) *(uint4*)(to + i * (256 / per_row) * stride) = r[i];
   }
-  static __device__ uint32_t top_of(uint32_t top, const uint4* r, int count) {
+  // marks the steps of a chunk (bit t of the two words) whose keys or values are not finite; nearly always none
+  static __device__ void mark_sick(const uint4* k, int count_k, const uint4* v, int count_v, uint32_t* sick) {
+    float odd[2] = {0.f, 0.f};
+    const auto look = [&](const uint4* r, int count) {
 #pragma unroll
-    for (int i = 0; i < count; ++i) {
-      top = top_bits<T>(top, r[i].x);
-      top = top_bits<T>(top, r[i].y);
-      top = top_bits<T>(top, r[i].z);
-      top = top_bits<T>(top, r[i].w);
-    }
-    return top;
+      for (int i = 0; i < count; ++i) {
+        odd[0] = plus_nothing(odd[0], r[i].x, T{});
+        odd[1] = plus_nothing(odd[1], r[i].y, T{});
+        odd[0] = plus_nothing(odd[0], r[i].z, T{});
+        odd[1] = plus_nothing(odd[1], r[i].w, T{});
+      }
+    };
+    look(k, count_k);
+    look(v, count_v);
+    if (odd[0] + odd[1] == 0.f) return;
+    const auto mark = [&](const uint4* r, int count, int padded) {
+      const int per_row = padded / kVec;
+#pragma unroll
+      for (int i = 0; i < count; ++i) {
+        const int t = threadIdx.x / per_row + i * (256 / per_row);
+        const uint32_t top = top_bits<T>(top_bits<T>(top_bits<T>(top_bits<T>(0, r[i].x), r[i].y), r[i].z), r[i].w);
+        if (not_finite<T>(top)) atomicOr(&sick[t >> 5], 1u << (t & 31));
+      }
+    };
+    mark(k, count_k, DK);
+    mark(v, count_v, DV);
+  }
+  static __device__ uint64_t marked(const uint32_t* sick) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(sick[0]), hi = __builtin_amdgcn_readfirstlane(sick[1]);
+    return (uint64_t)hi << 32 | lo;
   }
 
   static __device__ void load_state(const Scan& p, bool state_vec, int64_t row, int h, int lane, int wave, State& s) {
@@ -354,14 +385,15 @@ template <class T, int DK, int DV, bool kAligned, bool rev> struct Walk {
       }
   }
 
-  // the weights of the chunk's steps: in the state that leaves it, and of the state that enters it in their outputs
+  // the weights of the chunk's steps: in the state that leaves it, and of the state that enters it in their outputs (NaN:
+  // it does not reach them, which a weight that is 0 for its smallness must not be taken for where the state is infinite)
   static __device__ void weights(const Scan& p, const Now& c) {
     if (threadIdx.x < 2 * kChunk) {
       const int t = threadIdx.x % kChunk;
       const uint64_t until = c.starts & ((2ull << t) - 1), later = t < 63 ? c.starts >> (t + 1) : 0;
       const float from_0 = __builtin_amdgcn_exp2f(c.l2 * (t + 1)), to_end = __builtin_amdgcn_exp2f(c.l2 * (c.n - 1 - t));
       if (threadIdx.x < kChunk) c.w_up[t] = t < c.n && (rev ? until : later) == 0 ? (rev ? from_0 : to_end) * (M::kNarrow ? 1.f : p.inc_scale) : 0.f;
-      else c.w_in[t] = t < c.n && (rev ? later : until) == 0 ? (rev ? to_end : from_0) * p.out_scale : 0.f;
+      else c.w_in[t] = t < c.n && (rev ? later : until) == 0 ? (rev ? to_end : from_0) * p.out_scale : __builtin_nanf("");
     }
   }
 
@@ -521,7 +553,7 @@ template <class T, int DK, int DV, bool kAligned, bool rev> struct Walk {
 #pragma unroll
       for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) a[b][j][r] = w != 0.f ? a[b][j][r] * ws_ : 0.f;
+        for (int r = 0; r < 4; ++r) a[b][j][r] = w == w ? a[b][j][r] * ws_ : 0.f;
 #pragma unroll
       for (int k = 0; k < kChunk / K; ++k)
         if (rev ? (k + 1) * K > 16 * b : k * K <= 16 * b) {
@@ -624,12 +656,18 @@ template <class T, int DK, int DV, bool kAligned, bool rev> struct Walk {
   }
 };
 
-// where a chunk that holds the start of an episode and something that is not finite ends: 0 * inf would carry it
-// across, so the chunk keeps its outer episode only and the rest is a chunk of its own
-template <bool rev> __device__ inline void cut_chunk(uint64_t starts, int64_t& start, int& n) {
+// Where a chunk that holds something not finite ends. The products inside a chunk run over all of its steps, those that
+// do not reach a result with the weight 0, and 0 * inf is NaN. So a chunk with a sick step ends where an episode does, and
+// at the sick step: forward in time it starts one (and reaches all later steps, as it should), back in time it ends one.
+template <bool rev> __device__ inline void cut_chunk(uint64_t starts, uint64_t sick, int64_t& start, int& n) {
   int from = 0, to = n;
-  if (rev) from = 63 - __clzll(starts);
-  else if ((starts & ~1ull) != 0) to = __ffsll((unsigned long long)(starts & ~1ull)) - 1;
+  if (rev) {
+    const uint64_t before_last = sick & ((1ull << (n - 1)) - 1);
+    from = max(starts ? 63 - __clzll(starts) : 0, before_last ? 64 - __clzll(before_last) : 0);
+  } else {
+    const uint64_t ends = (starts | sick) & ~1ull;
+    if (ends) to = __ffsll((unsigned long long)ends) - 1;
+  }
   start += from;
   n = to - from;
 }
@@ -653,7 +691,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
   c.w_up = (float*)(ps + kChunk * Tile::SP);
   c.w_in = c.w_up + kChunk;
   c.p_top = c.w_in + kChunk;             // kNarrow: what a step's scores were multiplied by
-  int* odd = (int*)(c.p_top + kChunk);   // a key or value of this chunk is not finite
+  uint32_t* sick = (uint32_t*)(c.p_top + kChunk);  // steps of this chunk whose key or value is not finite, two words of bits
 
   const int64_t rh = blockIdx.x;
   const int64_t row = rh / p.heads;
@@ -689,7 +727,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
 
   int64_t start = rev ? seg1 - (seg1 - seg0 < kChunk ? seg1 - seg0 : kChunk) : seg0;
   int n = (int)(seg1 - seg0 < kChunk ? seg1 - seg0 : kChunk);
-  if (threadIdx.x == 0) *odd = 0;
+  if (threadIdx.x < 2) sick[threadIdx.x] = 0;
   if (n > 0) load(start, n);
 
   // ---- the state the part starts from
@@ -707,7 +745,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
   } else if (!parts.state_only && p.state_in) {
     W::load_state(p, parts.state_vec, row, h, lane, c.wave, s);
   }
-  float through = 1.f;
+  float through = 1.f;  // how far the part lets the state before it through, -1: not at all (an episode starts)
 
   while (n > 0) {
     // (opaque to the compiler here, or it would keep every step's powers of the decay, and every address, in
@@ -718,12 +756,12 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
     __syncthreads();  // (the tiles of the chunk before have been read)
     put();
     c.starts = __ballot(rf != 0);
-    if (c.starts && not_finite<T>(W::top_of(W::top_of(0, rk, Tile::kQ), rv, Tile::kV))) *odd = 1;
+    W::mark_sick(rk, Tile::kQ, rv, Tile::kV, sick);
     __syncthreads();
-    if (c.starts && *odd) {
+    if (const uint64_t bad = W::marked(sick)) {
       __syncthreads();
-      if (threadIdx.x == 0) *odd = 0;
-      cut_chunk<rev>(c.starts, start, n);
+      if (threadIdx.x < 2) sick[threadIdx.x] = 0;
+      cut_chunk<rev>(c.starts, bad, start, n);
       load(start, n);
       put();
       c.starts = __ballot(rf != 0);
@@ -738,7 +776,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
     if (n > 0) load(start, n);
 
     W::weights(p, c);
-    through = c.starts ? 0.f : through * __builtin_amdgcn_exp2f(c.l2 * c.n);
+    through = c.starts || through < 0.f ? -1.f : through * __builtin_amdgcn_exp2f(c.l2 * c.n);
     if (!parts.state_only) {
       typename W::Outs a;
       typename W::Seconds second;
@@ -796,7 +834,7 @@ template <class T> __global__ __launch_bounds__(256, 3) void scan_pair(Scan a, S
   c.w_up = (float*)(ps + kChunk * Tile::SP);
   c.w_in = c.w_up + kChunk;
   c.p_top = c.w_in + kChunk;
-  int* odd = (int*)(c.p_top + kChunk);
+  uint32_t* sick = (uint32_t*)(c.p_top + kChunk);
 
   const int64_t row = blockIdx.x / a.heads;
   const int h = (int)(blockIdx.x % a.heads);
@@ -827,7 +865,7 @@ template <class T> __global__ __launch_bounds__(256, 3) void scan_pair(Scan a, S
   };
   int n = (int)(a.steps < kChunk ? a.steps : kChunk);
   int64_t start = a.steps - n;
-  if (threadIdx.x == 0) *odd = 0;
+  if (threadIdx.x < 2) sick[threadIdx.x] = 0;
   if (n > 0) load(start, n);
   typename W::State sa, sb;
 #pragma unroll
@@ -842,12 +880,12 @@ template <class T> __global__ __launch_bounds__(256, 3) void scan_pair(Scan a, S
     __syncthreads();
     put();
     c.starts = __ballot(rf != 0);
-    if (c.starts && not_finite<T>(W::top_of(W::top_of(0, rq, N), rg, N))) *odd = 1;
+    W::mark_sick(rq, N, rg, N, sick);
     __syncthreads();
-    if (c.starts && *odd) {
+    if (const uint64_t bad = W::marked(sick)) {
       __syncthreads();
-      if (threadIdx.x == 0) *odd = 0;
-      cut_chunk<true>(c.starts, start, n);
+      if (threadIdx.x < 2) sick[threadIdx.x] = 0;
+      cut_chunk<true>(c.starts, bad, start, n);
       load(start, n);
       put();
       c.starts = __ballot(rf != 0);
@@ -917,7 +955,7 @@ template <int DK, int DV> __global__ __launch_bounds__(256) void join_parts(Scan
       if (n < parts.n_seg) ws[(int64_t)seg * (DK * DV / 4)] = s;
       if (n + 1 < parts.n_seg) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[r] = (carry[i] != 0.f ? s[r] * carry[i] : 0.f) + own[i][r];
+        for (int r = 0; r < 4; ++r) s[r] = (carry[i] < 0.f ? 0.f : s[r] * carry[i]) + own[i][r];
       }
     }
   }

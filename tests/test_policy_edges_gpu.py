@@ -191,3 +191,37 @@ def test_a_step_between_a_scan_and_its_backward_pass_is_noticed():
     memory = policy.EnvMemory(3, 2, 8, 8, decay)
     memory.step(q[0], k[0], v[0])
   memory.step(q[0], k[0], v[0])
+
+
+# ---- values that are not finite ----------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("filler", [math.inf, math.nan])
+@pytest.mark.parametrize("case", [(150, 4, 2, 2, 64, 64), (150, 4, 2, 1, 33, 21), (140, 530, 2, 2, 64, 48), (700, 4, 2, 2, 128, 128), (16, 4, 2, 2, 32, 32)],
+                         ids=lambda c: "-".join(str(x) for x in c))
+def test_what_is_not_finite_goes_where_the_recurrence_takes_it(case, filler, dtype):
+  """A query, key, value or gradient that is not finite, in a row each: later steps of its episode have it in their state,
+  earlier ones do not (and the other way round in the gradients), whatever shares a chunk with it. Everything else is
+  within the bound of test_results_in_16_bits_are_rounded_once; in 32 bits the same without its pieces."""
+  t, n, h, hk, dk, dv = case
+  q, k, v, decay, _, state, do, ds = _scan_problem(*case, 0.0, dtype)
+  fresh = torch.zeros(t, n, dtype=torch.bool)
+  at = 5 * t // 8  # inside a chunk of 32 and of 64
+  for row in range(4):
+    fresh[[at - 3, t - 2], row] = row % 2 == 0  # an episode that starts soon before and one that starts after, or neither
+    (q, k, v, do)[row][at, row, :, :] = filler
+  if t > 100:
+    v[at + 1, 1, 0, 0] = k[at + 30, 1, -1, -1] = filler  # several, a step and most of a chunk apart
+  got = _scan_all(q, k, v, decay, fresh, state, do, ds)
+  rows = torch.arange(4)
+  part = lambda x, dim: x.index_select(dim, rows)  # noqa: E731
+  args = dict(fresh=part(fresh, 1), state=part(state, 0), scale=dk**-0.5, grad_out=part(do, 1), reverse_from=part(ds, 0))
+  want = ref.scan(part(q, 1), part(k, 1), part(v, 1), decay, **args)
+  size = ref.scan(part(q, 1), part(k, 1), part(v, 1), decay, absolute=True, **args)
+  for name, x in got.items():
+    x, w, s = part(x, 0 if name in ("final", "grad_state") else 1).double(), want[name], size[name]
+    there = torch.isfinite(w)
+    assert torch.equal(torch.isfinite(x), there), (name, [sorted(set((torch.isfinite(x) != there).nonzero()[:, 0].tolist()))][:1])
+    half = ref.HALF[got[name].dtype]
+    inner = 1.01 * ref.HALF[dtype]**2 + H32 * (2 * max(dk, dv) + 2 * 64 + 2 * 27 + t + 4 * (t / 32 + 1) + h // hk + 8)
+    tol = s * inner + half * (w.abs() + s * inner) + ref.TINY[dtype] + 2.0**-34 * float(s[there].max())
+    assert ((x - w).abs() <= tol)[there].all(), (name, float((x - w).abs()[there].max()))
