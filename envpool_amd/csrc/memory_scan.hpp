@@ -656,6 +656,12 @@ template <class T, int DK, int DV, bool kAligned, bool rev> struct Walk {
   }
 };
 
+// (a decay of 0 as a very small one, whose power 0 is still 1; NaN stays)
+__device__ inline float log2_of_decay(float log_decay) {
+  const float x = log_decay * 1.44269504088896f;
+  return x < -1e30f ? -1e30f : x;
+}
+
 // Where a chunk that holds something not finite ends. The products inside a chunk run over all of its steps, those that
 // do not reach a result with the weight 0, and 0 * inf is NaN. So a chunk with a sick step ends where an episode does, and
 // at the sick step: forward in time it starts one (and reaches all later steps, as it should), back in time it ends one.
@@ -700,7 +706,7 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
   const int seg = blockIdx.y + (parts.state_only && rev ? 1 : 0);
   const int lane = threadIdx.x & 63;
   c.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const float log2_decay = fmaxf(p.log_decay[h] * 1.44269504088896f, -1e30f);  // (decay 0: its power 0 is still 1)
+  const float log2_decay = log2_of_decay(p.log_decay[h]);
   c.lambda = __builtin_amdgcn_exp2f(log2_decay);
 
   const T* gq = (const T*)p.q + row * p.q_stride[1] + (h / p.q_group) * p.q_stride[2];
@@ -840,7 +846,7 @@ template <class T> __global__ __launch_bounds__(256, 3) void scan_pair(Scan a, S
   const int h = (int)(blockIdx.x % a.heads);
   const int lane = threadIdx.x & 63;
   c.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const float log2_decay = fmaxf(a.log_decay[h] * 1.44269504088896f, -1e30f);
+  const float log2_decay = log2_of_decay(a.log_decay[h]);
   c.lambda = __builtin_amdgcn_exp2f(log2_decay);
   const T* gk = (const T*)a.q + row * a.q_stride[1] + (h / a.q_group) * a.q_stride[2];
   const T* gq = (const T*)a.k + row * a.k_stride[1] + (h / a.k_group) * a.k_stride[2];

@@ -225,3 +225,28 @@ def test_what_is_not_finite_goes_where_the_recurrence_takes_it(case, filler, dty
     inner = 1.01 * ref.HALF[dtype]**2 + H32 * (2 * max(dk, dv) + 2 * 64 + 2 * 27 + t + 4 * (t / 32 + 1) + h // hk + 8)
     tol = s * inner + half * (w.abs() + s * inner) + ref.TINY[dtype] + 2.0**-34 * float(s[there].max())
     assert ((x - w).abs() <= tol)[there].all(), (name, float((x - w).abs()[there].max()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,n,d", [(12, 3, 16), (130, 3, 40), (300, 520, 64), (700, 1, 128)])
+def test_a_decay_that_is_nan_shows(t, n, d, dtype):
+  """In steps, in short segments and in chunks alike: its head is NaN, the others are as they were."""
+  from envpool_amd import policy
+  q, k, v, _, _, state, do, ds = (x.to(DEV) for x in _scan_problem(t, n, 2, 2, d, d, 0.0, dtype))
+  decay = torch.tensor([math.nan, -0.1], device=DEV)
+
+  def run(decay):
+    leaves = [x.detach().requires_grad_() for x in (q, k, v, state)]
+    out, final = policy.memory_scan(*leaves[:3], decay, state=leaves[3])
+    return [x.detach() for x in (out, final, *torch.autograd.grad([out, final], leaves, [do, ds]))]
+
+  got, plain = run(decay), run(torch.tensor([-0.1, -0.1], device=DEV))
+  for i, (x, w) in enumerate(zip(got, plain)):
+    h = 1 if i in (1, 5) else 2
+    sick, well = x.select(h, 0), x.select(h, 1)
+    if i in (3, 4):  # (the last step's gradients of k and v do not pass a decay in the recurrence)
+      sick = sick[:-1]
+    assert torch.isnan(sick).all() and torch.equal(well, w.select(h, 1)), i
+  memory = policy.EnvMemory(n, 2, d, d, decay, state=state.clone())
+  out = memory.step(q[0], k[0], v[0])
+  assert torch.isnan(out[:, 0]).all() and torch.isfinite(out[:, 1]).all()
