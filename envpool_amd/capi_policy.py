@@ -36,7 +36,7 @@ class MemoryScanArgs(C.Structure):
 
 SYMBOLS = [
   "ep_policy_choose", "ep_policy_choose_workspace", "ep_policy_evaluate", "ep_policy_evaluate_workspace", "ep_policy_evaluate_grad",
-  "ep_policy_evaluate_grad_workspace", "ep_memory_step", "ep_memory_step_workspace", "ep_memory_scan", "ep_memory_scan_workspace",
+  "ep_policy_evaluate_grad_workspace", "ep_memory_step", "ep_memory_step_workspace", "ep_memory_reset", "ep_memory_scan", "ep_memory_scan_workspace",
   "ep_memory_scan_pair", "ep_memory_scan_pair_workspace",
   "ep_memory_sum_heads",
 ]
@@ -54,6 +54,7 @@ def lib():
     L.ep_policy_evaluate.argtypes = [rows, _vp, _vp, _vp, _vp]
     L.ep_policy_evaluate_grad.argtypes = [rows, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64]
     L.ep_memory_step.argtypes = [step]
+    L.ep_memory_reset.argtypes = [step]
     L.ep_memory_scan.argtypes = [scan]
     L.ep_memory_scan_pair.argtypes = [scan, scan]
     L.ep_memory_sum_heads.argtypes = [_i32, _vp, _i64, _i32, _i32, _i32, _vp, _i32, _vp]

@@ -270,6 +270,28 @@ int ep_memory_step(const ep_memory_step_args* a) {
   return EP_OK;
 }
 
+int ep_memory_reset(const ep_memory_step_args* a) {
+  if (!a) return fail(EP_ERR_INVALID, "null argument");
+  if (a->num_envs < 1 || a->num_envs > INT32_MAX) return fail(EP_ERR_INVALID, "num_envs = %lld", (long long)a->num_envs);
+  if (a->rows < 0 || a->rows > INT32_MAX) return fail(EP_ERR_INVALID, "rows = %lld", (long long)a->rows);
+  if (a->heads < 1 || a->heads > 65535) return fail(EP_ERR_INVALID, "heads = %d is outside [1, 65535]", a->heads);
+  if (a->key_dim < 1 || a->key_dim > 256 || a->value_dim < 1 || a->value_dim > 256)
+    return fail(EP_ERR_INVALID, "key_dim = %d, value_dim = %d: not both in [1, 256]", a->key_dim, a->value_dim);
+  if (!a->env_id && a->rows > a->num_envs) return fail(EP_ERR_INVALID, "rows = %lld of %lld envs without env_id", (long long)a->rows, (long long)a->num_envs);
+  if (a->rows > 0 && !a->state) return fail(EP_ERR_INVALID, "state: null pointer");
+  const void* words[] = {a->state, a->env_id, a->error};
+  for (const void* ptr : words)
+    if ((uintptr_t)ptr % 4) return fail(EP_ERR_INVALID, "an array of 4-byte values is not aligned to 4 bytes");
+  if (a->rows == 0) return EP_OK;
+  EP_ENTER_GPU(a->device_id);
+  epm::Step k{};
+  k.num_envs = a->num_envs, k.rows = a->rows, k.state = a->state, k.env_id = a->env_id, k.env_id_offset = a->env_id_offset, k.error = a->error;
+  const int64_t size = (int64_t)a->heads * a->key_dim * a->value_dim, stretches = std::min<int64_t>((size + 2047) / 2048, 256);
+  hipLaunchKernelGGL(epm::reset_rows, dim3((unsigned)std::min<int64_t>(a->rows * stretches, kMaxGroups256)), dim3(256), 0, (hipStream_t)a->stream, k, size, stretches);
+  HIP_TRY(hipGetLastError());
+  return EP_OK;
+}
+
 int64_t ep_memory_scan_workspace(const ep_memory_scan_args* a) { return a ? scan_workspace(a, scan_parts(a)) : 0; }
 
 int ep_memory_scan(const ep_memory_scan_args* a) {

@@ -45,6 +45,18 @@ static __global__ __launch_bounds__(256) void count_claims(Step p) {
   if (e >= 0 && e < p.num_envs) atomicAdd(&p.claims[e], 1);
 }
 
+// the states of the envs that a batch names, zeroed: a workgroup per row and stretch of it
+static __global__ __launch_bounds__(256) void reset_rows(Step p, int64_t size, int64_t stretches) {
+  for (int64_t i = blockIdx.x; i < p.rows * stretches; i += gridDim.x) {
+    const int64_t row = i / stretches, e = p.env_id ? (int64_t)p.env_id[row] - p.env_id_offset : row;
+    if (e < 0 || e >= p.num_envs) {
+      if (threadIdx.x == 0 && p.error) *p.error = 1;
+      continue;
+    }
+    for (int64_t j = i % stretches * 256 + threadIdx.x; j < size; j += stretches * 256) p.state[e * size + j] = 0.f;
+  }
+}
+
 // One wave per (row, head) streams the state through its registers: a lane holds kVec neighbouring value columns (or
 // kCols such pieces, 64 apart) and walks down the keys, 64 / (lanes per key row) keys an instruction, so that the load
 // instructions of the wave are one contiguous stretch. Nothing is read twice; HBM bounds it (8 bytes moved per 5 flops), so what matters

@@ -110,6 +110,16 @@ struct Step {
     }
     epy::check(rc);
   }
+  void reset(int64_t rows, u64 env_id, u64 stream) const {
+    ep_memory_step_args b = a;
+    b.rows = rows, b.env_id = at<const int32_t>(env_id), b.stream = at<void>(stream);
+    int rc;
+    {
+      py::gil_scoped_release rel;
+      rc = ep_memory_reset(&b);
+    }
+    epy::check(rc);
+  }
 };
 
 using Stride3 = std::array<int64_t, 3>;
@@ -165,7 +175,8 @@ PYBIND11_MODULE(policy_native, m) {
   py::class_<Step>(m, "Step")
       .def(py::init<int, int64_t, int, int, int, u64, u64, int, u64>())
       .def("workspace", &Step::workspace)
-      .def("run", &Step::run);
+      .def("run", &Step::run)
+      .def("reset", &Step::reset);
   py::class_<Scan>(m, "Scan")
       .def(py::init<int, int, int64_t, int64_t, int, int, int, u64, u64, int64_t, int64_t, u64>())
       .def("operands", &Scan::operands)

@@ -361,18 +361,27 @@ class EnvMemory:
                                 self._error.data_ptr())
 
   def poll_errors(self) -> None:
-    """Raises if a step so far named an env that is not in the memory. Never waits: what a running kernel has
+    """Raises if a step or a reset so far named an env that is not in the memory. Never waits: what a running kernel has
     yet to flag is seen by a later call (every `step` polls first)."""
     if self._error_np[0]:
       self._error_np[0] = 0
-      raise RuntimeError(f"EnvMemory: an earlier step named an env id outside [{self.env_id_offset}, {self.env_id_offset + self.num_envs})")
+      raise RuntimeError(f"EnvMemory: an earlier step or reset named an env id outside [{self.env_id_offset}, {self.env_id_offset + self.num_envs})")
 
   def reset(self, env_id: Optional[torch.Tensor] = None) -> None:
-    """Zeroes the state of the envs in `env_id` (all if None)."""
+    """Zeroes the state of the envs in `env_id` (whole numbers `[n]`; all envs if None). An id outside the memory touches
+    nothing and is reported by a later step, as a step's own are."""
     if env_id is None:
       self.state.zero_()
-    else:
-      self.state.index_fill_(0, env_id.long() - self.env_id_offset, 0.0)
+      return
+    if env_id.dim() > 1 or env_id.dtype == torch.bool or env_id.is_floating_point() or env_id.is_complex():
+      raise ValueError(f"env_id must be whole numbers [n], got {env_id.dtype} {list(env_id.shape)}")
+    _same_device(self.device, env_id=env_id)
+    with torch.no_grad():
+      if env_id.dtype != torch.int32:  # (what 32 bits do not hold is outside)
+        env_id = env_id.long().clamp(self.env_id_offset - 1, self.env_id_offset + self.num_envs).int()
+      env_id = _dense(env_id)
+      self._native.reset(env_id.numel(), env_id.data_ptr(), current_stream_handle(self.device))
+      torch.autograd.graph.increment_version(self.state)
 
   def step(self, q, k, v, *, env_id=None, fresh=None, elapsed_step=None, scale: Optional[float] = None) -> torch.Tensor:
     """One step of the rows of a batch: `q` `[B, num_heads, key_dim]`, `k` `[B, kv_heads, key_dim]`, `v`

@@ -127,6 +127,11 @@ typedef struct {
 int ep_memory_step(const ep_memory_step_args* args);
 int64_t ep_memory_step_workspace(const ep_memory_step_args* args);
 
+/* Zeroes the states of the envs that `env_id` [rows] names (NULL: envs 0 .. rows-1), as often as it names them. Of `args`
+ * only device_id, num_envs, rows, heads, key_dim, value_dim, state, env_id, env_id_offset, error and stream are looked at. An
+ * id outside touches nothing and sets *error, as in a step. */
+int ep_memory_reset(const ep_memory_step_args* args);
+
 /* `steps` steps of `rows` independent rows at once (a rollout segment, time first; any strides with a dense
  * last dimension). reverse != 0 runs time backwards with the recurrence of the gradients:
  *   forward:  S_t = d_t S_{t-1} + inc_scale k_t^T v_t,  d_t = fresh[t] ? 0 : exp(log_decay);  S_{-1} = state_in,

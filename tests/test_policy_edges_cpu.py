@@ -157,3 +157,50 @@ def test_send_choice_tells_rows_without_options_from_rows_without_a_distribution
   with pytest.raises(RuntimeError, match="1 rows.*row 1, env 3"):
     pool.send_choice(Choice(action, torch.tensor([-0.5, float("nan"), -1.0]), torch.zeros(3)))
   assert len(pool.sent) == 1
+
+
+def test_reset_leaves_envs_alone_that_it_was_not_asked_for(monkeypatch):
+  """An id below the memory's first is not its last env; what 32 bits do not hold is not what they wrap to."""
+  from envpool_amd import policy
+  monkeypatch.setattr(policy, "_same_device", lambda dev, **tensors: None)
+  monkeypatch.setattr(policy, "current_stream_handle", lambda dev: 0)
+  seen = []
+
+  class Native:
+    def reset(self, rows, env_id, stream):
+      import ctypes
+      seen.append(list((ctypes.c_int32 * rows).from_address(env_id)) if rows else [])
+
+  memory = object.__new__(policy.EnvMemory)
+  memory.num_envs, memory.env_id_offset, memory.device, memory._native = 4, 10, torch.device("cpu"), Native()
+  memory.state = torch.ones(4, 1, 2, 2)
+  memory.reset(torch.tensor([9, 11], dtype=torch.int32))
+  memory.reset(torch.tensor([2**32 + 11, 12, -2**40, 13]))
+  memory.reset(torch.zeros(0, dtype=torch.int64))
+  assert torch.equal(memory.state, torch.ones(4, 1, 2, 2))  # (the stand-in zeroes nothing)
+  assert seen == [[9, 11], [14, 12, 9, 13], []]
+  for bad in (torch.tensor([True, False]), torch.tensor([1.0]), torch.zeros(2, 2, dtype=torch.int32)):
+    with pytest.raises(ValueError, match="whole numbers"):
+      memory.reset(bad)
+  memory.reset()
+  assert not memory.state.any()
+
+
+def test_resets_that_are_refused():
+  import ctypes as C
+
+  from envpool_amd import capi, capi_policy as cp
+  L = cp.lib()
+  ptr = 4096  # (never followed)
+
+  def args(**kw):
+    a = dict(device_id=0, num_envs=8, rows=4, heads=2, key_dim=16, value_dim=16, state=ptr, env_id=ptr)
+    return cp.MemoryStepArgs(**dict(a, **kw))
+
+  for bad, word in ((dict(num_envs=0), "num_envs"), (dict(rows=-1), "rows"), (dict(heads=0), "heads"), (dict(key_dim=257), "key_dim"), (dict(value_dim=0), "value_dim"),
+                    (dict(rows=9, env_id=None), "without env_id"), (dict(state=None), "state"), (dict(env_id=ptr + 2), "aligned")):
+    assert L.ep_memory_reset(C.byref(args(**bad))) == capi.EP_ERR_INVALID and word in L.ep_last_error().decode(), bad
+  assert L.ep_memory_reset(None) == capi.EP_ERR_INVALID
+  assert L.ep_memory_reset(C.byref(args(rows=0, state=None))) == capi.EP_OK
+  if L.ep_device_count() == 0:
+    assert L.ep_memory_reset(C.byref(args())) == capi.EP_ERR_NO_DEVICE

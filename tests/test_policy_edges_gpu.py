@@ -250,3 +250,27 @@ def test_a_decay_that_is_nan_shows(t, n, d, dtype):
   memory = policy.EnvMemory(n, 2, d, d, decay, state=state.clone())
   out = memory.step(q[0], k[0], v[0])
   assert torch.isnan(out[:, 0]).all() and torch.isfinite(out[:, 1]).all()
+
+
+@pytest.mark.parametrize("shape", [(6, 1, 1, 1), (9, 3, 5, 7), (40, 4, 64, 64), (3, 8, 256, 256)])
+def test_reset_by_id(shape):
+  from envpool_amd import policy
+  g = _gen(1)
+  table = torch.randn(*shape, generator=g).to(DEV)
+  n = shape[0]
+  memory = policy.EnvMemory(*shape, torch.zeros(shape[1], device=DEV), state=table.clone(), env_id_offset=100)
+  memory.reset(torch.tensor([101, 99, 101, 100 + n, 100], dtype=torch.int32, device=DEV))  # twice, and outside on both ends
+  assert not memory.state[:2].any() and torch.equal(memory.state[2:], table[2:])
+  torch.cuda.synchronize()
+  with pytest.raises(RuntimeError, match="outside"):
+    memory.poll_errors()
+  memory.reset(torch.tensor([2**32 + 102, 102], device=DEV)[1:])
+  memory.reset(torch.arange(100, 100 + n, device=DEV)[::2])  # (strided, 64 bits)
+  torch.cuda.synchronize()
+  memory.poll_errors()
+  assert not memory.state[::2].any() and torch.equal(memory.state[3::2], table[3::2])
+  memory.reset(torch.tensor([2**32 + 103], device=DEV))
+  assert torch.equal(memory.state[3::2], table[3::2])
+  torch.cuda.synchronize()
+  with pytest.raises(RuntimeError, match="outside"):
+    memory.poll_errors()
