@@ -293,16 +293,22 @@ template <class T> __device__ inline float hold_range(const Rows& p, int64_t row
   return fabsf(x) < INFINITY && fabsf(b) < INFINITY ? (y > 0.f ? Num<float>::kHigh : Num<float>::kLow) : y;
 }
 
-// load_y made ready for sums: kNone where there is no weight, m the largest. Returns whether a legal one is NaN or +inf. Nearly
+// What a row, or a part of it, holds among its legal values
+enum : int {
+  kBad = 1,    // NaN or +inf
+  kBelow = 2,  // in 32 bits, a sum below the range, held at its end
+  kGone = 4,   // in 32 bits, a logit or a bias of -inf
+};
+// load_y made ready for sums: kNone where there is no weight, m the largest. Returns what of the above there is. Nearly
 // always all are finite, which one product with 0 per option shows (0 * inf and 0 * NaN are NaN).
 template <class T, class R, bool kHist, bool kWhole>
-__device__ inline bool load_ready(const Rows& p, const RowConst<R>& c, int64_t row, int64_t j0, bool whole, const Raw<T, kWhole>& raw, const Seen<R>& seen,
+__device__ inline int load_ready(const Rows& p, const RowConst<R>& c, int64_t row, int64_t j0, bool whole, const Raw<T, kWhole>& raw, const Seen<R>& seen,
                                   R (&y)[kPer], R& m) {
   m = Num<R>::kNone;
   if (j0 >= c.n_legal) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) y[i] = Num<R>::kNone;
-    return false;
+    return 0;
   }
   const uint32_t legal = load_y<T, R, kHist, kWhole>(p, c, row, j0, whole, raw, seen, y);
   R odd = (R)0;
@@ -312,18 +318,23 @@ __device__ inline bool load_ready(const Rows& p, const RowConst<R>& c, int64_t r
     odd = mul_add(y[i], (R)0, odd);
     m = larger(m, y[i]);
   }
-  if (odd == (R)0 && (m > Num<R>::kNone || !legal)) return false;
-  bool bad = false;
+  if (odd == (R)0 && (m > Num<R>::kNone || !legal)) return 0;
+  int what = 0;
+  m = Num<R>::kNone;  // (of the values as they are held)
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     if (!bit(legal, i)) continue;
-    if constexpr (sizeof(R) == 4) y[i] = hold_range<T>(p, row, j0 + i, y[i]);
-    if (!(y[i] < (R)INFINITY)) bad = true;
+    if constexpr (sizeof(R) == 4) {
+      const bool below = y[i] == -INFINITY;
+      y[i] = hold_range<T>(p, row, j0 + i, y[i]);
+      if (below) what |= y[i] == -INFINITY ? kGone : kBelow;
+    }
+    if (!(y[i] < (R)INFINITY)) what |= kBad;
     if (y[i] == -(R)INFINITY) y[i] = Num<R>::kNone;
     else if constexpr (sizeof(R) == 4) y[i] = larger(y[i], Num<float>::kLow);
     m = larger(m, y[i]);
   }
-  return bad;
+  return what;
 }
 
 // running statistics of a row, or of a part of it
@@ -331,7 +342,7 @@ template <class R> struct Stat {
   R m;           // largest y
   R s, e;        // sum w, sum w d with d = (y - m) k, w = exp(d kUnit)
   int64_t best;  // lowest index with y == m
-  int32_t bad;
+  int32_t what;  // kBad, kBelow, kGone
 };
 template <class R> __device__ inline Stat<R> stat_zero() { return {Num<R>::kNone, (R)0, (R)0, INT64_MAX, 0}; }
 template <class R> __device__ inline R exponent(R y, R m, R k) { return larger((y - m) * k, Num<R>::kFloor); }
@@ -400,6 +411,9 @@ template <class V> __device__ inline V lanes_max(V v, int width) {
 template <class V> __device__ inline V lanes_min(V v, int width) {
   return lanes_reduce(v, width, [](V a, V b) { return a < b ? a : b; });
 }
+__device__ inline int32_t lanes_or(int32_t v, int width) {
+  return lanes_reduce(v, width, [](int32_t a, int32_t b) { return a | b; });
+}
 template <class V> __device__ inline V lanes_sum(V v, int width) {
   return lanes_reduce(v, width, [](V a, V b) { return a + b; });
 }
@@ -427,13 +441,13 @@ template <class R, bool kBest> __device__ inline Stat<R> stat_block(Stat<R> a, R
   const int64_t best = kBest ? lanes_min((long long)(a.m == m ? a.best : INT64_MAX), 64) : INT64_MAX;
   stat_rebase(a, m, k);
   const R sum = lanes_sum(a.s, 64), e = lanes_sum(a.e, 64);
-  const int bad = __any(a.bad);
+  const int what = lanes_or(a.what, 64);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[wave] = {m, sum, e, best, bad};
+  if ((threadIdx.x & 63) == 0) lds[wave] = {m, sum, e, best, what};
   __syncthreads();
   Stat<R> r = lds[0];
   for (int i = 1; i < kWaves; ++i) {
-    r.s += lds[i].s, r.e += lds[i].e, r.bad |= lds[i].bad;
+    r.s += lds[i].s, r.e += lds[i].e, r.what |= lds[i].what;
     if (lds[i].best < r.best) r.best = lds[i].best;
   }
   return r;
@@ -488,7 +502,7 @@ struct ChooseOut {
   float *log_prob, *entropy;
 };
 __device__ inline void finish_choose(const ChooseOut& o, int64_t row, const Stat<double>& a, const RowConst<double>& c, int64_t pick, double y_pick) {
-  const bool bad = a.bad || c.bad;
+  const bool bad = (a.what & kBad) || c.bad;
   const bool empty = !bad && a.m == Num<double>::kNone;
   const double log_s = log(a.s);
   o.action[row] = bad || empty ? -1 : (int32_t)pick;
@@ -498,11 +512,15 @@ __device__ inline void finish_choose(const ChooseOut& o, int64_t row, const Stat
 
 struct EvaluateOut {
   const int32_t* action;
-  float *log_prob, *entropy, *stats;  // stats: {largest y, log2 of the sum of weights}; {-inf, 0}: EMPTY; {NaN, NaN}: BAD
+  // stats: {largest y, log2 of the sum of weights}; {-inf, 0}: EMPTY; {NaN, NaN}: BAD. A row whose largest y is the lower end
+  // of the range that values are held at has {kLow, ..} if sums below the range are among them, which the gradients'
+  // kernels see as -inf: all legal options are equal then. With -inf logits or biases beside such sums {kLow, NaN}: the gradients cannot
+  // tell them apart, and are NaN. Without such sums {the lowest value, ..}, from which the others' distance shows.
+  float *log_prob, *entropy, *stats;
 };
 __device__ inline void finish_evaluate(const EvaluateOut& o, int64_t row, int64_t options, const Stat<float>& a, const RowConst<float>& c, int32_t act,
                                        float y_act) {
-  const bool bad = a.bad || c.bad;
+  const bool bad = (a.what & kBad) || c.bad;
   const bool empty = !bad && a.m == Num<float>::kNone;
   const float log_s = __builtin_amdgcn_logf(a.s);
   float lp;
@@ -512,8 +530,9 @@ __device__ inline void finish_evaluate(const EvaluateOut& o, int64_t row, int64_
   else lp = ((y_act - a.m) * c.k - log_s) * Num<float>::kUnit;
   o.log_prob[row] = bad ? quiet_nan<float>() : lp;
   o.entropy[row] = bad ? quiet_nan<float>() : empty ? 0.f : (log_s - a.e / a.s) * Num<float>::kUnit;
-  o.stats[2 * row] = bad ? quiet_nan<float>() : empty ? -INFINITY : a.m;
-  o.stats[2 * row + 1] = bad ? quiet_nan<float>() : empty ? 0.f : log_s;
+  const bool lowest = a.m == Num<float>::kLow, below = lowest && (a.what & kBelow);
+  o.stats[2 * row] = bad ? quiet_nan<float>() : empty ? -INFINITY : lowest && !below ? Num<float>::kNone : a.m;
+  o.stats[2 * row + 1] = bad || (below && (a.what & kGone)) ? quiet_nan<float>() : empty ? 0.f : log_s;
 }
 
 // ---- rows of up to 64 * 8 * NP options: `width` lanes per row, a lane's options in registers -----------
@@ -568,11 +587,11 @@ __global__ __launch_bounds__(kThreads) void choose_group(Rows p, int width_log, 
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
     double m;
-    a.bad |= load_ready<T, double, kHist, kWhole>(p, c, g.row, g.j(k), whole, raw[k], Seen<double>{n}.at(kHist ? g.j(k) : 0), y[k], m);
+    a.what |= load_ready<T, double, kHist, kWhole>(p, c, g.row, g.j(k), whole, raw[k], Seen<double>{n}.at(kHist ? g.j(k) : 0), y[k], m);
     a.m = larger(a.m, m);
   }
   a.m = lanes_max(a.m, g.width);
-  a.bad = lanes_max(a.bad, g.width);
+  a.what = lanes_or(a.what, g.width);
   double w[NP][kPer];
 #pragma unroll
   for (int k = 0; k < NP; ++k)
@@ -655,7 +674,7 @@ template <class T, int NP, bool kHist, bool kWhole> __global__ __launch_bounds__
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
     float m;
-    a.bad |= load_ready<T, float, kHist, kWhole>(p, c, g.row, g.j(k), whole, raw[k], Seen<float>{n}.at(kHist ? g.j(k) : 0), y[k], m);
+    a.what |= load_ready<T, float, kHist, kWhole>(p, c, g.row, g.j(k), whole, raw[k], Seen<float>{n}.at(kHist ? g.j(k) : 0), y[k], m);
     a.m = larger(a.m, m);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
@@ -663,7 +682,7 @@ template <class T, int NP, bool kHist, bool kWhole> __global__ __launch_bounds__
     }
   }
   a.m = lanes_max(a.m, g.width);
-  a.bad = lanes_max(a.bad, g.width);
+  a.what = lanes_or(a.what, g.width);
   y_act = lanes_max(y_act, g.width);
 #pragma unroll
   for (int k = 0; k < NP; ++k)
@@ -701,7 +720,7 @@ __global__ __launch_bounds__(kThreads) void choose_parts(Rows p, int pieces, int
     const auto seen = mem.count(p, c, row, j0);
     const int64_t j = j0 + threadIdx.x * kPer;
     double y[kPer], m;
-    a.bad |= load_ready<T, double, kHist, kWhole>(p, c, row, j, p.vec && j0 + kPiece <= p.options, raw, seen, y, m);
+    a.what |= load_ready<T, double, kHist, kWhole>(p, c, row, j, p.vec && j0 + kPiece <= p.options, raw, seen, y, m);
     ask(j + kPiece);
     stat_add<double, kBest>(a, y, m, j, c.k);
   }
@@ -729,12 +748,12 @@ __global__ __launch_bounds__(kThreads) void choose_join(Rows p, int pieces, int 
     const int64_t best = a.m > b.m ? a.best : (b.m > a.m ? b.best : min(a.best, b.best));
     stat_rebase(a, m, c.k);
     stat_rebase(b, m, c.k);
-    a = {m, a.s + b.s, a.e + b.e, best, a.bad | b.bad};
+    a = {m, a.s + b.s, a.e + b.e, best, a.what | b.what};
   }
   a = stat_block<double, true>(a, c.k, red);
   int64_t pick = a.best;
   double y_pick = a.m;
-  if (u && !a.bad && !c.bad && a.m != Num<double>::kNone) {
+  if (u && !(a.what & kBad) && !c.bad && a.m != Num<double>::kNone) {
     const double target = (u_f64 ? ((const double*)u)[row] : (double)((const float*)u)[row]) * a.s;
     // the part: its weights, moved to the row's maximum, cumulated 64 parts at a time by one wave
     if (threadIdx.x < 64) {
@@ -846,7 +865,7 @@ __global__ __launch_bounds__(kThreads, kHist ? 6 : 8) void evaluate_parts(Rows p
     const auto seen = mem.count(p, c, row, j0);
     const int64_t j = j0 + threadIdx.x * kPer;
     float y[kPer], m;
-    a.bad |= load_ready<T, float, kHist, kWhole>(p, c, row, j, p.vec && j0 + kPiece <= p.options, raw, seen, y, m);
+    a.what |= load_ready<T, float, kHist, kWhole>(p, c, row, j, p.vec && j0 + kPiece <= p.options, raw, seen, y, m);
     ask(j + kPiece);
     stat_add<float, false>(a, y, m, j, c.k);
     if ((uint64_t)(act - j) < kPer) {
@@ -873,12 +892,12 @@ __global__ __launch_bounds__(kThreads) inline void evaluate_join(Rows p, int n_p
     const float m = larger(a.m, b.stat.m);
     stat_rebase(a, m, c.k);
     stat_rebase(b.stat, m, c.k);
-    a.s += b.stat.s, a.e += b.stat.e, a.bad |= b.stat.bad;
+    a.s += b.stat.s, a.e += b.stat.e, a.what |= b.stat.what;
     y_act = larger(y_act, b.y_act);
   }
   const float m = lanes_max(a.m, 64);
   stat_rebase(a, m, c.k);
-  a.s = lanes_sum(a.s, 64), a.e = lanes_sum(a.e, 64), a.bad = lanes_max(a.bad, 64);
+  a.s = lanes_sum(a.s, 64), a.e = lanes_sum(a.e, 64), a.what = lanes_or(a.what, 64);
   y_act = lanes_max(y_act, 64);
   if ((threadIdx.x & 63) == 0) finish_evaluate(out, row, p.options, a, c, out.action[row], y_act);
 }
@@ -913,12 +932,12 @@ template <bool kHist> __device__ inline GradRow grad_row(const GradArgs& g, cons
   GradRow r;
   r.m = g.stats[2 * row];
   r.log_s = g.stats[2 * row + 1];
-  r.k = c.k;
+  r.k = r.m == Num<float>::kLow ? -2e-38f : c.k;  // (all are equal, see EvaluateOut: what is below the largest counts as above)
   r.act = g.action[row];
   const float g_lp = g.g_lp ? g.g_lp[row] : 0.f, g2 = g.g_h ? g.g_h[row] : 0.f, entropy = g.entropy[row];
   const float g1 = r.act != -1 ? g_lp : 0.f;
   r.empty = r.m == -INFINITY;
-  const float nan = r.m != r.m ? r.m : 0.f;  // a BAD row: its gradient is NaN where legal
+  const float nan = r.log_s != r.log_s ? r.log_s : 0.f;  // (a BAD row) its gradient is NaN where legal
   r.g1 = g1 * c.inv_t;
   r.flat = (g1 + g2 * entropy) * c.inv_t + nan;
   r.lean = g2 * Num<float>::kUnit * c.inv_t;
@@ -928,8 +947,8 @@ template <bool kHist> __device__ inline GradRow grad_row(const GradArgs& g, cons
 __device__ inline void grad_y(const GradRow& r, const float (&y)[kPer], uint32_t legal, int64_t j, float (&out)[kPer]) {
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    // (no probability is above 1: a sum that left the range of 32 bits upwards counts as the row's largest)
-    const float d = __builtin_amdgcn_fmed3f(fmaf(y[i] - r.m, r.k, -r.log_s), Num<float>::kFloor, 0.f);
+    // (no probability is above that of the row's largest value, which a sum that left the range of 32 bits upwards is)
+    const float d = __builtin_amdgcn_fmed3f(fmaf(y[i] - r.m, r.k, -r.log_s), Num<float>::kFloor, -r.log_s);
     out[i] = pick(legal, i, -weight(d) * fmaf(r.lean, d, r.flat), 0.f);
   }
   if ((uint64_t)(r.act - j) < kPer) {

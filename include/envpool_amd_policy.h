@@ -74,8 +74,8 @@ int ep_policy_choose(const ep_policy_rows* rows, const void* u, int32_t u_dtype,
                      float* entropy);
 int64_t ep_policy_choose_workspace(const ep_policy_rows* rows);
 
-/* log_prob[b] = log p of action[b], entropy[b] = -sum p log p, in 32 bits, and stats[b] = {maximum,
- * log-sum} for ep_policy_evaluate_grad. action -1 ("none", what EMPTY rows choose): log_prob 0 without
+/* log_prob[b] = log p of action[b], entropy[b] = -sum p log p, in 32 bits, and in stats[b] (two floats)
+ * what ep_policy_evaluate_grad needs of the row. action -1 ("none", what EMPTY rows choose): log_prob 0 without
  * gradient; an illegal action: -inf; any other value outside [0, options): NaN. EMPTY rows: entropy 0,
  * log_prob 0 (-1) or -inf; BAD rows: NaN. */
 int ep_policy_evaluate(const ep_policy_rows* rows, const int32_t* action, float* log_prob, float* entropy, float* stats);

@@ -274,3 +274,52 @@ def test_reset_by_id(shape):
   torch.cuda.synchronize()
   with pytest.raises(RuntimeError, match="outside"):
     memory.poll_errors()
+
+
+# ---- logits at the ends of the type's range ---------------------------------------------------------
+def _evaluate_all(x, action, g1, g2, **kw):
+  from envpool_amd import policy
+  leaf = x.to(DEV).requires_grad_()
+  lp, ent = policy.evaluate(leaf, action.to(DEV), **{k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in kw.items()})
+  gx, = torch.autograd.grad([lp, ent], leaf, [g1.to(DEV), g2.to(DEV)])
+  return lp.detach().cpu().double(), ent.detach().cpu().double(), gx.cpu().double()
+
+
+def _agrees(got, want, size, tol):
+  """Within tol of the magnitude `size` (infinite and too large values have to be the same)."""
+  top = float(torch.finfo(torch.float32).max)
+  want = torch.where(want.abs() > top * (1 + H32), want.sign() * math.inf, want)
+  same = (got == want) | ((got - want).abs() <= tol * size)
+  return bool(same.all())
+
+
+@pytest.mark.parametrize("a", [6, 40, 300, 5000])
+def test_sums_beyond_32_bits(a):
+  """Finite logits and biases whose sum leaves the range: its end stands for them, forward and in the gradients."""
+  top = 3e38
+  x = torch.randn(3, a, generator=_gen(a))
+  b = torch.zeros(3, a)
+  x[0, [1, 4]], b[0, [1, 4]] = top, top    # two above everything: a half each
+  x[1], b[1] = -top, -top                  # nothing but sums below the range: uniform
+  x[2, 3], b[2, 3] = top, top              # one above everything
+  action = torch.tensor([1, 2, 3], dtype=torch.int32)
+  g1, g2 = torch.ones(3), torch.full((3,), 0.5)
+  want = ref.evaluate(x, action, g1, g2, bias=b)
+  lp, ent, gx = _evaluate_all(x, action, g1, g2, bias=b)
+  tol = 64 * H32
+  assert _agrees(lp, want["log_prob"], 1 + want["log_prob"].abs(), tol) and _agrees(ent, want["entropy"], 1 + want["entropy"].abs(), tol)
+  assert ((gx - want["grad_logits"]).abs() <= 4 * 12 * tol * (want["grad_logits"].abs() + 1e-3 / a)).all(), (gx - want["grad_logits"]).abs().max(1)
+
+
+def test_sums_below_32_bits_beside_nothing():
+  """A row of nothing but sums below the range and logits of -inf: forward the sums share it; the gradients cannot tell the
+  two apart and say so, NaN."""
+  x = torch.full((3, 12), -3e38)
+  b = torch.full((12,), -3e38)
+  x[0, 4] = x[1, 0] = -math.inf
+  action = torch.tensor([1, 1, 1], dtype=torch.int32)
+  mask = torch.ones(3, 12, dtype=torch.bool)
+  mask[1, 0] = False  # (not legal: not looked at)
+  lp, ent, gx = _evaluate_all(x, action, torch.ones(3), torch.ones(3), bias=b, mask=mask)
+  assert torch.allclose(lp, -torch.log(torch.tensor([11.0, 11.0, 12.0]).double()), atol=1e-6) and torch.allclose(ent, -lp, atol=1e-6)
+  assert torch.isnan(gx[0]).all() and torch.isfinite(gx[1:]).all() and gx[1, 0] == 0
