@@ -299,6 +299,17 @@ enum : int {
   kBelow = 2,  // in 32 bits, a sum below the range, held at its end
   kGone = 4,   // in 32 bits, a logit or a bias of -inf
 };
+// Option j of a row, where load_ready says that it has no weight: the lower end of the range, if that is only because its
+// neighbours are larger (it is legal, and has the lowest value), else still kNone.
+template <class T> __device__ inline float lowest_or_none(const Rows& p, const RowConst<float>& c, int64_t row, int64_t j) {
+  if (j < 0 || j >= c.n_legal) return Num<float>::kNone;
+  if (p.mask) {
+    const int64_t at = row * p.mask_stride;
+    if (p.mask_bits ? !((((const uint32_t*)p.mask)[at + (j >> 5)] >> (j & 31)) & 1u) : !((const uint8_t*)p.mask)[at + j]) return Num<float>::kNone;
+  }
+  return larger(hold_range<T>(p, row, j, -INFINITY), Num<float>::kNone);
+}
+
 // load_y made ready for sums: kNone where there is no weight, m the largest. Returns what of the above there is. Nearly
 // always all are finite, which one product with 0 per option shows (0 * inf and 0 * NaN are NaN).
 template <class T, class R, bool kHist, bool kWhole>
@@ -527,6 +538,7 @@ __device__ inline void finish_evaluate(const EvaluateOut& o, int64_t row, int64_
   if (act == -1) lp = 0.f;
   else if (act < 0 || act >= options) lp = quiet_nan<float>();
   else if (empty || y_act == Num<float>::kNone) lp = -INFINITY;
+  else if (y_act - a.m < -1e38f) lp = (y_act - a.m) * c.inv_t;  // (times k first it may leave the range)
   else lp = ((y_act - a.m) * c.k - log_s) * Num<float>::kUnit;
   o.log_prob[row] = bad ? quiet_nan<float>() : lp;
   o.entropy[row] = bad ? quiet_nan<float>() : empty ? 0.f : (log_s - a.e / a.s) * Num<float>::kUnit;
@@ -695,7 +707,10 @@ template <class T, int NP, bool kHist, bool kWhole> __global__ __launch_bounds__
     }
   a.s = lanes_sum(a.s, g.width);
   a.e = lanes_sum(a.e, g.width);
-  if (g.lane == 0 && g.there) finish_evaluate(out, g.row, p.options, a, c, act, y_act);
+  if (g.lane == 0 && g.there) {
+    if (y_act == Num<float>::kNone) y_act = lowest_or_none<T>(p, c, g.row, act);
+    finish_evaluate(out, g.row, p.options, a, c, act, y_act);
+  }
 }
 
 // ---- longer rows: a workgroup per part of a row (`pieces` pieces of kPiece options), parts joined after ---
@@ -852,8 +867,6 @@ __global__ __launch_bounds__(kThreads, kHist ? 6 : 8) void evaluate_parts(Rows p
   const RowConst<float> c = row_const<float, kHist>(p, row);
   const int32_t act = out.action[row];
   Stat<float> a = stat_zero<float>();
-  if (threadIdx.x == 0) y_act = Num<float>::kNone;
-  __syncthreads();
   const int64_t j_end = min((part + 1) * pieces * (int64_t)kPiece, c.n_legal);
   const int64_t j_first = part * pieces * (int64_t)kPiece;
   Raw<T, kWhole> raw;
@@ -861,6 +874,9 @@ __global__ __launch_bounds__(kThreads, kHist ? 6 : 8) void evaluate_parts(Rows p
     if (j < j_end) raw.ask_row(p, row, j), raw.ask_bias(p, row, j);
   };
   ask(j_first + threadIdx.x * kPer);
+  // (what the action has if the walk finds no weight there; here, where few registers are held)
+  if (threadIdx.x == 0) y_act = act >= j_first && act < j_end ? lowest_or_none<T>(p, c, row, act) : Num<float>::kNone;
+  __syncthreads();
   for (int64_t j0 = j_first; j0 < j_end; j0 += kPiece) {
     const auto seen = mem.count(p, c, row, j0);
     const int64_t j = j0 + threadIdx.x * kPer;
@@ -871,7 +887,7 @@ __global__ __launch_bounds__(kThreads, kHist ? 6 : 8) void evaluate_parts(Rows p
     if ((uint64_t)(act - j) < kPer) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
-        if (act == j + i) y_act = y[i];
+        if (act == j + i && y[i] != Num<float>::kNone) y_act = y[i];
     }
   }
   a = stat_block<float, false>(a, c.k, red);

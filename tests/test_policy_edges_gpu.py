@@ -323,3 +323,39 @@ def test_sums_below_32_bits_beside_nothing():
   lp, ent, gx = _evaluate_all(x, action, torch.ones(3), torch.ones(3), bias=b, mask=mask)
   assert torch.allclose(lp, -torch.log(torch.tensor([11.0, 11.0, 12.0]).double()), atol=1e-6) and torch.allclose(ent, -lp, atol=1e-6)
   assert torch.isnan(gx[0]).all() and torch.isfinite(gx[1:]).all() and gx[1, 0] == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("a", [6, 40, 300, 5000])
+def test_rows_masked_with_the_lowest_value(a, dtype):
+  """Options masked by the type's lowest value instead of by a mask: among others they keep their tiny probability (a
+  log-probability of the value's size, not -inf), and a row of nothing else is uniform, its gradients too. The sums have up
+  to 5000 equal terms in 32 bits: (5000 / 2048 * 8 + 20) half steps of their 1."""
+  low = torch.finfo(dtype).min
+  x = torch.randn(5, a, generator=_gen(a)).to(dtype)
+  x[0] = low
+  x[1] = low
+  x[1, a - 1] = -math.inf  # no probability at all: the others are uniform
+  x[2, ::2] = low          # action there
+  x[3, 1::2] = low         # action not there
+  x[4] = low
+  x[4, 2] = 1.0
+  action = torch.tensor([3, 2, 4, 4, 2], dtype=torch.int32)
+  g1, g2 = torch.tensor([1.0, -2.0, 0.5, 1.5, 1.0]), torch.tensor([0.3, 1.0, -1.0, 0.5, 0.1])
+  for kw in (dict(), dict(temperature=2.5), dict(num_options=torch.full((5,), a - 1, dtype=torch.int32)), dict(mask=torch.arange(a)[None].expand(5, a) != 5)):
+    want = ref.evaluate(x, action, g1, g2, **kw)
+    lp, ent, gx = _evaluate_all(x, action, g1, g2, **kw)
+    tol = 64 * H32
+    assert _agrees(lp, want["log_prob"], 1 + want["log_prob"].abs().nan_to_num(0, 0, 0), tol), (lp, want["log_prob"])
+    assert _agrees(ent, want["entropy"], 1 + want["entropy"].abs(), tol), (ent, want["entropy"])
+    # dy = g1 (one - p) - g2 p (ln p + H). p is off by r: the sum's 64 half steps, and (y - m) / T, of magnitudes up to 10,
+    # in the exponent, 5 roundings; H by what was allowed above; ln p by r and its own two roundings. One rounding each of the sums
+    y = ref.processed(x, **kw)[0]
+    m, w, total, _, _ = ref.distribution(y)
+    p = w / total[:, None]
+    logp = torch.where(w > 0, y - m - torch.log(total)[:, None], 0.0)
+    r, h = (64 + 50) * H32, want["entropy"][:, None]
+    g_1, g_2 = g1.double().abs()[:, None], g2.double().abs()[:, None]
+    bound = g_1 * (p * r + 4 * H32) + g_2 * p * ((logp + h).abs() * (r + 4 * H32) + (1 + h) * tol + r + 2 * H32 * logp.abs())
+    slack = bound / kw.get("temperature", 1.0) + (4 * H32 + ref.HALF[dtype]) * want["grad_logits"].abs() + ref.TINY[dtype]
+    assert ((gx - want["grad_logits"]).abs() <= slack).all(), ((gx - want["grad_logits"]).abs() - slack).max(1)
