@@ -49,12 +49,14 @@ template <> struct Num<double> {
   static constexpr double kNone = -1.7976931348623157e308;
   static constexpr double kUnit = 0.6931471805599453;
   static constexpr double kFloor = -1100.0;  // 2^d of this and less is 0
+  static constexpr double kLeast = 6.2e-306;  // kNone times this is below kFloor, a difference of logits times it nothing
 };
 template <> struct Num<float> {
   static constexpr float kNone = -3.40282347e38f;
   static constexpr float kLow = -3.40282326e38f, kHigh = 3.40282326e38f;
   static constexpr float kUnit = 0.693147181f;  // exponents d count octaves, weights are 2^d
   static constexpr float kFloor = -10000.f;
+  static constexpr float kLeast = 4.5e-37f;  // kNone times this is an exponent of -153 (the differences of logits up to 1e29 nothing)
 };
 
 // 2^d for d in [-1100, 0] in 64 bits: d = n + r, |r| <= 1/2, the series of exp(r ln 2) to the 11th power (the first
@@ -101,6 +103,7 @@ template <class R, bool kHist> __device__ inline RowConst<R> row_const(const Row
   else c.inv_t = sizeof(R) == 8 ? (R)p.inv_t_all : (R)p.inv_t_all_32;
   c.k = c.inv_t * ((R)1 / Num<R>::kUnit);
   c.bad = !(t > (R)0) || !(t < (R)INFINITY) || !(c.k < (R)INFINITY);
+  c.k = larger(c.k, Num<R>::kLeast);  // (however high the temperature, what has no weight gets none)
   if (kHist) {
     c.rep = p.repetition ? (R)p.repetition[row] : (R)p.repetition_all;
     c.inv_rep = (R)1 / c.rep;

@@ -359,3 +359,26 @@ def test_rows_masked_with_the_lowest_value(a, dtype):
     bound = g_1 * (p * r + 4 * H32) + g_2 * p * ((logp + h).abs() * (r + 4 * H32) + (1 + h) * tol + r + 2 * H32 * logp.abs())
     slack = bound / kw.get("temperature", 1.0) + (4 * H32 + ref.HALF[dtype]) * want["grad_logits"].abs() + ref.TINY[dtype]
     assert ((gx - want["grad_logits"]).abs() <= slack).all(), ((gx - want["grad_logits"]).abs() - slack).max(1)
+
+
+@pytest.mark.parametrize("a", [6, 40, 5000])
+@pytest.mark.parametrize("per_row", [False, True])
+def test_temperatures_at_the_end_of_the_range(a, per_row):
+  """However hot, an option that is not legal has no probability."""
+  from envpool_amd import policy
+  x = torch.randn(4, a, generator=_gen(a))
+  count = torch.tensor([2, a // 2, a, 1], dtype=torch.int32)
+  action = torch.zeros(4, dtype=torch.int32)
+  g = torch.ones(4)
+  for t in (1e30, 1e37, 3.4e38):
+    temp = torch.full((4,), t) if per_row else t
+    kw = dict(num_options=count, temperature=temp)
+    want = ref.evaluate(x, action, g, g, **kw)
+    lp, ent, gx = _evaluate_all(x, action, g, g, **kw)
+    tol = 64 * H32
+    assert _agrees(lp, want["log_prob"], 1 + want["log_prob"].abs(), tol) and _agrees(ent, want["entropy"], 1 + want["entropy"].abs(), tol), (t, lp, ent)
+    c = policy.choose(x.to(DEV), torch.full((4,), 0.999, device=DEV), num_options=count.to(DEV), temperature=temp.to(DEV) if per_row else t)
+    assert torch.equal(c.action.cpu().long(), ref.choose(x, torch.full((4,), 0.999), **kw)[0])
+  if not per_row:
+    c = policy.choose(x.to(DEV), torch.full((4,), 0.999, device=DEV), num_options=count.to(DEV), temperature=1e307)
+    assert (c.action.cpu() < count).all() and torch.allclose(c.entropy.cpu(), torch.log(count.float()), atol=1e-6)
