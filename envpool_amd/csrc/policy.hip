@@ -82,6 +82,17 @@ int check_rows(const ep_policy_rows* r, epp::Rows* k) {
   return EP_OK;
 }
 
+// evaluate computes in 32 bits: a number for all rows that those do not hold would make every row BAD
+int check_narrow(const ep_policy_rows* r) {
+  const auto holds = [](double v) { return v < INFINITY && (float)v > 0.f && (float)v < INFINITY && 1.f / (float)v < INFINITY; };
+  if (!r->temperature && !holds(r->temperature_all)) return fail(EP_ERR_INVALID, "temperature = %g: 32 bits do not hold it and its reciprocal", r->temperature_all);
+  if (!r->history || r->history_len == 0) return EP_OK;
+  if (!r->repetition && !holds(r->repetition_all)) return fail(EP_ERR_INVALID, "repetition = %g: 32 bits do not hold it and its reciprocal", r->repetition_all);
+  if (!r->frequency && !std::isfinite((float)r->frequency_all)) return fail(EP_ERR_INVALID, "frequency = %g: 32 bits do not hold it", r->frequency_all);
+  if (!r->presence && !std::isfinite((float)r->presence_all)) return fail(EP_ERR_INVALID, "presence = %g: 32 bits do not hold it", r->presence_all);
+  return EP_OK;
+}
+
 int check_workspace(const ep_policy_rows* r, int64_t need) {
   if (need > 0 && (!r->workspace || r->workspace_bytes < need))
     return fail(EP_ERR_INVALID, "workspace of %lld bytes is smaller than the %lld this call needs", (long long)(r->workspace ? r->workspace_bytes : 0),
@@ -215,6 +226,7 @@ int64_t ep_policy_evaluate_workspace(const ep_policy_rows* r) {
 int ep_policy_evaluate(const ep_policy_rows* r, const int32_t* action, float* log_prob, float* entropy, float* stats) {
   epp::Rows k;
   if (int rc = check_rows(r, &k)) return rc;
+  if (int rc = check_narrow(r)) return rc;
   if (r->rows > 0 && (!action || !log_prob || !entropy || !stats)) return fail(EP_ERR_INVALID, "action, log_prob, entropy, stats: null pointer");
   if (r->rows == 0) return EP_OK;
   if (int rc = check_groups(r, k, kFill)) return rc;
@@ -256,6 +268,7 @@ int ep_policy_evaluate_grad(const ep_policy_rows* r, const int32_t* action, cons
                             void* grad_bias, int64_t grad_bias_stride) {
   epp::Rows k;
   if (int rc = check_rows(r, &k)) return rc;
+  if (int rc = check_narrow(r)) return rc;
   if (r->rows > 0 && (!action || !entropy || !stats)) return fail(EP_ERR_INVALID, "action, entropy, stats: null pointer");
   if (!grad_logits && !grad_bias) return fail(EP_ERR_INVALID, "neither grad_logits nor grad_bias is wanted");
   if (grad_logits && r->rows > 1 && grad_logits_stride < r->options) return fail(EP_ERR_INVALID, "grad_logits_stride = %lld is less than options", (long long)grad_logits_stride);

@@ -109,7 +109,7 @@ template <class R, bool kHist> __device__ inline RowConst<R> row_const(const Row
     c.inv_rep = (R)1 / c.rep;
     c.freq = p.frequency ? (R)p.frequency[row] : (R)p.frequency_all;
     c.pres = p.presence ? (R)p.presence[row] : (R)p.presence_all;
-    c.bad = c.bad || !(c.rep > (R)0);
+    c.bad = c.bad || !(c.rep > (R)0) || !(c.rep < (R)INFINITY) || !(c.inv_rep < (R)INFINITY);
   }
   int64_t n = p.options;
   if (p.num_options) {

@@ -39,8 +39,7 @@ enum {
  *   p_j = exp(y_j) / sum over the legal options;  0 for the others, whose logits, biases and history are
  *   never used (they may hold anything, NaN included).
  * A row without a legal option, or whose legal options are all -inf, is EMPTY. A row with a NaN or +inf among
- * its legal y, a per-row temperature that is not > 0 and finite, or (with a history) a per-row repetition
- * that is not > 0, is BAD. */
+ * its legal y, or a per-row temperature or (with a history) repetition that is not > 0 and finite, is BAD. */
 typedef struct {
   int32_t device_id;
   int32_t dtype;          /* of the logits: EP_F32, EP_F16 or EP_BF16 */
@@ -57,7 +56,8 @@ typedef struct {
   const int32_t* history; /* NULL or [rows][history_len]: options chosen before; entries outside [0, options) count for nothing */
   int64_t history_len, history_stride;
   /* one value per row when the pointer is given, else the value beside it for all rows
-   * (temperature, repetition: > 0; all finite) */
+   * (temperature, repetition: > 0; all finite; ep_policy_evaluate takes them in 32 bits, which have to hold them and the
+   * reciprocals of those two: a number for all rows that is used is refused otherwise, a row's own makes it BAD) */
   const float *repetition, *frequency, *presence, *temperature;
   double repetition_all, frequency_all, presence_all, temperature_all;
   void* workspace;

@@ -204,3 +204,23 @@ def test_resets_that_are_refused():
   assert L.ep_memory_reset(C.byref(args(rows=0, state=None))) == capi.EP_OK
   if L.ep_device_count() == 0:
     assert L.ep_memory_reset(C.byref(args())) == capi.EP_ERR_NO_DEVICE
+
+
+@pytest.mark.parametrize("name,bad", [("temperature", 1e39), ("temperature", 1e-39), ("temperature", 1e-300), ("repetition", 1e-46), ("repetition", 1e300),
+                                      ("frequency", 1e39), ("presence", -1e39)])
+def test_numbers_that_32_bits_do_not_hold_are_refused_by_evaluate(name, bad):
+  """They would make every row one without a distribution. choose computes in 64 bits and takes them."""
+  import ctypes as C
+
+  from envpool_amd import capi, capi_policy as cp
+  L, ptr = cp.lib(), 4096  # (never followed)
+  rows = cp.PolicyRows(dtype=capi.EP_F32, rows=4, options=10, logits=ptr, logits_stride=10, repetition_all=1.0, temperature_all=1.0, history=ptr, history_len=3,
+                       history_stride=3)
+  setattr(rows, name + "_all", bad)
+  r = C.byref(rows)
+  for rc in (L.ep_policy_evaluate(r, ptr, ptr, ptr, ptr), L.ep_policy_evaluate_grad(r, ptr, ptr, ptr, ptr, ptr, ptr, 10, None, 0)):
+    assert rc == capi.EP_ERR_INVALID and name in L.ep_last_error().decode()
+  rows.rows = 0
+  assert L.ep_policy_choose(r, None, 0, None, None, None) == capi.EP_OK
+  setattr(rows, name, ptr)  # (one per row is on the device)
+  assert L.ep_policy_evaluate(r, None, None, None, None) == capi.EP_OK

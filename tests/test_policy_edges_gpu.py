@@ -382,3 +382,18 @@ def test_temperatures_at_the_end_of_the_range(a, per_row):
   if not per_row:
     c = policy.choose(x.to(DEV), torch.full((4,), 0.999, device=DEV), num_options=count.to(DEV), temperature=1e307)
     assert (c.action.cpu() < count).all() and torch.allclose(c.entropy.cpu(), torch.log(count.float()), atol=1e-6)
+
+
+def test_repetitions_of_a_row_that_are_no_numbers():
+  from envpool_amd import policy
+  x = torch.randn(4, 9, generator=_gen(0)).to(DEV).requires_grad_()
+  kw = dict(history=torch.full((4, 2), 3, dtype=torch.int32, device=DEV), repetition=torch.tensor([1.2, math.inf, 1e-40, math.nan], device=DEV))
+  lp, ent = policy.evaluate(x, torch.zeros(4, dtype=torch.int32, device=DEV), **kw)
+  gx, = torch.autograd.grad(lp.sum() + ent.sum(), x)
+  c = policy.choose(x, **kw)
+  for t in (lp, ent, gx[:, 0]):
+    assert torch.isfinite(t[0]) and torch.isnan(t[1:]).all()
+  assert c.action[0] >= 0 and c.action[[1, 3]].tolist() == [-1, -1]  # (64 bits hold 1e-40 and its reciprocal)
+  # without a history there is nothing to repeat
+  lp, _ = policy.evaluate(x, torch.zeros(4, dtype=torch.int32, device=DEV), repetition=1e300)
+  assert torch.isfinite(lp).all()
