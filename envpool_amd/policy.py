@@ -306,6 +306,8 @@ def evaluate(logits, action, *, num_options=None, mask=None, bias=None, history=
   illegal option -inf, a value outside [-1, A) NaN. The statistics of a row and the gradients' sums are kept in
   32 bits; gradients come in the type of the tensor they belong to."""
   _no_tangents("evaluate", logits=logits, bias=bias, repetition=repetition, frequency=frequency, presence=presence, temperature=temperature)
+  differentiable = torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad))
+  given = bias
   if bias is not None and bias.requires_grad and bias.dim() == 2 and bias.shape[0] > 1 and bias.stride(0) == 0:
     bias = bias.contiguous()  # one row of biases expanded by the caller: its gradient is one per row
   p = _prepare(logits, num_options, mask, bias, history, repetition, frequency, presence, temperature)
@@ -314,11 +316,11 @@ def evaluate(logits, action, *, num_options=None, mask=None, bias=None, history=
   _same_device(p.dev, action=action)
   if not action.is_contiguous():
     action = action.contiguous()
-  if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
+  if differentiable:
     # (copies that were laid out for the kernels are no part of the graph: the gradients are those of the originals)
     if p.tensors[0] is not logits or p.tensors[_BIAS] is not bias:
       p.tensors = tuple(t.detach() if i in (0, _BIAS) and t is not None else t for i, t in enumerate(p.tensors))
-    nodes = _guard_capture(logits, bias)  # noqa: F841
+    nodes = _guard_capture(logits, given)  # noqa: F841 (not the copy in the leaf's place)
     return _Evaluate.apply(logits, bias, action, p)
   return _evaluate_forward(p, action)[:2]
 
@@ -563,9 +565,10 @@ def memory_scan(q, k, v, log_decay, *, fresh=None, state=None, scale: Optional[f
   if state is not None and (state.dtype != torch.float32 or state.shape != (n, h, dk, dv)):
     raise ValueError(f"state must be float32 [{n}, {h}, {dk}, {dv}], got {state.dtype} {list(state.shape)}")
   _same_device(q.device, k=k, v=v, log_decay=log_decay, fresh=fresh, state=state)
-  q, k, v, log_decay = _dense_last(q), _dense_last(k), _dense_last(v), log_decay.contiguous()
   scale = dk ** -0.5 if scale is None else float(scale)
-  if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, state)):
-    nodes = _guard_capture(q, k, v, state)  # noqa: F841
+  differentiable = torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, state))
+  nodes = _guard_capture(q, k, v, state) if differentiable else ()  # noqa: F841 (before copies take the leaves' place)
+  q, k, v, log_decay = _dense_last(q), _dense_last(k), _dense_last(v), log_decay.contiguous()
+  if differentiable:
     return _MemoryScan.apply(q, k, v, state, log_decay, fresh, scale)
   return _scan_forward(q, k, v, state, log_decay, fresh, scale)

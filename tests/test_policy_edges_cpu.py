@@ -224,3 +224,24 @@ def test_numbers_that_32_bits_do_not_hold_are_refused_by_evaluate(name, bad):
   assert L.ep_policy_choose(r, None, 0, None, None, None) == capi.EP_OK
   setattr(rows, name, ptr)  # (one per row is on the device)
   assert L.ep_policy_evaluate(r, None, None, None, None) == capi.EP_OK
+
+
+def test_the_guard_of_captures_sees_the_leaves_themselves(stand_in, monkeypatch):
+  """Not the copies that are made of those whose rows have gaps: behind a copy the leaf's node would go unnoticed."""
+
+  class Seen(Exception):
+    pass
+
+  def guard(*inputs):
+    raise Seen(inputs)
+
+  monkeypatch.setattr(stand_in, "_guard_capture", guard)
+  leaf = torch.randn(5, 2, 4, 3).requires_grad_()
+  state = torch.randn(2, 3, 4, 4)
+  with pytest.raises(Seen) as e:
+    stand_in.memory_scan(leaf.detach().transpose(2, 3).requires_grad_(), *(torch.randn(5, 2, 3, 4) for _ in range(2)), torch.zeros(3), state=state)
+  assert all(t.is_leaf for t in e.value.args[0])
+  logits, bias = torch.randn(6, 3).t().requires_grad_(), torch.randn(1, 6).expand(3, 6).requires_grad_()
+  with pytest.raises(Seen) as e:
+    stand_in.evaluate(logits, torch.zeros(3, dtype=torch.int32), bias=bias)
+  assert e.value.args[0][0] is logits and e.value.args[0][1] is bias
