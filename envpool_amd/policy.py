@@ -14,6 +14,7 @@ overwritten when the ring comes round: clone what a later backward pass needs.
 
 The reference has no counterpart (its policies see numpy arrays, envpool2/python/envpool.py:135-142)."""
 import math
+import threading
 from typing import NamedTuple, Optional
 
 import torch
@@ -188,26 +189,28 @@ def choose(logits, u=None, *, num_options=None, mask=None, bias=None, history=No
     return Choice(action, log_prob, entropy)
 
 
-_CAPTURE = None  # a token that lasts from one capture's first differentiable call to the next eager one
+_capture = threading.local()  # .token: lasts from a capture's first differentiable call to the thread's next eager one
 
 
 def _guard_capture(*inputs):
   """Refuses a differentiable call inside a graph capture where a leaf among its inputs is still part of a graph
   recorded outside it: torch would make that graph's stream wait inside the capture, which ends the process
   when the capture ends. (Whether somebody holds a leaf's accumulation node shows in a mark left on it: with no
-  other holder the node goes, and the mark with it.) Returns the nodes, to be held until the call is recorded."""
-  global _CAPTURE
+  other holder the node goes, and the mark with it. Any holder counts: a wrapper that keeps the nodes of a module's
+  parameters, to reduce their gradients, has them refused as well, since on which stream a node was made cannot be asked.)
+  Returns the nodes, to be held until the call is recorded."""
   if not torch.cuda.is_current_stream_capturing():
-    _CAPTURE = None
+    _capture.token = None
     return ()
-  if _CAPTURE is None:
-    _CAPTURE = object()
+  token = getattr(_capture, "token", None)
+  if token is None:
+    token = _capture.token = object()
   nodes = []
   for t in inputs:
     if t is None or not t.requires_grad or not t.is_leaf:
       continue
     node = torch.autograd.graph.get_gradient_edge(t).node
-    if node.metadata.get("envpool_amd_capture") is _CAPTURE:
+    if node.metadata.get("envpool_amd_capture") is token:
       continue
     node.metadata["envpool_amd_probe"] = True
     del node
@@ -215,8 +218,8 @@ def _guard_capture(*inputs):
     if "envpool_amd_probe" in node.metadata:
       del node.metadata["envpool_amd_probe"]
       raise RuntimeError("graph capture: a leaf input still belongs to an autograd graph recorded outside this capture; "
-                         "drop that graph (its outputs) before capturing, or capture over other leaves")
-    node.metadata["envpool_amd_capture"] = _CAPTURE
+                         "drop that graph (its outputs), or what else holds the leaf's accumulation node, before capturing, or capture over other leaves")
+    node.metadata["envpool_amd_capture"] = token
     nodes.append(node)
   return nodes
 

@@ -245,3 +245,30 @@ def test_the_guard_of_captures_sees_the_leaves_themselves(stand_in, monkeypatch)
   with pytest.raises(Seen) as e:
     stand_in.evaluate(logits, torch.zeros(3, dtype=torch.int32), bias=bias)
   assert e.value.args[0][0] is logits and e.value.args[0][1] is bias
+
+
+def test_an_eager_call_in_another_thread_is_no_business_of_a_capture(monkeypatch):
+  """Two calls over one leaf in one capture, while another thread works without one."""
+  import threading
+
+  from envpool_amd import policy
+  capturing = threading.local()
+  monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: getattr(capturing, "yes", False))
+  leaf, other = torch.zeros(3).requires_grad_(), torch.zeros(3).requires_grad_()
+  capturing.yes = True
+  first = policy._guard_capture(leaf)
+  recorded = leaf * 2  # (the first call's graph holds the leaf's node)
+  thread = threading.Thread(target=lambda: policy._guard_capture(other))
+  thread.start()
+  thread.join()
+  policy._guard_capture(leaf)
+  del first, recorded
+  # a graph recorded outside the capture is still found
+  capturing.yes = False
+  policy._guard_capture(leaf)
+  living = leaf * 2
+  capturing.yes = True
+  with pytest.raises(RuntimeError, match="recorded outside this capture"):
+    policy._guard_capture(leaf)
+  del living
+  assert len(policy._guard_capture(leaf)) == 1
