@@ -58,11 +58,11 @@ def _no_tangents(call, **tensors):
 def _row_operand(t, name, rows, cols):
   """A `[cols]`, `[1, cols]` or `[rows, cols]` tensor -> (tensor, stride from row to row, 0: shared)."""
   if t.dim() == 1 and t.shape[0] == cols:
-    return (t if t.stride(0) == 1 or cols == 1 else t.contiguous()), 0
+    return (t if t.stride(0) == 1 or cols == 1 else t.detach().contiguous()), 0
   if t.dim() != 2 or t.shape[1] != cols or t.shape[0] not in (1, rows):
     raise ValueError(f"{name} must be [{cols}] or [{rows}, {cols}], got {list(t.shape)}")
   if (cols > 1 and t.stride(1) != 1) or 0 < t.stride(0) < cols:
-    t = t.contiguous()
+    t = t.detach().contiguous()
   return t, 0 if t.shape[0] == 1 and rows != 1 else t.stride(0)
 
 
@@ -92,11 +92,12 @@ def _dense(t):
 
 def _bind(p):
   """Lays `p.tensors` (of checked types and shapes) out as the kernels read them and fills `p.native` with where they are
-  now. The backward pass does it anew where what autograd hands back is laid out otherwise than what was saved."""
+  now. The backward pass does it anew where what autograd hands back is laid out otherwise than what was saved. (Copies
+  are no part of the graph: the gradients are those of the originals, and _guard_capture must not find a leaf held by them.)"""
   logits, num_options, mask, bias, history, *per_row = p.tensors
   n, a = logits.shape
   if (a > 1 and logits.stride(1) != 1) or (n > 1 and logits.stride(0) < a):
-    logits = logits.contiguous()
+    logits = logits.detach().contiguous()
   if num_options is not None and not num_options.is_contiguous():
     num_options = num_options.contiguous()
   mask_ptr = mask_dt = mask_stride = bias_ptr = bias_dt = bias_stride = hist_ptr = hist_len = hist_stride = 0
@@ -310,9 +311,6 @@ def evaluate(logits, action, *, num_options=None, mask=None, bias=None, history=
   32 bits; gradients come in the type of the tensor they belong to."""
   _no_tangents("evaluate", logits=logits, bias=bias, repetition=repetition, frequency=frequency, presence=presence, temperature=temperature)
   differentiable = torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad))
-  given = bias
-  if bias is not None and bias.requires_grad and bias.dim() == 2 and bias.shape[0] > 1 and bias.stride(0) == 0:
-    bias = bias.contiguous()  # one row of biases expanded by the caller: its gradient is one per row
   p = _prepare(logits, num_options, mask, bias, history, repetition, frequency, presence, temperature)
   if action.dtype != torch.int32 or action.shape != (p.n,):
     raise ValueError(f"action must be int32 [{p.n}], got {action.dtype} {list(action.shape)}")
@@ -320,10 +318,11 @@ def evaluate(logits, action, *, num_options=None, mask=None, bias=None, history=
   if not action.is_contiguous():
     action = action.contiguous()
   if differentiable:
-    # (copies that were laid out for the kernels are no part of the graph: the gradients are those of the originals)
-    if p.tensors[0] is not logits or p.tensors[_BIAS] is not bias:
-      p.tensors = tuple(t.detach() if i in (0, _BIAS) and t is not None else t for i, t in enumerate(p.tensors))
-    nodes = _guard_capture(logits, given)  # noqa: F841 (not the copy in the leaf's place)
+    nodes = _guard_capture(logits, bias)  # noqa: F841
+    if bias is not None and bias.requires_grad and bias.dim() == 2 and bias.shape[0] > 1 and bias.stride(0) == 0:
+      bias = _dense(bias)  # one row of biases expanded by the caller: its gradient is one per row
+      p.tensors = (*p.tensors[:_BIAS], bias, *p.tensors[_BIAS + 1:])
+      _bind(p)
     return _Evaluate.apply(logits, bias, action, p)
   return _evaluate_forward(p, action)[:2]
 

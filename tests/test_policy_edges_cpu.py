@@ -42,6 +42,7 @@ def stand_in(monkeypatch):
   from envpool_amd import policy
   monkeypatch.setattr(policy, "_same_device", lambda dev, **tensors: None)
   monkeypatch.setattr(policy, "current_stream_handle", lambda dev: 0)
+  _FakeRows.guard = staticmethod(policy._guard_capture)
   monkeypatch.setattr(policy, "_guard_capture", lambda *inputs: ())
   monkeypatch.setattr(policy, "_native", types.SimpleNamespace(Rows=_FakeRows))
   _FakeRows.calls = []
@@ -272,3 +273,18 @@ def test_an_eager_call_in_another_thread_is_no_business_of_a_capture(monkeypatch
     policy._guard_capture(leaf)
   del living
   assert len(policy._guard_capture(leaf)) == 1
+
+
+def test_copies_of_a_call_do_not_count_as_holders_of_its_leaves(stand_in, monkeypatch):
+  """Inside a capture: leaves whose rows have gaps, or are one row expanded, and no graph outside."""
+  monkeypatch.setattr(stand_in, "_guard_capture", _FakeRows.guard)
+  monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+  act = torch.zeros(3, dtype=torch.int32)
+  for bias in (None, torch.randn(1, 6).expand(3, 6), torch.randn(6, 3).t(), torch.randn(12)[::2]):
+    stand_in._capture.token = None
+    logits = torch.randn(6, 3).t().requires_grad_()
+    bias = None if bias is None else bias.requires_grad_()
+    lp, ent = stand_in.evaluate(logits, act, bias=bias)
+    (lp.sum() + ent.sum()).backward()
+    assert logits.grad.shape == (3, 6) and (bias is None or bias.grad.shape == bias.shape)
+  stand_in._capture.token = None

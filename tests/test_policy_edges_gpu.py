@@ -397,3 +397,40 @@ def test_repetitions_of_a_row_that_are_no_numbers():
   # without a history there is nothing to repeat
   lp, _ = policy.evaluate(x, torch.zeros(4, dtype=torch.int32, device=DEV), repetition=1e300)
   assert torch.isfinite(lp).all()
+
+
+def test_captured_over_leaves_with_gaps():
+  """Transposed and expanded leaves in a captured forward and backward pass: every replay against the eager result."""
+  from envpool_amd import policy
+  g = _gen(4)
+  n, a, t = 5, 12, 130
+  logits = torch.randn(a, n, generator=g).to(DEV).t().requires_grad_()
+  bias = torch.randn(1, a, generator=g).to(DEV).expand(n, a).requires_grad_()
+  q = torch.randn(t, 3, 8, 2, generator=g).to(DEV).transpose(2, 3).requires_grad_()
+  k, v = (torch.randn(t, 3, 2, 8, generator=g).to(DEV).requires_grad_() for _ in range(2))
+  action = torch.arange(n, dtype=torch.int32, device=DEV)
+  decay = torch.tensor([-0.1, -0.2], device=DEV)
+
+  def work():
+    lp, ent = policy.evaluate(logits, action, bias=bias)
+    out, final = policy.memory_scan(q, k, v, decay)
+    outs = [lp, ent, out, final]
+    return [x.detach() for x in outs] + list(torch.autograd.grad(outs, [logits, bias, q, k, v], [torch.ones_like(x) for x in outs]))
+
+  side = torch.cuda.Stream()
+  with torch.cuda.stream(side):
+    work()
+  torch.cuda.current_stream().wait_stream(side)
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    captured = work()
+  for _ in range(3):
+    with torch.no_grad():
+      logits.copy_(torch.randn(n, a, generator=g).to(DEV))
+      k.copy_(torch.randn(t, 3, 2, 8, generator=g).to(DEV))
+    graph.replay()
+    got = [x.clone() for x in captured]
+    torch.cuda.synchronize()
+    want = work()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, w) for x, w in zip(got, want))
