@@ -332,6 +332,20 @@ def _dense_last(t):
   return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+_error_pages, _error_lock = [], threading.Lock()
+
+
+def _error_word():
+  """A pinned word for a memory's kernels to flag an error in. Never freed: a step that is still under way when its memory
+  is dropped must not write into what somebody else has been given meanwhile."""
+  with _error_lock:
+    if not _error_pages or _error_pages[-1][1] == 1024:
+      _error_pages.append([torch.zeros(1024, dtype=torch.int32, pin_memory=True), 0])
+    page, used = _error_pages[-1]
+    _error_pages[-1][1] += 1
+  return page[used:used + 1]
+
+
 class EnvMemory:
   """The memory of a policy over the envs of a pool: per env and head a state `[key_dim, value_dim]` in
   float32, S <- exp(log_decay[head]) S + k^T v, out = scale * q S, zeroed where an episode starts.
@@ -359,7 +373,7 @@ class EnvMemory:
     self.env_id_offset, self.device = env_id_offset, dev
     self.log_decay = log_decay.detach().contiguous()
     self.state = torch.zeros(shape, dtype=torch.float32, device=dev) if state is None else state.detach()
-    self._error = torch.zeros(1, dtype=torch.int32, pin_memory=True)  # the kernel's word: an env id out of range
+    self._error = _error_word()  # set by a kernel: an env id out of range
     self._error_np = self._error.numpy()
     self._native = _native.Step(dev.index, num_envs, num_heads, key_dim, value_dim, self.log_decay.data_ptr(), self.state.data_ptr(), env_id_offset,
                                 self._error.data_ptr())

@@ -434,3 +434,25 @@ def test_captured_over_leaves_with_gaps():
     want = work()
     torch.cuda.synchronize()
     assert all(torch.equal(x, w) for x, w in zip(got, want))
+
+
+def test_the_error_word_of_a_dropped_memory_is_nobody_elses():
+  """A step under way may still flag an error when its memory is gone: not in memory that has a new owner."""
+  from envpool_amd import policy
+  words = []
+  for _ in range(3):
+    memory = policy.EnvMemory(2, 1, 4, 4, torch.zeros(1, device=DEV))
+    words.append(memory._error.data_ptr())
+    del memory
+    new = [torch.zeros(1, dtype=torch.int32, pin_memory=True) for _ in range(8)]
+    assert not any(t.data_ptr() <= w < t.data_ptr() + 4 for t in new for w in words)
+  assert len(set(words)) == 3
+  memories = [policy.EnvMemory(2, 1, 4, 4, torch.zeros(1, device=DEV)) for _ in range(1100)]
+  assert len({m._error.data_ptr() for m in memories}) == 1100
+  one = torch.ones(1, 1, 4, device=DEV)
+  memories[700].step(one, one, one, env_id=torch.tensor([5], dtype=torch.int32, device=DEV))
+  torch.cuda.synchronize()
+  for i in (0, 699, 701, 1099):
+    memories[i].poll_errors()
+  with pytest.raises(RuntimeError, match="outside"):
+    memories[700].poll_errors()
