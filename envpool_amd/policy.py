@@ -489,6 +489,9 @@ def _scan_forward(q, k, v, state, log_decay, fresh, scale):
 
 def _scan_backward(ctx, g_out, g_final):
   q, k, v, state, log_decay, fresh = ctx.saved_tensors
+  # (a hook for saved tensors may hand back another layout)
+  q, k, v, log_decay = _dense_last(q), _dense_last(k), _dense_last(v), _dense(log_decay)
+  _same_device(ctx.dev, q=q, k=k, v=v, state=state, log_decay=log_decay, fresh=fresh)
   t, n, h, dk = q.shape
   dv, hk = v.shape[3], k.shape[2]
   group, scale = h // hk, ctx.scale
@@ -539,7 +542,7 @@ class _MemoryScan(torch.autograd.Function):
   def forward(ctx, q, k, v, state, log_decay, fresh, scale):
     ctx.set_materialize_grads(False)
     ctx.save_for_backward(q, k, v, state, log_decay, fresh)
-    ctx.scale = scale
+    ctx.scale, ctx.dev = scale, q.device
     return _scan_forward(q, k, v, state, log_decay, fresh, scale)
 
   @staticmethod

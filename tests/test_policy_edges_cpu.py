@@ -288,3 +288,43 @@ def test_copies_of_a_call_do_not_count_as_holders_of_its_leaves(stand_in, monkey
     (lp.sum() + ent.sum()).backward()
     assert logits.grad.shape == (3, 6) and (bias is None or bias.grad.shape == bias.shape)
   stand_in._capture.token = None
+
+
+@pytest.mark.parametrize("where", ["last", "decay"])
+def test_the_backward_pass_of_a_scan_takes_any_layout(stand_in, monkeypatch, where):
+  """The kernels read rows whose last dimension is dense, and a dense log_decay: whatever a hook hands back."""
+  scans = []
+
+  class Scan:
+    def __init__(self, dev, dtype, steps, rows, heads, key_dim, value_dim, log_decay, *rest):
+      self.decay, self.seen = log_decay, {}
+      scans.append(self)
+
+    def operands(self, q, qs, qg, k, ks, kg, v, vs, vg):
+      self.seen = {q: qs, k: ks, v: vs}
+
+    def workspace(self):
+      return 0
+
+    output = states = direction = run = lambda self, *args: None
+
+  monkeypatch.setattr(stand_in, "_native", types.SimpleNamespace(Scan=Scan, scan_pair_workspace=lambda x, y: 0, scan_pair=lambda x, y, ws, n: None))
+  q, k, v = (torch.randn(5, 2, 3, 4).requires_grad_() for _ in range(3))
+  handed = []
+
+  def unpack(t):
+    if where == "last" and t.dim() == 4:
+      t = t.transpose(2, 3).contiguous().transpose(2, 3)
+    if where == "decay" and t.dim() == 1:
+      t = torch.stack([t, t], 1)[:, 0]
+    handed.append(t)
+    return t
+
+  with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(), unpack):
+    out, final = stand_in.memory_scan(q, k, v, torch.zeros(3))
+  del scans[:]
+  (out.sum() + final.sum()).backward()
+  gaps = {t.data_ptr() for t in handed if t.stride(-1) != 1}
+  assert gaps and len(scans) == 3
+  for s in scans:
+    assert s.decay not in gaps and not gaps & set(s.seen), where
