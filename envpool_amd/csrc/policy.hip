@@ -270,7 +270,7 @@ int ep_policy_evaluate_grad(const ep_policy_rows* r, const int32_t* action, cons
   if (int rc = check_rows(r, &k)) return rc;
   if (int rc = check_narrow(r)) return rc;
   if (r->rows > 0 && (!action || !entropy || !stats)) return fail(EP_ERR_INVALID, "action, entropy, stats: null pointer");
-  if (!grad_logits && !grad_bias) return fail(EP_ERR_INVALID, "neither grad_logits nor grad_bias is wanted");
+  if (r->rows > 0 && !grad_logits && !grad_bias) return fail(EP_ERR_INVALID, "neither grad_logits nor grad_bias is wanted");
   if (grad_logits && r->rows > 1 && grad_logits_stride < r->options) return fail(EP_ERR_INVALID, "grad_logits_stride = %lld is less than options", (long long)grad_logits_stride);
   if ((uintptr_t)grad_logits % size_of(r->dtype)) return fail(EP_ERR_INVALID, "grad_logits: not aligned to its type");
   if (grad_bias && !r->bias) return fail(EP_ERR_INVALID, "grad_bias without a bias");

@@ -456,3 +456,37 @@ def test_the_error_word_of_a_dropped_memory_is_nobody_elses():
     memories[i].poll_errors()
   with pytest.raises(RuntimeError, match="outside"):
     memories[700].poll_errors()
+
+
+def test_gradients_of_segments_without_steps_or_rows():
+  """No steps: the first state is the last one, gradient included. No rows: empty gradients."""
+  from envpool_amd import policy
+  g = _gen(1)
+  for t, n in ((0, 3), (7, 0), (130, 0), (0, 0)):
+    q, k, v = (torch.randn(t, n, h, 8, generator=g).to(DEV).requires_grad_() for h in (4, 2, 2))
+    state = torch.randn(n, 4, 8, 8, generator=g).to(DEV).requires_grad_()
+    out, final = policy.memory_scan(q, k, v, torch.full((4,), -0.5, device=DEV), state=state)
+    ds = torch.randn(n, 4, 8, 8, generator=g).to(DEV)
+    grads = torch.autograd.grad([out, final], [q, k, v, state], [torch.ones_like(out), ds])
+    assert [x.shape for x in grads] == [x.shape for x in (q, k, v, state)]
+    assert torch.equal(grads[3], ds) and torch.equal(final, state)
+
+
+@pytest.mark.parametrize("a", [24, 5000])
+@pytest.mark.parametrize("rows", [0, 1, 37])
+def test_the_gradient_of_a_bias_alone(a, rows):
+  """Logits that require none, a bias for all rows and one for each."""
+  from envpool_amd import policy
+  g = _gen(a)
+  x = torch.randn(rows, a, generator=g).to(DEV)
+  action = torch.randint(0, a, (rows,), generator=g, dtype=torch.int32).to(DEV)
+  for b in (torch.randn(a, generator=g), torch.randn(1, a, generator=g), torch.randn(rows, a, generator=g)):
+    alone, both = b.to(DEV).requires_grad_(), b.to(DEV).requires_grad_()
+    leaf = x.clone().requires_grad_()
+    lp, ent = policy.evaluate(x, action, bias=alone)
+    one, = torch.autograd.grad(lp.sum() + ent.sum(), alone)
+    lp, ent = policy.evaluate(leaf, action, bias=both)
+    _, two = torch.autograd.grad(lp.sum() + ent.sum(), [leaf, both])
+    assert one.shape == b.shape and torch.equal(one, two) and (rows or not one.any())
+  lp, ent = policy.evaluate(leaf, action)
+  assert torch.autograd.grad(lp.sum() + ent.sum(), leaf)[0].shape == (rows, a)
