@@ -58,7 +58,7 @@ int64_t per_cu(const ep_memory_scan_args* a) { return a->dtype == EP_F32 ? per_c
 // Split of the time axis. One part per state keeps everything single-pass. With fewer states than the chip holds at
 // once, the axis is cut into parts that are walked side by side: keys and values are then read twice (first for the
 // states between the parts), which counts as 1.6 times the chunks plus the join. 32768 steps of 16 states of 128 x 128
-// in bf16: 77 + 14 + 169 us in 32 parts, 2982 in one; 777 steps of 30 states in f32: 16 + 9 + 28 us, 166 in one.
+// in bf16: 82 + 14 + 187 us in 32 parts, 3230 in one; 777 steps of 30 states in f32: 15 + 9 + 28 us, 167 in one.
 int64_t scan_parts(const ep_memory_scan_args* a) {
   const int64_t states = a->rows * a->heads, chunk = chunk_steps(a->dtype), chunks = (a->steps + chunk - 1) / chunk;
   if (states <= 0 || chunks < 2) return 1;
@@ -140,10 +140,10 @@ bool state_vec(const ep_memory_scan_args* a) {
 }
 
 // Short segments are walked step by step (scan_few). Forward / with all gradients, us, walk of chunks against it:
-//   65536 states of 16 x 16 bf16: 4 steps 401 / 1537, 107 / 418; 16 steps 405 / 1546, 310 / 1252; 32 steps 451 / 1668, 611 / 2436
-//   65536 states of 32 x 32 bf16: 4 steps 406 / 1542, 131 / 469; 16 steps 423 / 1584, 315 / 1227; 32 steps 510 / 1845, 574 / 2273
-//   16384 states of 64 x 64 f32:  4 steps 190 / 711, 126 / 576;  8 steps 195 / 722, 148 / 676;    16 steps 203 / 740, 197 / 877
-// In 16 bits states of 64 x 64 stay with the chunks (4 steps 124 / 429, 118 / 556), whose gradients share a launch.
+//   65536 states of 16 x 16 bf16: 4 steps 468 / 1761, 110 / 421; 16 steps 470 / 1769, 310 / 1254; 32 steps 497 / 1834, 611 / 2436
+//   65536 states of 32 x 32 bf16: 4 steps 478 / 1781, 133 / 476; 16 steps 484 / 1788, 317 / 1235; 32 steps 537 / 1946, 574 / 2273
+//   16384 states of 64 x 64 f32:  4 steps 193 / 727, 125 / 577;  8 steps 198 / 737, 147 / 673;    16 steps 206 / 756, 197 / 877
+// In 16 bits states of 64 x 64 stay with the chunks (4 steps 143 / 489, 118 / 556), whose gradients share a launch.
 constexpr int64_t kFewSteps = 16, kFewKeySteps = 128;
 // how scan_few lays a state over a wave: 2^width_log lanes of four values, `keys` keys a lane; keys 0: not its size
 struct Few {
@@ -152,7 +152,7 @@ struct Few {
 Few few_steps(const ep_memory_scan_args* a);
 
 // whether two scans are the gradients of values (a) and keys (b) of one call, in a form that one kernel covers (128
-// steps of 4096 states of 64 x 64 in bf16: 161 us, one after the other 204). Other sizes' two states and six tiles would
+// steps of 4096 states of 64 x 64 in bf16: 175 us, one after the other 204). Other sizes' two states and six tiles would
 // leave a CU one workgroup, and a split axis has two walks that start from different states.
 bool pairs_up(const ep_memory_scan_args* a, const ep_memory_scan_args* b) {
   const auto same = [](const int64_t* x, const int64_t* y, int n) { return std::equal(x, x + n, y); };

@@ -11,7 +11,8 @@
 // computes 16 of the query columns and needs all of them for its quarter of the value columns, and an output row is
 // written 4 values a lane.
 // What 32-bit values become as operands of 16-bit products (every sum is kept in 32 bits):
-//   weighted values in K^T V   three pieces (bf16) or two scaled ones (f16): the state keeps what 32 bits keep
+//   weighted values in K^T V   three pieces (bf16) or two scaled ones (f16): the state keeps what 32 bits keep (f16: of terms
+//                              below 2^-14, where the type's own steps stop shrinking, 2^-36 each)
 //   the state in Q S           two pieces: 16 bits of it in bf16, 22 in f16
 //   scores in P V              two pieces, the same
 // so that an output is off by 2^-16 (2^-22) of its terms before it is rounded to its type once. (With the scores in one
@@ -678,9 +679,9 @@ template <bool rev> __device__ inline void cut_chunk(uint64_t starts, uint64_t s
   n = to - from;
 }
 
-// One walk. 128 steps of 4096 states of 64 x 64 in bf16, states in and out: 105 us = 3.8 TB/s of the 403 MB it moves,
-// 78 % of a large copy; vector and matrix instructions share the rest (half of the cycles issue vector instructions).
-// 32768 steps of 16 states of 128 x 128 in 32 parts: 169 us for 537 MB and 103 Gflop with the pieces (matrix floor 85
+// One walk. 128 steps of 4096 states of 64 x 64 in bf16, states in and out: 108 us = 3.7 TB/s of the 403 MB it moves,
+// 76 % of a large copy; vector and matrix instructions share the rest (half of the cycles issue vector instructions).
+// 32768 steps of 16 states of 128 x 128 in 32 parts: 187 us for 537 MB and 109 Gflop with the pieces (matrix floor 90
 // us). In f32 two chunks of 32 steps of 80 x 112 take 28 us in 390 workgroups: a CU's two workgroups need 11 us on the
 // matrix cores, the rest is the state's way in and out and loads that nothing hides.
 template <class T, int DK, int DV, bool kAligned, bool rev>
@@ -819,8 +820,8 @@ __global__ __launch_bounds__(256, (ScanTile<T, DK, DV>::kWaves(kAligned))) void 
 
 // Two walks back in time over the same four tensors, for the gradients of keys and values (a: values, from keys,
 // queries and the outputs' gradients; b: keys, from values, the outputs' gradients and queries): the tiles of a chunk
-// are read once for both. 16-bit types, sizes up to 64, time not split. 128 steps of 4096 states in bf16: 161 us for the
-// 604 MB that the two move (3.75 TB/s); three workgroups a CU (149 and 160 registers, 48 KB of LDS).
+// are read once for both. 16-bit types, sizes up to 64, time not split. 128 steps of 4096 states in bf16: 175 us for the
+// 604 MB that the two move (3.45 TB/s); three workgroups a CU (165 and 168 registers, 48 KB of LDS).
 template <class T> struct PairTile {
   using Tile = ScanTile<T, 64, 64>;
   static constexpr size_t kLds = (size_t)Tile::kChunk * (2 * Tile::SQ + 2 * Tile::SK + Tile::SP) * sizeof(T) + 4 * Tile::kChunk * sizeof(float);

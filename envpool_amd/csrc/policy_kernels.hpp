@@ -671,7 +671,7 @@ __global__ __launch_bounds__(kThreads) void choose_group(Rows p, int width_log, 
 }
 
 // evaluate: the same in 32 bits. Bound by instructions (30 an option of a lane, whether the row has it or not: a quarter
-// of the lanes of 24 options): 524288 x 24 bf16 15.4 us = 3 TB/s of 46 MB.
+// of the lanes of 24 options): 524288 x 24 bf16 16 us = 2.9 TB/s of 46 MB.
 template <class T, int NP, bool kHist, bool kWhole> __global__ __launch_bounds__(kThreads) void evaluate_group(Rows p, int width_log, EvaluateOut out) {
   extern __shared__ uint32_t counts[];
   const Group g = group_of(p, blockIdx.x, width_log);
@@ -855,7 +855,7 @@ __global__ __launch_bounds__(kThreads) void choose_join(Rows p, int pieces, int 
 }
 
 // The same walk in 32 bits. One part: the row's results at once; several: partial sums, with the logit of the
-// action from the part that holds it. 2048 x 32768 bf16 with bit masks: 45 us = 3.2 TB/s of 142 MB, bound by
+// action from the part that holds it. 2048 x 32768 bf16 with bit masks: 45 us = 3.1 TB/s of 142 MB, bound by
 // instructions (20 an option: 45 us with the registers kept to eight workgroups a CU, one round of them; 60 in two).
 struct EvaluatePart {
   Stat<float> stat;

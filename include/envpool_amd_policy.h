@@ -139,7 +139,10 @@ int ep_memory_reset(const ep_memory_step_args* args);
  *   reverse:  S_t = d_{t+1} S_{t+1} + inc_scale k_t^T v_t, S_{steps-1} = state_in + inc_scale k^T v;
  *             out_t = out_scale q_t S_t;  state_out = d_0 S_0
  * so that, with o = forward(q, k, v) under `scale`, grad_q = forward(do, v, k; state_in^T) with out_scale = scale,
- * grad_v = reverse(k, q, do; d state_out) and grad_k = reverse(v, do, q; (d state_out)^T), both with inc_scale = scale. */
+ * grad_v = reverse(k, q, do; d state_out) and grad_k = reverse(v, do, q; (d state_out)^T), both with inc_scale = scale.
+ * S and all sums are kept in 32 bits; as operands of 16-bit products S and the scores q_t k_s^T enter with 16 bits (bf16) or 22
+ * (f16), before out is rounded to out_dtype once. Values that are not finite reach the steps that the recurrence takes them to
+ * and no others. */
 typedef struct {
   int32_t device_id;
   int32_t dtype;
