@@ -170,8 +170,9 @@ def choose(logits, u=None, *, num_options=None, mask=None, bias=None, history=No
   is divided by `temperature`. The four numbers may be float32 tensors `[B]`.
 
   `u` (`[B]`, float32 or float64, in [0, 1)): the option where the cumulated probability first exceeds it.
-  None: the most probable option, the lowest of equals. Returns a `Choice` (no gradients: `evaluate` has them); a row without a legal option gets
-  action -1, log_prob 0 and entropy 0, a row with a NaN or +inf among its legal options -1, NaN and NaN."""
+  None: the most probable option, the lowest of equals. Returns a `Choice` (no gradients: `evaluate` has them); a row
+  without a legal option gets action -1, log_prob 0 and entropy 0, a row with a NaN or +inf among its legal options -1,
+  NaN and NaN."""
   with torch.no_grad():
     p = _prepare(logits, num_options, mask, bias, history, repetition, frequency, presence, temperature)
     u_ptr = u_dt = 0
@@ -352,9 +353,10 @@ class EnvMemory:
 
   `log_decay` float32 `[num_heads]` on the GPU, values <= 0 (not differentiated). `state`: an existing
   `[num_envs, num_heads, key_dim, value_dim]` float32 tensor to work on (dense); made, all zero, when None.
-  Dimensions 1 to 256 (`memory_scan`, and so training, 1 to 128). Steps of one memory are ordered by the caller (one stream). A step changes `state` in place, and
-  autograd is told so: a `memory_scan` that starts from it and is differentiated after another step needs a copy
-  (`memory.state.clone()`), without one its backward pass raises. (Replays of a captured step go unnoticed.)"""
+  Dimensions 1 to 256 (`memory_scan`, and so training, 1 to 128). Steps of one memory are ordered by the caller (one
+  stream). A step changes `state` in place, and autograd is told so: a `memory_scan` that starts from it and is
+  differentiated after another step needs a copy (`memory.state.clone()`), without one its backward pass raises.
+  (Replays of a captured step go unnoticed.)"""
 
   def __init__(self, num_envs: int, num_heads: int, key_dim: int, value_dim: int, log_decay: torch.Tensor, *, state: Optional[torch.Tensor] = None,
                env_id_offset: int = 0):
@@ -557,8 +559,8 @@ def memory_scan(q, k, v, log_decay, *, fresh=None, state=None, scale: Optional[f
 
   `log_decay` float32 `[H]`, values <= 0, not differentiated. `fresh` bool / uint8 `[T, B]`: steps at which an
   episode starts, so that nothing from before reaches them (None: no such step). `state` float32
-  `[B, H, key_dim, value_dim]`: where the rows start (None: zero). Dimensions 1 to 128 (`EnvMemory` acts with up to 256). What
-  is not finite goes where the recurrence takes it, to later steps of its episode and, in the gradients, to earlier ones.
+  `[B, H, key_dim, value_dim]`: where the rows start (None: zero). Dimensions 1 to 128 (`EnvMemory` acts with up to
+  256). What is not finite goes where the recurrence takes it: to later steps of its episode, in the gradients to earlier.
   Differentiable (once, backwards: dual numbers are refused) in q, k, v and state; gradients come in the type of the tensor they belong to. States and sums
   are kept in 32 bits. As operands of 16-bit products the states and the scores of a chunk enter as two pieces of the type
   (16 bits together in bfloat16, 22 in float16), so that outputs and gradients are in effect rounded once, at the end;
